@@ -288,6 +288,103 @@ int rq_linear_rows(const void* x, int64_t x_stride, const void* weight, void* y,
                    int64_t out_features, int64_t in_features, hipStream_t stream);
 
 /*
+ * A paged cache held in 8 bits: OCP E4M3 codes [2, num_blocks, kv_heads,
+ * page_tokens, head_dim] (plane 0 K, plane 1 V; 16-byte aligned) and one FP32
+ * scale per (plane, block, head), [2, num_blocks, kv_heads]; a value is
+ * code x scale.  head_dim 96 or 128, page_tokens 16 or 32.  No counterpart in
+ * the reference, which compares its packed pages with a BF16 cache: this is
+ * the 8-bit cache of serving engines, between the two.
+ *
+ * rq_quantize_fp8 writes the K/V of a call's new tokens: request b's n rows
+ * query_start_loc[b]..query_start_loc[b + 1] are the last n of its
+ * seq_lens[b] tokens, token t in slot t % page_tokens of block
+ * block_table[b][t / page_tokens].  Per (plane, page, head) the scale is the
+ * least power of two s >= 2^-126 with |x| <= 448 s for every finite new value
+ * x of the page, or the page's present scale if that is larger and the page
+ * holds earlier tokens of the request; earlier tokens' codes are rounded
+ * again (to nearest, ties to even) where the scale grows.  NaN and infinities
+ * are stored as NaN.  Slots past seq_lens[b] keep their bytes, rows outside
+ * query_start_loc and tokens whose page the table does not hold (or holds
+ * with an invalid block) are skipped.  A block that is written must belong to
+ * one request of the call.  The call may be repeated: it writes the same.
+ * key, value: BF16 [rows, kv_heads, head_dim], 8-byte aligned, token strides
+ * multiples of 4 elements.
+ */
+int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int64_t value_stride, int64_t rows,
+                    int kv_heads, int head_dim, void* cache, float* scales, int64_t num_blocks, int page_tokens,
+                    const int32_t* query_start_loc, const int32_t* seq_lens, int64_t requests,
+                    const int32_t* block_table, int64_t block_table_stride, int64_t max_pages, hipStream_t stream);
+
+/*
+ * Attention over such a cache: request b's n rows are its last n of
+ * seq_lens[b] tokens; row i of them attends to the first seq_lens[b] - n
+ * tokens through block_table (any positive scales, not powers of two only)
+ * and, causally, to the request's new BF16 key/value rows 0..i, which need
+ * not be in the cache:
+ *   out = sum_j softmax_j(softmax_scale q . k_j) v_j.
+ * Query head h reads K/V head h / (heads / kv_heads).  query, output BF16
+ * [rows, heads, head_dim], key, value [rows, kv_heads, head_dim], 8-byte
+ * aligned, token strides multiples of 4 elements.  A request may have no new
+ * rows; rows outside query_start_loc are left as they are; tokens on invalid
+ * blocks are skipped.  `workspace`: device memory of
+ * rq_paged_attention_fp8_workspace_bytes(...), any address; calls that may
+ * overlap need one each.
+ */
+int rq_paged_attention_fp8(const void* query, int64_t query_stride, const void* key, int64_t key_stride,
+                           const void* value, int64_t value_stride, void* output, int64_t output_stride, int64_t rows,
+                           int heads, int kv_heads, int head_dim, const void* cache, const float* scales,
+                           int64_t num_blocks, int page_tokens, const int32_t* query_start_loc,
+                           const int32_t* seq_lens, int64_t requests, const int32_t* block_table,
+                           int64_t block_table_stride, int64_t max_pages, float softmax_scale, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+size_t rq_paged_attention_fp8_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim, int64_t max_pages,
+                                              int page_tokens);
+
+/*
+ * Projections with 4-bit weights: a weight [out_features, in_features] as
+ * codes c in -8..7 and one BF16 scale per output row and group of 32, 64 or
+ * 128 inputs (in_features a multiple of the group), laid out once for the
+ * kernel in rq_int4_weight_bytes(...) bytes of 16-byte aligned device memory
+ * (0 for an invalid shape).
+ * rq_pack_weight_int4 takes codes (INT8 [out, in], limited to -8..7) and
+ * scales (BF16 [out, in / group]); rq_quantize_weight_int4 a BF16 weight:
+ * scale = bf16(largest |w| of the group / 7), code = w / scale to nearest,
+ * ties to even (a group with a NaN or an infinity yields NaN);
+ * rq_dequantize_weight_int4 restores bf16(c x scale).
+ * rq_linear_rows_int4: y[m, n] = bf16(sum_g scale[n, g] sum_{k in g} c[n, k] x[m, k])
+ * for 1-64 BF16 rows x [rows, in_features] (16-byte aligned, x_stride a
+ * multiple of 8), FP32 accumulation.  More rows return RQ_ENOKERNEL.  The
+ * projections of a decode step, as rq_linear_rows, at a quarter of its bytes.
+ */
+size_t rq_int4_weight_bytes(int64_t out_features, int64_t in_features, int group);
+int rq_pack_weight_int4(const int8_t* codes, const void* scales, int64_t out_features, int64_t in_features, int group,
+                        void* packed, size_t packed_bytes, hipStream_t stream);
+int rq_quantize_weight_int4(const void* weight, int64_t out_features, int64_t in_features, int group, void* packed,
+                            size_t packed_bytes, hipStream_t stream);
+int rq_dequantize_weight_int4(const void* packed, size_t packed_bytes, int64_t out_features, int64_t in_features,
+                              int group, void* weight, hipStream_t stream);
+int rq_linear_rows_int4(const void* x, int64_t x_stride, const void* packed, size_t packed_bytes, void* y,
+                        int64_t y_stride, int64_t rows, int64_t out_features, int64_t in_features, int group,
+                        hipStream_t stream);
+
+/* Element types of rq_token_logprobs' logits. */
+enum { RQ_DTYPE_BF16 = 0, RQ_DTYPE_F32 = 1 };
+
+/*
+ * Per row of logits [rows, vocab] (unit column stride, row stride in
+ * elements), with m the row's maximum and S = sum_j e^(x_j - m):
+ *   logprob = x[token] - m - log S  (NaN for a token outside 0..vocab - 1),
+ *   entropy = log S - sum_j e^(x_j - m) (x_j - m) / S  (-inf logits add nothing),
+ *   top_logprobs, top_tokens [rows, top]: the `top` (0 to 32) largest logits,
+ *   largest first, ties to the lower token, as x - m - log S and token.
+ * A row of -inf alone, or with a NaN or +inf, gives NaN; NaN logits rank above all.
+ * Any alignment of whole elements.
+ */
+int rq_token_logprobs(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, const int64_t* tokens,
+                      float* logprob, float* entropy, int top, float* top_logprobs, int64_t* top_tokens,
+                      hipStream_t stream);
+
+/*
  * Kernel timing for measurement: when enabled, rq_attention and
  * rq_paged_attention_bf16 record HIP events around their split-K kernel on
  * the caller's stream; rq_timing_read() synchronizes the recorded events and

@@ -10,10 +10,10 @@ src/residual_quantization/packed_backend.py:63-77.
 """
 
 from .ops import (attention, dequantize, flash_attn_varlen_func, packed_prefill_attention,  # noqa: F401
-                  paged_attention_bf16, prefill_attention, quantize)
+                  paged_attention_bf16, paged_attention_fp8, prefill_attention, quantize, quantize_fp8)
 from .layout import page_width  # noqa: F401
 from .group import DeferredKVGroup  # noqa: F401
 
 __all__ = ("attention", "quantize", "dequantize", "flash_attn_varlen_func", "prefill_attention",
            "packed_prefill_attention",
-           "paged_attention_bf16", "page_width", "DeferredKVGroup")
+           "paged_attention_bf16", "paged_attention_fp8", "quantize_fp8", "page_width", "DeferredKVGroup")

@@ -35,6 +35,15 @@ EXPORTED_SYMBOLS = (
     "rq_rope_qkv",
     "rq_silu_mul",
     "rq_linear_rows",
+    "rq_quantize_fp8",
+    "rq_paged_attention_fp8",
+    "rq_paged_attention_fp8_workspace_bytes",
+    "rq_int4_weight_bytes",
+    "rq_pack_weight_int4",
+    "rq_quantize_weight_int4",
+    "rq_dequantize_weight_int4",
+    "rq_linear_rows_int4",
+    "rq_token_logprobs",
     "rq_timing_enable",
     "rq_timing_read",
     "rq_set_split_target",
@@ -108,6 +117,25 @@ def _declare(l: ctypes.CDLL) -> None:
     l.rq_silu_mul.argtypes = [vp, i64, vp, i64, i64, i32, vp]
     l.rq_linear_rows.restype = i32
     l.rq_linear_rows.argtypes = [vp, i64, vp, vp, i64, i64, i64, i64, vp]
+    l.rq_quantize_fp8.restype = i32
+    l.rq_quantize_fp8.argtypes = [vp, i64, vp, i64, i64, i32, i32, vp, vp, i64, i32, vp, vp, i64, vp, i64, i64, vp]
+    l.rq_paged_attention_fp8.restype = i32
+    l.rq_paged_attention_fp8.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, i32, i32, vp, vp, i64, i32,
+                                         vp, vp, i64, vp, i64, i64, ctypes.c_float, vp, sz, vp]
+    l.rq_paged_attention_fp8_workspace_bytes.restype = sz
+    l.rq_paged_attention_fp8_workspace_bytes.argtypes = [i64, i32, i32, i32, i64, i32]
+    l.rq_int4_weight_bytes.restype = sz
+    l.rq_int4_weight_bytes.argtypes = [i64, i64, i32]
+    l.rq_pack_weight_int4.restype = i32
+    l.rq_pack_weight_int4.argtypes = [vp, vp, i64, i64, i32, vp, sz, vp]
+    l.rq_quantize_weight_int4.restype = i32
+    l.rq_quantize_weight_int4.argtypes = [vp, i64, i64, i32, vp, sz, vp]
+    l.rq_dequantize_weight_int4.restype = i32
+    l.rq_dequantize_weight_int4.argtypes = [vp, sz, i64, i64, i32, vp, vp]
+    l.rq_linear_rows_int4.restype = i32
+    l.rq_linear_rows_int4.argtypes = [vp, i64, vp, sz, vp, i64, i64, i64, i64, i32, vp]
+    l.rq_token_logprobs.restype = i32
+    l.rq_token_logprobs.argtypes = [vp, i64, i32, i64, i64, vp, vp, vp, i32, vp, vp, vp]
     l.rq_timing_enable.argtypes = [i32]
     l.rq_timing_read.restype = i32
     l.rq_timing_read.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]

@@ -21,6 +21,7 @@
 #include "../../include/rq_hip.h"
 #include "rq_kernels.h"
 #include "rq_plan.h"
+#include "rq_reduced.h"
 
 namespace {
 
@@ -1157,6 +1158,246 @@ size_t rq_prefill_workspace_bytes(int64_t batch, int heads_q, int head_dim, int6
     p.causal = causal != 0;
     (void)same_lengths;
     return rq::prefill_plan(p, max_seqlen_k);
+}
+
+// ------------------------------------------------- 8-bit cache, 4-bit weights, log probabilities
+
+// What the writer and the reader of an 8-bit cache both take.
+static int check_fp8_pages(const void* cache, const float* scales, int64_t num_blocks, int kv_heads, int head_dim,
+                           int page_tokens, int64_t rows, const int32_t* query_start_loc, const int32_t* seq_lens,
+                           int64_t requests, const int32_t* block_table, int64_t block_table_stride,
+                           int64_t max_pages) {
+    if ((head_dim != 96 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32))
+        return fail(RQ_ENOKERNEL, "No compiled 8-bit paged kernel for head_dim=%d, page_tokens=%d", head_dim,
+                    page_tokens);
+    if (rows < 0 || rows > (int64_t)INT32_MAX || kv_heads <= 0 || kv_heads > 65535)
+        return fail(RQ_EINVAL, "K/V of 0 or more rows and 1 to 65535 heads required");
+    if (cache == nullptr || scales == nullptr || num_blocks < 0 || (reinterpret_cast<uintptr_t>(cache) % 16) != 0 ||
+        (reinterpret_cast<uintptr_t>(scales) % 4) != 0)
+        return fail(RQ_EINVAL, "16-byte aligned 8-bit cache and its FP32 scales required");
+    if (requests < 0 || (requests > 0 && (query_start_loc == nullptr || seq_lens == nullptr)))
+        return fail(RQ_EINVAL, "Contiguous INT32 query starts with one final boundary required");
+    if ((rows > 0 && requests > 0 && block_table == nullptr) || max_pages < 0 || block_table_stride < max_pages ||
+        max_pages > (int64_t)INT32_MAX / page_tokens)
+        return fail(RQ_EINVAL, "INT32 page table with packed rows required");
+    return RQ_OK;
+}
+
+static int check_bf16_rows(const void* data, int64_t stride, int64_t rows, int64_t heads, int head_dim) {
+    if (stride < heads * head_dim || stride % 4 != 0)
+        return fail(RQ_EINVAL, "BF16 [tokens, heads, channels] with packed trailing strides, a multiple of 4 elements "
+                               "per token, required");
+    if (rows > 0 && (data == nullptr || (reinterpret_cast<uintptr_t>(data) % 8) != 0))
+        return fail(RQ_EINVAL, "8-byte aligned Q/K/V/output required");
+    return RQ_OK;
+}
+
+int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int64_t value_stride, int64_t rows,
+                    int kv_heads, int head_dim, void* cache, float* scales, int64_t num_blocks, int page_tokens,
+                    const int32_t* query_start_loc, const int32_t* seq_lens, int64_t requests,
+                    const int32_t* block_table, int64_t block_table_stride, int64_t max_pages, hipStream_t stream) {
+    int status = check_fp8_pages(cache, scales, num_blocks, kv_heads, head_dim, page_tokens, rows, query_start_loc,
+                                 seq_lens, requests, block_table, block_table_stride, max_pages);
+    if (status == RQ_OK) status = check_bf16_rows(key, key_stride, rows, kv_heads, head_dim);
+    if (status == RQ_OK) status = check_bf16_rows(value, value_stride, rows, kv_heads, head_dim);
+    if (status != RQ_OK) return status;
+    if (rows == 0 || requests == 0 || num_blocks == 0 || max_pages == 0) return ok();
+    rq::Fp8WriteParams p{};
+    p.key = static_cast<const uint16_t*>(key);
+    p.key_stride = key_stride;
+    p.value = static_cast<const uint16_t*>(value);
+    p.value_stride = value_stride;
+    p.rows = rows;
+    p.kv_heads = kv_heads;
+    p.head_dim = head_dim;
+    p.cache = static_cast<uint8_t*>(cache);
+    p.scales = scales;
+    p.num_blocks = num_blocks;
+    p.page_tokens = page_tokens;
+    p.query_start_loc = query_start_loc;
+    p.seq_lens = seq_lens;
+    p.requests = requests;
+    p.block_table = block_table;
+    p.block_table_stride = block_table_stride;
+    p.max_pages = max_pages;
+    return check_launch(rq::launch_quantize_fp8(p, stream), "8-bit cache write launch");
+}
+
+size_t rq_paged_attention_fp8_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim, int64_t max_pages,
+                                              int page_tokens) {
+    (void)rows, (void)heads, (void)kv_heads, (void)head_dim, (void)max_pages, (void)page_tokens;
+    return 256;
+}
+
+int rq_paged_attention_fp8(const void* query, int64_t query_stride, const void* key, int64_t key_stride,
+                           const void* value, int64_t value_stride, void* output, int64_t output_stride, int64_t rows,
+                           int heads, int kv_heads, int head_dim, const void* cache, const float* scales,
+                           int64_t num_blocks, int page_tokens, const int32_t* query_start_loc,
+                           const int32_t* seq_lens, int64_t requests, const int32_t* block_table,
+                           int64_t block_table_stride, int64_t max_pages, float softmax_scale, void* workspace,
+                           size_t workspace_bytes, hipStream_t stream) {
+    int status = check_fp8_pages(cache, scales, num_blocks, kv_heads, head_dim, page_tokens, rows, query_start_loc,
+                                 seq_lens, requests, block_table, block_table_stride, max_pages);
+    if (status != RQ_OK) return status;
+    if (heads <= 0 || heads % kv_heads != 0 || heads > 65535)
+        return fail(RQ_EINVAL, "Query heads must be a positive multiple of key/value heads");
+    if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return fail(RQ_EINVAL, "softmax_scale must be positive");
+    const void* inputs[4] = {query, key, value, output};
+    const int64_t strides[4] = {query_stride, key_stride, value_stride, output_stride};
+    for (int i = 0; i < 4 && status == RQ_OK; ++i)
+        status = check_bf16_rows(inputs[i], strides[i], rows, i == 1 || i == 2 ? kv_heads : heads, head_dim);
+    if (status != RQ_OK) return status;
+    if (rows == 0 || requests == 0) return ok();
+    const size_t needed = rq_paged_attention_fp8_workspace_bytes(rows, heads, kv_heads, head_dim, max_pages, page_tokens);
+    if (workspace == nullptr || workspace_bytes < needed)
+        return fail(RQ_ENOSPACE, "Attention workspace of %zu bytes required, %zu given", needed, workspace_bytes);
+    rq::Fp8AttentionParams p{};
+    p.query = static_cast<const uint16_t*>(query);
+    p.query_stride = query_stride;
+    p.key = static_cast<const uint16_t*>(key);
+    p.key_stride = key_stride;
+    p.value = static_cast<const uint16_t*>(value);
+    p.value_stride = value_stride;
+    p.output = static_cast<uint16_t*>(output);
+    p.output_stride = output_stride;
+    p.rows = rows;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.head_dim = head_dim;
+    p.cache = static_cast<const uint8_t*>(cache);
+    p.scales = scales;
+    p.num_blocks = num_blocks;
+    p.page_tokens = page_tokens;
+    p.query_start_loc = query_start_loc;
+    p.seq_lens = seq_lens;
+    p.requests = requests;
+    p.block_table = block_table;
+    p.block_table_stride = block_table_stride;
+    p.max_pages = max_pages;
+    p.softmax_scale = softmax_scale;
+    return check_launch(rq::launch_attention_fp8(p, stream), "8-bit attention launch");
+}
+
+// The largest sides and elements keep every index of the kernels in range.
+static int check_int4_shape(int64_t out_features, int64_t in_features, int group) {
+    if (group != 32 && group != 64 && group != 128)
+        return fail(RQ_ENOKERNEL, "No compiled 4-bit projection kernel for groups of %d (32, 64 or 128)", group);
+    if (out_features <= 0 || in_features <= 0 || in_features % group != 0 || out_features > (1 << 24) ||
+        in_features > (1 << 20) || out_features * in_features > ((int64_t)1 << 40))
+        return fail(RQ_EINVAL, "4-bit weights need out_features up to 2^24, in_features, a multiple of the group, up "
+                               "to 2^20 and at most 2^40 elements");
+    return RQ_OK;
+}
+
+size_t rq_int4_weight_bytes(int64_t out_features, int64_t in_features, int group) {
+    if (check_int4_shape(out_features, in_features, group) != RQ_OK) return 0;
+    ok();
+    return rq::int4_weight_bytes(out_features, in_features, group);
+}
+
+static int int4_pack_params(rq::Int4PackParams* p, const void* packed, size_t packed_bytes, int64_t out_features,
+                            int64_t in_features, int group) {
+    const int status = check_int4_shape(out_features, in_features, group);
+    if (status != RQ_OK) return status;
+    const size_t needed = rq::int4_weight_bytes(out_features, in_features, group);
+    if (packed == nullptr || (reinterpret_cast<uintptr_t>(packed) % 16) != 0 || packed_bytes < needed)
+        return fail(RQ_EINVAL, "16-byte aligned packed weight of %zu bytes required", needed);
+    *p = rq::Int4PackParams{};
+    p->packed = const_cast<uint32_t*>(static_cast<const uint32_t*>(packed));
+    p->packed_scales = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(p->packed) +
+                                                   rq::int4_code_bytes(out_features, in_features));
+    p->out_features = out_features;
+    p->in_features = in_features;
+    p->group = group;
+    return RQ_OK;
+}
+
+int rq_pack_weight_int4(const int8_t* codes, const void* scales, int64_t out_features, int64_t in_features, int group,
+                        void* packed, size_t packed_bytes, hipStream_t stream) {
+    rq::Int4PackParams p;
+    const int status = int4_pack_params(&p, packed, packed_bytes, out_features, in_features, group);
+    if (status != RQ_OK) return status;
+    if (codes == nullptr || scales == nullptr || (reinterpret_cast<uintptr_t>(scales) % 2) != 0)
+        return fail(RQ_EINVAL, "INT8 codes and BF16 scales required");
+    p.codes = codes;
+    p.scales = static_cast<const uint16_t*>(scales);
+    return check_launch(rq::launch_pack_int4(p, stream), "4-bit weight pack launch");
+}
+
+int rq_quantize_weight_int4(const void* weight, int64_t out_features, int64_t in_features, int group, void* packed,
+                            size_t packed_bytes, hipStream_t stream) {
+    rq::Int4PackParams p;
+    const int status = int4_pack_params(&p, packed, packed_bytes, out_features, in_features, group);
+    if (status != RQ_OK) return status;
+    if (weight == nullptr || (reinterpret_cast<uintptr_t>(weight) % 2) != 0)
+        return fail(RQ_EINVAL, "BF16 weight required");
+    p.weight = static_cast<const uint16_t*>(weight);
+    return check_launch(rq::launch_pack_int4(p, stream), "4-bit weight quantize launch");
+}
+
+int rq_dequantize_weight_int4(const void* packed, size_t packed_bytes, int64_t out_features, int64_t in_features,
+                              int group, void* weight, hipStream_t stream) {
+    rq::Int4PackParams p;
+    const int status = int4_pack_params(&p, packed, packed_bytes, out_features, in_features, group);
+    if (status != RQ_OK) return status;
+    if (weight == nullptr || (reinterpret_cast<uintptr_t>(weight) % 2) != 0)
+        return fail(RQ_EINVAL, "BF16 weight required");
+    return check_launch(rq::launch_unpack_int4(p, static_cast<uint16_t*>(weight), stream), "4-bit weight restore launch");
+}
+
+int rq_linear_rows_int4(const void* x, int64_t x_stride, const void* packed, size_t packed_bytes, void* y,
+                        int64_t y_stride, int64_t rows, int64_t out_features, int64_t in_features, int group,
+                        hipStream_t stream) {
+    if (rows < 0 || rows > rq::kLinearInt4MaxRows)
+        return fail(RQ_ENOKERNEL, "No compiled 4-bit projection kernel for %lld rows (at most %d)", (long long)rows,
+                    rq::kLinearInt4MaxRows);
+    rq::Int4PackParams w;
+    const int status = int4_pack_params(&w, packed, packed_bytes, out_features, in_features, group);
+    if (status != RQ_OK) return status;
+    if (x_stride < in_features || x_stride % 8 != 0 || y_stride < out_features)
+        return fail(RQ_EINVAL, "x rows of in_features (stride a multiple of 8) and y rows of out_features required");
+    if (rows == 0) return ok();
+    if (x == nullptr || y == nullptr || (reinterpret_cast<uintptr_t>(x) % 16) || (reinterpret_cast<uintptr_t>(y) % 2))
+        return fail(RQ_EINVAL, "16-byte aligned x and a BF16 output required");
+    rq::LinearInt4Params p{};
+    p.x = static_cast<const uint16_t*>(x);
+    p.x_stride = x_stride;
+    p.packed = w.packed;
+    p.packed_scales = w.packed_scales;
+    p.y = static_cast<uint16_t*>(y);
+    p.y_stride = y_stride;
+    p.rows = rows;
+    p.out_features = out_features;
+    p.in_features = in_features;
+    p.group = group;
+    return check_launch(rq::launch_linear_int4(p, stream), "4-bit projection launch");
+}
+
+int rq_token_logprobs(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, const int64_t* tokens,
+                      float* logprob, float* entropy, int top, float* top_logprobs, int64_t* top_tokens,
+                      hipStream_t stream) {
+    if (dtype != RQ_DTYPE_BF16 && dtype != RQ_DTYPE_F32) return fail(RQ_EINVAL, "BF16 or FP32 logits required");
+    if (rows < 0 || rows > (int64_t)INT32_MAX || vocab <= 0 || vocab > (int64_t)INT32_MAX || stride < vocab)
+        return fail(RQ_EINVAL, "Logits [rows, vocab] of at least one column with unit column stride required");
+    if (top < 0 || top > rq::kLogprobMaxTop || top > vocab)
+        return fail(RQ_EINVAL, "0 to %d alternatives, at most the vocabulary, required", rq::kLogprobMaxTop);
+    if (rows == 0) return ok();
+    if (logits == nullptr || (reinterpret_cast<uintptr_t>(logits) % (dtype == RQ_DTYPE_BF16 ? 2 : 4)) || tokens == nullptr ||
+        logprob == nullptr || entropy == nullptr || (top > 0 && (top_logprobs == nullptr || top_tokens == nullptr)))
+        return fail(RQ_EINVAL, "Logits, tokens and outputs required");
+    rq::LogprobParams p{};
+    p.logits = logits;
+    p.stride = stride;
+    p.bf16 = dtype == RQ_DTYPE_BF16;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.tokens = tokens;
+    p.logprob = logprob;
+    p.entropy = entropy;
+    p.top = top;
+    p.top_logprobs = top_logprobs;
+    p.top_tokens = top_tokens;
+    return check_launch(rq::launch_logprobs(p, stream), "log probability launch");
 }
 
 void rq_timing_enable(int enabled) {

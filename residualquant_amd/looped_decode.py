@@ -48,13 +48,19 @@ from .layout import page_width
 LINEAR_ROWS_MAX = 8
 
 
-def _project(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
-    """``x @ weight.T`` for a linear weight held ``[out, in]``.
+def _project(x: torch.Tensor, weight) -> torch.Tensor:
+    """``x @ weight.T`` for a linear weight held ``[out, in]``, in BF16 or in 4 bits (``Int4Weight``).
 
     At up to eight rows the product is a weight stream: ``step_ops.linear_rows``
     reads every weight row once with 16-byte loads and FP32 accumulation.
-    Larger batches take hipBLASLt through ``F.linear``."""
+    Larger batches take hipBLASLt through ``F.linear``.  A 4-bit weight takes
+    ``step_ops.linear_rows_int4`` at up to 64 rows; above, it is restored to
+    BF16 for the product."""
     rows, in_features = x.shape
+    if isinstance(weight, step_ops.Int4Weight):
+        if rows <= step_ops.LINEAR_INT4_MAX_ROWS:
+            return step_ops.linear_rows_int4(x, weight)
+        return F.linear(x, weight.dequantize())
     if (rows <= LINEAR_ROWS_MAX and in_features % 8 == 0 and in_features <= 6144 and x.stride(1) == 1
             and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 and weight.is_contiguous()
             and weight.data_ptr() % 16 == 0):
@@ -68,7 +74,9 @@ class LoopedConfig:
 
     ``intermediate`` is not given by the benchmark configuration; 5632 (the
     Ouro-1.4B MLP width at the same hidden size) is an assumption, as are
-    ``rope_theta`` and ``rms_eps``.
+    ``rope_theta`` and ``rms_eps``.  ``projection_bits`` 4 holds the
+    projections and the vocabulary projection as 4-bit codes with a BF16 scale
+    per ``projection_group`` inputs.
     """
 
     layers: int = 48
@@ -84,15 +92,28 @@ class LoopedConfig:
     anchor: int = 3
     coefficient: str = "ls"
     page_tokens: int = 16
+    projection_bits: int = 16
+    projection_group: int = 32
 
 
 class LoopedDecoder:
-    """Synthetic Ouro-shaped model with a packed paged cache for ``batch`` requests."""
+    """Synthetic Ouro-shaped model with a packed paged cache for ``batch`` requests.
+
+    With ``top_logprobs`` (0 to 32) every step also leaves the log probability
+    of each next token, the entropy and that many alternatives in ``logprobs``
+    (``step_ops.TokenLogprobs``)."""
 
     def __init__(self, config: LoopedConfig, batch: int, context: int, max_new_tokens: int,
-                 device: torch.device, seed: int = 0, weights_from: Optional["LoopedDecoder"] = None):
+                 device: torch.device, seed: int = 0, weights_from: Optional["LoopedDecoder"] = None,
+                 top_logprobs: Optional[int] = None):
         if config.loops != len(config.schedule):
             raise ValueError("one packed record per loop is required")
+        if config.projection_bits not in (4, 16):
+            raise ValueError("projections are held in 16 or 4 bits")
+        if top_logprobs is not None and not 0 <= top_logprobs <= min(step_ops.LOGPROBS_MAX_TOP, config.vocab):
+            raise ValueError(f"0 to {step_ops.LOGPROBS_MAX_TOP} alternatives, at most the vocabulary, required")
+        self.top_logprobs = top_logprobs
+        self.logprobs: Optional[step_ops.TokenLogprobs] = None
         self.config = c = config
         self.batch, self.context, self.device = batch, context, device
         self.max_tokens = context + max_new_tokens
@@ -100,7 +121,8 @@ class LoopedDecoder:
 
         def weight(fan_out, fan_in):
             scale = 1.0 / math.sqrt(fan_in)
-            return (torch.randn((fan_out, fan_in), generator=generator, device=device) * scale).to(torch.bfloat16)
+            drawn = (torch.randn((fan_out, fan_in), generator=generator, device=device) * scale).to(torch.bfloat16)
+            return step_ops.quantize_weight_int4(drawn, c.projection_group) if c.projection_bits == 4 else drawn
 
         q_size = c.heads * c.head_dim
         if weights_from is not None:
@@ -175,10 +197,13 @@ class LoopedDecoder:
         model's loops, as the reference binds them (install_model.py:154-196).
         4-D value rotations are folded into this decoder's QKV and O weights
         (weights.py:8-37), in place: call before building the history, and
-        before sharing the weights with another decoder."""
+        before sharing the weights with another decoder (weights held in 4
+        bits cannot take them)."""
         c = self.config
         q_size = c.heads * c.head_dim
         prepared, folded = artifact_module.prepare_value_rotation(artifact)
+        if folded is not None and c.projection_bits != 16:
+            raise ValueError("4-D value rotations fold into BF16 projections only")
         slots = artifact_module.bind_slots(prepared, [c.schedule], c.layers, self.device)[0]
         # Own lists (a decoder built with weights_from shares the originals).
         self.key_rotation, self.value_rotation = list(self.key_rotation), list(self.value_rotation)
@@ -277,6 +302,8 @@ class LoopedDecoder:
         logits = _project(h, self.lm_head)
         # Greedy next token and the next position, slot and sequence length.
         self.tokens.copy_(logits.argmax(dim=-1))
+        if self.top_logprobs is not None:
+            self.logprobs = step_ops.token_logprobs(logits, self.tokens, top=self.top_logprobs)
         self.positions.add_(1)
         self.seq_lens.add_(1)
         self._update_slots()

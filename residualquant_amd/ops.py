@@ -342,6 +342,119 @@ def paged_attention_bf16(query: torch.Tensor, key: torch.Tensor, value: torch.Te
     _lib.check(status)
 
 
+def _validate_fp8_cache(cache, scales, device, kv_heads, head_dim):
+    shape = cache.shape
+    _require(cache.get_device() == device and cache.dtype is torch.float8_e4m3fn and cache.is_contiguous()
+             and len(shape) == 5 and shape[0] == 2 and shape[2] == kv_heads and shape[4] == head_dim,
+             "Contiguous E4M3 [2, blocks, heads, page tokens, channels] cache required")
+    _require(scales.get_device() == device and scales.dtype is torch.float32 and scales.is_contiguous()
+             and scales.shape == shape[:3], "Contiguous FP32 [2, blocks, heads] scales on the cache device required")
+    return shape
+
+
+def _validate_sequences(query_start_loc, seq_lens, block_table, device):
+    """The number of requests."""
+    requests = seq_lens.numel()
+    _require(query_start_loc.get_device() == device and query_start_loc.dtype is torch.int32
+             and query_start_loc.dim() == 1 and query_start_loc.is_contiguous()
+             and query_start_loc.numel() == requests + 1,
+             "Contiguous INT32 query starts with one final boundary required")
+    _require(seq_lens.get_device() == device and seq_lens.dtype is torch.int32 and seq_lens.dim() == 1
+             and seq_lens.is_contiguous(), "Contiguous INT32 sequence lengths required")
+    _require(block_table.get_device() == device and block_table.dtype is torch.int32 and block_table.dim() == 2
+             and (block_table.stride(1) == 1 or block_table.size(1) <= 1) and block_table.size(0) >= requests
+             and (block_table.stride(0) >= block_table.size(1) or block_table.size(0) <= 1),
+             "INT32 page table with packed rows required")
+    return requests
+
+
+def quantize_fp8(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor,
+                 query_start_loc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor) -> None:
+    """Write a call's new K/V tokens into a paged cache held in 8 bits, in place.
+
+    ``cache`` is E4M3 ``[2, blocks, kv_heads, page_tokens, D]`` with FP32
+    ``scales`` ``[2, blocks, kv_heads]``; a value is code x scale.  Request
+    b's rows ``query_start_loc[b]..query_start_loc[b+1]`` of ``key`` and
+    ``value`` (BF16 ``[rows, kv_heads, D]``) are the last of its
+    ``seq_lens[b]`` tokens and go to the slots that ``block_table`` gives
+    them.  A page's scale is the least power of two that keeps its values
+    within E4M3; it grows with a larger value, and the codes of the request's
+    earlier tokens in the page are then rounded again.  NaN and infinities are
+    stored as NaN; slots behind a request's last token keep their bytes; a
+    block that is written belongs to one request of the call.
+    """
+    shape, key_stride = _validate_bf16_token_tensor(key)
+    value_shape, value_stride = _validate_bf16_token_tensor(value)
+    device = key.get_device()
+    _require(value.get_device() == device and value_shape == shape, "K/V must have matching shapes and devices")
+    rows, kv_heads, head_dim = shape
+    _, blocks, _, page_tokens, _ = _validate_fp8_cache(cache, scales, device, kv_heads, head_dim)
+    requests = _validate_sequences(query_start_loc, seq_lens, block_table, device)
+    with _on_device(device):
+        status = _lib.lib().rq_quantize_fp8(
+            key.data_ptr(), key_stride, value.data_ptr(), value_stride, rows, kv_heads, head_dim, cache.data_ptr(),
+            scales.data_ptr(), blocks, page_tokens, query_start_loc.data_ptr(), seq_lens.data_ptr(), requests,
+            block_table.data_ptr(), max(block_table.stride(0), block_table.size(1)), block_table.size(1),
+            _stream(device))
+    _lib.check(status)
+
+
+def paged_attention_fp8_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_pages: int,
+                                        page_tokens: int) -> int:
+    """Device workspace (bytes) for ``paged_attention_fp8``; depends on shapes only."""
+    return int(_lib.lib().rq_paged_attention_fp8_workspace_bytes(rows, heads, kv_heads, head_dim, max_pages,
+                                                                 page_tokens))
+
+
+def paged_attention_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor,
+                        scales: torch.Tensor, output: torch.Tensor, query_start_loc: torch.Tensor,
+                        seq_lens: torch.Tensor, block_table: torch.Tensor, softmax_scale: Optional[float] = None,
+                        workspace: Optional[torch.Tensor] = None) -> None:
+    """Attention over a paged cache held in 8 bits, writing ``output``.
+
+    Request b's rows ``query_start_loc[b]..query_start_loc[b+1]`` are the
+    last n of its ``seq_lens[b]`` tokens: they attend to the first
+    ``seq_lens[b] - n`` tokens from the cache (``quantize_fp8``'s layout, any
+    positive scales) and, causally, to the request's own new ``key``/``value``
+    rows, which need not be in the cache.  One row per request is a decode
+    step, more are draft rows or a prompt chunk.  ``query``/``output`` are BF16
+    ``[rows, heads, D]``, ``key``/``value`` ``[rows, kv_heads, D]`` with
+    ``heads`` a multiple of ``kv_heads``.  A request may have no new rows; rows
+    outside ``query_start_loc`` are left as they are.  ``softmax_scale``
+    defaults to ``D ** -0.5``; ``workspace`` as in ``attention``, of
+    ``paged_attention_fp8_workspace_bytes(...)`` bytes.
+    """
+    shape, query_stride = _validate_bf16_token_tensor(query)
+    key_shape, key_stride = _validate_bf16_token_tensor(key)
+    value_shape, value_stride = _validate_bf16_token_tensor(value)
+    out_shape, out_stride = _validate_bf16_token_tensor(output)
+    device = query.get_device()
+    rows, heads, head_dim = shape
+    kv_heads = key_shape[1]
+    _require(key.get_device() == device and value.get_device() == device and output.get_device() == device
+             and out_shape == shape and value_shape == key_shape and key_shape[0] == rows
+             and key_shape[2] == head_dim, "Q/K/V/output must have matching shapes and devices")
+    _, blocks, _, page_tokens, _ = _validate_fp8_cache(cache, scales, device, kv_heads, head_dim)
+    requests = _validate_sequences(query_start_loc, seq_lens, block_table, device)
+    max_pages = block_table.size(1)
+    library = _lib.lib()
+    if workspace is None:
+        needed = library.rq_paged_attention_fp8_workspace_bytes(rows, heads, kv_heads, head_dim, max_pages, page_tokens)
+        workspace = torch.empty(needed, dtype=torch.uint8, device=query.device)
+    else:
+        _require(workspace.get_device() == device and workspace.is_contiguous(),
+                 "Contiguous attention workspace on the query device required")
+    with _on_device(device):
+        status = library.rq_paged_attention_fp8(
+            query.data_ptr(), query_stride, key.data_ptr(), key_stride, value.data_ptr(), value_stride,
+            output.data_ptr(), out_stride, rows, heads, kv_heads, head_dim, cache.data_ptr(), scales.data_ptr(),
+            blocks, page_tokens, query_start_loc.data_ptr(), seq_lens.data_ptr(), requests, block_table.data_ptr(),
+            max(block_table.stride(0), max_pages), max_pages,
+            head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _stream(device))
+    _lib.check(status)
+
+
 def flash_attn_varlen_func(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, max_seqlen_q: int,
                            cu_seqlens_q: torch.Tensor, max_seqlen_k: int,
                            cu_seqlens_k: Optional[torch.Tensor] = None, dropout_p: float = 0.0,

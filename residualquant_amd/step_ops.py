@@ -2,19 +2,22 @@
 
 One Ouro layer (plugins/looped_transformers/src/looped_transformers/ouro.py:101-157)
 brackets its attention with vLLM's fused add + RMSNorm, the rotary embedding
-of Q and K, and Qwen2MLP's SiLU(gate) * up.  Each op here is one HIP launch
-through ``librq_hip.so`` (rq_rms_norm, rq_rope_qkv, rq_silu_mul); there is no
-CPU or torch fallback.  Work is enqueued on the current HIP stream of the
+of Q and K, and Qwen2MLP's SiLU(gate) * up.  Beside them stand the projections at a few rows,
+with BF16 and with 4-bit weights, and the log probabilities of a step's
+tokens.  Each op here is a HIP launch through ``librq_hip.so`` (rq_rms_norm,
+rq_rope_qkv, rq_silu_mul, rq_linear_rows, rq_linear_rows_int4,
+rq_token_logprobs); there is no CPU or torch fallback.  Work is enqueued on the current HIP stream of the
 input's device.
 """
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
 from . import _lib
+from .ops import _on_device
 
 
 def _require(condition: bool, message: str) -> None:
@@ -146,3 +149,143 @@ def linear_rows(x: torch.Tensor, weight: torch.Tensor, out: Optional[torch.Tenso
                                           rows, weight.size(0), in_features, _stream(x.device))
     _lib.check(status)
     return out
+
+
+LINEAR_INT4_MAX_ROWS = 64
+
+
+class Int4Weight:
+    """A linear weight ``[out_features, in_features]`` in 4 bits, laid out for ``linear_rows_int4``.
+
+    Codes in -8..7 with one BF16 scale per output row and ``group`` inputs;
+    made by ``quantize_weight_int4`` or ``pack_weight_int4``.
+    """
+
+    def __init__(self, data: torch.Tensor, out_features: int, in_features: int, group: int):
+        self.data, self.out_features, self.in_features, self.group = data, out_features, in_features, group
+        self.device = data.device
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.out_features, self.in_features
+
+    def dequantize(self) -> torch.Tensor:
+        """The BF16 weight ``[out_features, in_features]``: ``bf16(code * scale)``."""
+        weight = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
+        with _on_device(self.data.get_device()):
+            status = _lib.lib().rq_dequantize_weight_int4(self.data.data_ptr(), self.data.numel(), self.out_features,
+                                                          self.in_features, self.group, weight.data_ptr(),
+                                                          _stream(self.device))
+        _lib.check(status)
+        return weight
+
+
+def _int4_weight(out_features: int, in_features: int, group: int, device: torch.device) -> Int4Weight:
+    needed = _lib.lib().rq_int4_weight_bytes(out_features, in_features, group)
+    if needed == 0:
+        raise RuntimeError(_lib.lib().rq_last_error().decode(errors="replace"))
+    return Int4Weight(torch.empty(needed, dtype=torch.uint8, device=device), out_features, in_features, group)
+
+
+def quantize_weight_int4(weight: torch.Tensor, group: int = 32) -> Int4Weight:
+    """A contiguous BF16 weight ``[out_features, in_features]`` in 4 bits.
+
+    Per output row and ``group`` (32, 64 or 128) inputs: scale = bf16(largest
+    |w| / 7), code = w / scale to nearest, ties to even.
+    """
+    _require(weight.is_cuda and weight.dtype == torch.bfloat16 and weight.dim() == 2 and weight.is_contiguous(),
+             "weight must be a contiguous BF16 [out_features, in_features] tensor on a HIP device")
+    packed = _int4_weight(weight.size(0), weight.size(1), group, weight.device)
+    with _on_device(weight.get_device()):
+        status = _lib.lib().rq_quantize_weight_int4(weight.data_ptr(), packed.out_features, packed.in_features, group,
+                                                    packed.data.data_ptr(), packed.data.numel(), _stream(weight.device))
+    _lib.check(status)
+    return packed
+
+
+def pack_weight_int4(codes: torch.Tensor, scales: torch.Tensor) -> Int4Weight:
+    """A weight given as INT8 ``codes`` ``[out_features, in_features]`` (limited
+    to -8..7) and BF16 ``scales`` ``[out_features, in_features / group]``, both contiguous."""
+    _require(codes.is_cuda and codes.dtype == torch.int8 and codes.dim() == 2 and codes.is_contiguous(),
+             "codes must be a contiguous INT8 [out_features, in_features] tensor on a HIP device")
+    _require(scales.device == codes.device and scales.dtype == torch.bfloat16 and scales.dim() == 2
+             and scales.is_contiguous() and scales.size(0) == codes.size(0) and scales.size(1) > 0
+             and codes.size(1) % scales.size(1) == 0,
+             "scales must be a contiguous BF16 [out_features, in_features / group] tensor on the codes' device")
+    packed = _int4_weight(codes.size(0), codes.size(1), codes.size(1) // scales.size(1), codes.device)
+    with _on_device(codes.get_device()):
+        status = _lib.lib().rq_pack_weight_int4(codes.data_ptr(), scales.data_ptr(), packed.out_features,
+                                                packed.in_features, packed.group, packed.data.data_ptr(),
+                                                packed.data.numel(), _stream(codes.device))
+    _lib.check(status)
+    return packed
+
+
+def linear_rows_int4(x: torch.Tensor, weight: Int4Weight, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``bf16(x @ weight.T)`` for 1-64 BF16 rows and a 4-bit weight (rq_linear_rows_int4), FP32 accumulation.
+
+    The codes are exact in the products and the scales multiply each group's
+    sum; the weight itself is never rounded to BF16.  ``x`` rows are 16-byte aligned.
+    """
+    _rows(x, "x")
+    rows, in_features = x.shape
+    device = x.get_device()
+    _require(in_features == weight.in_features and weight.data.get_device() == device,
+             "x must have the weight's in_features and device")
+    if out is None:
+        out = torch.empty((rows, weight.out_features), dtype=torch.bfloat16, device=x.device)
+    else:
+        _rows(out, "out")
+        _require(out.shape == (rows, weight.out_features) and out.device == x.device,
+                 "out must be [rows, out_features]")
+    with _on_device(device):
+        status = _lib.lib().rq_linear_rows_int4(
+            x.data_ptr(), x.stride(0) if rows > 1 else in_features, weight.data.data_ptr(), weight.data.numel(),
+            out.data_ptr(), out.stride(0) if rows > 1 else weight.out_features, rows, weight.out_features, in_features, weight.group, torch._C._cuda_getCurrentRawStream(device))
+    _lib.check(status)
+    return out
+
+
+LOGPROBS_MAX_TOP = 32
+
+
+class TokenLogprobs(NamedTuple):
+    """Log probabilities (natural logarithm) of a call's tokens and their rows' distributions."""
+
+    logprob: torch.Tensor       # FP32 [rows]
+    entropy: torch.Tensor       # FP32 [rows]
+    top_logprobs: torch.Tensor  # FP32 [rows, top], largest first
+    top_tokens: torch.Tensor    # INT64 [rows, top]
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> TokenLogprobs:
+    """Log probability of ``tokens[i]`` under ``logits[i]``, the row's entropy and its ``top`` alternatives.
+
+    ``logits`` is BF16 or FP32 ``[rows, vocab]`` with unit column stride,
+    ``tokens`` INT64 ``[rows]`` (a token outside the vocabulary gives NaN),
+    ``top`` 0 to 32.  Logits of -inf (ruled-out tokens) have probability 0 and
+    add nothing to the entropy; a row of -inf alone, or with a NaN or +inf,
+    gives NaN.  Equal logits rank by the lower token.
+    """
+    _require(logits.is_cuda and logits.dim() == 2 and (logits.stride(1) == 1 or logits.size(1) == 1)
+             and logits.dtype in (torch.bfloat16, torch.float32),
+             "logits must be BF16 or FP32 [rows, vocab] on a HIP device with unit column stride")
+    rows, vocab = logits.shape
+    device = logits.get_device()
+    _require(tokens.get_device() == device and tokens.dtype is torch.int64 and tokens.dim() == 1
+             and tokens.is_contiguous() and tokens.numel() == rows,
+             "Contiguous INT64 tokens, one per row, on the logits' device required")
+    top = int(top)
+    _require(0 <= top <= min(LOGPROBS_MAX_TOP, vocab),
+             f"0 to {LOGPROBS_MAX_TOP} alternatives, at most the vocabulary, required")
+    logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    entropy = torch.empty_like(logprob)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
+    top_tokens = torch.empty((rows, top), dtype=torch.int64, device=logits.device)
+    with _on_device(device):
+        status = _lib.lib().rq_token_logprobs(
+            logits.data_ptr(), max(logits.stride(0), vocab), 0 if logits.dtype is torch.bfloat16 else 1, rows, vocab,
+            tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), top, top_logprobs.data_ptr(),
+            top_tokens.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
+    _lib.check(status)
+    return TokenLogprobs(logprob, entropy, top_logprobs, top_tokens)
