@@ -1223,10 +1223,61 @@ int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int6
     return check_launch(rq::launch_quantize_fp8(p, stream), "8-bit cache write launch");
 }
 
+// Least steps of 32 tokens of one split of an 8-bit attention call, the
+// workgroups per compute unit that its work is spread over, and the most
+// columns of a workgroup's tile.
+constexpr int kFp8MinSteps = 8, kFp8PerCu = 2, kFp8MaxTile = 128, kFp8MaxSplits = 256;
+
+// Steps that the page table and the new rows of a call can hold.
+static int64_t fp8_most_steps(int64_t rows, int64_t max_pages, int page_tokens) {
+    return (max_pages * page_tokens + 31) / 32 + (rows + 31) / 32 + 1;
+}
+
+static int fp8_max_splits(int64_t rows, int64_t max_pages, int page_tokens) {
+    const int64_t steps = fp8_most_steps(rows, max_pages, page_tokens);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(steps / kFp8MinSteps, kFp8MaxSplits));
+}
+
+// Partial entries per K/V head that a plan may use: every column split
+// max_splits times, or `target` splits of whole tiles beside one entry per
+// column (0: no call of this size is split).
+static int64_t fp8_entries(int64_t rows, int heads, int kv_heads, int head_dim, int64_t max_pages, int page_tokens) {
+    const int64_t columns = rows * (heads / kv_heads);
+    const int64_t target = (kFp8PerCu * (int64_t)compute_units() + kv_heads - 1) / kv_heads;
+    const int max_splits = fp8_max_splits(rows, max_pages, page_tokens);
+    if (max_splits == 1) return 0;
+    const int64_t entries = std::min<int64_t>(columns * max_splits, columns + target * kFp8MaxTile);
+    // (The kernels address a head's entries in 32 bits.)
+    return entries * (head_dim + 4) * 4 < ((int64_t)1 << 31) ? entries : 0;
+}
+
 size_t rq_paged_attention_fp8_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim, int64_t max_pages,
                                               int page_tokens) {
-    (void)rows, (void)heads, (void)kv_heads, (void)head_dim, (void)max_pages, (void)page_tokens;
-    return 256;
+    if (rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || head_dim <= 0 || max_pages < 0 ||
+        page_tokens <= 0 || max_pages > (int64_t)INT32_MAX / page_tokens || rows > (int64_t)INT32_MAX)
+        return 256;
+    return 256 + (size_t)fp8_entries(rows, heads, kv_heads, head_dim, max_pages, page_tokens) * kv_heads * (head_dim + 4) * 4;
+}
+
+static void plan_fp8(rq::Fp8AttentionParams& p) {
+    const int64_t columns = p.rows * (p.heads / p.kv_heads);
+    const int64_t average = (columns + p.requests - 1) / p.requests;
+    p.tile = average <= 16 ? 16 : average <= 48 ? 32 : kFp8MaxTile;
+    const int64_t target = (kFp8PerCu * (int64_t)compute_units() + p.kv_heads - 1) / p.kv_heads;
+    const int64_t most_steps = fp8_most_steps(p.rows, p.max_pages, p.page_tokens);
+    const int64_t tiles = columns / p.tile + p.requests;  // at most, over all requests
+    const bool split = p.entries > 0;
+    p.plan_min = kFp8MinSteps;
+    p.plan_max_splits = split ? fp8_max_splits(p.rows, p.max_pages, p.page_tokens) : 1;
+    const int64_t average_tiles = p.requests * std::max<int64_t>(1, (average + p.tile - 1) / p.tile);
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>(target / average_tiles, p.plan_max_splits));
+    if (split) splits = std::max<int64_t>(1, std::min<int64_t>(splits, p.entries / columns));
+    p.splits = split ? (int)splits : 1;
+    p.items = 0;
+    // The device sums tiles x steps in 31 bits.
+    if (p.requests > rq::kPlanRequests || tiles > INT32_MAX / most_steps) return;
+    p.plan_target = split ? (int)target : 0;
+    p.items = (int)(std::max<int64_t>(tiles * p.splits, tiles + p.plan_target));
 }
 
 int rq_paged_attention_fp8(const void* query, int64_t query_stride, const void* key, int64_t key_stride,
@@ -1275,6 +1326,12 @@ int rq_paged_attention_fp8(const void* query, int64_t query_stride, const void* 
     p.block_table_stride = block_table_stride;
     p.max_pages = max_pages;
     p.softmax_scale = softmax_scale;
+    p.entries = fp8_entries(rows, heads, kv_heads, head_dim, max_pages, page_tokens);
+    p.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + to_boundary(workspace));
+    p.call_tag = next_call_tag();
+    plan_fp8(p);
+    const int64_t workgroups = p.items > 0 ? p.items : (rows * (heads / kv_heads) / p.tile + requests) * p.splits;
+    if (workgroups > (int64_t)INT32_MAX / kv_heads) return fail(RQ_EINVAL, "Too many rows, heads and requests for one call");
     return check_launch(rq::launch_attention_fp8(p, stream), "8-bit attention launch");
 }
 

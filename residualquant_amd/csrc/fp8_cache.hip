@@ -4,6 +4,7 @@
 // quantize_fp8_kernel writes a call's new tokens, attention_fp8_kernel reads
 // the cache: the 8-bit member beside the packed (2 + 4 bit) and the BF16 pages.
 #include "rq_device.h"
+#include "rq_plan.h"
 #include "rq_reduced.h"
 
 namespace rq {
@@ -95,74 +96,577 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams 
 }
 
 // ------------------------------------------------------------------ attention
+//
+// Queries are laid out as columns: the n new rows of a request times the
+// `group` query heads that share a K/V head, column c = row (c / group), head
+// c % group.  A wave streams the tokens of one (request, K/V head) for NT tiles
+// of 16 columns, 32 tokens per step:
+//   S^T = K Q^T    2 x D / 32 v_mfma_f32_16x16x32_bf16 (16 tokens x 16 columns),
+//   O^T += V^T P^T  one per tile of 16 channels and part of P.
+// Lane l = (i = l % 16, g = l / 16).  S^T leaves lane (q, g) the scores of
+// tokens 4 g + r of both 16-token units for column q: exactly the slots that a
+// B operand of the second product takes from this lane if its k slot
+// (g, 4 u + r) stands for token 16 u + 4 g + r, so P never leaves the lane.
+// The A operand then needs, per lane, channel (row) i of tokens 16 u + 4 g + r:
+// lane (i, g) loads 8 channels 8 i.. of those 8 tokens and transposes 4 x 4
+// bytes by v_perm; tile e holds channels 8 i + e, so lane (q, g) ends with the
+// 32 channels 32 g.. of column q.  E4M3 becomes BF16 exactly.  Neither K nor V
+// passes LDS.
+//
+// A page's K scale multiplies its scores (FP32), its V scale the weights
+// (FP32), which are then split into two BF16 parts (16 bits of the weight
+// multiply V; one part alone would round each weight by up to 2^-8, as much
+// again as the rounding of the output).  The running maximum of a column moves
+// only when a score exceeds it by 2^8, so most steps neither exchange lanes
+// nor rescale; weights are then at most 2^8.
 
-// One workgroup per (row, query head): each wave takes every fourth token, a
-// lane two channels, with a running maximum and sum per wave.
-__global__ __launch_bounds__(256) void attention_fp8_kernel(const Fp8AttentionParams p) {
-    __shared__ int counts[4];
-    __shared__ float merged[4][kFp8MaxDim + 2];
-    const int64_t row = blockIdx.x;
-    const int head = blockIdx.y, kv_head = head / (p.heads / p.kv_heads);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const RowPlace at = place_row(p.query_start_loc, p.seq_lens, p.requests, row, counts);
-    if (at.request < 0) return;
-    const int PT = p.page_tokens, D = p.head_dim;
-    const bool active = 2 * lane < D;
-    const int64_t history = min(at.history, p.max_pages * PT);
-    const uint16_t* q = p.query + row * p.query_stride + (int64_t)head * D;
-    float q0 = 0.f, q1 = 0.f;
-    if (active) q0 = bf16_f32(q[2 * lane]) * p.softmax_scale, q1 = bf16_f32(q[2 * lane + 1]) * p.softmax_scale;
-    float m = -__builtin_inff(), l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int64_t t = wave; t < history + at.index + 1; t += 4) {
-        float k0 = 0.f, k1 = 0.f, v0 = 0.f, v1 = 0.f;
-        if (t < history) {
-            const int64_t block = p.block_table[(int64_t)at.request * p.block_table_stride + t / PT];
-            if (block < 0 || block >= p.num_blocks) continue;
-            const int64_t index = block * p.kv_heads + kv_head;
-            const int64_t plane = p.num_blocks * p.kv_heads;
-            const uint8_t* k = p.cache + (index * PT + t % PT) * D;
-            const uint8_t* v = k + plane * PT * D;
-            const float ks = p.scales[index], vs = p.scales[index + plane];
-            if (active) {
-                k0 = e4m3_f32(k[2 * lane]) * ks, k1 = e4m3_f32(k[2 * lane + 1]) * ks;
-                v0 = e4m3_f32(v[2 * lane]) * vs, v1 = e4m3_f32(v[2 * lane + 1]) * vs;
+typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 Bf16x2 __attribute__((ext_vector_type(2)));
+typedef float F32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kStreamThreads = 256;
+constexpr float kLowest = -3.402823466e+38f;
+constexpr float kMaxSlack = 8.0f;  // log2 units
+
+__device__ __forceinline__ F32x4 mfma(U32x4 a, U32x4 b, F32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
+}
+
+// Two E4M3 codes (low or high half word of x) as two BF16, exactly.
+template <bool High>
+__device__ __forceinline__ uint32_t bf16x2_of_fp8(uint32_t x) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, High));
+}
+
+// t[c] = byte c of x[0..3] (x[0] lowest).
+__device__ __forceinline__ void transpose_bytes(const uint32_t (&x)[4], uint32_t (&t)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400);  // x0.0 x1.0 x0.1 x1.1
+    const uint32_t b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400);
+    const uint32_t c = __builtin_amdgcn_perm(x[1], x[0], 0x07030602);  // x0.2 x1.2 x0.3 x1.3
+    const uint32_t d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602);
+    t[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
+    t[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    t[2] = __builtin_amdgcn_perm(d, c, 0x05040100);
+    t[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
+}
+
+__device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
+    return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+}
+
+// One request's new rows (as columns) and history.
+struct Fp8Request {
+    int first, rows, history;
+};
+
+__device__ __forceinline__ Fp8Request fp8_request(const Fp8AttentionParams& p, int request) {
+    Fp8Request r;
+    r.first = p.query_start_loc[request];
+    const int n = p.query_start_loc[request + 1] - r.first;
+    // Rows past the query tensor are not read or written.
+    r.rows = r.first < 0 || r.first >= p.rows ? 0 : (int)min((int64_t)max(n, 0), p.rows - r.first);
+    const int seq = p.seq_lens[request];
+    // Tokens past the page table are never read.
+    r.history = p.num_blocks > 0 ? (int)min((int64_t)(seq > n ? (int64_t)seq - n : 0), p.max_pages * p.page_tokens) : 0;
+    return r;
+}
+
+// Steps (of 32 tokens) of a request: its history, then its new rows.
+__device__ __forceinline__ int fp8_steps(int tokens) { return (tokens + 31) / 32; }
+
+// The item of a workgroup: PlanItem's rows are columns, its length steps.
+template <int Tile>
+__device__ __forceinline__ PlanItem fp8_item(const Fp8AttentionParams& p, int key) {
+    const int group = p.heads / p.kv_heads, requests = (int)p.requests;
+    const int lane = threadIdx.x & 63;
+    if (p.items > 0) {
+        const Fp8Request q = fp8_request(p, lane < requests ? lane : requests - 1);
+        const int columns = lane < requests ? q.rows * group : 0;
+        const PlanEntry own{(columns + Tile - 1) / Tile, fp8_steps(q.history) + fp8_steps(q.rows), q.first, q.history, columns};
+        const PlanSizes sizes{p.plan_target, p.splits, p.plan_min, 1 << 24, p.plan_max_splits, 0, 1, 9, 0};
+        return plan_find(requests, key, sizes, own);
+    }
+    // More requests than a wave has lanes: tile i of request b has slot
+    // floor(first column of b / Tile) + b + i, each slot `splits` workgroups.
+    const int slot = key / p.splits;
+    int count = 0;
+    for (int b = 1 + lane; b < requests; b += 64)
+        count += (int64_t)p.query_start_loc[b] * group / Tile + b <= slot ? 1 : 0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) count += __shfl_xor(count, d);
+    const Fp8Request q = fp8_request(p, count);
+    const int index = slot - (int)((int64_t)q.first * group / Tile + count);
+    const int columns = q.rows * group;
+    if (index < 0 || index * Tile >= columns) return PlanItem{-1, 0, 0, 1, 0, 0, 0, 0, 0, 0, 0};
+    return PlanItem{count, index, key % p.splits, p.splits, fp8_steps(q.history) + fp8_steps(q.rows), q.first, q.history,
+                    columns, 0, q.first * group * p.splits, 0};
+}
+
+// Codes of one step: 16 tokens' K rows and this lane's 8 tokens of V, for both units.
+template <int D>
+struct Fp8Step {
+    U32x4 k[2][D == 128 ? 2 : 1];
+    U32x2 k_rest[2];  // D = 96
+    U32x2 v[2][4];
+    float key_scale[2], value_scale[2];
+    int valid[2];  // tokens of the unit inside the history
+};
+
+// The columns' statistics and sums of a wave.
+template <int NT>
+struct Fp8Columns {
+    F32x4 out[NT][8];   // [tile][e]: channels 8 (4 g + r) + e
+    float high[NT];     // the maximum that weights refer to (log2 units)
+    float sum[NT];      // of this lane's tokens
+};
+
+// Weights of one step's scores and their product with V (operand a[e]).
+template <int NT>
+__device__ __forceinline__ void fp8_softmax(Fp8Columns<NT>& columns, const float (&s)[NT][2][4],
+                                            const float (&value_scale)[2], float (&weight)[NT][2][4],
+                                            U32x4 (&upper)[NT], U32x4 (&lower)[NT]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float most = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                           fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+        if (__any(most > columns.high[t] + kMaxSlack)) {
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const float next = fmaxf(columns.high[t], most);
+            const float keep = next == columns.high[t] ? 1.0f : __builtin_amdgcn_exp2f(columns.high[t] - next);
+            columns.high[t] = next;
+            columns.sum[t] *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) columns.out[t][e][r] *= keep;
+        }
+        uint32_t up[4], low[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                weight[t][u][r] = __builtin_amdgcn_exp2f(s[t][u][r] - columns.high[t]);
+                columns.sum[t] += weight[t][u][r];
             }
-        } else {
-            const int64_t live = row - at.index + (t - history);
-            const uint16_t* k = p.key + live * p.key_stride + (int64_t)kv_head * D;
-            const uint16_t* v = p.value + live * p.value_stride + (int64_t)kv_head * D;
-            if (active) {
-                k0 = bf16_f32(k[2 * lane]), k1 = bf16_f32(k[2 * lane + 1]);
-                v0 = bf16_f32(v[2 * lane]), v1 = bf16_f32(v[2 * lane + 1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float a = weight[t][u][2 * h] * value_scale[u], b = weight[t][u][2 * h + 1] * value_scale[u];
+                const uint32_t both = bf16x2_rn(a, b);
+                up[2 * u + h] = both;
+                low[2 * u + h] = bf16x2_rn(a - __uint_as_float(both << 16), b - __uint_as_float(both & 0xffff0000u));
             }
         }
-        float s = q0 * k0 + q1 * k1;
+        upper[t] = U32x4{up[0], up[1], up[2], up[3]};
+        lower[t] = U32x4{low[0], low[1], low[2], low[3]};
+    }
+}
+
+// One workgroup per (item, K/V head).  Rows false: its four waves take every
+// fourth step of the item's 16 NT columns; true: every step, 16 NT columns each.
+template <int D, int NT, bool Rows>
+__global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8AttentionParams p) {
+    constexpr int kTile = 16 * NT * (Rows ? 4 : 1);
+    constexpr int kSteps = D / 32;
+    constexpr int kEntry = D + 4;  // m, l, arrival word, O
+    __shared__ __align__(16) float merged[Rows ? 1 : 4][Rows ? 1 : 16][Rows ? 1 : kEntry];
+    __shared__ int last_flag;
+    const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
+    const int request = __builtin_amdgcn_readfirstlane(item.request);
+    if (request < 0) return;  // uniform over the workgroup, before any barrier
+    const int group = p.heads / p.kv_heads;
+    const int first = __builtin_amdgcn_readfirstlane(item.first), columns_in = __builtin_amdgcn_readfirstlane(item.rows);
+    const int rows = columns_in / group;
+    const int history = __builtin_amdgcn_readfirstlane(item.tokens);
+    const int splits = __builtin_amdgcn_readfirstlane(item.splits), split = __builtin_amdgcn_readfirstlane(item.split);
+    const int begin = split_begin(__builtin_amdgcn_readfirstlane(item.length), split, splits);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int item_column = __builtin_amdgcn_readfirstlane(item.index) * kTile;
+    const int column0 = item_column + (Rows ? wave * 16 * NT : 0);
+    // (A wave past the request's columns has no steps.)
+    const int end = column0 < columns_in ? split_begin(__builtin_amdgcn_readfirstlane(item.length), split + 1, splits) : begin;
+    const int stride = Rows ? 1 : 4;
+    const int history_steps = fp8_steps(history);
+
+    // The item's arrival word lies in the two unused floats of its first entry.
+    float* const entries = p.partials + ((int64_t)head * p.entries + item.entry) * kEntry;
+    uint64_t* const arrivals = reinterpret_cast<uint64_t*>(entries + (int64_t)item_column * splits * kEntry + 2);
+    const uint64_t arrivals_seen = splits > 1 ? peek_arrivals(arrivals) : 0;
+
+    // Queries: column q's channels of each k step (the K loads' order), and the
+    // last new row that the column sees.
+    U32x4 query[NT][kSteps];
+    int seen[NT];
+    auto k_channel = [&](int s) { return D == 128 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 24 * g + 8 * s; };
 #pragma unroll
-        for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-        if (s == -__builtin_inff()) continue;
-        const float next = fmaxf(m, s);
-        const float keep = m == next ? 1.f : expf(m - next), weight = expf(s - next);
-        l = l * keep + weight;
-        o0 = o0 * keep + weight * v0;
-        o1 = o1 * keep + weight * v1;
-        m = next;
+    for (int t = 0; t < NT; ++t) {
+        const int column = column0 + 16 * t + i;
+        seen[t] = column < columns_in ? column / group : -1;
+        const int row = column < columns_in ? column / group : 0;
+        const uint16_t* q = p.query + (int64_t)(first + row) * p.query_stride +
+                            ((int64_t)head * group + (column < columns_in ? column % group : 0)) * D;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const U32x2 a = *reinterpret_cast<const U32x2*>(q + k_channel(s));
+            const U32x2 b = *reinterpret_cast<const U32x2*>(q + k_channel(s) + 4);
+            query[t][s] = column < columns_in ? U32x4{a[0], a[1], b[0], b[1]} : U32x4{0u, 0u, 0u, 0u};
+        }
     }
-    if (active) merged[wave][2 * lane] = o0, merged[wave][2 * lane + 1] = o1;
-    if (lane == 0) merged[wave][D] = m, merged[wave][D + 1] = l;
-    __syncthreads();
-    if (wave != 0 || !active) return;
-    float top = -__builtin_inff();
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, merged[w][D]);
-    float total = 0.f, a = 0.f, b = 0.f;
-    for (int w = 0; w < 4; ++w) {
-        const float keep = merged[w][D] == top ? 1.f : expf(merged[w][D] - top);
-        total += merged[w][D + 1] * keep;
-        a += merged[w][2 * lane] * keep;
-        b += merged[w][2 * lane + 1] * keep;
+    Fp8Columns<NT> columns;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        columns.high[t] = kLowest;
+        columns.sum[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) columns.out[t][e] = F32x4{0.f, 0.f, 0.f, 0.f};
     }
-    uint16_t* out = p.output + row * p.output_stride + (int64_t)head * D;
-    out[2 * lane] = (uint16_t)bf16_rn(a / total);
-    out[2 * lane + 1] = (uint16_t)bf16_rn(b / total);
+    const float to_log2 = p.softmax_scale * 1.44269504088896341f;
+
+    // ---------------------------------------------------------------- history
+    // Lane l holds the place, scales and valid tokens of unit l % 2 of the
+    // wave's step l / 2 of a batch of 32.
+    const int64_t plane_bytes = p.num_blocks * p.kv_heads * p.page_tokens * D;
+    const int my_steps = max(0, (min(end, history_steps) - begin - (Rows ? 0 : wave) + stride - 1) / stride);
+    const int step0 = begin + (Rows ? 0 : wave);
+    uint32_t place_low = 0, place_high = 0, unit_valid = 0;
+    float unit_key_scale = 1.f, unit_value_scale = 1.f;
+    auto look_up = [&](int batch) {
+        const int step = step0 + (32 * batch + (lane >> 1)) * stride;
+        const int token = 32 * step + 16 * (lane & 1);
+        const int left = step < min(end, history_steps) ? history - token : 0;
+        const int page = token / p.page_tokens;
+        int64_t block = left > 0 ? p.block_table[(int64_t)request * p.block_table_stride + page] : -1;
+        const bool held = block >= 0 && block < p.num_blocks;
+        if (!held) block = 0;
+        const int64_t index = block * p.kv_heads + head;
+        const int64_t place = (index * p.page_tokens + token % p.page_tokens) * D;
+        place_low = (uint32_t)place;
+        place_high = (uint32_t)((uint64_t)place >> 32);
+        unit_valid = held ? (uint32_t)min(left, 16) : 0u;
+        unit_key_scale = held ? p.scales[index] * to_log2 : 1.f;
+        unit_value_scale = held ? p.scales[index + p.num_blocks * p.kv_heads] : 1.f;
+    };
+    auto load = [&](Fp8Step<D>& x, int number) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int from = 2 * (number & 31) + u;
+            const int64_t place = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane(place_high, from) << 32) |
+                                            (uint32_t)__builtin_amdgcn_readlane(place_low, from));
+            x.valid[u] = __builtin_amdgcn_readlane(unit_valid, from);
+            x.key_scale[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(unit_key_scale), from));
+            x.value_scale[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(unit_value_scale), from));
+            const uint8_t* k = p.cache + place;
+            const uint8_t* v = k + plane_bytes;
+            if constexpr (D == 128) {
+                x.k[u][0] = *reinterpret_cast<const U32x4*>(k + (i * D + 16 * g));
+                x.k[u][1] = *reinterpret_cast<const U32x4*>(k + (i * D + 16 * g + 64));
+            } else {
+                const U32x2 a = *reinterpret_cast<const U32x2*>(k + (i * D + 24 * g));
+                const U32x2 b = *reinterpret_cast<const U32x2*>(k + (i * D + 24 * g + 8));
+                x.k[u][0] = U32x4{a[0], a[1], b[0], b[1]};
+                x.k_rest[u] = *reinterpret_cast<const U32x2*>(k + (i * D + 24 * g + 16));
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                x.v[u][r] = *reinterpret_cast<const U32x2*>(v + ((4 * g + r) * D + (8 * i < D ? 8 * i : 0)));
+        }
+    };
+    auto compute = [&](const Fp8Step<D>& x) {
+        float s[NT][2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            F32x4 dot[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) dot[t] = F32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int m = 0; m < kSteps; ++m) {
+                uint32_t a0, a1;
+                if constexpr (D == 128) {
+                    a0 = x.k[u][m >> 1][2 * (m & 1)], a1 = x.k[u][m >> 1][2 * (m & 1) + 1];
+                } else {
+                    a0 = m < 2 ? x.k[u][0][2 * (m & 1)] : x.k_rest[u][0];
+                    a1 = m < 2 ? x.k[u][0][2 * (m & 1) + 1] : x.k_rest[u][1];
+                }
+                const U32x4 a = {bf16x2_of_fp8<false>(a0), bf16x2_of_fp8<true>(a0), bf16x2_of_fp8<false>(a1),
+                                 bf16x2_of_fp8<true>(a1)};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) dot[t] = mfma(a, query[t][m], dot[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[t][u][r] = dot[t][r] * x.key_scale[u];
+            if (x.valid[u] < 16) {
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[t][u][r] = 4 * g + r < x.valid[u] ? s[t][u][r] : -__builtin_inff();
+            }
+        }
+        float weight[NT][2][4];
+        U32x4 upper[NT], lower[NT];
+        fp8_softmax<NT>(columns, s, x.value_scale, weight, upper, lower);
+        uint32_t v[2][4][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) v[u][r][w] = x.v[u][r][w];
+        // Slots past the history may hold NaN, which a weight of zero does not remove.
+        if (x.valid[0] < 16 || x.valid[1] < 16) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) v[u][r][w] = 4 * g + r < x.valid[u] ? v[u][r][w] : 0u;
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            uint32_t t0[4], t1[4];
+            const uint32_t x0[4] = {v[0][0][w], v[0][1][w], v[0][2][w], v[0][3][w]};
+            const uint32_t x1[4] = {v[1][0][w], v[1][1][w], v[1][2][w], v[1][3][w]};
+            transpose_bytes(x0, t0);
+            transpose_bytes(x1, t1);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const U32x4 a = {bf16x2_of_fp8<false>(t0[c]), bf16x2_of_fp8<true>(t0[c]), bf16x2_of_fp8<false>(t1[c]),
+                                 bf16x2_of_fp8<true>(t1[c])};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    columns.out[t][4 * w + c] = mfma(a, upper[t], columns.out[t][4 * w + c]);
+                    columns.out[t][4 * w + c] = mfma(a, lower[t], columns.out[t][4 * w + c]);
+                }
+            }
+        }
+    };
+    if (my_steps > 0) {
+        Fp8Step<D> even, odd;
+        look_up(0);
+        load(even, 0);
+        for (int n = 0; n < my_steps; n += 2) {
+            if (n + 1 < my_steps) load(odd, n + 1);
+            compute(even);
+            if (n + 1 >= my_steps) break;
+            if (n + 2 < my_steps) {
+                if (((n + 2) & 31) == 0) look_up((n + 2) >> 5);
+                load(even, n + 2);
+            }
+            compute(odd);
+        }
+    }
+
+    // ---------------------------------------------------------------- new rows
+    // (BF16 rows of this call, row j seen by the columns of rows j and later.)
+    {
+        const int most = min(rows - 1, (column0 + 16 * NT - 1) / group);  // the last row that any column sees
+        int step = begin + (Rows ? 0 : wave);
+        if (step < history_steps) step += (history_steps - step + stride - 1) / stride * stride;
+        for (; step < end; step += stride) {
+            const int base = 32 * (step - history_steps);
+            if (base > most) break;
+            float s[NT][2][4];
+            U32x4 v[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                F32x4 dot[NT];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) dot[t] = F32x4{0.f, 0.f, 0.f, 0.f};
+                const uint16_t* k = p.key + (int64_t)(first + min(base + 16 * u + i, rows - 1)) * p.key_stride + (int64_t)head * D;
+#pragma unroll
+                for (int m = 0; m < kSteps; ++m) {
+                    const U32x2 a = *reinterpret_cast<const U32x2*>(k + k_channel(m));
+                    const U32x2 b = *reinterpret_cast<const U32x2*>(k + k_channel(m) + 4);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) dot[t] = mfma(U32x4{a[0], a[1], b[0], b[1]}, query[t][m], dot[t]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int token = base + 16 * u + 4 * g + r;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) s[t][u][r] = token <= seen[t] ? dot[t][r] * to_log2 : -__builtin_inff();
+                    const uint16_t* row = p.value + (int64_t)(first + min(token, rows - 1)) * p.value_stride +
+                                          (int64_t)head * D + (8 * i < D ? 8 * i : 0);
+                    const U32x2 a = *reinterpret_cast<const U32x2*>(row), b = *reinterpret_cast<const U32x2*>(row + 4);
+                    v[u][r] = U32x4{a[0], a[1], b[0], b[1]};
+                }
+            }
+            float weight[NT][2][4];
+            U32x4 upper[NT], lower[NT];
+            const float one[2] = {1.f, 1.f};
+            fp8_softmax<NT>(columns, s, one, weight, upper, lower);
+            // Infinities and NaN, which a weight of zero does not remove, are added apart.
+            bool odd_values = false;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) odd_values |= not_finite_bf16x2(v[u][r][w]);
+            const bool any_odd = __any(odd_values);
+            if (any_odd) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t x = v[u][r][w];
+                            if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+                            if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
+                            v[u][r][w] = x;
+                        }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;  // the upper or lower halves of two words
+                const U32x4 a = {__builtin_amdgcn_perm(v[0][1][e >> 1], v[0][0][e >> 1], pick),
+                                 __builtin_amdgcn_perm(v[0][3][e >> 1], v[0][2][e >> 1], pick),
+                                 __builtin_amdgcn_perm(v[1][1][e >> 1], v[1][0][e >> 1], pick),
+                                 __builtin_amdgcn_perm(v[1][3][e >> 1], v[1][2][e >> 1], pick)};
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    columns.out[t][e] = mfma(a, upper[t], columns.out[t][e]);
+                    columns.out[t][e] = mfma(a, lower[t], columns.out[t][e]);
+                }
+            }
+            if (any_odd) {
+                for (int j = 0; j < 32; ++j) {
+                    const int token = base + j;
+                    if (token >= rows) break;
+                    const uint16_t* row = p.value + (int64_t)(first + token) * p.value_stride + (int64_t)head * D;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        // (selected without an index, so that the weights stay in registers)
+                        float mine = 0.f;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (16 * u + r == (j & 19)) mine = weight[t][u][r];
+                        const float w = __shfl(mine, i + 16 * ((j >> 2) & 3));
+                        if (token > seen[t]) continue;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int channel = 32 * g + 8 * r + e;
+                                if (channel >= D) continue;
+                                const float x = bf16_f32(row[channel]);
+                                if (!(fabsf(x) < __builtin_inff())) columns.out[t][e][r] += w * x;
+                            }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        columns.sum[t] += __shfl_xor(columns.sum[t], 16);
+        columns.sum[t] += __shfl_xor(columns.sum[t], 32);
+    }
+
+    // ---------------------------------------------------------------- finish
+    const __amdgpu_buffer_rsrc_t handoff = handoff_resource(entries, (uint32_t)min((int64_t)columns_in * splits * kEntry * 4, (int64_t)0xfffffffc));
+    auto output_row = [&](int column) {
+        return p.output + (int64_t)(first + column / group) * p.output_stride + ((int64_t)head * group + column % group) * D;
+    };
+    // Eight channels of a column: the output, or this split's part of it.
+    auto emit = [&](int column, int channel, const float (&o)[8], float high, float sum) {
+        if (splits == 1) {
+            const float scale = 1.0f / sum;
+            uint16_t* out = output_row(column) + channel;
+            *reinterpret_cast<U32x2*>(out) = U32x2{bf16x2_rn(o[0] * scale, o[1] * scale), bf16x2_rn(o[2] * scale, o[3] * scale)};
+            *reinterpret_cast<U32x2*>(out + 4) = U32x2{bf16x2_rn(o[4] * scale, o[5] * scale), bf16x2_rn(o[6] * scale, o[7] * scale)};
+            return;
+        }
+        const uint32_t at = (uint32_t)(column * splits + split) * kEntry * 4;
+        handoff_store4(handoff, at + 16 + 4 * channel, o[0], o[1], o[2], o[3]);
+        handoff_store4(handoff, at + 32 + 4 * channel, o[4], o[5], o[6], o[7]);
+        if (channel == 0) {
+            handoff_store(handoff, at, high);
+            handoff_store(handoff, at + 4, sum);
+        }
+    };
+    if (splits > 1 && tid == 0) tag_arrivals(arrivals, p.call_tag, arrivals_seen);
+    if constexpr (Rows) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int column = column0 + 16 * t + i;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = columns.out[t][e][r];
+                const int channel = 32 * g + 8 * r;
+                if (column < columns_in && channel < D) emit(column, channel, o, columns.high[t], columns.sum[t]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (t > 0) __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int channel = 32 * g + 8 * r;
+                if (channel >= D) continue;
+                float* to = &merged[wave][i][channel];
+                *reinterpret_cast<F32x4*>(to) = F32x4{columns.out[t][0][r], columns.out[t][1][r], columns.out[t][2][r], columns.out[t][3][r]};
+                *reinterpret_cast<F32x4*>(to + 4) = F32x4{columns.out[t][4][r], columns.out[t][5][r], columns.out[t][6][r], columns.out[t][7][r]};
+            }
+            if (g == 0) {
+                merged[wave][i][D] = columns.high[t];
+                merged[wave][i][D + 1] = columns.sum[t];
+            }
+            __syncthreads();
+            const int local = tid >> 4, channel = 8 * (tid & 15), column = item_column + 16 * t + local;
+            if (column < columns_in && channel < D) {
+                float high = kLowest;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) high = fmaxf(high, merged[w][local][D]);
+                float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float m = merged[w][local][D];
+                    const float keep = m == high ? 1.0f : __builtin_amdgcn_exp2f(m - high);
+                    sum += merged[w][local][D + 1] * keep;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] += merged[w][local][channel + e] * keep;
+                }
+                emit(column, channel, o, high, sum);
+            }
+        }
+    }
+    if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
+    // The last split of the item to finish joins them, in their order.
+    for (int c = tid >> 4; c < kTile; c += 16) {
+        const int column = item_column + c, channel = 8 * (tid & 15);
+        if (column >= columns_in || channel >= D) continue;
+        const uint32_t at = (uint32_t)(column * splits) * kEntry * 4;
+        float high = kLowest;
+        for (int k = 0; k < splits; ++k) high = fmaxf(high, handoff_load2(handoff, at + (uint32_t)k * kEntry * 4).x);
+        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+        for (int k = 0; k < splits; ++k) {
+            const uint32_t part = at + (uint32_t)k * kEntry * 4;
+            const float2 stats = handoff_load2(handoff, part);
+            const float4 a = handoff_load4(handoff, part + 16 + 4 * channel), b = handoff_load4(handoff, part + 32 + 4 * channel);
+            const float keep = stats.x == high ? 1.0f : __builtin_amdgcn_exp2f(stats.x - high);
+            sum += stats.y * keep;
+            o[0] += a.x * keep, o[1] += a.y * keep, o[2] += a.z * keep, o[3] += a.w * keep;
+            o[4] += b.x * keep, o[5] += b.y * keep, o[6] += b.z * keep, o[7] += b.w * keep;
+        }
+        const float scale = 1.0f / sum;
+        uint16_t* out = output_row(column) + channel;
+        *reinterpret_cast<U32x2*>(out) = U32x2{bf16x2_rn(o[0] * scale, o[1] * scale), bf16x2_rn(o[2] * scale, o[3] * scale)};
+        *reinterpret_cast<U32x2*>(out + 4) = U32x2{bf16x2_rn(o[4] * scale, o[5] * scale), bf16x2_rn(o[6] * scale, o[7] * scale)};
+    }
 }
 
 }  // namespace
@@ -173,9 +677,29 @@ hipError_t launch_quantize_fp8(const Fp8WriteParams& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
+namespace {
+
+template <int D>
+void launch_attention(const Fp8AttentionParams& p, hipStream_t stream) {
+    const int64_t columns = p.rows * (p.heads / p.kv_heads);
+    const int64_t items = p.items > 0 ? p.items : (columns / p.tile + p.requests) * p.splits;
+    const dim3 grid((unsigned)(items * p.kv_heads)), threads(kStreamThreads);
+    if (p.tile == 16)
+        hipLaunchKernelGGL((attention_fp8_kernel<D, 1, false>), grid, threads, 0, stream, p);
+    else if (p.tile == 32)
+        hipLaunchKernelGGL((attention_fp8_kernel<D, 2, false>), grid, threads, 0, stream, p);
+    else
+        hipLaunchKernelGGL((attention_fp8_kernel<D, 2, true>), grid, threads, 0, stream, p);
+}
+
+}  // namespace
+
 hipError_t launch_attention_fp8(const Fp8AttentionParams& p, hipStream_t stream) {
-    if (p.rows == 0) return hipSuccess;
-    hipLaunchKernelGGL(attention_fp8_kernel, dim3((unsigned)p.rows, (unsigned)p.heads), dim3(256), 0, stream, p);
+    if (p.rows == 0 || p.requests == 0) return hipSuccess;
+    if (p.head_dim == 128)
+        launch_attention<128>(p, stream);
+    else
+        launch_attention<96>(p, stream);
     return hipGetLastError();
 }
 

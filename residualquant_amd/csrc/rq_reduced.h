@@ -94,6 +94,18 @@ struct Fp8AttentionParams {
     int64_t block_table_stride;
     int64_t max_pages;
     float softmax_scale;
+    // Work plan (rq_plan.h).  A request's rows x group query heads per K/V
+    // head are its columns, in tiles of `tile`; its history and new rows are
+    // read in steps of 32 tokens.  Up to kPlanRequests requests, `items`
+    // workgroups per K/V head are planned on the device; with more (items 0)
+    // every tile takes `splits`.
+    int tile;                 // 16, 32 or 128 columns per workgroup
+    int items;
+    int splits;               // of every tile of equal requests
+    int plan_target, plan_min, plan_max_splits;  // PlanSizes, in steps
+    int64_t entries;          // partials per K/V head
+    float* partials;          // workspace [kv_heads, entries, D + 4]
+    uint64_t call_tag;        // of this call (48 bits, rq_plan.h)
 };
 hipError_t launch_quantize_fp8(const Fp8WriteParams& p, hipStream_t stream);
 hipError_t launch_attention_fp8(const Fp8AttentionParams& p, hipStream_t stream);
