@@ -4,8 +4,9 @@
 // Packed layout, made once from the codes: tiles of 16 output rows, in a tile
 // blocks of 128 inputs of 1 KB each.  Lane l of a wave reads 16 bytes at
 // 16 l: word i holds the codes of row l % 16 at inputs 32 i + 8 (l / 16) + e,
-// e = 0..7 (code_shift).  Rows and inputs past the weight hold code 0.  The
-// scales follow: [tile][group][16 rows].
+// e = 0..7 (code_shift), the A operand of v_mfma_f32_16x16x32 for 16 output
+// rows.  Rows and inputs past the weight hold code 0.  The scales follow (scale_place),
+// in the order in which the lanes of the product's result need them.
 #include "rq_device.h"
 #include "rq_reduced.h"
 
@@ -31,6 +32,13 @@ __device__ __forceinline__ int code_at(uint32_t word, int e) {
 __host__ __device__ __forceinline__ int64_t int4_tiles(int64_t out_features) { return (out_features + 15) / 16; }
 __host__ __device__ __forceinline__ int64_t int4_blocks(int64_t in_features) { return (in_features + 127) / 128; }
 
+// Place of the scale of output row 16 tile + row and input group `group`:
+// [tile][block of 128 inputs][row / 4][group of the block][row % 4].
+__device__ __forceinline__ int64_t scale_place(int64_t tile, int64_t blocks, int64_t group, int group_size, int row) {
+    const int per = 128 / group_size;
+    return (((tile * blocks + group / per) * 4 + (row >> 2)) * per + group % per) * 4 + (row & 3);
+}
+
 // One thread per word.  From codes (int8 [out, in]) and scales, or from a BF16
 // weight: scale = bf16(largest |w| of the group / 7), code = round to even of
 // w / scale, limited to -8..7 (0 where the scale is 0).
@@ -44,9 +52,9 @@ __global__ __launch_bounds__(256) void pack_int4_kernel(const Int4PackParams p) 
     uint32_t word = 0;
     const bool inside = n < p.out_features && k < p.in_features;
     float scale = 0.f;
+    uint32_t scale_bits = 0;
     if (inside) {
         const int64_t group = k / p.group, groups = p.in_features / p.group;
-        uint32_t scale_bits;
         if (p.weight != nullptr) {
             float largest = 0.f;
             for (int e = 0; e < p.group; ++e) {
@@ -58,10 +66,9 @@ __global__ __launch_bounds__(256) void pack_int4_kernel(const Int4PackParams p) 
             scale_bits = p.scales[n * groups + group];
         }
         scale = bf16_f32(scale_bits);
-        if (k % p.group == 0) p.packed_scales[(tile * groups + group) * 16 + (lane & 15)] = (uint16_t)scale_bits;
-    } else if (n >= p.out_features && k < p.in_features && k % p.group == 0) {
-        p.packed_scales[(tile * (p.in_features / p.group) + k / p.group) * 16 + (lane & 15)] = 0;
     }
+    if (k % p.group == 0)
+        p.packed_scales[scale_place(tile, blocks, k / p.group, p.group, lane & 15)] = (uint16_t)scale_bits;
     for (int e = 0; e < 8; ++e) {
         int code = 0;
         if (inside && p.weight != nullptr) {
@@ -84,30 +91,174 @@ __global__ __launch_bounds__(256) void unpack_int4_kernel(const Int4PackParams p
     const int64_t block = (w >> 8) % blocks, tile = (w >> 8) / blocks;
     const int64_t n = 16 * tile + (lane & 15), k = 128 * block + 32 * i + 8 * (lane >> 4);
     if (n >= p.out_features || k >= p.in_features) return;
-    const float scale = bf16_f32(p.packed_scales[(tile * (p.in_features / p.group) + k / p.group) * 16 + (lane & 15)]);
+    const float scale = bf16_f32(p.packed_scales[scale_place(tile, blocks, k / p.group, p.group, lane & 15)]);
     for (int e = 0; e < 8; ++e)
         weight[n * p.in_features + k + e] = (uint16_t)bf16_rn((float)code_at(p.packed[w], e) * scale);
 }
 
-// One wave per (tile of 16 output rows, row of x): a lane sums its 8 inputs of
-// every 32, the four lanes of an output row meet at the end.
-__global__ __launch_bounds__(64) void linear_int4_kernel(const LinearInt4Params p) {
-    const int lane = threadIdx.x;
-    const int64_t tile = blockIdx.x, row = blockIdx.y;
+typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
+typedef float F32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ F32x4 mfma(U32x4 a, U32x4 b, F32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
+}
+
+// The eight codes of a word as BF16 numbers 1 + (c + 8) / 16, in three shifts
+// and four v_and_or: a code takes the upper four mantissa bits of a 1.
+__device__ __forceinline__ U32x4 codes_bf16(uint32_t word) {
+    constexpr uint32_t kMantissa = 0x00780078u, kOne = 0x3f803f80u;
+    return U32x4{(word & kMantissa) | kOne, ((word >> 4) & kMantissa) | kOne, ((word >> 8) & kMantissa) | kOne,
+                 (__builtin_amdgcn_alignbit(word, word, 12) & kMantissa) | kOne};
+}
+
+// y of the outputs 16 tile0.. of NB tiles in plain steps, for results that are
+// not finite: the products of shifted codes overflow earlier than the sum
+// itself, and turn an infinity in x into NaN.
+__device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int tiles, int threads) {
     const int64_t blocks = int4_blocks(p.in_features);
-    const int groups = (int)(p.in_features / p.group);
-    const uint16_t* x = p.x + row * p.x_stride;
-    float sum = 0.f;
-    for (int64_t step = 0; step < p.in_features / 32; ++step) {
-        const uint32_t word = p.packed[((tile * blocks + step / 4) * 64 + lane) * 4 + (step & 3)];
-        const int64_t k = 32 * step + 8 * (lane >> 4);
-        const float scale = bf16_f32(p.packed_scales[(tile * groups + k / p.group) * 16 + (lane & 15)]);
-        for (int e = 0; e < 8; ++e) sum += (float)code_at(word, e) * (bf16_f32(x[k + e]) * scale);
+    for (int64_t o = threadIdx.x; o < (int64_t)tiles * 16 * p.rows; o += threads) {
+        const int64_t tile = tile0 + o / 16 % tiles, n = 16 * tile + o % 16, m = o / (16 * tiles);
+        if (n >= p.out_features) continue;
+        float sum = 0.f;
+        for (int64_t k = 0; k < p.in_features; k += 8) {
+            const uint32_t word = p.packed[((tile * blocks + k / 128) * 64 + (n & 15) + 16 * (k / 8 % 4)) * 4 + k / 32 % 4];
+            const float scale = bf16_f32(p.packed_scales[scale_place(tile, blocks, k / p.group, p.group, (int)(n & 15))]);
+            for (int e = 0; e < 8; ++e) sum += (float)code_at(word, e) * (bf16_f32(p.x[m * p.x_stride + k + e]) * scale);
+        }
+        p.y[m * p.y_stride + n] = (uint16_t)bf16_rn(sum);
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    const int64_t n = 16 * tile + (lane & 15);
-    if (lane < 16 && n < p.out_features) p.y[row * p.y_stride + n] = (uint16_t)bf16_rn(sum);
+}
+
+// One workgroup per NB tiles of 16 outputs, for all rows (T tiles of 16).  Its
+// W waves share the inputs out in blocks of 128.  With u = c + 8 and
+// v = 1 + u / 16 (codes_bf16), sum c x = 16 (sum v x - 1.5 sum x): the second
+// sum, from a constant operand, is the accumulator that the first starts with,
+// once per group for all tiles.
+template <int Group, int T, int NB, int W>
+__global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Params p) {
+    constexpr int kPer = 128 / Group, kGroupSteps = Group / 32;
+    __shared__ F32x4 partial[W][NB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int64_t blocks = int4_blocks(p.in_features), tiles = int4_tiles(p.out_features);
+    const int64_t tile0 = (int64_t)blockIdx.x * NB;
+    const int64_t begin = blocks * wave / W, end = blocks * (wave + 1) / W;
+    F32x4 total[NB][T];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < T; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
+    struct Block {
+        U32x4 words[NB];
+        uint2 scales[NB][kPer];
+        U32x4 x[T][4];
+    };
+    auto load = [&](Block& b, int64_t block) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int64_t place = min(tile0 + j, tiles - 1) * blocks + block;
+            b.words[j] = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(p.packed) + place * 64 + lane);
+            const uint2* scales = reinterpret_cast<const uint2*>(p.packed_scales) + (place * 4 + g) * kPer;
+#pragma unroll
+            for (int h = 0; h < kPer; ++h) b.scales[j][h] = scales[h];
+        }
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int64_t k = 128 * block + 32 * s + 8 * g;
+                b.x[t][s] = U32x4{0u, 0u, 0u, 0u};
+                if (16 * t + i < p.rows && k < p.in_features)
+                    b.x[t][s] = *reinterpret_cast<const U32x4*>(p.x + (16 * t + i) * p.x_stride + k);
+            }
+    };
+    auto compute = [&](const Block& b) {
+        const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) {
+            F32x4 start[T];
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                start[t] = F32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < kGroupSteps; ++s) start[t] = mfma(shift, b.x[t][h * kGroupSteps + s], start[t]);
+            }
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                F32x4 sum[T];
+#pragma unroll
+                for (int t = 0; t < T; ++t) sum[t] = start[t];
+#pragma unroll
+                for (int s = 0; s < kGroupSteps; ++s) {
+                    const U32x4 a = codes_bf16(b.words[j][h * kGroupSteps + s]);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) sum[t] = mfma(a, b.x[t][h * kGroupSteps + s], sum[t]);
+                }
+                const uint2 raw = b.scales[j][h];
+                const float scale[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
+                                        __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(scale[r], sum[t][r], total[j][t][r]);
+            }
+        }
+    };
+    if (begin < end) {
+        Block even, odd;
+        load(even, begin);
+        for (int64_t b = begin; b < end; b += 2) {
+            if (b + 1 < end) load(odd, b + 1);
+            compute(even);
+            if (b + 1 >= end) break;
+            if (b + 2 < end) load(even, b + 2);
+            compute(odd);
+        }
+    }
+    bool finite = true;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        if (t > 0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NB; ++j) partial[wave][j][lane] = total[j][t];
+        __syncthreads();
+        const int j = wave;
+        if (j < NB) {
+            F32x4 sum = partial[0][j][lane];
+#pragma unroll
+            for (int w = 1; w < W; ++w) sum += partial[w][j][lane];
+            const int64_t n = 16 * (tile0 + j) + 4 * g, m = 16 * t + i;
+            if (m < p.rows) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (n + r >= p.out_features) break;
+                    finite = finite && fabsf(sum[r]) < __builtin_inff();
+                    p.y[m * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * sum[r]);
+                }
+            }
+        }
+    }
+    if (__syncthreads_or(!finite)) linear_int4_plain(p, tile0, (int)min((int64_t)NB, tiles - tile0), 64 * W);
+}
+
+template <int Group, int T>
+void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
+    const int64_t tiles = int4_tiles(p.out_features);
+    if (tiles >= 1024)
+        hipLaunchKernelGGL((linear_int4_kernel<Group, T, 4, 4>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, stream, p);
+    else
+        hipLaunchKernelGGL((linear_int4_kernel<Group, T, 1, 8>), dim3((unsigned)tiles), dim3(512), 0, stream, p);
+}
+
+template <int Group>
+void launch_rows(const LinearInt4Params& p, hipStream_t stream) {
+    switch ((p.rows + 15) / 16) {
+        case 1: return launch_tiles<Group, 1>(p, stream);
+        case 2: return launch_tiles<Group, 2>(p, stream);
+        case 3: return launch_tiles<Group, 3>(p, stream);
+        default: return launch_tiles<Group, 4>(p, stream);
+    }
 }
 
 }  // namespace
@@ -117,7 +268,7 @@ size_t int4_code_bytes(int64_t out_features, int64_t in_features) {
 }
 
 size_t int4_weight_bytes(int64_t out_features, int64_t in_features, int group) {
-    return int4_code_bytes(out_features, in_features) + (size_t)int4_tiles(out_features) * (in_features / group) * 32;
+    return int4_code_bytes(out_features, in_features) + (size_t)int4_tiles(out_features) * int4_blocks(in_features) * (128 / group) * 32;
 }
 
 hipError_t launch_pack_int4(const Int4PackParams& p, hipStream_t stream) {
@@ -133,8 +284,12 @@ hipError_t launch_unpack_int4(const Int4PackParams& p, uint16_t* weight, hipStre
 }
 
 hipError_t launch_linear_int4(const LinearInt4Params& p, hipStream_t stream) {
-    hipLaunchKernelGGL(linear_int4_kernel, dim3((unsigned)int4_tiles(p.out_features), (unsigned)p.rows), dim3(64), 0,
-                       stream, p);
+    if (p.group == 32)
+        launch_rows<32>(p, stream);
+    else if (p.group == 64)
+        launch_rows<64>(p, stream);
+    else
+        launch_rows<128>(p, stream);
     return hipGetLastError();
 }
 

@@ -1,6 +1,18 @@
 // Log probability of given tokens, entropy and top alternatives of logits:
 // with m = max x and S = sum e^(x - m), log p = x - m - log S and
 // H = log S - sum e^(x - m) (x - m) / S, where entries of -inf add nothing.
+//
+// One workgroup reads a row once, in chunks of 8 logits per thread.  A thread
+// keeps the sums against a reference that follows its running maximum only
+// when a logit exceeds it by 2^8 (log2 units), and its largest logit with the
+// chunk that holds it first.  Alternatives: the threads of one lane number
+// form one of 64 owners.  With T the `top`-th largest of the owners' largest
+// (value, chunk) - greater values first, then lower chunks - at least `top`
+// logits lie at or above T, so every alternative does; and logits at or above
+// T belong to threads whose own largest is, some 20 to 40 of them in a row in
+// any order.  Their chunks are read again, by all threads, and the few logits
+// found (at most kMaxCandidates, else the row takes one pass per alternative,
+// as rows with NaN or infinities do) are ranked by counting.
 #include "rq_device.h"
 #include "rq_reduced.h"
 
@@ -8,7 +20,10 @@ namespace rq {
 
 namespace {
 
-constexpr int kLogprobThreads = 256;
+constexpr int kChunk = 8;
+constexpr int kMaxCandidates = 2048;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr float kSlack = 8.0f;
 
 template <bool Bf16>
 __device__ __forceinline__ float logit_at(const void* logits, int64_t i) {
@@ -18,27 +33,91 @@ __device__ __forceinline__ float logit_at(const void* logits, int64_t i) {
         return static_cast<const float*>(logits)[i];
 }
 
-// Order of (value, index) as one number: greater values first, equal ones
-// (-0 and +0 among them) by the lower index, NaN above all.
-__device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
+// Order of values as numbers: -0 and +0 alike, NaN above all.
+__device__ __forceinline__ uint32_t ordered_bits(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
-    const uint32_t ordered = x != x ? 0xffffffffu : (u >> 31) ? ~u : u | 0x80000000u;
-    return ((uint64_t)ordered << 32) | (0xffffffffu - index);
+    return x != x ? 0xffffffffu : (u >> 31) ? ~u : u | 0x80000000u;
 }
 
+// Order of (value, index): equal values by the lower index.
+__device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
+    return ((uint64_t)ordered_bits(x) << 32) | (0xffffffffu - index);
+}
+
+__device__ __forceinline__ uint64_t shuffle_xor_u64(uint64_t v, int d) {
+    return ((uint64_t)__shfl_xor((uint32_t)(v >> 32), d) << 32) | __shfl_xor((uint32_t)v, d);
+}
+
+// A row's chunks: chunk q holds logits 8 q - shift.. of it, so that every
+// chunk starts on a 16-byte boundary (32 bytes of FP32: on a 16-byte one).
+template <bool Bf16>
+struct Row {
+    const void* base;
+    int vocab, shift, chunks;
+    __device__ Row(const LogprobParams& p, int64_t row) {
+        base = static_cast<const uint8_t*>(p.logits) + row * p.stride * (Bf16 ? 2 : 4);
+        vocab = (int)p.vocab;
+        shift = (int)(reinterpret_cast<uintptr_t>(base) % 16) / (Bf16 ? 2 : 4);
+        chunks = (int)(((int64_t)vocab + shift + kChunk - 1) / kChunk);
+    }
+    // The chunk's logits; -inf outside the row.
+    __device__ __forceinline__ void load(int q, float (&x)[kChunk]) const {
+        const int64_t at = (int64_t)kChunk * q - shift;
+        if (at >= 0 && at + kChunk <= vocab) {
+            if constexpr (Bf16) {
+                const Chunk16 raw = *reinterpret_cast<const Chunk16*>(static_cast<const uint16_t*>(base) + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[2 * e] = __uint_as_float(raw[e] << 16);
+                    x[2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u);
+                }
+            } else {
+                const Chunk16* raw = reinterpret_cast<const Chunk16*>(static_cast<const float*>(base) + at);
+                const Chunk16 a = raw[0], b = raw[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(a[e]), x[4 + e] = __uint_as_float(b[e]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e)
+            x[e] = at + e >= 0 && at + e < vocab ? logit_at<Bf16>(base, at + e) : -__builtin_inff();
+    }
+};
+
+// a * b, 0 where a is 0 (whatever b).
+__device__ __forceinline__ float mul_zero(float a, float b) { return a == 0.f ? 0.f : a * b; }
+
+// Sums of e^(x - m) and of e^(x - m) (x - m) in log2 units, with m = high.
+struct Sums {
+    float high, sum, weighted;
+};
+
+// The two sums against the larger reference.
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+    const float high = fmaxf(a.high, b.high);
+    const float da = a.high - high, db = b.high - high;
+    const float wa = da == 0.f ? 1.f : __builtin_amdgcn_exp2f(da), wb = db == 0.f ? 1.f : __builtin_amdgcn_exp2f(db);
+    // (A product with a weight of 0 is 0, whatever the distance.)
+    return Sums{high, a.sum * wa + b.sum * wb,
+                (a.weighted + mul_zero(a.sum, da)) * wa + (b.weighted + mul_zero(b.sum, db)) * wb};
+}
+
+template <int Threads>
 __device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t* partial) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
-        const uint64_t other = ((uint64_t)__shfl_xor((uint32_t)(v >> 32), d) << 32) | __shfl_xor((uint32_t)v, d);
+        const uint64_t other = shuffle_xor_u64(v, d);
         v = other > v ? other : v;
     }
     __syncthreads();
     if ((threadIdx.x & 63) == 0) partial[threadIdx.x >> 6] = v;
     __syncthreads();
-    for (int w = 0; w < kLogprobThreads / 64; ++w) v = partial[w] > v ? partial[w] : v;
+    for (int w = 0; w < Threads / 64; ++w) v = partial[w] > v ? partial[w] : v;
     return v;
 }
 
+template <int Threads>
 __device__ __forceinline__ float block_sum(float v, float* partial) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
@@ -46,34 +125,30 @@ __device__ __forceinline__ float block_sum(float v, float* partial) {
     if ((threadIdx.x & 63) == 0) partial[threadIdx.x >> 6] = v;
     __syncthreads();
     float total = 0.f;
-    for (int w = 0; w < kLogprobThreads / 64; ++w) total += partial[w];
+    for (int w = 0; w < Threads / 64; ++w) total += partial[w];
     return total;
 }
 
-// One workgroup per row: one pass for the maximum, one for the sums, one for
-// each alternative.
-template <bool Bf16>
-__global__ __launch_bounds__(kLogprobThreads) void logprobs_kernel(const LogprobParams p) {
-    __shared__ uint64_t keys[kLogprobThreads / 64];
-    __shared__ float sums[kLogprobThreads / 64];
-    const int64_t row = blockIdx.x;
+// The row by plain passes: the maximum, the sums, one pass per alternative
+// (those only if `sums_done`).
+template <bool Bf16, int Threads>
+__device__ __noinline__ void logprobs_plain(const LogprobParams& p, int64_t row, bool sums_done, uint64_t* keys, float* sums) {
     const int64_t base = row * p.stride;
     float largest = -__builtin_inff();
-    for (int64_t i = threadIdx.x; i < p.vocab; i += kLogprobThreads) largest = fmaxf(largest, logit_at<Bf16>(p.logits, base + i));
-    const uint64_t top_key = block_max_u64(rank_key(largest, 0), keys);
-    const uint32_t ordered = (uint32_t)(top_key >> 32);
+    for (int64_t i = threadIdx.x; i < p.vocab; i += Threads) largest = fmaxf(largest, logit_at<Bf16>(p.logits, base + i));
+    const uint32_t ordered = (uint32_t)(block_max_u64<Threads>(rank_key(largest, 0), keys) >> 32);
     largest = __uint_as_float((ordered >> 31) ? ordered & 0x7fffffffu : ~ordered);
     float sum = 0.f, weighted = 0.f;
-    for (int64_t i = threadIdx.x; i < p.vocab; i += kLogprobThreads) {
+    for (int64_t i = threadIdx.x; i < p.vocab; i += Threads) {
         const float x = logit_at<Bf16>(p.logits, base + i);
         const float d = x - largest, w = x == -__builtin_inff() ? 0.f : expf(d);
         sum += w;
         weighted += w > 0.f ? w * d : 0.f;
     }
-    sum = block_sum(sum, sums);
-    weighted = block_sum(weighted, sums);
+    sum = block_sum<Threads>(sum, sums);
+    weighted = block_sum<Threads>(weighted, sums);
     const float log_sum = logf(sum);
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0 && !sums_done) {
         const int64_t token = p.tokens[row];
         p.logprob[row] = token >= 0 && token < p.vocab ? logit_at<Bf16>(p.logits, base + token) - largest - log_sum
                                                        : __builtin_nanf("");
@@ -82,11 +157,11 @@ __global__ __launch_bounds__(kLogprobThreads) void logprobs_kernel(const Logprob
     uint64_t below = ~0ull;
     for (int k = 0; k < p.top; ++k) {
         uint64_t best = 0;
-        for (int64_t i = threadIdx.x; i < p.vocab; i += kLogprobThreads) {
+        for (int64_t i = threadIdx.x; i < p.vocab; i += Threads) {
             const uint64_t key = rank_key(logit_at<Bf16>(p.logits, base + i), (uint32_t)i);
             if (key < below && key > best) best = key;
         }
-        below = best = block_max_u64(best, keys);
+        below = best = block_max_u64<Threads>(best, keys);
         if (threadIdx.x == 0) {
             const int64_t index = 0xffffffffu - (uint32_t)best;
             p.top_tokens[row * p.top + k] = index;
@@ -95,13 +170,163 @@ __global__ __launch_bounds__(kLogprobThreads) void logprobs_kernel(const Logprob
     }
 }
 
+template <bool Bf16, int Threads>
+__global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p) {
+    constexpr int kWaves = Threads / 64;
+    __shared__ uint64_t keys[kWaves * 64];
+    __shared__ Sums wave_sums[kWaves];
+    __shared__ uint64_t candidates[kMaxCandidates];
+    __shared__ uint16_t listed[Threads];
+    __shared__ uint64_t threshold;
+    __shared__ int listed_count, candidate_count;
+    const int64_t row_number = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Row<Bf16> row(p, row_number);
+    float token_logit = 0.f;
+    int64_t token = 0;
+    if (tid == 0) {
+        token = p.tokens[row_number];
+        token_logit = token >= 0 && token < p.vocab ? logit_at<Bf16>(row.base, token) : __builtin_nanf("");
+        listed_count = candidate_count = 0;
+    }
+
+    // One pass: the sums, and the thread's largest logit with its first chunk.
+    Sums own{-3.0e38f, 0.f, 0.f};
+    float largest = -__builtin_inff();
+    uint32_t largest_chunk = 0xffffffffu;
+    auto take = [&](int q, const float (&x)[kChunk]) {
+        const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (most > largest || largest_chunk == 0xffffffffu) {
+            largest_chunk = (uint32_t)q;
+            largest = fmaxf(most, largest);
+        }
+        if (__any(most * kLog2e > own.high + kSlack)) {
+            const float high = fmaxf(own.high, most * kLog2e);
+            const float down = own.high - high, keep = __builtin_amdgcn_exp2f(down);
+            own.weighted = (own.weighted + mul_zero(own.sum, down)) * keep;
+            own.sum *= keep;
+            own.high = high;
+        }
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            const float d = fmaf(x[e], kLog2e, -own.high);
+            const float w = __builtin_amdgcn_exp2f(d);
+            own.sum += w;
+            own.weighted = fmaf(w, fmaxf(d, -1000.0f), own.weighted);  // 0 where w is 0, also at d = -inf
+        }
+    };
+    constexpr int kAhead = 4;
+    for (int q = tid; q < row.chunks; q += kAhead * Threads) {
+        float x[kAhead][kChunk];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (q + a * Threads < row.chunks) row.load(q + a * Threads, x[a]);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+            if (q + a * Threads < row.chunks) take(q + a * Threads, x[a]);
+    }
+    Sums all = own;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) all = join(all, Sums{__shfl_xor(all.high, d), __shfl_xor(all.sum, d), __shfl_xor(all.weighted, d)});
+    const uint64_t own_key = ((uint64_t)ordered_bits(largest) << 32) | (0xffffffffu - largest_chunk);
+    if (lane == 0) wave_sums[wave] = all;
+    keys[tid] = own_key;
+    __syncthreads();
+    all = wave_sums[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) all = join(all, wave_sums[w]);
+    // The largest logit itself: owners' largest, then the largest of all.
+    uint64_t owner = keys[lane];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) owner = keys[64 * w + lane] > owner ? keys[64 * w + lane] : owner;
+    uint64_t best = owner;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const uint64_t other = shuffle_xor_u64(best, d);
+        best = other > best ? other : best;
+    }
+    const uint32_t ordered = (uint32_t)(best >> 32);
+    const float m = __uint_as_float((ordered >> 31) ? ordered & 0x7fffffffu : ~ordered);
+    // The sums against m itself.  Their reference is a rounded m' log2(e); one
+    // rounding of the difference keeps large logits exact.
+    const float above_reference = fmaf(m, kLog2e, -all.high), keep = __builtin_amdgcn_exp2f(-above_reference);
+    const float exact_sum = all.sum * keep;
+    const float weighted = (all.weighted - above_reference * all.sum) * keep;
+    const float log_sum = logf(exact_sum);
+    // NaN, infinities (S is NaN), nothing but -inf (m), or values near the lowest.
+    if (!(m > -1.0e38f && m < 1.0e38f && exact_sum < 1.0e38f)) {
+        logprobs_plain<Bf16, Threads>(p, row_number, false, keys, reinterpret_cast<float*>(wave_sums));
+        return;
+    }
+    if (tid == 0) {
+        p.logprob[row_number] = token_logit - m - log_sum;
+        p.entropy[row_number] = log_sum - weighted * kLn2 / exact_sum;
+    }
+    if (p.top == 0) return;
+
+    // T: the `top`-th of the owners.
+    if (wave == 0) {
+        int above = 0;
+        for (int o = 0; o < 64; ++o) {
+            const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(owner >> 32), o) << 32) |
+                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)owner, o);
+            above += other > owner || (other == owner && o < lane) ? 1 : 0;
+        }
+        if (above == p.top - 1) threshold = owner;
+    }
+    __syncthreads();
+    const uint64_t limit = threshold;
+    if (own_key >= limit && largest_chunk != 0xffffffffu) listed[atomicAdd(&listed_count, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int each = (row.chunks + Threads - 1) / Threads, work = listed_count * each;
+    for (int o = tid; o < work; o += Threads) {
+        const int q = listed[o / each] + o % each * Threads;
+        if (q >= row.chunks) continue;
+        float x[kChunk];
+        row.load(q, x);
+#pragma unroll
+        for (int e = 0; e < kChunk; ++e) {
+            const int64_t index = (int64_t)kChunk * q - row.shift + e;
+            const uint64_t key = ((uint64_t)ordered_bits(x[e]) << 32) | (0xffffffffu - (uint32_t)q);
+            if (key >= limit && index >= 0 && index < row.vocab) {
+                const int place = atomicAdd(&candidate_count, 1);
+                if (place < kMaxCandidates) candidates[place] = rank_key(x[e], (uint32_t)index);
+            }
+        }
+    }
+    __syncthreads();
+    const int found = candidate_count;
+    if (found > kMaxCandidates) {
+        logprobs_plain<Bf16, Threads>(p, row_number, true, keys, reinterpret_cast<float*>(wave_sums));
+        return;
+    }
+    for (int c = tid; c < found; c += Threads) {
+        const uint64_t key = candidates[c];
+        int rank = 0;
+        for (int o = 0; o < found; ++o) rank += candidates[o] > key ? 1 : 0;
+        if (rank >= p.top) continue;
+        const uint32_t bits = (uint32_t)(key >> 32);
+        const float x = __uint_as_float((bits >> 31) ? bits & 0x7fffffffu : ~bits);
+        p.top_tokens[row_number * p.top + rank] = (int64_t)(0xffffffffu - (uint32_t)key);
+        p.top_logprobs[row_number * p.top + rank] = x - m - log_sum;
+    }
+}
+
+template <bool Bf16>
+void launch_rows(const LogprobParams& p, hipStream_t stream) {
+    if (p.rows <= 256)
+        hipLaunchKernelGGL((logprobs_kernel<Bf16, 1024>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    else
+        hipLaunchKernelGGL((logprobs_kernel<Bf16, 512>), dim3((unsigned)p.rows), dim3(512), 0, stream, p);
+}
+
 }  // namespace
 
 hipError_t launch_logprobs(const LogprobParams& p, hipStream_t stream) {
     if (p.bf16)
-        hipLaunchKernelGGL((logprobs_kernel<true>), dim3((unsigned)p.rows), dim3(kLogprobThreads), 0, stream, p);
+        launch_rows<true>(p, stream);
     else
-        hipLaunchKernelGGL((logprobs_kernel<false>), dim3((unsigned)p.rows), dim3(kLogprobThreads), 0, stream, p);
+        launch_rows<false>(p, stream);
     return hipGetLastError();
 }
 
