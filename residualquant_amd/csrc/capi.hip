@@ -1170,12 +1170,13 @@ static int check_fp8_pages(const void* cache, const float* scales, int64_t num_b
     if ((head_dim != 96 && head_dim != 128) || (page_tokens != 16 && page_tokens != 32))
         return fail(RQ_ENOKERNEL, "No compiled 8-bit paged kernel for head_dim=%d, page_tokens=%d", head_dim,
                     page_tokens);
-    if (rows < 0 || rows > (int64_t)INT32_MAX || kv_heads <= 0 || kv_heads > 65535)
+    if (rows < 0 || rows > (int64_t)INT32_MAX / 4 || kv_heads <= 0 || kv_heads > 65535)
         return fail(RQ_EINVAL, "K/V of 0 or more rows and 1 to 65535 heads required");
     if (cache == nullptr || scales == nullptr || num_blocks < 0 || (reinterpret_cast<uintptr_t>(cache) % 16) != 0 ||
         (reinterpret_cast<uintptr_t>(scales) % 4) != 0)
         return fail(RQ_EINVAL, "16-byte aligned 8-bit cache and its FP32 scales required");
-    if (requests < 0 || (requests > 0 && (query_start_loc == nullptr || seq_lens == nullptr)))
+    if (requests < 0 || requests > (int64_t)INT32_MAX / 4 ||
+        (requests > 0 && (query_start_loc == nullptr || seq_lens == nullptr)))
         return fail(RQ_EINVAL, "Contiguous INT32 query starts with one final boundary required");
     if ((rows > 0 && requests > 0 && block_table == nullptr) || max_pages < 0 || block_table_stride < max_pages ||
         max_pages > (int64_t)INT32_MAX / page_tokens)

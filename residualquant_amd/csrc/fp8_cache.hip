@@ -11,27 +11,26 @@ namespace rq {
 
 namespace {
 
+typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
+typedef U32x4 U32x4At8 __attribute__((aligned(8)));  // 16 bytes on an 8-byte boundary
+
 // ------------------------------------------------------------------ write
+//
+// One wave per (page that the call writes, head, plane): the page's new
+// values stay in registers between the maximum and the conversion, so each is
+// read once.  Request b's pages take the slots from floor(first row / PT) + 2 b
+// (n rows touch at most n / PT + 2 pages), so a wave finds its request by
+// counting.
 
-// The request of a row, its place among the request's new rows and its
-// position in the sequence.
-struct RowPlace {
-    int request;      // -1: the row belongs to no request
-    int index, count; // place among the request's `count` new rows
-    int64_t history;  // tokens before the first of them
-};
-
-__device__ __forceinline__ RowPlace place_row(const int32_t* qsl, const int32_t* seq_lens, int64_t requests,
-                                              int64_t row, int* lds_counts) {
-    RowPlace r;
-    r.request = find_request_parallel(qsl, requests, row, lds_counts);
-    if (r.request < 0) return r;
-    const int32_t begin = qsl[r.request];
-    r.index = (int)(row - begin);
-    r.count = qsl[r.request + 1] - begin;
-    const int64_t history = (int64_t)seq_lens[r.request] - r.count;
-    r.history = history > 0 ? history : 0;
-    return r;
+// The request of slot `slot` (the last whose first slot is at or below it).
+__device__ __forceinline__ int write_request(const int32_t* qsl, int requests, int page_shift, int slot) {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int b = 1 + lane; b < requests; b += 64) count += (int64_t)(qsl[b] >> page_shift) + 2 * (int64_t)b <= slot ? 1 : 0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) count += __shfl_xor(count, d);
+    return __builtin_amdgcn_readfirstlane(count);
 }
 
 // The least power of two s >= 2^-126 with largest <= 448 s.  largest = m 2^e,
@@ -43,56 +42,105 @@ __device__ __forceinline__ float needed_scale(float largest) {
     return __uint_as_float((uint32_t)exponent << 23);
 }
 
-// E4M3 of x; infinities, which the format lacks, become NaN.
-__device__ __forceinline__ uint32_t e4m3_code(float x) {
-    return fabsf(x) == __builtin_inff() ? 0x7fu : e4m3_rn(x);
+// Four E4M3 codes (ties to even) of values within +-448; what is not finite becomes NaN.
+__device__ __forceinline__ uint32_t fp8x4_rn(float a, float b, float c, float d) {
+    auto nan_unless_finite = [](float x) { return fabsf(x) < __builtin_inff() ? x : __builtin_nanf(""); };
+    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(a), nan_unless_finite(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(c), nan_unless_finite(d), low, true);
 }
 
-// One workgroup per (row, head, plane); the first new row of a page writes
-// all of the page's new rows and, where the scale grows, rounds the codes of
-// the page's older tokens again.
-__global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams p) {
-    __shared__ int counts[4];
-    __shared__ float wave_largest[4];
-    const int64_t row = blockIdx.x;
-    const int head = blockIdx.y, plane = blockIdx.z;
-    const int tid = threadIdx.x;
-    const RowPlace at = place_row(p.query_start_loc, p.seq_lens, p.requests, row, counts);
-    if (at.request < 0) return;
-    const int PT = p.page_tokens, D = p.head_dim;
-    const int64_t position = at.history + at.index;
-    const int slot = (int)(position % PT);
-    const int64_t page = position / PT;
-    if ((at.index != 0 && slot != 0) || page >= p.max_pages) return;
-    const int64_t block = p.block_table[(int64_t)at.request * p.block_table_stride + page];
-    if (block < 0 || block >= p.num_blocks) return;
-    const int rows = min(PT - slot, at.count - at.index);
-    const uint16_t* in = (plane == 0 ? p.key : p.value) + row * (plane == 0 ? p.key_stride : p.value_stride) +
-                         (int64_t)head * D;
-    const int64_t in_stride = plane == 0 ? p.key_stride : p.value_stride;
-    const int64_t index = ((int64_t)plane * p.num_blocks + block) * p.kv_heads + head;
-    uint8_t* codes = p.cache + index * PT * D;
+__device__ __forceinline__ bool power_of_two(float x) { return (__float_as_uint(x) & 0x7fffffu) == 0; }
 
-    float largest = 0.f;
-    for (int i = tid; i < rows * D; i += 256) {
-        const float x = fabsf(bf16_f32(in[(i / D) * in_stride + i % D]));
-        if (x < __builtin_inff()) largest = fmaxf(largest, x);
+template <int D, int PT>
+__global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams p) {
+    constexpr int kRow = D / 8;                      // chunks of 8 values per row
+    constexpr int kChunks = (PT * kRow + 63) / 64;   // per lane
+    constexpr int kShift = PT == 16 ? 4 : 5;
+    const int lane = threadIdx.x & 63;
+    const int head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int plane = blockIdx.z;
+    if (head >= p.kv_heads) return;
+    const int request = write_request(p.query_start_loc, (int)p.requests, kShift, (int)blockIdx.x);
+    const int first = p.query_start_loc[request];
+    const int n = p.query_start_loc[request + 1] - first;
+    const int64_t seq = p.seq_lens[request];
+    const int64_t history = seq > n ? seq - n : 0;
+    // The page: the slot's number among the request's, the rows from `begin` on at `slot`.
+    const int64_t number = (int64_t)blockIdx.x - ((int64_t)(first >> kShift) + 2 * (int64_t)request);
+    const int64_t page = (history >> kShift) + number;
+    const int64_t begin = number == 0 ? 0 : (page << kShift) - history;
+    if (n <= 0 || first < 0 || first + begin >= p.rows || number < 0 || begin >= n || page >= p.max_pages) return;
+    const int slot = (int)((history + begin) & (PT - 1));
+    const int rows = (int)min(min((int64_t)(PT - slot), n - begin), p.rows - first - begin);
+    const int64_t block = p.block_table[(int64_t)request * p.block_table_stride + page];
+    if (block < 0 || block >= p.num_blocks) return;
+    const int64_t index = ((int64_t)plane * p.num_blocks + block) * p.kv_heads + head;
+    uint8_t* const codes = p.cache + index * (PT * D);
+    const float before = p.scales[index];
+    const int64_t stride = plane == 0 ? p.key_stride : p.value_stride;
+    const uint16_t* in = (plane == 0 ? p.key : p.value) + (first + begin) * stride + (int64_t)head * D;
+
+    U32x4 values[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int chunk = 64 * c + lane, r = chunk / kRow;
+        values[c] = U32x4{0u, 0u, 0u, 0u};
+        if (r < rows) values[c] = *reinterpret_cast<const U32x4At8*>(in + r * stride + 8 * (chunk - r * kRow));
     }
+    float largest = 0.f;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float a = __uint_as_float(values[c][e] << 16), b = __uint_as_float(values[c][e] & 0xffff0000u);
+            largest = fmaxf(largest, fabsf(a) < __builtin_inff() ? fabsf(a) : 0.f);
+            largest = fmaxf(largest, fabsf(b) < __builtin_inff() ? fabsf(b) : 0.f);
+        }
 #pragma unroll
     for (int d = 32; d; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
-    if ((tid & 63) == 0) wave_largest[tid >> 6] = largest;
-    const float before = p.scales[index];
-    __syncthreads();
-    largest = fmaxf(fmaxf(wave_largest[0], wave_largest[1]), fmaxf(wave_largest[2], wave_largest[3]));
     const float need = needed_scale(largest);
     const float scale = slot > 0 && before >= need ? before : need;
+
     if (slot > 0 && scale > before) {
         const float shrink = before / scale;
-        for (int i = tid; i < slot * D; i += 256) codes[i] = (uint8_t)e4m3_rn(e4m3_f32(codes[i]) * shrink);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const int chunk = 64 * c + lane;
+            if (chunk >= slot * kRow) continue;
+            U32x2* place = reinterpret_cast<U32x2*>(codes) + chunk;
+            U32x2 word = *place;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(word[w], false), high = __builtin_amdgcn_cvt_pk_f32_fp8(word[w], true);
+                word[w] = fp8x4_rn(low[0] * shrink, low[1] * shrink, high[0] * shrink, high[1] * shrink);
+            }
+            *place = word;
+        }
     }
-    for (int i = tid; i < rows * D; i += 256)
-        codes[slot * D + i] = (uint8_t)e4m3_code(bf16_f32(in[(i / D) * in_stride + i % D]) / scale);
-    if (tid == 0) p.scales[index] = scale;
+    // A division by a power of two is a product (a scale that the caller made may be any number).
+    const bool exact = power_of_two(scale);
+    const float inverse = 1.0f / scale;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int chunk = 64 * c + lane;
+        if (chunk >= rows * kRow) continue;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[2 * e] = __uint_as_float(values[c][e] << 16);
+            x[2 * e + 1] = __uint_as_float(values[c][e] & 0xffff0000u);
+        }
+        if (exact) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= inverse;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] /= scale;
+        }
+        reinterpret_cast<U32x2*>(codes)[slot * kRow + chunk] =
+            U32x2{fp8x4_rn(x[0], x[1], x[2], x[3]), fp8x4_rn(x[4], x[5], x[6], x[7])};
+    }
+    if (lane == 0) p.scales[index] = scale;
 }
 
 // ------------------------------------------------------------------ attention
@@ -123,8 +171,6 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams 
 typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 Bf16x2 __attribute__((ext_vector_type(2)));
 typedef float F32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kStreamThreads = 256;
 constexpr float kLowest = -3.402823466e+38f;
@@ -672,8 +718,16 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
 }  // namespace
 
 hipError_t launch_quantize_fp8(const Fp8WriteParams& p, hipStream_t stream) {
-    if (p.rows == 0) return hipSuccess;
-    hipLaunchKernelGGL(quantize_fp8_kernel, dim3((unsigned)p.rows, (unsigned)p.kv_heads, 2), dim3(256), 0, stream, p);
+    if (p.rows == 0 || p.requests == 0) return hipSuccess;
+    const dim3 grid((unsigned)(p.rows / p.page_tokens + 2 * p.requests), (unsigned)((p.kv_heads + 3) / 4), 2), threads(256);
+    if (p.head_dim == 128 && p.page_tokens == 16)
+        hipLaunchKernelGGL((quantize_fp8_kernel<128, 16>), grid, threads, 0, stream, p);
+    else if (p.head_dim == 128)
+        hipLaunchKernelGGL((quantize_fp8_kernel<128, 32>), grid, threads, 0, stream, p);
+    else if (p.page_tokens == 16)
+        hipLaunchKernelGGL((quantize_fp8_kernel<96, 16>), grid, threads, 0, stream, p);
+    else
+        hipLaunchKernelGGL((quantize_fp8_kernel<96, 32>), grid, threads, 0, stream, p);
     return hipGetLastError();
 }
 
