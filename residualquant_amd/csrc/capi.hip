@@ -1227,7 +1227,7 @@ int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int6
 // Least steps of 32 tokens of one split of an 8-bit attention call, the
 // workgroups per compute unit that its work is spread over, and the most
 // columns of a workgroup's tile.
-constexpr int kFp8MinSteps = 8, kFp8PerCu = 2, kFp8MaxTile = 128, kFp8MaxSplits = 256;
+constexpr int kFp8MinSteps = 8, kFp8PerCu = 2, kFp8MaxTile = 256, kFp8MaxSplits = 256;
 
 // Steps that the page table and the new rows of a call can hold.
 static int64_t fp8_most_steps(int64_t rows, int64_t max_pages, int page_tokens) {
@@ -1264,7 +1264,7 @@ static void plan_fp8(rq::Fp8AttentionParams& p) {
     const int64_t columns = p.rows * (p.heads / p.kv_heads);
     const int64_t average = (columns + p.requests - 1) / p.requests;
     p.tile = average <= 16 ? 16 : average <= 48 ? 32 : kFp8MaxTile;
-    const int64_t target = (kFp8PerCu * (int64_t)compute_units() + p.kv_heads - 1) / p.kv_heads;
+    const int64_t target = ((p.tile == kFp8MaxTile ? 3 * (int64_t)compute_units() / 4 : kFp8PerCu * (int64_t)compute_units()) + p.kv_heads - 1) / p.kv_heads;
     const int64_t most_steps = fp8_most_steps(p.rows, p.max_pages, p.page_tokens);
     const int64_t tiles = columns / p.tile + p.requests;  // at most, over all requests
     const bool split = p.entries > 0;

@@ -261,40 +261,53 @@ struct Fp8Step {
 };
 
 // The columns' statistics and sums of a wave.
-template <int NT>
+template <int NT, int Channels>
 struct Fp8Columns {
-    F32x4 out[NT][8];   // [tile][e]: channels 8 (4 g + r) + e
-    float high[NT];     // the maximum that weights refer to (log2 units)
-    float sum[NT];      // of this lane's tokens
+    F32x4 out[NT][Channels];  // [tile][e]
+    float high[NT];  // the maximum that weights refer to (log2 units)
+    float sum[NT];   // of this lane's tokens
 };
 
-// Weights of one step's scores and their product with V (operand a[e]).
-template <int NT>
-__device__ __forceinline__ void fp8_softmax(Fp8Columns<NT>& columns, const float (&s)[NT][2][4],
-                                            const float (&value_scale)[2], float (&weight)[NT][2][4],
-                                            U32x4 (&upper)[NT], U32x4 (&lower)[NT]) {
+// Weights of U units of 16 tokens: of the products dot (masked: -inf) with their
+// K scales (positive, softmax scale and log2(e) included), as two BF16 parts of
+// weight x V scale.  Channels: the product's tiles of 16.
+template <int NT, int Channels, int U>
+__device__ __forceinline__ void fp8_softmax(Fp8Columns<NT, Channels>& columns, const F32x4 (&dot)[NT][U],
+                                            const float (&key_scale)[U], const float (&value_scale)[U],
+                                            float (&weight)[NT][U][4], U32x4 (&upper)[NT][U / 2], U32x4 (&lower)[NT][U / 2]) {
+    float top[NT];
+    bool above = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        float most = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                           fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-        if (__any(most > columns.high[t] + kMaxSlack)) {
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            const float next = fmaxf(columns.high[t], most);
+        top[t] = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            top[t] = fmaxf(top[t], fmaxf(fmaxf(dot[t][u][0], dot[t][u][1]), fmaxf(dot[t][u][2], dot[t][u][3])) * key_scale[u]);
+        above = above || top[t] > columns.high[t] + kMaxSlack;
+    }
+    if (__any(above)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            top[t] = fmaxf(top[t], __shfl_xor(top[t], 16));
+            top[t] = fmaxf(top[t], __shfl_xor(top[t], 32));
+            const float next = fmaxf(columns.high[t], top[t]);
             const float keep = next == columns.high[t] ? 1.0f : __builtin_amdgcn_exp2f(columns.high[t] - next);
             columns.high[t] = next;
             columns.sum[t] *= keep;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < Channels; ++e)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) columns.out[t][e][r] *= keep;
         }
-        uint32_t up[4], low[4];
+    }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+    for (int t = 0; t < NT; ++t) {
+        uint32_t up[2 * U], low[2 * U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                weight[t][u][r] = __builtin_amdgcn_exp2f(s[t][u][r] - columns.high[t]);
+                weight[t][u][r] = __builtin_amdgcn_exp2f(fmaf(dot[t][u][r], key_scale[u], -columns.high[t]));
                 columns.sum[t] += weight[t][u][r];
             }
 #pragma unroll
@@ -305,19 +318,53 @@ __device__ __forceinline__ void fp8_softmax(Fp8Columns<NT>& columns, const float
                 low[2 * u + h] = bf16x2_rn(a - __uint_as_float(both << 16), b - __uint_as_float(both & 0xffff0000u));
             }
         }
-        upper[t] = U32x4{up[0], up[1], up[2], up[3]};
-        lower[t] = U32x4{low[0], low[1], low[2], low[3]};
+#pragma unroll
+        for (int s = 0; s < U / 2; ++s) {
+            upper[t][s] = U32x4{up[4 * s], up[4 * s + 1], up[4 * s + 2], up[4 * s + 3]};
+            lower[t][s] = U32x4{low[4 * s], low[4 * s + 1], low[4 * s + 2], low[4 * s + 3]};
+        }
     }
 }
 
-// One workgroup per (item, K/V head).  Rows false: its four waves take every
-// fourth step of the item's 16 NT columns; true: every step, 16 NT columns each.
-template <int D, int NT, bool Rows>
+// The last split of an item to finish joins the splits' parts of its columns, in their order.
+template <int D, int Threads, int Tile, class OutputRow>
+__device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int item_column, int columns_in, int splits,
+                                         OutputRow output_row) {
+    constexpr int kEntry = D + 4;
+    const int tid = threadIdx.x;
+    for (int c = tid >> 4; c < Tile; c += Threads / 16) {
+        const int column = item_column + c, channel = 8 * (tid & 15);
+        if (column >= columns_in || channel >= D) continue;
+        const uint32_t at = (uint32_t)(column * splits) * kEntry * 4;
+        float high = kLowest;
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) high = fmaxf(high, handoff_load2(handoff, at + (uint32_t)k * kEntry * 4).x);
+        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) {
+            const uint32_t part = at + (uint32_t)k * kEntry * 4;
+            const float2 stats = handoff_load2(handoff, part);
+            const float4 a = handoff_load4(handoff, part + 16 + 4 * channel), b = handoff_load4(handoff, part + 32 + 4 * channel);
+            const float keep = stats.x == high ? 1.0f : __builtin_amdgcn_exp2f(stats.x - high);
+            sum += stats.y * keep;
+            o[0] += a.x * keep, o[1] += a.y * keep, o[2] += a.z * keep, o[3] += a.w * keep;
+            o[4] += b.x * keep, o[5] += b.y * keep, o[6] += b.z * keep, o[7] += b.w * keep;
+        }
+        const float scale = 1.0f / sum;
+        uint16_t* out = output_row(column) + channel;
+        *reinterpret_cast<U32x2*>(out) = U32x2{bf16x2_rn(o[0] * scale, o[1] * scale), bf16x2_rn(o[2] * scale, o[3] * scale)};
+        *reinterpret_cast<U32x2*>(out + 4) = U32x2{bf16x2_rn(o[4] * scale, o[5] * scale), bf16x2_rn(o[6] * scale, o[7] * scale)};
+    }
+}
+
+// One workgroup per (item, K/V head): its four waves take every fourth step of
+// the item's 16 NT columns.
+template <int D, int NT>
 __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8AttentionParams p) {
-    constexpr int kTile = 16 * NT * (Rows ? 4 : 1);
+    constexpr int kTile = 16 * NT, kWaves = kStreamThreads / 64;
     constexpr int kSteps = D / 32;
     constexpr int kEntry = D + 4;  // m, l, arrival word, O
-    __shared__ __align__(16) float merged[Rows ? 1 : 4][Rows ? 1 : 16][Rows ? 1 : kEntry];
+    __shared__ __align__(16) float merged[kWaves][16][kEntry];
     __shared__ int last_flag;
     const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
     const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
@@ -333,14 +380,11 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int item_column = __builtin_amdgcn_readfirstlane(item.index) * kTile;
-    const int column0 = item_column + (Rows ? wave * 16 * NT : 0);
-    // (A wave past the request's columns has no steps.)
-    const int end = column0 < columns_in ? split_begin(__builtin_amdgcn_readfirstlane(item.length), split + 1, splits) : begin;
-    const int stride = Rows ? 1 : 4;
+    const int end = split_begin(__builtin_amdgcn_readfirstlane(item.length), split + 1, splits);
     const int history_steps = fp8_steps(history);
 
     // The item's arrival word lies in the two unused floats of its first entry.
-    float* const entries = p.partials + ((int64_t)head * p.entries + item.entry) * kEntry;
+    float* const entries = p.partials + ((int64_t)head * p.entries + __builtin_amdgcn_readfirstlane(item.entry)) * kEntry;
     uint64_t* const arrivals = reinterpret_cast<uint64_t*>(entries + (int64_t)item_column * splits * kEntry + 2);
     const uint64_t arrivals_seen = splits > 1 ? peek_arrivals(arrivals) : 0;
 
@@ -351,7 +395,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
     auto k_channel = [&](int s) { return D == 128 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 24 * g + 8 * s; };
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int column = column0 + 16 * t + i;
+        const int column = item_column + 16 * t + i;
         seen[t] = column < columns_in ? column / group : -1;
         const int row = column < columns_in ? column / group : 0;
         const uint16_t* q = p.query + (int64_t)(first + row) * p.query_stride +
@@ -363,7 +407,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
             query[t][s] = column < columns_in ? U32x4{a[0], a[1], b[0], b[1]} : U32x4{0u, 0u, 0u, 0u};
         }
     }
-    Fp8Columns<NT> columns;
+    Fp8Columns<NT, 8> columns;  // tile e: channels 8 (4 g + r) + e
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         columns.high[t] = kLowest;
@@ -376,21 +420,22 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
     // ---------------------------------------------------------------- history
     // Lane l holds the place, scales and valid tokens of unit l % 2 of the
     // wave's step l / 2 of a batch of 32.
-    const int64_t plane_bytes = p.num_blocks * p.kv_heads * p.page_tokens * D;
-    const int my_steps = max(0, (min(end, history_steps) - begin - (Rows ? 0 : wave) + stride - 1) / stride);
-    const int step0 = begin + (Rows ? 0 : wave);
+    const int page_shift = p.page_tokens == 16 ? 4 : 5;
+    const int64_t plane_bytes = ((p.num_blocks * p.kv_heads) << page_shift) * D;
+    const int step0 = begin + wave;
+    const int my_steps = max(0, (min(end, history_steps) - step0 + kWaves - 1) / kWaves);
     uint32_t place_low = 0, place_high = 0, unit_valid = 0;
     float unit_key_scale = 1.f, unit_value_scale = 1.f;
     auto look_up = [&](int batch) {
-        const int step = step0 + (32 * batch + (lane >> 1)) * stride;
+        const int step = step0 + (32 * batch + (lane >> 1)) * kWaves;
         const int token = 32 * step + 16 * (lane & 1);
         const int left = step < min(end, history_steps) ? history - token : 0;
-        const int page = token / p.page_tokens;
+        const int page = token >> page_shift;
         int64_t block = left > 0 ? p.block_table[(int64_t)request * p.block_table_stride + page] : -1;
         const bool held = block >= 0 && block < p.num_blocks;
         if (!held) block = 0;
         const int64_t index = block * p.kv_heads + head;
-        const int64_t place = (index * p.page_tokens + token % p.page_tokens) * D;
+        const int64_t place = ((index << page_shift) + (token & (p.page_tokens - 1))) * D;
         place_low = (uint32_t)place;
         place_high = (uint32_t)((uint64_t)place >> 32);
         unit_valid = held ? (uint32_t)min(left, 16) : 0u;
@@ -423,12 +468,11 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         }
     };
     auto compute = [&](const Fp8Step<D>& x) {
-        float s[NT][2][4];
+        F32x4 dot[NT][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            F32x4 dot[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) dot[t] = F32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < NT; ++t) dot[t][u] = F32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m < kSteps; ++m) {
                 uint32_t a0, a1;
@@ -441,23 +485,19 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
                 const U32x4 a = {bf16x2_of_fp8<false>(a0), bf16x2_of_fp8<true>(a0), bf16x2_of_fp8<false>(a1),
                                  bf16x2_of_fp8<true>(a1)};
 #pragma unroll
-                for (int t = 0; t < NT; ++t) dot[t] = mfma(a, query[t][m], dot[t]);
+                for (int t = 0; t < NT; ++t) dot[t][u] = mfma(a, query[t][m], dot[t][u]);
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][u][r] = dot[t][r] * x.key_scale[u];
             if (x.valid[u] < 16) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        s[t][u][r] = 4 * g + r < x.valid[u] ? s[t][u][r] : -__builtin_inff();
+                        dot[t][u][r] = 4 * g + r < x.valid[u] ? dot[t][u][r] : -__builtin_inff();
             }
         }
         float weight[NT][2][4];
-        U32x4 upper[NT], lower[NT];
-        fp8_softmax<NT>(columns, s, x.value_scale, weight, upper, lower);
+        U32x4 upper[NT][1], lower[NT][1];
+        fp8_softmax<NT, 8, 2>(columns, dot, x.key_scale, x.value_scale, weight, upper, lower);
         uint32_t v[2][4][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -487,8 +527,8 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
                                  bf16x2_of_fp8<true>(t1[c])};
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    columns.out[t][4 * w + c] = mfma(a, upper[t], columns.out[t][4 * w + c]);
-                    columns.out[t][4 * w + c] = mfma(a, lower[t], columns.out[t][4 * w + c]);
+                    columns.out[t][4 * w + c] = mfma(a, upper[t][0], columns.out[t][4 * w + c]);
+                    columns.out[t][4 * w + c] = mfma(a, lower[t][0], columns.out[t][4 * w + c]);
                 }
             }
         }
@@ -512,32 +552,31 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
     // ---------------------------------------------------------------- new rows
     // (BF16 rows of this call, row j seen by the columns of rows j and later.)
     {
-        const int most = min(rows - 1, (column0 + 16 * NT - 1) / group);  // the last row that any column sees
-        int step = begin + (Rows ? 0 : wave);
-        if (step < history_steps) step += (history_steps - step + stride - 1) / stride * stride;
-        for (; step < end; step += stride) {
+        const int most = min(rows - 1, (item_column + 16 * NT - 1) / group);  // the last row that any column sees
+        int step = step0;
+        if (step < history_steps) step += (history_steps - step + kWaves - 1) / kWaves * kWaves;
+        for (; step < end; step += kWaves) {
             const int base = 32 * (step - history_steps);
             if (base > most) break;
-            float s[NT][2][4];
+            F32x4 dot[NT][2];
             U32x4 v[2][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                F32x4 dot[NT];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) dot[t] = F32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < NT; ++t) dot[t][u] = F32x4{0.f, 0.f, 0.f, 0.f};
                 const uint16_t* k = p.key + (int64_t)(first + min(base + 16 * u + i, rows - 1)) * p.key_stride + (int64_t)head * D;
 #pragma unroll
                 for (int m = 0; m < kSteps; ++m) {
                     const U32x2 a = *reinterpret_cast<const U32x2*>(k + k_channel(m));
                     const U32x2 b = *reinterpret_cast<const U32x2*>(k + k_channel(m) + 4);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) dot[t] = mfma(U32x4{a[0], a[1], b[0], b[1]}, query[t][m], dot[t]);
+                    for (int t = 0; t < NT; ++t) dot[t][u] = mfma(U32x4{a[0], a[1], b[0], b[1]}, query[t][m], dot[t][u]);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int token = base + 16 * u + 4 * g + r;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) s[t][u][r] = token <= seen[t] ? dot[t][r] * to_log2 : -__builtin_inff();
+                    for (int t = 0; t < NT; ++t) dot[t][u][r] = token <= seen[t] ? dot[t][u][r] : -__builtin_inff();
                     const uint16_t* row = p.value + (int64_t)(first + min(token, rows - 1)) * p.value_stride +
                                           (int64_t)head * D + (8 * i < D ? 8 * i : 0);
                     const U32x2 a = *reinterpret_cast<const U32x2*>(row), b = *reinterpret_cast<const U32x2*>(row + 4);
@@ -545,9 +584,9 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
                 }
             }
             float weight[NT][2][4];
-            U32x4 upper[NT], lower[NT];
-            const float one[2] = {1.f, 1.f};
-            fp8_softmax<NT>(columns, s, one, weight, upper, lower);
+            U32x4 upper[NT][1], lower[NT][1];
+            const float key_scale[2] = {to_log2, to_log2}, value_scale[2] = {1.f, 1.f};
+            fp8_softmax<NT, 8, 2>(columns, dot, key_scale, value_scale, weight, upper, lower);
             // Infinities and NaN, which a weight of zero does not remove, are added apart.
             bool odd_values = false;
 #pragma unroll
@@ -579,8 +618,8 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
                                  __builtin_amdgcn_perm(v[1][3][e >> 1], v[1][2][e >> 1], pick)};
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    columns.out[t][e] = mfma(a, upper[t], columns.out[t][e]);
-                    columns.out[t][e] = mfma(a, lower[t], columns.out[t][e]);
+                    columns.out[t][e] = mfma(a, upper[t][0], columns.out[t][e]);
+                    columns.out[t][e] = mfma(a, lower[t][0], columns.out[t][e]);
                 }
             }
             if (any_odd) {
@@ -642,77 +681,409 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         }
     };
     if (splits > 1 && tid == 0) tag_arrivals(arrivals, p.call_tag, arrivals_seen);
-    if constexpr (Rows) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int column = column0 + 16 * t + i;
+    for (int t = 0; t < NT; ++t) {
+        if (t > 0) __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float o[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = columns.out[t][e][r];
-                const int channel = 32 * g + 8 * r;
-                if (column < columns_in && channel < D) emit(column, channel, o, columns.high[t], columns.sum[t]);
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int channel = 32 * g + 8 * r;
+            if (channel >= D) continue;
+            float* to = &merged[wave][i][channel];
+            *reinterpret_cast<F32x4*>(to) = F32x4{columns.out[t][0][r], columns.out[t][1][r], columns.out[t][2][r], columns.out[t][3][r]};
+            *reinterpret_cast<F32x4*>(to + 4) = F32x4{columns.out[t][4][r], columns.out[t][5][r], columns.out[t][6][r], columns.out[t][7][r]};
         }
-    } else {
+        if (g == 0) {
+            merged[wave][i][D] = columns.high[t];
+            merged[wave][i][D + 1] = columns.sum[t];
+        }
+        __syncthreads();
+        const int local = tid >> 4, channel = 8 * (tid & 15), column = item_column + 16 * t + local;
+        if (column < columns_in && channel < D) {
+            float high = kLowest;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (t > 0) __syncthreads();
+            for (int w = 0; w < kWaves; ++w) high = fmaxf(high, merged[w][local][D]);
+            float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int channel = 32 * g + 8 * r;
-                if (channel >= D) continue;
-                float* to = &merged[wave][i][channel];
-                *reinterpret_cast<F32x4*>(to) = F32x4{columns.out[t][0][r], columns.out[t][1][r], columns.out[t][2][r], columns.out[t][3][r]};
-                *reinterpret_cast<F32x4*>(to + 4) = F32x4{columns.out[t][4][r], columns.out[t][5][r], columns.out[t][6][r], columns.out[t][7][r]};
+            for (int w = 0; w < kWaves; ++w) {
+                const float m = merged[w][local][D];
+                const float keep = m == high ? 1.0f : __builtin_amdgcn_exp2f(m - high);
+                sum += merged[w][local][D + 1] * keep;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] += merged[w][local][channel + e] * keep;
             }
-            if (g == 0) {
-                merged[wave][i][D] = columns.high[t];
-                merged[wave][i][D + 1] = columns.sum[t];
-            }
-            __syncthreads();
-            const int local = tid >> 4, channel = 8 * (tid & 15), column = item_column + 16 * t + local;
-            if (column < columns_in && channel < D) {
-                float high = kLowest;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) high = fmaxf(high, merged[w][local][D]);
-                float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float m = merged[w][local][D];
-                    const float keep = m == high ? 1.0f : __builtin_amdgcn_exp2f(m - high);
-                    sum += merged[w][local][D + 1] * keep;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] += merged[w][local][channel + e] * keep;
-                }
-                emit(column, channel, o, high, sum);
-            }
+            emit(column, channel, o, high, sum);
         }
     }
     if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
-    // The last split of the item to finish joins them, in their order.
-    for (int c = tid >> 4; c < kTile; c += 16) {
-        const int column = item_column + c, channel = 8 * (tid & 15);
-        if (column >= columns_in || channel >= D) continue;
-        const uint32_t at = (uint32_t)(column * splits) * kEntry * 4;
-        float high = kLowest;
-        for (int k = 0; k < splits; ++k) high = fmaxf(high, handoff_load2(handoff, at + (uint32_t)k * kEntry * 4).x);
-        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-        for (int k = 0; k < splits; ++k) {
-            const uint32_t part = at + (uint32_t)k * kEntry * 4;
-            const float2 stats = handoff_load2(handoff, part);
-            const float4 a = handoff_load4(handoff, part + 16 + 4 * channel), b = handoff_load4(handoff, part + 32 + 4 * channel);
-            const float keep = stats.x == high ? 1.0f : __builtin_amdgcn_exp2f(stats.x - high);
-            sum += stats.y * keep;
-            o[0] += a.x * keep, o[1] += a.y * keep, o[2] += a.z * keep, o[3] += a.w * keep;
-            o[4] += b.x * keep, o[5] += b.y * keep, o[6] += b.z * keep, o[7] += b.w * keep;
+    fp8_join<D, kStreamThreads, kTile>(handoff, item_column, columns_in, splits, output_row);
+}
+
+// ------------------------------------------------------------------ many columns
+//
+// The same products for requests of many columns: kWideWaves waves of 16 NT
+// columns share tiles of 64 tokens, which they convert to BF16 once, into LDS:
+// K as it is read ([token][channel]), V transposed ([channel][token], the tokens
+// in the order in which the second product's k slots stand for them).  Rows of
+// 256 and 128 bytes; the 16-byte chunks of a row are permuted by its number so
+// that the 16 rows an operand read touches lie in different banks.  A tile's
+// global loads are issued a tile ahead and converted into the other buffer
+// after the products of the present one: one barrier per tile.
+
+constexpr int kWideTokens = 64;
+
+// Distinct for channels c..c + 7 (an operand read) and for every fourth (the transposing writes).
+__device__ __forceinline__ int v_swizzle(int channel) { return (channel ^ (channel >> 2)) & 7; }
+
+template <int D>
+struct WideTile {
+    U32x4 k[kWideTokens][16];  // [token][chunk of 8 channels, chunk ^ (token % 16)]
+    U32x4 v[D][8];             // [channel][chunk of 8 tokens, chunk ^ v_swizzle(channel)]
+    float key_scale[4], value_scale[4];  // of the tile's units of 16 tokens
+    int valid[4];              // tokens of the unit that count (0 to 16)
+    int odd;                   // the number of the last tile of new rows with infinities or NaN among its values
+};
+
+template <int D, int NT, int Waves>
+__global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp8AttentionParams p) {
+    constexpr int kThreads = 64 * Waves, kTile = 16 * NT * Waves, kSteps = D / 32, kOut = D / 16, kEntry = D + 4;
+    constexpr int kPasses = 512 / kThreads;       // 128 threads fill a unit at a time
+    constexpr int kChunks = D / 16;               // 16-byte chunks of a row of codes
+    static_assert(kPasses * kThreads == 512, "units are filled by whole waves");
+    __shared__ WideTile<D> tiles[2];
+    __shared__ int last_flag;
+    const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
+    const int request = __builtin_amdgcn_readfirstlane(item.request);
+    if (request < 0) return;  // uniform over the workgroup, before any barrier
+    const int group = p.heads / p.kv_heads;
+    const int first = __builtin_amdgcn_readfirstlane(item.first), columns_in = __builtin_amdgcn_readfirstlane(item.rows);
+    const int rows = columns_in / group;
+    const int history = __builtin_amdgcn_readfirstlane(item.tokens);
+    const int splits = __builtin_amdgcn_readfirstlane(item.splits), split = __builtin_amdgcn_readfirstlane(item.split);
+    // The split's steps of 32 tokens: of the history, then of the new rows that the tile's columns see.
+    const int begin = split_begin(__builtin_amdgcn_readfirstlane(item.length), split, splits);
+    const int end = split_begin(__builtin_amdgcn_readfirstlane(item.length), split + 1, splits);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int item_column = __builtin_amdgcn_readfirstlane(item.index) * kTile;
+    const int column0 = item_column + wave * 16 * NT;
+    const int history_steps = fp8_steps(history);
+    const int old_end = min(end, history_steps);
+    const int old_tokens = min(history, 32 * old_end);                   // of the history, tokens below this
+    const int old_tiles = old_end > begin ? (old_end - begin + 1) / 2 : 0;
+    const int seen_rows = min(rows, (item_column + kTile - 1) / group + 1);  // new rows that any column sees
+    const int new_begin = 32 * (max(begin, history_steps) - history_steps);
+    const int new_end = min(32 * (end - history_steps), seen_rows);
+    const int new_tiles = new_end > new_begin ? (new_end - new_begin + kWideTokens - 1) / kWideTokens : 0;
+    const int all_tiles = old_tiles + new_tiles;
+
+    float* const entries = p.partials + ((int64_t)head * p.entries + __builtin_amdgcn_readfirstlane(item.entry)) * kEntry;
+    uint64_t* const arrivals = reinterpret_cast<uint64_t*>(entries + (int64_t)item_column * splits * kEntry + 2);
+    const uint64_t arrivals_seen = splits > 1 ? peek_arrivals(arrivals) : 0;
+
+    U32x4 query[NT][kSteps];
+    int seen[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int column = column0 + 16 * t + i;
+        seen[t] = column < columns_in ? column / group : -1;
+        const int row = column < columns_in ? column / group : 0;
+        const uint16_t* q = p.query + (int64_t)(first + row) * p.query_stride +
+                            ((int64_t)head * group + (column < columns_in ? column % group : 0)) * D;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const U32x4 a = *reinterpret_cast<const U32x4At8*>(q + 32 * s + 8 * g);
+            query[t][s] = column < columns_in ? a : U32x4{0u, 0u, 0u, 0u};
         }
-        const float scale = 1.0f / sum;
-        uint16_t* out = output_row(column) + channel;
-        *reinterpret_cast<U32x2*>(out) = U32x2{bf16x2_rn(o[0] * scale, o[1] * scale), bf16x2_rn(o[2] * scale, o[3] * scale)};
-        *reinterpret_cast<U32x2*>(out + 4) = U32x2{bf16x2_rn(o[4] * scale, o[5] * scale), bf16x2_rn(o[6] * scale, o[7] * scale)};
     }
+    Fp8Columns<NT, kOut> columns;  // tile e: channels 16 e + 4 g + r
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        columns.high[t] = kLowest;
+        columns.sum[t] = 0.f;
+#pragma unroll
+        for (int e = 0; e < kOut; ++e) columns.out[t][e] = F32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float to_log2 = p.softmax_scale * 1.44269504088896341f;
+    const int page_shift = p.page_tokens == 16 ? 4 : 5;
+    const int64_t plane_bytes = ((p.num_blocks * p.kv_heads) << page_shift) * D;
+
+    // ---------------------------------------------------------------- fill
+    // Thread `place` of a unit's 128: chunk place % kChunks of K token
+    // place / kChunks; channels 4 (place % (D / 4)).. of V tokens
+    // 4 (place / (D / 4))..  (D = 96: 96 of the 128.)
+    const bool filler = (tid & 127) < 16 * kChunks;
+    const int place = filler ? tid & 127 : 0;
+    const int k_token = place / kChunks, k_chunk = place % kChunks;
+    const int v_quad = place / (D / 4), v_word = place % (D / 4);
+    // What a thread holds of a tile of the history in flight.  (Tiles of new rows are few: they are
+    // loaded where they are stored.)
+    struct Stage {
+        U32x4 k[kPasses];
+        uint32_t v[kPasses][4];
+        float key_scale[kPasses], value_scale[kPasses];
+    };
+    // (Not made uniform: a scalar load in flight would hold back every LDS wait.)
+    auto unit_of = [&](int pass) { return (tid + pass * kThreads) >> 7; };
+    auto block_of = [&](int tile, int pass) {  // -1: no tokens of the unit, or no block
+        const int token = 32 * begin + kWideTokens * tile + 16 * unit_of(pass);
+        if (token >= old_tokens) return -1;
+        const int block = p.block_table[(int64_t)request * p.block_table_stride + (token >> page_shift)];
+        return block >= 0 && block < p.num_blocks ? block : -1;
+    };
+    int next_block[kPasses], stage_block[kPasses];
+    auto fetch = [&](Stage& x, int tile) {
+        if (tile >= old_tiles) return;
+#pragma unroll
+        for (int pass = 0; pass < kPasses; ++pass) {
+            const int block = next_block[pass];
+            const int token = 32 * begin + kWideTokens * tile + 16 * unit_of(pass);
+            const int64_t index = (int64_t)max(block, 0) * p.kv_heads + head;
+            x.key_scale[pass] = x.value_scale[pass] = 1.f;
+            if (block >= 0) {
+                x.key_scale[pass] = p.scales[index];
+                x.value_scale[pass] = p.scales[index + p.num_blocks * p.kv_heads];
+            }
+            // (Without a block: the first one's bytes, of which no token counts.)
+            const uint8_t* unit = p.cache + ((index << page_shift) + (token & (p.page_tokens - 1))) * D;
+            x.k[pass] = *reinterpret_cast<const U32x4*>(unit + k_token * D + 16 * k_chunk);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                x.v[pass][r] = *reinterpret_cast<const uint32_t*>(unit + plane_bytes + (4 * v_quad + r) * D + 4 * v_word);
+            stage_block[pass] = block;
+            next_block[pass] = block_of(tile + 1, pass);
+        }
+    };
+    auto v_place = [&](WideTile<D>& tile, int channel, int unit, int quad) -> U32x2* {
+        const int chunk = 4 * (unit >> 1) + quad;
+        return reinterpret_cast<U32x2*>(&tile.v[channel][chunk ^ v_swizzle(channel)]) + (unit & 1);
+    };
+    auto store = [&](const Stage& x, int number) {
+        WideTile<D>& tile = tiles[number & 1];
+        bool odd = false;
+#pragma unroll
+        for (int pass = 0; pass < kPasses; ++pass) {
+            const int unit = unit_of(pass), token = 16 * unit + k_token;
+            if (number < old_tiles) {
+                const int valid = stage_block[pass] >= 0 ? min(old_tokens - 32 * begin - kWideTokens * number - 16 * unit, 16) : 0;
+                if (filler) {
+                    const U32x4 k = x.k[pass];
+                    tile.k[token][(2 * k_chunk) ^ k_token] =
+                        U32x4{bf16x2_of_fp8<false>(k[0]), bf16x2_of_fp8<true>(k[0]), bf16x2_of_fp8<false>(k[1]), bf16x2_of_fp8<true>(k[1])};
+                    tile.k[token][(2 * k_chunk + 1) ^ k_token] =
+                        U32x4{bf16x2_of_fp8<false>(k[2]), bf16x2_of_fp8<true>(k[2]), bf16x2_of_fp8<false>(k[3]), bf16x2_of_fp8<true>(k[3])};
+                    // Slots past the history may hold NaN, which a weight of zero does not remove.
+                    uint32_t w[4], y[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[r] = 4 * v_quad + r < valid ? x.v[pass][r] : 0u;
+                    transpose_bytes(w, y);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        *v_place(tile, 4 * v_word + c, unit, v_quad) = U32x2{bf16x2_of_fp8<false>(y[c]), bf16x2_of_fp8<true>(y[c])};
+                }
+                if ((tid & 127) == 0) {
+                    tile.key_scale[unit] = x.key_scale[pass] * to_log2;
+                    tile.value_scale[unit] = x.value_scale[pass];
+                    tile.valid[unit] = valid;
+                }
+                continue;
+            }
+            // New rows (clamped to the request's; what lies past them is masked).
+            const int base = new_begin + kWideTokens * (number - old_tiles) + 16 * unit;
+            if (filler) {
+                const uint16_t* k = p.key + (int64_t)(first + min(base + k_token, rows - 1)) * p.key_stride + (int64_t)head * D + 16 * k_chunk;
+                tile.k[token][(2 * k_chunk) ^ k_token] = *reinterpret_cast<const U32x4At8*>(k);
+                tile.k[token][(2 * k_chunk + 1) ^ k_token] = *reinterpret_cast<const U32x4At8*>(k + 8);
+                // Infinities and NaN, which a weight of zero does not remove, are left out here and added apart.
+                U32x2 w[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    w[r] = *reinterpret_cast<const U32x2*>(
+                        p.value + (int64_t)(first + min(base + 4 * v_quad + r, rows - 1)) * p.value_stride + (int64_t)head * D + 4 * v_word);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t v = w[r][h];
+                        odd |= not_finite_bf16x2(v);
+                        if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
+                        if ((v & 0x7f800000u) == 0x7f800000u) v &= 0x0000ffffu;
+                        w[r][h] = v;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t pick = c & 1 ? 0x07060302u : 0x05040100u;
+                    *v_place(tile, 4 * v_word + c, unit, v_quad) =
+                        U32x2{__builtin_amdgcn_perm(w[1][c >> 1], w[0][c >> 1], pick), __builtin_amdgcn_perm(w[3][c >> 1], w[2][c >> 1], pick)};
+                }
+            }
+            if ((tid & 127) == 0) {
+                tile.key_scale[unit] = to_log2;
+                tile.value_scale[unit] = 1.f;
+                tile.valid[unit] = 16;
+            }
+        }
+        if (odd) tile.odd = number;
+    };
+
+    // ---------------------------------------------------------------- products
+    const bool idle = column0 >= columns_in;
+    // The last new row of the split that the wave's columns see.
+    const int new_last = min(new_end - 1, (column0 + 16 * NT - 1) / group);
+    // (base: the tile's first new row, or -1 for the history.)
+    auto compute = [&](int number) {
+        WideTile<D>& tile = tiles[number & 1];
+        const int base = number < old_tiles ? -1 : new_begin + kWideTokens * (number - old_tiles);
+        if (base >= 0 && base > new_last) return;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            if (base >= 0 && base + 32 * st > new_last) break;
+            float key_scale[2], value_scale[2];
+            int valid[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                key_scale[u] = tile.key_scale[2 * st + u];
+                value_scale[u] = tile.value_scale[2 * st + u];
+                valid[u] = tile.valid[2 * st + u];
+            }
+            F32x4 dot[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) dot[t][u] = F32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                U32x4 a[kSteps];
+#pragma unroll
+                for (int m = 0; m < kSteps; ++m) a[m] = tile.k[32 * st + 16 * u + i][(4 * m + g) ^ i];
+#pragma unroll
+                for (int m = 0; m < kSteps; ++m)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) dot[t][u] = mfma(a[m], query[t][m], dot[t][u]);
+            }
+            // V's operands arrive while the weights are computed.
+            __builtin_amdgcn_sched_barrier(0);
+            U32x4 operand[kOut];
+#pragma unroll
+            for (int e = 0; e < kOut; ++e) operand[e] = tile.v[16 * e + i][(4 * st + g) ^ v_swizzle(16 * e + i)];
+            __builtin_amdgcn_sched_barrier(0);
+            if (base < 0) {
+                if (__builtin_amdgcn_readfirstlane(valid[0] & valid[1]) != 16) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                dot[t][u][r] = 4 * g + r < valid[u] ? dot[t][u][r] : -__builtin_inff();
+                }
+            } else if (base + 32 * st + 31 > column0 / group || base + 32 * st + 31 >= new_end) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            dot[t][u][r] = base + 32 * st + 16 * u + 4 * g + r <= min(seen[t], new_end - 1) ? dot[t][u][r] : -__builtin_inff();
+            }
+            float weight[NT][2][4];
+            U32x4 upper[NT][1], lower[NT][1];
+            fp8_softmax<NT, kOut, 2>(columns, dot, key_scale, value_scale, weight, upper, lower);
+#pragma unroll
+            for (int e = 0; e < kOut; ++e)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) columns.out[t][e] = mfma(operand[e], upper[t][0], columns.out[t][e]);
+#pragma unroll
+            for (int e = 0; e < kOut; ++e)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) columns.out[t][e] = mfma(operand[e], lower[t][0], columns.out[t][e]);
+            if (base >= 0 && tile.odd == number) {
+                // Infinities and NaN among the new values, for the columns that see them.
+                for (int j = 0; j < 32; ++j) {
+                    const int token = base + 32 * st + j;
+                    if (token >= new_end) break;
+                    const uint16_t* row = p.value + (int64_t)(first + token) * p.value_stride + (int64_t)head * D;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        // The weight (both its parts) of token j.
+                        uint32_t up = 0, low = 0;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                if (16 * u + 2 * x == (j & 18)) up = upper[t][0][2 * u + x], low = lower[t][0][2 * u + x];
+                        if ((j & 1) == 0) up <<= 16, low <<= 16;
+                        const float mine = __uint_as_float(up & 0xffff0000u) + __uint_as_float(low & 0xffff0000u);
+                        const float w = __shfl(mine, i + 16 * ((j >> 2) & 3));
+                        if (token > seen[t]) continue;
+#pragma unroll
+                        for (int e = 0; e < kOut; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float x = bf16_f32(row[16 * e + 4 * g + r]);
+                                if (!(fabsf(x) < __builtin_inff())) columns.out[t][e][r] += w * x;
+                            }
+                    }
+                }
+            }
+        }
+    };
+
+    Stage stage;
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) next_block[pass] = block_of(0, pass);
+    if (tid < 2) tiles[tid].odd = -1;
+    __syncthreads();
+    if (all_tiles > 0) {
+        fetch(stage, 0);
+        store(stage, 0);
+        if (all_tiles > 1) fetch(stage, 1);
+    }
+    for (int n = 0; n < all_tiles; ++n) {
+        __syncthreads();
+        if (!idle) compute(n);
+        if (n + 1 < all_tiles) store(stage, n + 1);
+        if (n + 2 < all_tiles) fetch(stage, n + 2);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        columns.sum[t] += __shfl_xor(columns.sum[t], 16);
+        columns.sum[t] += __shfl_xor(columns.sum[t], 32);
+    }
+
+    // ---------------------------------------------------------------- finish
+    const __amdgpu_buffer_rsrc_t handoff = handoff_resource(entries, (uint32_t)min((int64_t)columns_in * splits * kEntry * 4, (int64_t)0xfffffffc));
+    auto output_row = [&](int column) {
+        return p.output + (int64_t)(first + column / group) * p.output_stride + ((int64_t)head * group + column % group) * D;
+    };
+    if (splits > 1 && tid == 0) tag_arrivals(arrivals, p.call_tag, arrivals_seen);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int column = column0 + 16 * t + i;
+        if (column >= columns_in) continue;
+        if (splits == 1) {
+            const float scale = 1.0f / columns.sum[t];
+            uint16_t* out = output_row(column) + 4 * g;
+#pragma unroll
+            for (int e = 0; e < kOut; ++e) {
+                const F32x4 o = columns.out[t][e] * scale;
+                *reinterpret_cast<U32x2*>(out + 16 * e) = U32x2{bf16x2_rn(o[0], o[1]), bf16x2_rn(o[2], o[3])};
+            }
+            continue;
+        }
+        const uint32_t at = (uint32_t)(column * splits + split) * kEntry * 4;
+#pragma unroll
+        for (int e = 0; e < kOut; ++e) {
+            const F32x4 o = columns.out[t][e];
+            handoff_store4(handoff, at + 16 + 4 * (16 * e + 4 * g), o[0], o[1], o[2], o[3]);
+        }
+        if (g == 0) {
+            handoff_store(handoff, at, columns.high[t]);
+            handoff_store(handoff, at + 4, columns.sum[t]);
+        }
+    }
+    if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
+    fp8_join<D, kThreads, kTile>(handoff, item_column, columns_in, splits, output_row);
 }
 
 }  // namespace
@@ -739,11 +1110,11 @@ void launch_attention(const Fp8AttentionParams& p, hipStream_t stream) {
     const int64_t items = p.items > 0 ? p.items : (columns / p.tile + p.requests) * p.splits;
     const dim3 grid((unsigned)(items * p.kv_heads)), threads(kStreamThreads);
     if (p.tile == 16)
-        hipLaunchKernelGGL((attention_fp8_kernel<D, 1, false>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((attention_fp8_kernel<D, 1>), grid, threads, 0, stream, p);
     else if (p.tile == 32)
-        hipLaunchKernelGGL((attention_fp8_kernel<D, 2, false>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((attention_fp8_kernel<D, 2>), grid, threads, 0, stream, p);
     else
-        hipLaunchKernelGGL((attention_fp8_kernel<D, 2, true>), grid, threads, 0, stream, p);
+        hipLaunchKernelGGL((attention_fp8_wide_kernel<D, 2, 8>), grid, dim3(512), 0, stream, p);
 }
 
 }  // namespace

@@ -73,6 +73,10 @@ ATTENTION = [
     ([257], [130], 2, 2, 128, 16),
     ([2050], [1], 16, 1, 128, 32),
     ([5], [300], 1, 1, 96, 16),
+    ([1500], [100], 2, 2, 128, 16),
+    ([2500, 70], [64, 130], 2, 1, 96, 32),
+    ([1300, 1200], [40, 25], 1, 1, 128, 16),
+    ([1700], [9], 4, 2, 96, 16),
 ]
 
 
