@@ -533,18 +533,18 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
             }
         }
     };
+    // (Loads without a condition, past the last step of that step again: after a
+    // load that one path leaves out, every wait would be for all loads in flight.)
     if (my_steps > 0) {
         Fp8Step<D> even, odd;
         look_up(0);
         load(even, 0);
         for (int n = 0; n < my_steps; n += 2) {
-            if (n + 1 < my_steps) load(odd, n + 1);
+            load(odd, min(n + 1, my_steps - 1));
             compute(even);
             if (n + 1 >= my_steps) break;
-            if (n + 2 < my_steps) {
-                if (((n + 2) & 31) == 0) look_up((n + 2) >> 5);
-                load(even, n + 2);
-            }
+            if (((n + 2) & 31) == 0) look_up((n + 2) >> 5);
+            load(even, min(n + 2, my_steps - 1));
             compute(odd);
         }
     }

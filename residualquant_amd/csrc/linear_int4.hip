@@ -130,50 +130,78 @@ __device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int 
     }
 }
 
+// y of every output in plain steps, for strides past what the buffer loads of x address.
+__global__ __launch_bounds__(256) void linear_int4_plain_kernel(const LinearInt4Params p) {
+    linear_int4_plain(p, blockIdx.x, 1, 256);
+}
+
 // One workgroup per NB tiles of 16 outputs, for all rows (T tiles of 16).  Its
 // W waves share the inputs out in blocks of 128.  With u = c + 8 and
 // v = 1 + u / 16 (codes_bf16), sum c x = 16 (sum v x - 1.5 sum x): the second
 // sum, from a constant operand, is the accumulator that the first starts with,
-// once per group for all tiles.
+// once per group for all tiles.  The next block's loads are in flight during a
+// block's products; x is read by buffer loads, which give 0 to lanes past its
+// rows without a branch per load.
 template <int Group, int T, int NB, int W>
 __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Params p) {
     constexpr int kPer = 128 / Group, kGroupSteps = Group / 32;
     __shared__ F32x4 partial[W][NB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int64_t blocks = int4_blocks(p.in_features), tiles = int4_tiles(p.out_features);
+    const int in_features = (int)p.in_features, blocks = (int)int4_blocks(p.in_features);
+    const int64_t tiles = int4_tiles(p.out_features);
     const int64_t tile0 = (int64_t)blockIdx.x * NB;
-    const int64_t begin = blocks * wave / W, end = blocks * (wave + 1) / W;
+    const int begin = blocks * wave / W, end = blocks * (wave + 1) / W;
     F32x4 total[NB][T];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int t = 0; t < T; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
-    struct Block {
+    // (The host takes other strides to linear_int4_plain_kernel.)
+    const uint32_t x_bytes = (uint32_t)((p.rows - 1) * p.x_stride + p.in_features) * 2;
+    const __amdgpu_buffer_rsrc_t x_rows = handoff_resource(p.x, x_bytes);
+    constexpr uint32_t kOutside = 0xfffffff0u;
+    uint32_t x_place[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) x_place[t] = 16 * t + i < p.rows ? (uint32_t)((16 * t + i) * p.x_stride + 8 * g) * 2 : kOutside;
+    struct Codes {
         U32x4 words[NB];
-        uint2 scales[NB][kPer];
+        uint32_t scales[NB][2 * kPer];
+    };
+    struct Inputs {
         U32x4 x[T][4];
     };
-    auto load = [&](Block& b, int64_t block) {
+    auto load_codes = [&](Codes& b, int block) {
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int64_t place = min(tile0 + j, tiles - 1) * blocks + block;
             b.words[j] = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(p.packed) + place * 64 + lane);
-            const uint2* scales = reinterpret_cast<const uint2*>(p.packed_scales) + (place * 4 + g) * kPer;
+            const uint32_t* scales = reinterpret_cast<const uint32_t*>(p.packed_scales) + place * (8 * kPer) + g * (2 * kPer);
+            if constexpr (kPer == 1) {
+                const uint2 v = *reinterpret_cast<const uint2*>(scales);
+                b.scales[j][0] = v.x, b.scales[j][1] = v.y;
+            } else {
 #pragma unroll
-            for (int h = 0; h < kPer; ++h) b.scales[j][h] = scales[h];
+                for (int h = 0; h < kPer / 2; ++h) {
+                    const U32x4 v = *reinterpret_cast<const U32x4*>(scales + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) b.scales[j][4 * h + e] = v[e];
+                }
+            }
         }
+    };
+    auto load_inputs = [&](Inputs& b, int block) {
+        const bool whole = 128 * block + 128 <= in_features;
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const int64_t k = 128 * block + 32 * s + 8 * g;
-                b.x[t][s] = U32x4{0u, 0u, 0u, 0u};
-                if (16 * t + i < p.rows && k < p.in_features)
-                    b.x[t][s] = *reinterpret_cast<const U32x4*>(p.x + (16 * t + i) * p.x_stride + k);
+                uint32_t place = x_place[t] + 64 * s;
+                if (16 * t + i >= p.rows || (!whole && 128 * block + 32 * s + 8 * g >= in_features)) place = kOutside;
+                b.x[t][s] = __builtin_amdgcn_raw_buffer_load_b128(x_rows, place, 256 * block, 0);
             }
     };
-    auto compute = [&](const Block& b) {
+    auto compute = [&](const Codes& b, const Inputs& in) {
         const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
@@ -182,7 +210,7 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
             for (int t = 0; t < T; ++t) {
                 start[t] = F32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < kGroupSteps; ++s) start[t] = mfma(shift, b.x[t][h * kGroupSteps + s], start[t]);
+                for (int s = 0; s < kGroupSteps; ++s) start[t] = mfma(shift, in.x[t][h * kGroupSteps + s], start[t]);
             }
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
@@ -193,11 +221,11 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
                 for (int s = 0; s < kGroupSteps; ++s) {
                     const U32x4 a = codes_bf16(b.words[j][h * kGroupSteps + s]);
 #pragma unroll
-                    for (int t = 0; t < T; ++t) sum[t] = mfma(a, b.x[t][h * kGroupSteps + s], sum[t]);
+                    for (int t = 0; t < T; ++t) sum[t] = mfma(a, in.x[t][h * kGroupSteps + s], sum[t]);
                 }
-                const uint2 raw = b.scales[j][h];
-                const float scale[4] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u),
-                                        __uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
+                const uint32_t low = b.scales[j][2 * h], high = b.scales[j][2 * h + 1];
+                const float scale[4] = {__uint_as_float(low << 16), __uint_as_float(low & 0xffff0000u),
+                                        __uint_as_float(high << 16), __uint_as_float(high & 0xffff0000u)};
 #pragma unroll
                 for (int t = 0; t < T; ++t)
 #pragma unroll
@@ -206,14 +234,22 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
         }
     };
     if (begin < end) {
-        Block even, odd;
-        load(even, begin);
-        for (int64_t b = begin; b < end; b += 2) {
-            if (b + 1 < end) load(odd, b + 1);
-            compute(even);
-            if (b + 1 >= end) break;
-            if (b + 2 < end) load(even, b + 2);
-            compute(odd);
+        Codes codes;
+        Inputs inputs;
+        load_codes(codes, begin);
+        load_inputs(inputs, begin);
+        // (Rolled: a wave runs two to six rounds, and code that runs once is fetched as it runs.)
+#pragma unroll 1
+        for (int b = begin; b < end; ++b) {
+            Codes next_codes = codes;
+            Inputs next_inputs = inputs;
+            if (b + 1 < end) {
+                load_codes(next_codes, b + 1);
+                load_inputs(next_inputs, b + 1);
+            }
+            compute(codes, inputs);
+            codes = next_codes;
+            inputs = next_inputs;
         }
     }
     bool finite = true;
@@ -284,7 +320,9 @@ hipError_t launch_unpack_int4(const Int4PackParams& p, uint16_t* weight, hipStre
 }
 
 hipError_t launch_linear_int4(const LinearInt4Params& p, hipStream_t stream) {
-    if (p.group == 32)
+    if (p.x_stride >= (1 << 24))  // 64 rows would pass the 2 GiB that the buffer loads of x address
+        hipLaunchKernelGGL(linear_int4_plain_kernel, dim3((unsigned)int4_tiles(p.out_features)), dim3(256), 0, stream, p);
+    else if (p.group == 32)
         launch_rows<32>(p, stream);
     else if (p.group == 64)
         launch_rows<64>(p, stream);
