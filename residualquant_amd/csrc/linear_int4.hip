@@ -7,6 +7,8 @@
 // e = 0..7 (code_shift), the A operand of v_mfma_f32_16x16x32 for 16 output
 // rows.  Rows and inputs past the weight hold code 0.  The scales follow (scale_place),
 // in the order in which the lanes of the product's result need them.
+#include <algorithm>
+
 #include "rq_device.h"
 #include "rq_reduced.h"
 
@@ -130,46 +132,46 @@ __device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int 
     }
 }
 
-// y of every output in plain steps, for strides past what the buffer loads of x address.
-__global__ __launch_bounds__(256) void linear_int4_plain_kernel(const LinearInt4Params p) {
-    linear_int4_plain(p, blockIdx.x, 1, 256);
+// One workgroup of eight waves per 8 / WK x NB tiles of 16 outputs, for all
+// rows (T tiles of 16).  x passes through LDS, in chunks of `chunk_blocks`
+// blocks of 128 inputs (all of them where they fit): rows of a large power of
+// two lie in one channel of the cache, so 16 rows read side by side by every
+// wave took most of the time (64 rows x 16 outputs x 2048 inputs, one
+// workgroup: 10.3 us, 8 of them for x).  WK waves share a tile's inputs out; a
+// wave keeps the codes of kAhead blocks in flight.
+//
+// With u = c + 8 and v = 1 + u / 16 (codes_bf16), sum c x = 16 (sum v x - 1.5
+// sum x): the second sum, from a constant operand, is the accumulator that the
+// first starts with, once per group for all tiles of a wave.
+typedef __attribute__((address_space(3))) void LdsVoid;
+
+// One DMA load: lane l's 16 bytes at `offset` of the resource go to lds + 16 l (lds wave-uniform).
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds, uint32_t offset) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsVoid*)lds, 16, offset, 0, 0, 0);
 }
 
-// One workgroup per NB tiles of 16 outputs, for all rows (T tiles of 16).  Its
-// W waves share the inputs out in blocks of 128.  With u = c + 8 and
-// v = 1 + u / 16 (codes_bf16), sum c x = 16 (sum v x - 1.5 sum x): the second
-// sum, from a constant operand, is the accumulator that the first starts with,
-// once per group for all tiles.  The next block's loads are in flight during a
-// block's products; x is read by buffer loads, which give 0 to lanes past its
-// rows without a branch per load.
-template <int Group, int T, int NB, int W>
-__global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Params p) {
-    constexpr int kPer = 128 / Group, kGroupSteps = Group / 32;
-    __shared__ F32x4 partial[W][NB][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+constexpr int kLinearInt4Threads = 512;
+constexpr int kRowPad = 16;  // bytes between the rows in LDS: operand reads of 16 rows meet different banks
+
+template <int Group, int T, int NB, int WK>
+__global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const LinearInt4Params p) {
+    constexpr int kPer = 128 / Group, kGroupSteps = Group / 32, kAhead = NB == 1 ? 4 : 2;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
+    const int part = wave % WK, rows = (int)p.rows;
     const int in_features = (int)p.in_features, blocks = (int)int4_blocks(p.in_features);
     const int64_t tiles = int4_tiles(p.out_features);
-    const int64_t tile0 = (int64_t)blockIdx.x * NB;
-    const int begin = blocks * wave / W, end = blocks * (wave + 1) / W;
+    const int64_t tile0 = ((int64_t)blockIdx.x * (8 / WK) + wave / WK) * NB;
+    const int row_bytes = (p.chunk_blocks + 3) / 4 * 1024 + kRowPad;
     F32x4 total[NB][T];
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
         for (int t = 0; t < T; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
-    // (The host takes other strides to linear_int4_plain_kernel.)
-    const uint32_t x_bytes = (uint32_t)((p.rows - 1) * p.x_stride + p.in_features) * 2;
-    const __amdgpu_buffer_rsrc_t x_rows = handoff_resource(p.x, x_bytes);
-    constexpr uint32_t kOutside = 0xfffffff0u;
-    uint32_t x_place[T];
-#pragma unroll
-    for (int t = 0; t < T; ++t) x_place[t] = 16 * t + i < p.rows ? (uint32_t)((16 * t + i) * p.x_stride + 8 * g) * 2 : kOutside;
     struct Codes {
         U32x4 words[NB];
         uint32_t scales[NB][2 * kPer];
-    };
-    struct Inputs {
-        U32x4 x[T][4];
     };
     auto load_codes = [&](Codes& b, int block) {
 #pragma unroll
@@ -190,18 +192,16 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
             }
         }
     };
-    auto load_inputs = [&](Inputs& b, int block) {
-        const bool whole = 128 * block + 128 <= in_features;
+    // Rows past the last read the last again; their outputs are not stored.
+    const uint8_t* x_row[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) x_row[t] = lds + min(16 * t + i, rows - 1) * row_bytes + 16 * g;
+    auto compute = [&](const Codes& b, int block) {
+        U32x4 x[T][4];
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint32_t place = x_place[t] + 64 * s;
-                if (16 * t + i >= p.rows || (!whole && 128 * block + 32 * s + 8 * g >= in_features)) place = kOutside;
-                b.x[t][s] = __builtin_amdgcn_raw_buffer_load_b128(x_rows, place, 256 * block, 0);
-            }
-    };
-    auto compute = [&](const Codes& b, const Inputs& in) {
+            for (int s = 0; s < 4; ++s) x[t][s] = *reinterpret_cast<const U32x4*>(x_row[t] + 256 * block + 64 * s);
         const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
             for (int t = 0; t < T; ++t) {
                 start[t] = F32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < kGroupSteps; ++s) start[t] = mfma(shift, in.x[t][h * kGroupSteps + s], start[t]);
+                for (int s = 0; s < kGroupSteps; ++s) start[t] = mfma(shift, x[t][h * kGroupSteps + s], start[t]);
             }
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
                 for (int s = 0; s < kGroupSteps; ++s) {
                     const U32x4 a = codes_bf16(b.words[j][h * kGroupSteps + s]);
 #pragma unroll
-                    for (int t = 0; t < T; ++t) sum[t] = mfma(a, in.x[t][h * kGroupSteps + s], sum[t]);
+                    for (int t = 0; t < T; ++t) sum[t] = mfma(a, x[t][h * kGroupSteps + s], sum[t]);
                 }
                 const uint32_t low = b.scales[j][2 * h], high = b.scales[j][2 * h + 1];
                 const float scale[4] = {__uint_as_float(low << 16), __uint_as_float(low & 0xffff0000u),
@@ -233,58 +233,212 @@ __global__ __launch_bounds__(64 * W) void linear_int4_kernel(const LinearInt4Par
             }
         }
     };
-    if (begin < end) {
-        Codes codes;
-        Inputs inputs;
-        load_codes(codes, begin);
-        load_inputs(inputs, begin);
-        // (Rolled: a wave runs two to six rounds, and code that runs once is fetched as it runs.)
-#pragma unroll 1
-        for (int b = begin; b < end; ++b) {
-            Codes next_codes = codes;
-            Inputs next_inputs = inputs;
-            if (b + 1 < end) {
-                load_codes(next_codes, b + 1);
-                load_inputs(next_inputs, b + 1);
+    // (The host sends larger x to linear_int4_plain_kernel.)
+    const int copy_rows = rows > 4 ? 8 : rows > 2 ? 4 : rows;  // rows that the waves copy at a time
+    const __amdgpu_buffer_rsrc_t x_all = handoff_resource(p.x, (uint32_t)(((p.rows - 1) * p.x_stride + p.in_features) * 2));
+    for (int first = 0; first < blocks; first += p.chunk_blocks) {
+        const int count = min(p.chunk_blocks, blocks - first);
+        const int begin = first + count * part / WK, end = first + count * (part + 1) / WK;
+        // (Loads without a condition, past the end of the last block again: after a
+        // load that one path leaves out, every wait is for all loads in flight.)
+        Codes codes[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) load_codes(codes[a], min(begin + a, blocks - 1));
+        if (first > 0) __syncthreads();
+        // 1 KB of a row per DMA load, all in flight; zeros past the inputs.
+        const int pieces = (count + 3) / 4;
+        for (int r = wave & (copy_rows - 1); r < rows; r += copy_rows) {
+            const uint32_t row = (uint32_t)(r * p.x_stride + 128 * first) * 2;
+            uint8_t* to = lds + r * row_bytes;
+            for (int c = wave / copy_rows; c < pieces; c += 8 / copy_rows) {
+                const int at = 512 * c + 8 * lane;  // of the chunk
+                load_to_lds(x_all, to + 1024 * c, 128 * first + at < in_features ? row + 2 * at : 0xfffffff0u);
             }
-            compute(codes, inputs);
-            codes = next_codes;
-            inputs = next_inputs;
         }
-    }
-    bool finite = true;
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-        if (t > 0) __syncthreads();
-#pragma unroll
-        for (int j = 0; j < NB; ++j) partial[wave][j][lane] = total[j][t];
+        wait_vector_memory();
         __syncthreads();
-        const int j = wave;
-        if (j < NB) {
-            F32x4 sum = partial[0][j][lane];
+        for (int b = begin; b < end; b += kAhead) {
 #pragma unroll
-            for (int w = 1; w < W; ++w) sum += partial[w][j][lane];
-            const int64_t n = 16 * (tile0 + j) + 4 * g, m = 16 * t + i;
-            if (m < p.rows) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (n + r >= p.out_features) break;
-                    finite = finite && fabsf(sum[r]) < __builtin_inff();
-                    p.y[m * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * sum[r]);
-                }
+            for (int a = 0; a < kAhead; ++a) {
+                if (b + a < end) compute(codes[a], b + a - first);
+                load_codes(codes[a], min(b + a + kAhead, blocks - 1));
             }
         }
     }
-    if (__syncthreads_or(!finite)) linear_int4_plain(p, tile0, (int)min((int64_t)NB, tiles - tile0), 64 * W);
+
+    // ---------------------------------------------------------------- join
+    bool finite = true;
+    auto write = [&](F32x4 sum, int64_t tile, int t) {
+        const int64_t n = 16 * tile + 4 * g, m = 16 * t + i;
+        if (m >= p.rows) return;
+        if (p.aligned && n + 4 <= p.out_features) {
+            finite = finite && fabsf(sum[0]) < __builtin_inff() && fabsf(sum[1]) < __builtin_inff() &&
+                     fabsf(sum[2]) < __builtin_inff() && fabsf(sum[3]) < __builtin_inff();
+            *reinterpret_cast<uint2*>(p.y + m * p.y_stride + n) =
+                make_uint2(bf16x2_rn(16.0f * sum[0], 16.0f * sum[1]), bf16x2_rn(16.0f * sum[2], 16.0f * sum[3]));
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (n + r >= p.out_features) break;
+            finite = finite && fabsf(sum[r]) < __builtin_inff();
+            p.y[m * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * sum[r]);
+        }
+    };
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int t = 0; t < T; ++t) write(total[j][t], tile0 + j, t);
+    } else {
+        F32x4(*const partial)[NB * T][64] = reinterpret_cast<F32x4(*)[NB * T][64]>(lds);  // [wave][output][lane]
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int t = 0; t < T; ++t) partial[wave][j * T + t][lane] = total[j][t];
+        __syncthreads();
+        // The waves of a group of tiles share its outputs out.
+        for (int q = part; q < NB * T; q += WK) {
+            F32x4 sum = partial[wave - part][q][lane];
+#pragma unroll
+            for (int w = 1; w < WK; ++w) sum += partial[wave - part + w][q][lane];
+            write(sum, tile0 + q / T, q % T);
+        }
+    }
+    const int64_t workgroup_tile = (int64_t)blockIdx.x * (8 / WK) * NB;
+    if (__syncthreads_or(!finite))
+        linear_int4_plain(p, workgroup_tile, (int)min((int64_t)(8 / WK) * NB, tiles - workgroup_tile), kLinearInt4Threads);
+}
+
+// One workgroup of W waves per tile of 16 outputs, for up to 16 rows: x goes from
+// global memory to the operands without LDS, which saves few rows a copy and a
+// barrier.  All of a wave's blocks, at most kBlocks, are in flight at once;
+// past its last one a wave reads that block again, with scales of 0 (a branch
+// around it would let the compiler move its loads behind the first block's products).
+template <int Group, int kBlocks, int W>
+__global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt4Params p) {
+    constexpr int kPer = 128 / Group, kGroupSteps = Group / 32;
+    __shared__ F32x4 partial[W][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int in_features = (int)p.in_features, blocks = (int)int4_blocks(p.in_features);
+    const int64_t tile = blockIdx.x;
+    const int begin = blocks * wave / W, end = blocks * (wave + 1) / W;
+    const uint16_t* x_row = p.x + min(i, (int)p.rows - 1) * p.x_stride + 8 * g;
+    U32x4 words[kBlocks], x[kBlocks][4];
+    uint32_t scales[kBlocks][2 * kPer];
+#pragma unroll
+    for (int a = 0; a < kBlocks; ++a) {
+        const int block = min(min(begin + a, end - 1), blocks - 1);
+        const int64_t place = tile * blocks + max(block, 0);
+        words[a] = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(p.packed) + place * 64 + lane);
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(p.packed_scales) + place * (8 * kPer) + g * (2 * kPer);
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) {
+            const uint2 v = reinterpret_cast<const uint2*>(from)[h];
+            scales[a][2 * h] = begin + a < end ? v.x : 0u;
+            scales[a][2 * h + 1] = begin + a < end ? v.y : 0u;
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int k = 128 * max(block, 0) + 32 * s;
+            x[a][s] = *reinterpret_cast<const U32x4*>(x_row + (k < in_features ? k : 0));
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    F32x4 total = {0.f, 0.f, 0.f, 0.f};
+    const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
+#pragma unroll
+    for (int a = 0; a < kBlocks; ++a) {
+        F32x4 sum[kPer];
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) {
+            sum[h] = F32x4{0.f, 0.f, 0.f, 0.f};
+            // (Groups past the inputs hold no scale: 0 times what is read there again.)
+#pragma unroll
+            for (int s = 0; s < kGroupSteps; ++s) sum[h] = mfma(shift, x[a][h * kGroupSteps + s], sum[h]);
+        }
+#pragma unroll
+        for (int s = 0; s < kGroupSteps; ++s)
+#pragma unroll
+            for (int h = 0; h < kPer; ++h)
+                sum[h] = mfma(codes_bf16(words[a][h * kGroupSteps + s]), x[a][h * kGroupSteps + s], sum[h]);
+#pragma unroll
+        for (int h = 0; h < kPer; ++h) {
+            const float scale[4] = {__uint_as_float(scales[a][2 * h] << 16), __uint_as_float(scales[a][2 * h] & 0xffff0000u),
+                                    __uint_as_float(scales[a][2 * h + 1] << 16), __uint_as_float(scales[a][2 * h + 1] & 0xffff0000u)};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) total[r] = fmaf(scale[r], sum[h][r], total[r]);
+        }
+    }
+    partial[wave][lane] = total;
+    __syncthreads();
+    bool finite = true;
+    if (wave == 0 && i < p.rows) {
+#pragma unroll
+        for (int w = 1; w < W; ++w) total += partial[w][lane];
+        const int64_t n = 16 * tile + 4 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (n + r >= p.out_features) break;
+            finite = finite && fabsf(total[r]) < __builtin_inff();
+            p.y[i * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * total[r]);
+        }
+    }
+    if (__syncthreads_or(!finite)) linear_int4_plain(p, tile, 1, 64 * W);
+}
+
+__global__ __launch_bounds__(256) void linear_int4_plain_kernel(const LinearInt4Params p) {
+    linear_int4_plain(p, blockIdx.x, 1, 256);
+}
+
+template <int Group, int T, int NB, int WK>
+void launch_one(const LinearInt4Params& p, hipStream_t stream) {
+    const int64_t per = 8 / WK * NB, tiles = int4_tiles(p.out_features);
+    LinearInt4Params q = p;
+    q.aligned = p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
+    const int blocks = (int)int4_blocks(p.in_features);
+    // x of one chunk: all of it up to 136 KB, else 128 KB.
+    const int64_t whole = p.rows * ((int64_t)(blocks + 3) / 4 * 1024 + kRowPad);
+    const int64_t most = whole <= 136 * 1024 ? whole : 128 * 1024;
+    const int kilobytes = std::max(1, (int)((most / p.rows - kRowPad) / 1024));  // of a row
+    q.chunk_blocks = std::min(blocks, 4 * kilobytes);
+    const size_t bytes = std::max<size_t>((size_t)p.rows * ((q.chunk_blocks + 3) / 4 * 1024 + kRowPad), WK > 1 ? 8 * NB * T * 1024 : 0);
+    hipLaunchKernelGGL((linear_int4_kernel<Group, T, NB, WK>), dim3((unsigned)((tiles + per - 1) / per)),
+                       dim3(kLinearInt4Threads), bytes, stream, q);
+}
+
+template <int Group, int W>
+void launch_few(const LinearInt4Params& p, int blocks, hipStream_t stream) {
+    const dim3 grid((unsigned)int4_tiles(p.out_features)), threads(64 * W);
+    if (blocks <= W)
+        hipLaunchKernelGGL((linear_int4_few_kernel<Group, 1, W>), grid, threads, 0, stream, p);
+    else if (blocks <= 2 * W)
+        hipLaunchKernelGGL((linear_int4_few_kernel<Group, 2, W>), grid, threads, 0, stream, p);
+    else
+        hipLaunchKernelGGL((linear_int4_few_kernel<Group, 3, W>), grid, threads, 0, stream, p);
 }
 
 template <int Group, int T>
 void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
     const int64_t tiles = int4_tiles(p.out_features);
-    if (tiles >= 1024)
-        hipLaunchKernelGGL((linear_int4_kernel<Group, T, 4, 4>), dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, stream, p);
+    const int blocks = (int)int4_blocks(p.in_features);
+    if (T == 1 && tiles < 1024 && blocks <= 48) {
+        if (blocks <= 24)
+            launch_few<Group, 8>(p, blocks, stream);
+        else
+            launch_few<Group, 16>(p, blocks, stream);
+        return;
+    }
+    if (tiles >= 2048)
+        launch_one<Group, T, 2, 1>(p, stream);
+    else if (tiles >= 1024)
+        launch_one<Group, T, 1, 2>(p, stream);
+    else if (tiles >= 512)
+        launch_one<Group, T, 1, 4>(p, stream);
     else
-        hipLaunchKernelGGL((linear_int4_kernel<Group, T, 1, 8>), dim3((unsigned)tiles), dim3(512), 0, stream, p);
+        launch_one<Group, T, 1, 8>(p, stream);
 }
 
 template <int Group>
@@ -320,7 +474,7 @@ hipError_t launch_unpack_int4(const Int4PackParams& p, uint16_t* weight, hipStre
 }
 
 hipError_t launch_linear_int4(const LinearInt4Params& p, hipStream_t stream) {
-    if (p.x_stride >= (1 << 24))  // 64 rows would pass the 2 GiB that the buffer loads of x address
+    if (p.x_stride >= (1 << 24))  // 64 rows would pass the 2 GiB that the DMA loads of x address
         hipLaunchKernelGGL(linear_int4_plain_kernel, dim3((unsigned)int4_tiles(p.out_features)), dim3(256), 0, stream, p);
     else if (p.group == 32)
         launch_rows<32>(p, stream);

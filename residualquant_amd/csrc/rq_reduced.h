@@ -28,6 +28,8 @@ struct LinearInt4Params {
     int64_t y_stride;
     int64_t rows, out_features, in_features;
     int group;
+    int chunk_blocks;         // set by the launch: blocks of 128 inputs of x in LDS at once
+    bool aligned;             // set by the launch: 8-byte stores of y
 };
 size_t int4_code_bytes(int64_t out_features, int64_t in_features);
 size_t int4_weight_bytes(int64_t out_features, int64_t in_features, int group);
