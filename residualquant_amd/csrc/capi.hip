@@ -1428,6 +1428,7 @@ int rq_linear_rows_int4(const void* x, int64_t x_stride, const void* packed, siz
     p.out_features = out_features;
     p.in_features = in_features;
     p.group = group;
+    p.compute_units = compute_units();
     return check_launch(rq::launch_linear_int4(p, stream), "4-bit projection launch");
 }
 

@@ -196,21 +196,21 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
     const uint8_t* x_row[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) x_row[t] = lds + min(16 * t + i, rows - 1) * row_bytes + 16 * g;
+    // [block][group][row]: -1.5 sum x, behind the rows of x.
+    float* const starts = reinterpret_cast<float*>(lds + rows * row_bytes);
     auto compute = [&](const Codes& b, int block) {
         U32x4 x[T][4];
 #pragma unroll
         for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int s = 0; s < 4; ++s) x[t][s] = *reinterpret_cast<const U32x4*>(x_row[t] + 256 * block + 64 * s);
-        const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
             F32x4 start[T];
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                start[t] = F32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < kGroupSteps; ++s) start[t] = mfma(shift, x[t][h * kGroupSteps + s], start[t]);
+                const float value = starts[(block * kPer + h) * (16 * T) + 16 * t + i];
+                start[t] = F32x4{value, value, value, value};
             }
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
@@ -256,6 +256,20 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
             }
         }
         wait_vector_memory();
+        __syncthreads();
+        for (int b = wave; b < count; b += 8) {
+            const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
+#pragma unroll
+            for (int h = 0; h < kPer; ++h)
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    F32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < kGroupSteps; ++s)
+                        sum = mfma(shift, *reinterpret_cast<const U32x4*>(x_row[t] + 256 * b + 64 * (h * kGroupSteps + s)), sum);
+                    if (g == 0) starts[(b * kPer + h) * (16 * T) + 16 * t + i] = sum[0];
+                }
+        }
         __syncthreads();
         for (int b = begin; b < end; b += kAhead) {
 #pragma unroll
@@ -394,19 +408,10 @@ __global__ __launch_bounds__(256) void linear_int4_plain_kernel(const LinearInt4
 }
 
 template <int Group, int T, int NB, int WK>
-void launch_one(const LinearInt4Params& p, hipStream_t stream) {
+void launch_one(const LinearInt4Params& p, size_t bytes, hipStream_t stream) {
     const int64_t per = 8 / WK * NB, tiles = int4_tiles(p.out_features);
-    LinearInt4Params q = p;
-    q.aligned = p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
-    const int blocks = (int)int4_blocks(p.in_features);
-    // x of one chunk: all of it up to 136 KB, else 128 KB.
-    const int64_t whole = p.rows * ((int64_t)(blocks + 3) / 4 * 1024 + kRowPad);
-    const int64_t most = whole <= 136 * 1024 ? whole : 128 * 1024;
-    const int kilobytes = std::max(1, (int)((most / p.rows - kRowPad) / 1024));  // of a row
-    q.chunk_blocks = std::min(blocks, 4 * kilobytes);
-    const size_t bytes = std::max<size_t>((size_t)p.rows * ((q.chunk_blocks + 3) / 4 * 1024 + kRowPad), WK > 1 ? 8 * NB * T * 1024 : 0);
     hipLaunchKernelGGL((linear_int4_kernel<Group, T, NB, WK>), dim3((unsigned)((tiles + per - 1) / per)),
-                       dim3(kLinearInt4Threads), bytes, stream, q);
+                       dim3(kLinearInt4Threads), std::max<size_t>(bytes, 8 * NB * T * 1024), stream, p);
 }
 
 template <int Group, int W>
@@ -431,14 +436,34 @@ void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
             launch_few<Group, 16>(p, blocks, stream);
         return;
     }
-    if (tiles >= 2048)
-        launch_one<Group, T, 2, 1>(p, stream);
-    else if (tiles >= 1024)
-        launch_one<Group, T, 1, 2>(p, stream);
-    else if (tiles >= 512)
-        launch_one<Group, T, 1, 4>(p, stream);
-    else
-        launch_one<Group, T, 1, 8>(p, stream);
+    LinearInt4Params q = p;
+    q.aligned = p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
+    // x of one chunk in LDS with its sums: all of it up to 152 KB, else chunks of at most that.
+    constexpr int kPer = 128 / Group;
+    auto chunk_bytes = [&](int64_t count) { return p.rows * ((count + 3) / 4 * 1024 + kRowPad) + count * kPer * 16 * T * 4; };
+    q.chunk_blocks = blocks;
+    while (chunk_bytes(q.chunk_blocks) > 152 * 1024) q.chunk_blocks = (q.chunk_blocks - 1) / 4 * 4;  // (whole KB of a row)
+    const size_t bytes = chunk_bytes(q.chunk_blocks);
+    // Tiles per workgroup: every compute unit takes ceil(workgroups / units)
+    // workgroups, each a copy of x (at 125 KB per us) and its tiles (21 KB of
+    // codes per us and compute unit, the even share of the memory's rate).
+    const double copy = p.rows * (double)blocks * 256 / 125e3 + 0.5, tile = blocks * 1024 / 21e3;
+    constexpr int kChoices[6][3] = {{1, 1, 8}, {2, 2, 8}, {3, 3, 8}, {4, 1, 2}, {8, 2, 2}, {12, 3, 2}};  // tiles, NB, WK
+    int best = 0;
+    double least = 0;
+    for (int c = 0; c < 6; ++c) {
+        const int64_t workgroups = (tiles + kChoices[c][0] - 1) / kChoices[c][0];
+        const double time = (double)((workgroups + q.compute_units - 1) / q.compute_units) * (copy + kChoices[c][0] * tile);
+        if (c == 0 || time < least) best = c, least = time;
+    }
+    switch (best) {
+        case 0: return launch_one<Group, T, 1, 8>(q, bytes, stream);
+        case 1: return launch_one<Group, T, 2, 8>(q, bytes, stream);
+        case 2: return launch_one<Group, T, 3, 8>(q, bytes, stream);
+        case 3: return launch_one<Group, T, 1, 2>(q, bytes, stream);
+        case 4: return launch_one<Group, T, 2, 2>(q, bytes, stream);
+        default: return launch_one<Group, T, 3, 2>(q, bytes, stream);
+    }
 }
 
 template <int Group>

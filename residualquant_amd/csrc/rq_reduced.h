@@ -28,6 +28,7 @@ struct LinearInt4Params {
     int64_t y_stride;
     int64_t rows, out_features, in_features;
     int group;
+    int compute_units;        // of the launching device
     int chunk_blocks;         // set by the launch: blocks of 128 inputs of x in LDS at once
     bool aligned;             // set by the launch: 8-byte stores of y
 };
