@@ -14,6 +14,7 @@
 // found (at most kMaxCandidates, else the row takes one pass per alternative,
 // as rows with NaN or infinities do) are ranked by counting.
 #include "rq_device.h"
+#include "rq_plan.h"
 #include "rq_reduced.h"
 
 namespace rq {
@@ -60,23 +61,37 @@ struct Row {
         shift = (int)(reinterpret_cast<uintptr_t>(base) % 16) / (Bf16 ? 2 : 4);
         chunks = (int)(((int64_t)vocab + shift + kChunk - 1) / kChunk);
     }
-    // The chunk's logits; -inf outside the row.
+    // Chunks first_whole..end_whole - 1 lie inside the row.
+    __device__ __forceinline__ int first_whole() const { return shift > 0 ? 1 : 0; }
+    __device__ __forceinline__ int end_whole() const { return (int)(((int64_t)vocab + shift) / kChunk); }
+    // The raw words of such a chunk, and its logits.
+    struct Raw {
+        Chunk16 words[Bf16 ? 1 : 2];
+    };
+    __device__ __forceinline__ Raw load_whole(int q) const {
+        Raw r;
+        const Chunk16* from = reinterpret_cast<const Chunk16*>(static_cast<const uint8_t*>(base) + ((int64_t)kChunk * q - shift) * (Bf16 ? 2 : 4));
+        r.words[0] = from[0];
+        if constexpr (!Bf16) r.words[1] = from[1];
+        return r;
+    }
+    __device__ __forceinline__ static void unpack(const Raw& r, float (&x)[kChunk]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (Bf16) {
+                x[2 * e] = __uint_as_float(r.words[0][e] << 16);
+                x[2 * e + 1] = __uint_as_float(r.words[0][e] & 0xffff0000u);
+            } else {
+                x[e] = __uint_as_float(r.words[0][e]);
+                x[4 + e] = __uint_as_float(r.words[1][e]);
+            }
+        }
+    }
+    // Any chunk's logits; -inf outside the row.
     __device__ __forceinline__ void load(int q, float (&x)[kChunk]) const {
         const int64_t at = (int64_t)kChunk * q - shift;
         if (at >= 0 && at + kChunk <= vocab) {
-            if constexpr (Bf16) {
-                const Chunk16 raw = *reinterpret_cast<const Chunk16*>(static_cast<const uint16_t*>(base) + at);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[2 * e] = __uint_as_float(raw[e] << 16);
-                    x[2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u);
-                }
-            } else {
-                const Chunk16* raw = reinterpret_cast<const Chunk16*>(static_cast<const float*>(base) + at);
-                const Chunk16 a = raw[0], b = raw[1];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(a[e]), x[4 + e] = __uint_as_float(b[e]);
-            }
+            unpack(load_whole(q), x);
             return;
         }
 #pragma unroll
@@ -93,14 +108,15 @@ struct Sums {
     float high, sum, weighted;
 };
 
-// The two sums against the larger reference.
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    const float high = fmaxf(a.high, b.high);
-    const float da = a.high - high, db = b.high - high;
-    const float wa = da == 0.f ? 1.f : __builtin_amdgcn_exp2f(da), wb = db == 0.f ? 1.f : __builtin_amdgcn_exp2f(db);
-    // (A product with a weight of 0 is 0, whatever the distance.)
-    return Sums{high, a.sum * wa + b.sum * wb,
-                (a.weighted + mul_zero(a.sum, da)) * wa + (b.weighted + mul_zero(b.sum, db)) * wb};
+// Sum over the wave, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+    v += __uint_as_float(plan_dpp<0xB1>(__float_as_uint(v)));   // quad_perm [1,0,3,2]
+    v += __uint_as_float(plan_dpp<0x4E>(__float_as_uint(v)));   // quad_perm [2,3,0,1]
+    v += __uint_as_float(plan_dpp<0x124>(__float_as_uint(v)));  // row_ror:4
+    v += __uint_as_float(plan_dpp<0x128>(__float_as_uint(v)));  // row_ror:8
+    const uint32_t u = __float_as_uint(v);
+    return (__uint_as_float(__builtin_amdgcn_readlane(u, 0)) + __uint_as_float(__builtin_amdgcn_readlane(u, 16))) +
+           (__uint_as_float(__builtin_amdgcn_readlane(u, 32)) + __uint_as_float(__builtin_amdgcn_readlane(u, 48)));
 }
 
 template <int Threads>
@@ -174,7 +190,7 @@ template <bool Bf16, int Threads>
 __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p) {
     constexpr int kWaves = Threads / 64;
     __shared__ uint64_t keys[kWaves * 64];
-    __shared__ Sums wave_sums[kWaves];
+    __shared__ float2 wave_sums[kWaves];
     __shared__ uint64_t candidates[kMaxCandidates];
     __shared__ uint16_t listed[Threads];
     __shared__ uint64_t threshold;
@@ -196,7 +212,8 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     uint32_t largest_chunk = 0xffffffffu;
     auto take = [&](int q, const float (&x)[kChunk]) {
         const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (most > largest || largest_chunk == 0xffffffffu) {
+        // (The first chunk that holds it: the row's first chunk is taken last.)
+        if (most > largest || largest_chunk == 0xffffffffu || (most == largest && (uint32_t)q < largest_chunk)) {
             largest_chunk = (uint32_t)q;
             largest = fmaxf(most, largest);
         }
@@ -215,46 +232,63 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
             own.weighted = fmaf(w, fmaxf(d, -1000.0f), own.weighted);  // 0 where w is 0, also at d = -inf
         }
     };
+    // (Loads without a condition, the next in flight while the present are summed; at the end the last again.)
     constexpr int kAhead = 4;
-    for (int q = tid; q < row.chunks; q += kAhead * Threads) {
-        float x[kAhead][kChunk];
+    const int end_whole = row.end_whole();
+    int at = row.first_whole() + tid;
+    if (row.first_whole() < end_whole) {
+        typename Row<Bf16>::Raw now[kAhead], next[kAhead];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-            if (q + a * Threads < row.chunks) row.load(q + a * Threads, x[a]);
+        for (int a = 0; a < kAhead; ++a) now[a] = row.load_whole(min(at + a * Threads, end_whole - 1));
+        for (int q = row.first_whole(); q < end_whole; q += kAhead * Threads, at += kAhead * Threads) {
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
-            if (q + a * Threads < row.chunks) take(q + a * Threads, x[a]);
+            for (int a = 0; a < kAhead; ++a) next[a] = row.load_whole(min(at + (kAhead + a) * Threads, end_whole - 1));
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                if (at + a * Threads >= end_whole) break;
+                float x[kChunk];
+                Row<Bf16>::unpack(now[a], x);
+                take(at + a * Threads, x);
+            }
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) now[a] = next[a];
+        }
     }
-    Sums all = own;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) all = join(all, Sums{__shfl_xor(all.high, d), __shfl_xor(all.sum, d), __shfl_xor(all.weighted, d)});
+    // The row's ends, by the last two threads (which have the fewest chunks).
+    auto edge_chunk = [&](int thread) {
+        if (thread == Threads - 1 && row.first_whole() > 0) return 0;
+        if (thread == Threads - 2 && end_whole < row.chunks && row.chunks - 1 >= row.first_whole()) return row.chunks - 1;
+        return -1;
+    };
+    if (edge_chunk(tid) >= 0) {
+        float x[kChunk];
+        row.load(edge_chunk(tid), x);
+        take(edge_chunk(tid), x);
+    }
     const uint64_t own_key = ((uint64_t)ordered_bits(largest) << 32) | (0xffffffffu - largest_chunk);
-    if (lane == 0) wave_sums[wave] = all;
     keys[tid] = own_key;
     __syncthreads();
-    all = wave_sums[0];
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) all = join(all, wave_sums[w]);
-    // The largest logit itself: owners' largest, then the largest of all.
+    // The owners' largest, then the largest of all.
     uint64_t owner = keys[lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) owner = keys[64 * w + lane] > owner ? keys[64 * w + lane] : owner;
-    uint64_t best = owner;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        const uint64_t other = shuffle_xor_u64(best, d);
-        best = other > best ? other : best;
-    }
-    const uint32_t ordered = (uint32_t)(best >> 32);
+    const uint32_t ordered = wave_max_u32((uint32_t)(owner >> 32));
     const float m = __uint_as_float((ordered >> 31) ? ordered & 0x7fffffffu : ~ordered);
-    // The sums against m itself.  Their reference is a rounded m' log2(e); one
+    // The thread's sums against m itself.  Its reference is a rounded m' log2(e); one
     // rounding of the difference keeps large logits exact.
-    const float above_reference = fmaf(m, kLog2e, -all.high), keep = __builtin_amdgcn_exp2f(-above_reference);
-    const float exact_sum = all.sum * keep;
-    const float weighted = (all.weighted - above_reference * all.sum) * keep;
+    const float above_reference = fmaf(m, kLog2e, -own.high), keep = __builtin_amdgcn_exp2f(-above_reference);
+    const float weighted_here = own.sum == 0.f ? 0.f : (own.weighted - above_reference * own.sum) * keep;
+    const float sum_here = own.sum == 0.f ? 0.f : own.sum * keep;
+    const float wave_total = wave_sum(sum_here), wave_weighted = wave_sum(weighted_here);
+    if (lane == 0) wave_sums[wave] = make_float2(wave_total, wave_weighted);
+    __syncthreads();
+    float2 part = make_float2(0.f, 0.f);
+    if (lane < kWaves) part = wave_sums[lane];
+    const float exact_sum = wave_sum(part.x), weighted = wave_sum(part.y);
     const float log_sum = logf(exact_sum);
     // NaN, infinities (S is NaN), nothing but -inf (m), or values near the lowest.
     if (!(m > -1.0e38f && m < 1.0e38f && exact_sum < 1.0e38f)) {
+        __syncthreads();
         logprobs_plain<Bf16, Threads>(p, row_number, false, keys, reinterpret_cast<float*>(wave_sums));
         return;
     }
@@ -264,8 +298,8 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     }
     if (p.top == 0) return;
 
-    // T: the `top`-th of the owners.
-    if (wave == 0) {
+    // T: the `top`-th of the owners; the first of them every wave knows.
+    if (p.top > 1 && wave == 0) {
         int above = 0;
         for (int o = 0; o < 64; ++o) {
             const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(owner >> 32), o) << 32) |
@@ -274,14 +308,24 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
         }
         if (above == p.top - 1) threshold = owner;
     }
-    __syncthreads();
-    const uint64_t limit = threshold;
+    uint64_t limit = ((uint64_t)ordered << 32) | wave_max_u32((uint32_t)(owner >> 32) == ordered ? (uint32_t)owner : 0u);
+    if (p.top > 1) {
+        __syncthreads();
+        limit = threshold;
+    }
     if (own_key >= limit && largest_chunk != 0xffffffffu) listed[atomicAdd(&listed_count, 1)] = (uint16_t)tid;
     __syncthreads();
-    const int each = (row.chunks + Threads - 1) / Threads, work = listed_count * each;
+    // A listed thread's chunks: its whole ones and, of the last two threads, the row's ends.
+    const int whole = end_whole - row.first_whole(), each = (max(whole, 0) + Threads - 1) / Threads + 1;
+    const int work = listed_count * each;
     for (int o = tid; o < work; o += Threads) {
-        const int q = listed[o / each] + o % each * Threads;
-        if (q >= row.chunks) continue;
+        const int owner_thread = listed[o / each], number = o % each;
+        int q = row.first_whole() + owner_thread + number * Threads;
+        if (number == each - 1)
+            q = edge_chunk(owner_thread);
+        else if (q >= end_whole)
+            q = -1;
+        if (q < 0) continue;
         float x[kChunk];
         row.load(q, x);
 #pragma unroll
