@@ -1224,10 +1224,18 @@ int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int6
     return check_launch(rq::launch_quantize_fp8(p, stream), "8-bit cache write launch");
 }
 
-// Least steps of 32 tokens of one split of an 8-bit attention call, the
-// workgroups per compute unit that its work is spread over, and the most
-// columns of a workgroup's tile.
-constexpr int kFp8MinSteps = 8, kFp8PerCu = 2, kFp8MaxTile = 256, kFp8MaxSplits = 256;
+// Least steps of 32 tokens of one split of an 8-bit attention call, and the
+// most columns of a workgroup's tile.  (Least steps of 8, 12 and 16: one
+// request of 2048 tokens 9.8, 11.0 and 10.7 us, 16 requests of 100..3000 tokens
+// 11.5, 12.0 and 12.5.)
+constexpr int kFp8MinSteps = 8, kFp8MaxTile = 256, kFp8MaxSplits = 256;
+
+// Workgroups per K/V head that a call's work is spread over: three quarters of
+// the compute units together, so that rounding up the splits still leaves one
+// round of workgroups.  (All of them: 8 grouped requests 20.3 us instead of
+// 18.3, 8 requests of 8 rows 17.5 instead of 14.9, one request of 8192 tokens
+// 13.7 instead of 14.3; two rounds: 21.5, 21.5 and 16.7 us.)
+static int64_t fp8_target(int kv_heads) { return (3 * (int64_t)compute_units() / 4 + kv_heads - 1) / kv_heads; }
 
 // Steps that the page table and the new rows of a call can hold.
 static int64_t fp8_most_steps(int64_t rows, int64_t max_pages, int page_tokens) {
@@ -1244,7 +1252,7 @@ static int fp8_max_splits(int64_t rows, int64_t max_pages, int page_tokens) {
 // column (0: no call of this size is split).
 static int64_t fp8_entries(int64_t rows, int heads, int kv_heads, int head_dim, int64_t max_pages, int page_tokens) {
     const int64_t columns = rows * (heads / kv_heads);
-    const int64_t target = (kFp8PerCu * (int64_t)compute_units() + kv_heads - 1) / kv_heads;
+    const int64_t target = fp8_target(kv_heads);
     const int max_splits = fp8_max_splits(rows, max_pages, page_tokens);
     if (max_splits == 1) return 0;
     const int64_t entries = std::min<int64_t>(columns * max_splits, columns + target * kFp8MaxTile);
@@ -1264,7 +1272,7 @@ static void plan_fp8(rq::Fp8AttentionParams& p) {
     const int64_t columns = p.rows * (p.heads / p.kv_heads);
     const int64_t average = (columns + p.requests - 1) / p.requests;
     p.tile = average <= 16 ? 16 : average <= 48 ? 32 : kFp8MaxTile;
-    const int64_t target = ((p.tile == kFp8MaxTile ? 3 * (int64_t)compute_units() / 4 : kFp8PerCu * (int64_t)compute_units()) + p.kv_heads - 1) / p.kv_heads;
+    const int64_t target = fp8_target(p.kv_heads);
     const int64_t most_steps = fp8_most_steps(p.rows, p.max_pages, p.page_tokens);
     const int64_t tiles = columns / p.tile + p.requests;  // at most, over all requests
     const bool split = p.entries > 0;

@@ -336,19 +336,45 @@ __device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int ite
         const int column = item_column + c, channel = 8 * (tid & 15);
         if (column >= columns_in || channel >= D) continue;
         const uint32_t at = (uint32_t)(column * splits) * kEntry * 4;
+        // Parts in groups of four whose loads are all in flight (past the last part that one again, with a weight
+        // of 0), the first group together with the maxima of the others: one wait for up to four parts, and no
+        // chain of rescaled sums for more. One pass with rescaling took 11.1 us against 9.8 for one request of
+        // 2048 tokens; loads that wait part by part 118 us against 113 for a chunk of 512 rows.
+        constexpr int kGroup = 4;
+        float2 stats[kGroup];
+        float4 low[kGroup], up[kGroup];
+        const auto load = [&](int first) {
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                const uint32_t part = at + (uint32_t)min(first + k, splits - 1) * kEntry * 4;
+                stats[k] = handoff_load2(handoff, part);
+                low[k] = handoff_load4(handoff, part + 16 + 4 * channel);
+                up[k] = handoff_load4(handoff, part + 32 + 4 * channel);
+            }
+        };
+        load(0);
         float high = kLowest;
-#pragma unroll 4
-        for (int k = 0; k < splits; ++k) high = fmaxf(high, handoff_load2(handoff, at + (uint32_t)k * kEntry * 4).x);
+        for (int first = kGroup; first < splits; first += 8) {
+            float largest[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) largest[k] = handoff_load2(handoff, at + (uint32_t)min(first + k, splits - 1) * kEntry * 4).x;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) high = fmaxf(high, largest[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kGroup; ++k) high = fmaxf(high, stats[k].x);
         float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < splits; ++k) {
-            const uint32_t part = at + (uint32_t)k * kEntry * 4;
-            const float2 stats = handoff_load2(handoff, part);
-            const float4 a = handoff_load4(handoff, part + 16 + 4 * channel), b = handoff_load4(handoff, part + 32 + 4 * channel);
-            const float keep = stats.x == high ? 1.0f : __builtin_amdgcn_exp2f(stats.x - high);
-            sum += stats.y * keep;
-            o[0] += a.x * keep, o[1] += a.y * keep, o[2] += a.z * keep, o[3] += a.w * keep;
-            o[4] += b.x * keep, o[5] += b.y * keep, o[6] += b.z * keep, o[7] += b.w * keep;
+        for (int first = 0;;) {
+#pragma unroll
+            for (int k = 0; k < kGroup; ++k) {
+                const float keep = first + k >= splits ? 0.0f : stats[k].x == high ? 1.0f : __builtin_amdgcn_exp2f(stats[k].x - high);
+                sum += stats[k].y * keep;
+                o[0] += low[k].x * keep, o[1] += low[k].y * keep, o[2] += low[k].z * keep, o[3] += low[k].w * keep;
+                o[4] += up[k].x * keep, o[5] += up[k].y * keep, o[6] += up[k].z * keep, o[7] += up[k].w * keep;
+            }
+            first += kGroup;
+            if (first >= splits) break;
+            load(first);
         }
         const float scale = 1.0f / sum;
         uint16_t* out = output_row(column) + channel;
