@@ -114,13 +114,13 @@ __device__ __forceinline__ U32x4 codes_bf16(uint32_t word) {
                  (__builtin_amdgcn_alignbit(word, word, 12) & kMantissa) | kOne};
 }
 
-// y of the outputs 16 tile0.. of NB tiles in plain steps, for results that are
+// y of `rows` rows and of the outputs 16 tile0.. of `tiles` tiles in plain steps, for results that are
 // not finite: the products of shifted codes overflow earlier than the sum
 // itself, and turn an infinity in x into NaN.
-__device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int tiles, int threads) {
+__device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int tiles, int64_t first_row, int rows, int threads) {
     const int64_t blocks = int4_blocks(p.in_features);
-    for (int64_t o = threadIdx.x; o < (int64_t)tiles * 16 * p.rows; o += threads) {
-        const int64_t tile = tile0 + o / 16 % tiles, n = 16 * tile + o % 16, m = o / (16 * tiles);
+    for (int64_t o = threadIdx.x; o < (int64_t)tiles * 16 * rows; o += threads) {
+        const int64_t tile = tile0 + o / 16 % tiles, n = 16 * tile + o % 16, m = first_row + o / (16 * tiles);
         if (n >= p.out_features) continue;
         float sum = 0.f;
         for (int64_t k = 0; k < p.in_features; k += 8) {
@@ -322,10 +322,10 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
     }
     const int64_t workgroup_tile = (int64_t)blockIdx.x * (8 / WK) * NB;
     if (__syncthreads_or(!finite))
-        linear_int4_plain(p, workgroup_tile, (int)min((int64_t)(8 / WK) * NB, tiles - workgroup_tile), kLinearInt4Threads);
+        linear_int4_plain(p, workgroup_tile, (int)min((int64_t)(8 / WK) * NB, tiles - workgroup_tile), 0, rows, kLinearInt4Threads);
 }
 
-// One workgroup of W waves per tile of 16 outputs, for up to 16 rows: x goes from
+// One workgroup of W waves per tile of 16 outputs and 16 rows: x goes from
 // global memory to the operands without LDS, which saves few rows a copy and a
 // barrier.  All of a wave's blocks, at most kBlocks, are in flight at once;
 // past its last one a wave reads that block again, with scales of 0 (a branch
@@ -337,9 +337,10 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int in_features = (int)p.in_features, blocks = (int)int4_blocks(p.in_features);
-    const int64_t tile = blockIdx.x;
+    const int64_t tile = blockIdx.x, first_row = 16 * blockIdx.y;
+    const int rows = min((int)(p.rows - first_row), 16);
     const int begin = blocks * wave / W, end = blocks * (wave + 1) / W;
-    const uint16_t* x_row = p.x + min(i, (int)p.rows - 1) * p.x_stride + 8 * g;
+    const uint16_t* x_row = p.x + (first_row + min(i, rows - 1)) * p.x_stride + 8 * g;
     U32x4 words[kBlocks], x[kBlocks][4];
     uint32_t scales[kBlocks][2 * kPer];
 #pragma unroll
@@ -389,7 +390,7 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
     partial[wave][lane] = total;
     __syncthreads();
     bool finite = true;
-    if (wave == 0 && i < p.rows) {
+    if (wave == 0 && i < rows) {
 #pragma unroll
         for (int w = 1; w < W; ++w) total += partial[w][lane];
         const int64_t n = 16 * tile + 4 * g;
@@ -397,14 +398,14 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
         for (int r = 0; r < 4; ++r) {
             if (n + r >= p.out_features) break;
             finite = finite && fabsf(total[r]) < __builtin_inff();
-            p.y[i * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * total[r]);
+            p.y[(first_row + i) * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * total[r]);
         }
     }
-    if (__syncthreads_or(!finite)) linear_int4_plain(p, tile, 1, 64 * W);
+    if (__syncthreads_or(!finite)) linear_int4_plain(p, tile, 1, first_row, rows, 64 * W);
 }
 
 __global__ __launch_bounds__(256) void linear_int4_plain_kernel(const LinearInt4Params p) {
-    linear_int4_plain(p, blockIdx.x, 1, 256);
+    linear_int4_plain(p, blockIdx.x, 1, 0, (int)p.rows, 256);
 }
 
 template <int Group, int T, int NB, int WK>
@@ -416,7 +417,7 @@ void launch_one(const LinearInt4Params& p, size_t bytes, hipStream_t stream) {
 
 template <int Group, int W>
 void launch_few(const LinearInt4Params& p, int blocks, hipStream_t stream) {
-    const dim3 grid((unsigned)int4_tiles(p.out_features)), threads(64 * W);
+    const dim3 grid((unsigned)int4_tiles(p.out_features), (unsigned)((p.rows + 15) / 16)), threads(64 * W);
     if (blocks <= W)
         hipLaunchKernelGGL((linear_int4_few_kernel<Group, 1, W>), grid, threads, 0, stream, p);
     else if (blocks <= 2 * W)
@@ -429,13 +430,6 @@ template <int Group, int T>
 void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
     const int64_t tiles = int4_tiles(p.out_features);
     const int blocks = (int)int4_blocks(p.in_features);
-    if (T == 1 && tiles < 1024 && blocks <= 48) {
-        if (blocks <= 24)
-            launch_few<Group, 8>(p, blocks, stream);
-        else
-            launch_few<Group, 16>(p, blocks, stream);
-        return;
-    }
     LinearInt4Params q = p;
     q.aligned = p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
     // x of one chunk in LDS with its sums: all of it up to 152 KB, else chunks of at most that.
@@ -466,8 +460,26 @@ void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
     }
 }
 
+// x beside the codes, or through LDS: by the rounds of workgroups, one per tile
+// and 16 rows, that the compute units take without it.  Without LDS (against
+// with it), for outputs x inputs and rows:
+//   1 round:   2048 x 5632, 16: 8.8 us (9.4); 32: 9.0 (13.3)
+//   2 rounds:  2048 x 5632, 64: 16.6 us (24.3); 4096 x 5632, 32: 16.7 (13.7)
+//   3 rounds:  11264 x 2048, 8: 6.8 us (7.4), 16: 9.0 (7.7); 6144 x 1024, 32: 5.7 (6.0)
+//   4 rounds:  16000 x 2048, 8: 8.3 us (7.1); 4096 x 1024, 64: 6.8 (6.5)
 template <int Group>
 void launch_rows(const LinearInt4Params& p, hipStream_t stream) {
+    const int blocks = (int)int4_blocks(p.in_features);
+    const int64_t workgroups = int4_tiles(p.out_features) * ((p.rows + 15) / 16);
+    const int64_t rounds = (workgroups + p.compute_units - 1) / p.compute_units;
+    const int64_t most = blocks <= 8 || (blocks <= 24 && p.rows <= 8) ? 3 : p.rows > 32 ? 2 : 1;
+    if (blocks <= 48 && rounds <= most) {
+        if (blocks <= 24)
+            launch_few<Group, 8>(p, blocks, stream);
+        else
+            launch_few<Group, 16>(p, blocks, stream);
+        return;
+    }
     switch ((p.rows + 15) / 16) {
         case 1: return launch_tiles<Group, 1>(p, stream);
         case 2: return launch_tiles<Group, 2>(p, stream);

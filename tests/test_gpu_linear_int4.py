@@ -67,6 +67,50 @@ def test_linear_is_exact_on_small_integers(device, rows, group):
     assert torch.equal(got.cpu(), want.to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("rows,group", [(1, 32), (9, 64), (16, 128), (30, 64), (48, 32), (49, 128), (64, 64)])
+@pytest.mark.parametrize("out,features", [(16643, 1152), (5000, 2048), (1037, 6400), (24, 6400)])
+def test_wide_and_deep_weights_are_exact_on_small_integers(device, rows, group, out, features):
+    """Many outputs or inputs, where x passes through shared memory, whole and in chunks."""
+    codes, _ = _weight(out, features, group, seed=rows + out)
+    g = torch.Generator().manual_seed(rows)
+    scales = torch.exp2(torch.randint(-2, 3, (out, features // group), generator=g).float()).to(torch.bfloat16)
+    x = torch.randint(-4, 5, (rows, features), generator=g).to(torch.bfloat16)
+    got = step_ops.linear_rows_int4(x.to(device), step_ops.pack_weight_int4(codes.to(device), scales.to(device)))
+    # (Below 2^24 in quarters: exact in float32 too, in any order.)
+    want = x.float() @ (codes.float() * scales.float().repeat_interleave(group, dim=1)).t()
+    assert torch.equal(got.cpu(), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("rows", [3, 40])
+def test_wide_weight_nan_and_infinity(device, rows):
+    """As the narrow ones: on the row of the NaN or infinity only, the others as without it."""
+    out, features = 16643, 256
+    codes, scales = _weight(out, features, 64, seed=8)
+    codes[codes == 0] = 1
+    weight = step_ops.pack_weight_int4(codes.to(device), scales.to(device))
+    x = torch.randn((rows, features), generator=torch.Generator().manual_seed(6)).to(torch.bfloat16)
+    plain = step_ops.linear_rows_int4(x.to(device), weight).cpu()
+    for value in (torch.inf, torch.nan, 3.3e38):
+        y = x.clone()
+        y[1, 100] = value
+        got = step_ops.linear_rows_int4(y.to(device), weight).cpu()
+        want = (y[1].double() @ (codes.double() * scales.double().repeat_interleave(64, dim=1)).t()).to(torch.bfloat16)
+        assert torch.equal(got[1].isnan(), want.isnan()) and torch.equal(got[1].isinf(), want.isinf())
+        rest = [m for m in range(rows) if m != 1]
+        assert torch.allclose(got[rest].double(), plain[rest].double(), rtol=2.0 ** -6, atol=2.0 ** -8)
+
+
+def test_rows_far_apart(device):
+    """Rows 2^24 and more elements apart."""
+    codes, scales = _weight(70, 256, 64, seed=5)
+    store = torch.zeros(2 * (1 << 24) + 256, dtype=torch.bfloat16, device=device)
+    x = store.as_strided((3, 256), (1 << 24, 1))
+    x.copy_(torch.randn((3, 256), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16))
+    got = step_ops.linear_rows_int4(x, step_ops.pack_weight_int4(codes.to(device), scales.to(device))).cpu().double()
+    want, bound = _reference(x.cpu(), codes, scales)
+    assert ((got - want).abs() / bound).max() <= 1.0
+
+
 def test_every_code_at_every_place(device):
     """One-hot inputs read the weight back: code x scale, exact in BF16."""
     out, features = 48, 256
