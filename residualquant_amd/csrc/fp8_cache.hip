@@ -326,15 +326,13 @@ __device__ __forceinline__ void fp8_softmax(Fp8Columns<NT, Channels>& columns, c
     }
 }
 
-// The last split of an item to finish joins the splits' parts of its columns, in their order.
-template <int D, int Threads, int Tile, class OutputRow>
-__device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int item_column, int columns_in, int splits,
-                                         OutputRow output_row) {
+// Joins the splits' parts of columns from..to - 1, in the splits' order.
+template <int D, int Threads, class OutputRow>
+__device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int from, int to, int splits, OutputRow output_row) {
     constexpr int kEntry = D + 4;
-    const int tid = threadIdx.x;
-    for (int c = tid >> 4; c < Tile; c += Threads / 16) {
-        const int column = item_column + c, channel = 8 * (tid & 15);
-        if (column >= columns_in || channel >= D) continue;
+    const int tid = threadIdx.x, channel = 8 * (tid & 15);
+    if (channel >= D) return;
+    for (int column = from + (tid >> 4); column < to; column += Threads / 16) {
         const uint32_t at = (uint32_t)(column * splits) * kEntry * 4;
         // Parts in groups of four whose loads are all in flight (past the last part that one again, with a weight
         // of 0), the first group together with the maxima of the others: one wait for up to four parts, and no
@@ -741,7 +739,8 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         }
     }
     if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
-    fp8_join<D, kStreamThreads, kTile>(handoff, item_column, columns_in, splits, output_row);
+    // The last split to finish joins.
+    fp8_join<D, kStreamThreads>(handoff, item_column, min(item_column + kTile, columns_in), splits, output_row);
 }
 
 // ------------------------------------------------------------------ many columns
@@ -755,7 +754,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
 // global loads are issued a tile ahead and converted into the other buffer
 // after the products of the present one: one barrier per tile.
 
-constexpr int kWideTokens = 64;
+constexpr int kWideTokens = 64, kJoinThreads = 512;
 
 // Distinct for channels c..c + 7 (an operand read) and for every fourth (the transposing writes).
 __device__ __forceinline__ int v_swizzle(int channel) { return (channel ^ (channel >> 2)) & 7; }
@@ -776,7 +775,6 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
     constexpr int kChunks = D / 16;               // 16-byte chunks of a row of codes
     static_assert(kPasses * kThreads == 512, "units are filled by whole waves");
     __shared__ WideTile<D> tiles[2];
-    __shared__ int last_flag;
     const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
     const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
     const int request = __builtin_amdgcn_readfirstlane(item.request);
@@ -805,8 +803,6 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
     const int all_tiles = old_tiles + new_tiles;
 
     float* const entries = p.partials + ((int64_t)head * p.entries + __builtin_amdgcn_readfirstlane(item.entry)) * kEntry;
-    uint64_t* const arrivals = reinterpret_cast<uint64_t*>(entries + (int64_t)item_column * splits * kEntry + 2);
-    const uint64_t arrivals_seen = splits > 1 ? peek_arrivals(arrivals) : 0;
 
     U32x4 query[NT][kSteps];
     int seen[NT];
@@ -1082,7 +1078,6 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
     auto output_row = [&](int column) {
         return p.output + (int64_t)(first + column / group) * p.output_stride + ((int64_t)head * group + column % group) * D;
     };
-    if (splits > 1 && tid == 0) tag_arrivals(arrivals, p.call_tag, arrivals_seen);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int column = column0 + 16 * t + i;
@@ -1108,8 +1103,30 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
             handoff_store(handoff, at + 4, columns.sum[t]);
         }
     }
-    if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
-    fp8_join<D, kThreads, kTile>(handoff, item_column, columns_in, splits, output_row);
+}
+
+// The join of the wide kernel's parts, over the same plan: the workgroup of a
+// split joins that share of its item's columns.  (The last of the splits alone
+// would read 1 MB for 256 columns in 8 parts: one request of 2048 + 256 tokens
+// took 68 us with that.)
+template <int D, int NT, int Waves>
+__global__ __launch_bounds__(kJoinThreads) void attention_fp8_join_kernel(const Fp8AttentionParams p) {
+    constexpr int kTile = 16 * NT * Waves, kEntry = D + 4;
+    const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
+    const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
+    const int request = __builtin_amdgcn_readfirstlane(item.request);
+    const int splits = __builtin_amdgcn_readfirstlane(item.splits), split = __builtin_amdgcn_readfirstlane(item.split);
+    if (request < 0 || splits == 1) return;
+    const int group = p.heads / p.kv_heads;
+    const int first = __builtin_amdgcn_readfirstlane(item.first), columns_in = __builtin_amdgcn_readfirstlane(item.rows);
+    const int item_column = __builtin_amdgcn_readfirstlane(item.index) * kTile, count = min(kTile, columns_in - item_column);
+    float* const entries = p.partials + ((int64_t)head * p.entries + __builtin_amdgcn_readfirstlane(item.entry)) * kEntry;
+    const __amdgpu_buffer_rsrc_t handoff = handoff_resource(entries, (uint32_t)min((int64_t)columns_in * splits * kEntry * 4, (int64_t)0xfffffffc));
+    fp8_join<D, kJoinThreads>(handoff, item_column + count * split / splits, item_column + count * (split + 1) / splits, splits,
+                              [&](int column) {
+                                  return p.output + (int64_t)(first + column / group) * p.output_stride +
+                                         ((int64_t)head * group + column % group) * D;
+                              });
 }
 
 }  // namespace
@@ -1139,8 +1156,11 @@ void launch_attention(const Fp8AttentionParams& p, hipStream_t stream) {
         hipLaunchKernelGGL((attention_fp8_kernel<D, 1>), grid, threads, 0, stream, p);
     else if (p.tile == 32)
         hipLaunchKernelGGL((attention_fp8_kernel<D, 2>), grid, threads, 0, stream, p);
-    else
+    else {
         hipLaunchKernelGGL((attention_fp8_wide_kernel<D, 2, 8>), grid, dim3(512), 0, stream, p);
+        if (p.splits > 1 || (p.items > 0 && p.plan_max_splits > 1))
+            hipLaunchKernelGGL((attention_fp8_join_kernel<D, 2, 8>), grid, dim3(kJoinThreads), 0, stream, p);
+    }
 }
 
 }  // namespace
