@@ -745,16 +745,25 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
 
 // ------------------------------------------------------------------ many columns
 //
-// The same products for requests of many columns: kWideWaves waves of 16 NT
-// columns share tiles of 64 tokens, which they convert to BF16 once, into LDS:
+// The same products for requests of many columns: eight waves of 32 columns
+// share tiles of 64 tokens, which they convert to BF16 once, into LDS:
 // K as it is read ([token][channel]), V transposed ([channel][token], the tokens
 // in the order in which the second product's k slots stand for them).  Rows of
 // 256 and 128 bytes; the 16-byte chunks of a row are permuted by its number so
 // that the 16 rows an operand read touches lie in different banks.  A tile's
 // global loads are issued a tile ahead and converted into the other buffer
 // after the products of the present one: one barrier per tile.
+//
+// One request of 8192 tokens + 1024 new rows, 16 heads of 128: 147 us, 3.8 us per
+// tile and compute unit, of which the matrix units work 1.6 (a third of it for the
+// weights' lower parts); the rest is the vector instructions of the weights and
+// conversions, about as long, and waits for LDS.  Two waves per SIMD hide
+// little of one another; four (16 columns each) spill registers (224 us), one
+// of 64 columns took 276, and the weights of one step beside the products of
+// the other in one wave 154.
 
-constexpr int kWideTokens = 64, kJoinThreads = 512;
+constexpr int kWideTokens = 64, kWideThreads = 512, kWideColumns = 32;  // columns of a wave
+constexpr int kWideTile = kWideColumns * kWideThreads / 64;
 
 // Distinct for channels c..c + 7 (an operand read) and for every fourth (the transposing writes).
 __device__ __forceinline__ int v_swizzle(int channel) { return (channel ^ (channel >> 2)) & 7; }
@@ -768,12 +777,10 @@ struct WideTile {
     int odd;                   // the number of the last tile of new rows with infinities or NaN among its values
 };
 
-template <int D, int NT, int Waves>
-__global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp8AttentionParams p) {
-    constexpr int kThreads = 64 * Waves, kTile = 16 * NT * Waves, kSteps = D / 32, kOut = D / 16, kEntry = D + 4;
-    constexpr int kPasses = 512 / kThreads;       // 128 threads fill a unit at a time
+template <int D>
+__global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const Fp8AttentionParams p) {
+    constexpr int NT = kWideColumns / 16, kTile = kWideTile, kSteps = D / 32, kOut = D / 16, kEntry = D + 4;
     constexpr int kChunks = D / 16;               // 16-byte chunks of a row of codes
-    static_assert(kPasses * kThreads == 512, "units are filled by whole waves");
     __shared__ WideTile<D> tiles[2];
     const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
     const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
@@ -839,43 +846,47 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
     const int place = filler ? tid & 127 : 0;
     const int k_token = place / kChunks, k_chunk = place % kChunks;
     const int v_quad = place / (D / 4), v_word = place % (D / 4);
-    // What a thread holds of a tile of the history in flight.  (Tiles of new rows are few: they are
-    // loaded where they are stored.)
+    // What a thread holds of a tile in flight: codes of the history, or new rows.
     struct Stage {
-        U32x4 k[kPasses];
-        uint32_t v[kPasses][4];
-        float key_scale[kPasses], value_scale[kPasses];
+        U32x4 k[2];  // (codes: the first)
+        U32x2 v[4];  // (codes: the first word)
+        float key_scale, value_scale;
     };
     // (Not made uniform: a scalar load in flight would hold back every LDS wait.)
-    auto unit_of = [&](int pass) { return (tid + pass * kThreads) >> 7; };
-    auto block_of = [&](int tile, int pass) {  // -1: no tokens of the unit, or no block
-        const int token = 32 * begin + kWideTokens * tile + 16 * unit_of(pass);
-        if (token >= old_tokens) return -1;
-        const int block = p.block_table[(int64_t)request * p.block_table_stride + (token >> page_shift)];
-        return block >= 0 && block < p.num_blocks ? block : -1;
+    const int unit = tid >> 7;
+    // The table's entry for a tile's unit, unchecked; past the history the last one again.  (Loads
+    // without a condition: behind one that a path leaves out, the wait is for all loads in flight.)
+    auto entry_of = [&](int tile) {
+        const int token = min(32 * begin + kWideTokens * tile + 16 * unit, old_tokens - 1);
+        return p.block_table[(int64_t)request * p.block_table_stride + (token >> page_shift)];
     };
-    int next_block[kPasses], stage_block[kPasses];
+    int next_entry, stage_block;  // stage_block: -1 if no token of the unit counts
     auto fetch = [&](Stage& x, int tile) {
-        if (tile >= old_tiles) return;
-#pragma unroll
-        for (int pass = 0; pass < kPasses; ++pass) {
-            const int block = next_block[pass];
-            const int token = 32 * begin + kWideTokens * tile + 16 * unit_of(pass);
-            const int64_t index = (int64_t)max(block, 0) * p.kv_heads + head;
-            x.key_scale[pass] = x.value_scale[pass] = 1.f;
-            if (block >= 0) {
-                x.key_scale[pass] = p.scales[index];
-                x.value_scale[pass] = p.scales[index + p.num_blocks * p.kv_heads];
-            }
-            // (Without a block: the first one's bytes, of which no token counts.)
-            const uint8_t* unit = p.cache + ((index << page_shift) + (token & (p.page_tokens - 1))) * D;
-            x.k[pass] = *reinterpret_cast<const U32x4*>(unit + k_token * D + 16 * k_chunk);
+        if (tile >= old_tiles) {
+            // New rows (clamped to the request's; what lies past them is masked).
+            const int base = new_begin + kWideTokens * (tile - old_tiles) + 16 * unit;
+            const uint16_t* k = p.key + (int64_t)(first + min(base + k_token, rows - 1)) * p.key_stride + (int64_t)head * D + 16 * k_chunk;
+            x.k[0] = *reinterpret_cast<const U32x4At8*>(k);
+            x.k[1] = *reinterpret_cast<const U32x4At8*>(k + 8);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                x.v[pass][r] = *reinterpret_cast<const uint32_t*>(unit + plane_bytes + (4 * v_quad + r) * D + 4 * v_word);
-            stage_block[pass] = block;
-            next_block[pass] = block_of(tile + 1, pass);
+                x.v[r] = *reinterpret_cast<const U32x2*>(
+                    p.value + (int64_t)(first + min(base + 4 * v_quad + r, rows - 1)) * p.value_stride + (int64_t)head * D + 4 * v_word);
+            return;
         }
+        const int token = 32 * begin + kWideTokens * tile + 16 * unit;
+        const int block = token < old_tokens && next_entry >= 0 && next_entry < p.num_blocks ? next_entry : -1;
+        const int64_t index = (int64_t)max(block, 0) * p.kv_heads + head;
+        next_entry = entry_of(tile + 1);
+        // (Without a block: the first one's bytes, of which no token counts.)
+        x.key_scale = p.scales[index];
+        x.value_scale = p.scales[index + p.num_blocks * p.kv_heads];
+        const uint8_t* from = p.cache + ((index << page_shift) + (token & (p.page_tokens - 1))) * D;
+        x.k[0] = *reinterpret_cast<const U32x4*>(from + k_token * D + 16 * k_chunk);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            x.v[r][0] = *reinterpret_cast<const uint32_t*>(from + plane_bytes + (4 * v_quad + r) * D + 4 * v_word);
+        stage_block = block;
     };
     auto v_place = [&](WideTile<D>& tile, int channel, int unit, int quad) -> U32x2* {
         const int chunk = 4 * (unit >> 1) + quad;
@@ -884,66 +895,58 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
     auto store = [&](const Stage& x, int number) {
         WideTile<D>& tile = tiles[number & 1];
         bool odd = false;
-#pragma unroll
-        for (int pass = 0; pass < kPasses; ++pass) {
-            const int unit = unit_of(pass), token = 16 * unit + k_token;
-            if (number < old_tiles) {
-                const int valid = stage_block[pass] >= 0 ? min(old_tokens - 32 * begin - kWideTokens * number - 16 * unit, 16) : 0;
-                if (filler) {
-                    const U32x4 k = x.k[pass];
-                    tile.k[token][(2 * k_chunk) ^ k_token] =
-                        U32x4{bf16x2_of_fp8<false>(k[0]), bf16x2_of_fp8<true>(k[0]), bf16x2_of_fp8<false>(k[1]), bf16x2_of_fp8<true>(k[1])};
-                    tile.k[token][(2 * k_chunk + 1) ^ k_token] =
-                        U32x4{bf16x2_of_fp8<false>(k[2]), bf16x2_of_fp8<true>(k[2]), bf16x2_of_fp8<false>(k[3]), bf16x2_of_fp8<true>(k[3])};
-                    // Slots past the history may hold NaN, which a weight of zero does not remove.
-                    uint32_t w[4], y[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) w[r] = 4 * v_quad + r < valid ? x.v[pass][r] : 0u;
-                    transpose_bytes(w, y);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        *v_place(tile, 4 * v_word + c, unit, v_quad) = U32x2{bf16x2_of_fp8<false>(y[c]), bf16x2_of_fp8<true>(y[c])};
-                }
-                if ((tid & 127) == 0) {
-                    tile.key_scale[unit] = x.key_scale[pass] * to_log2;
-                    tile.value_scale[unit] = x.value_scale[pass];
-                    tile.valid[unit] = valid;
-                }
-                continue;
-            }
-            // New rows (clamped to the request's; what lies past them is masked).
-            const int base = new_begin + kWideTokens * (number - old_tiles) + 16 * unit;
+        const int token = 16 * unit + k_token;
+        if (number < old_tiles) {
+            const int valid = stage_block >= 0 ? min(old_tokens - 32 * begin - kWideTokens * number - 16 * unit, 16) : 0;
             if (filler) {
-                const uint16_t* k = p.key + (int64_t)(first + min(base + k_token, rows - 1)) * p.key_stride + (int64_t)head * D + 16 * k_chunk;
-                tile.k[token][(2 * k_chunk) ^ k_token] = *reinterpret_cast<const U32x4At8*>(k);
-                tile.k[token][(2 * k_chunk + 1) ^ k_token] = *reinterpret_cast<const U32x4At8*>(k + 8);
-                // Infinities and NaN, which a weight of zero does not remove, are left out here and added apart.
-                U32x2 w[4];
+                const U32x4 k = x.k[0];
+                tile.k[token][(2 * k_chunk) ^ k_token] =
+                    U32x4{bf16x2_of_fp8<false>(k[0]), bf16x2_of_fp8<true>(k[0]), bf16x2_of_fp8<false>(k[1]), bf16x2_of_fp8<true>(k[1])};
+                tile.k[token][(2 * k_chunk + 1) ^ k_token] =
+                    U32x4{bf16x2_of_fp8<false>(k[2]), bf16x2_of_fp8<true>(k[2]), bf16x2_of_fp8<false>(k[3]), bf16x2_of_fp8<true>(k[3])};
+                // Slots past the history may hold NaN, which a weight of zero does not remove.
+                uint32_t w[4], y[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    w[r] = *reinterpret_cast<const U32x2*>(
-                        p.value + (int64_t)(first + min(base + 4 * v_quad + r, rows - 1)) * p.value_stride + (int64_t)head * D + 4 * v_word);
+                for (int r = 0; r < 4; ++r) w[r] = 4 * v_quad + r < valid ? x.v[r][0] : 0u;
+                transpose_bytes(w, y);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t v = w[r][h];
-                        odd |= not_finite_bf16x2(v);
-                        if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
-                        if ((v & 0x7f800000u) == 0x7f800000u) v &= 0x0000ffffu;
-                        w[r][h] = v;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t pick = c & 1 ? 0x07060302u : 0x05040100u;
-                    *v_place(tile, 4 * v_word + c, unit, v_quad) =
-                        U32x2{__builtin_amdgcn_perm(w[1][c >> 1], w[0][c >> 1], pick), __builtin_amdgcn_perm(w[3][c >> 1], w[2][c >> 1], pick)};
-                }
+                for (int c = 0; c < 4; ++c)
+                    *v_place(tile, 4 * v_word + c, unit, v_quad) = U32x2{bf16x2_of_fp8<false>(y[c]), bf16x2_of_fp8<true>(y[c])};
             }
             if ((tid & 127) == 0) {
-                tile.key_scale[unit] = to_log2;
-                tile.value_scale[unit] = 1.f;
-                tile.valid[unit] = 16;
+                tile.key_scale[unit] = stage_block >= 0 ? x.key_scale * to_log2 : 1.f;
+                tile.value_scale[unit] = stage_block >= 0 ? x.value_scale : 1.f;
+                tile.valid[unit] = valid;
             }
+            return;
+        }
+        if (filler) {
+            tile.k[token][(2 * k_chunk) ^ k_token] = x.k[0];
+            tile.k[token][(2 * k_chunk + 1) ^ k_token] = x.k[1];
+            // Infinities and NaN, which a weight of zero does not remove, are left out here and added apart.
+            U32x2 w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t v = x.v[r][h];
+                    odd |= not_finite_bf16x2(v);
+                    if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
+                    if ((v & 0x7f800000u) == 0x7f800000u) v &= 0x0000ffffu;
+                    w[r][h] = v;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t pick = c & 1 ? 0x07060302u : 0x05040100u;
+                *v_place(tile, 4 * v_word + c, unit, v_quad) =
+                    U32x2{__builtin_amdgcn_perm(w[1][c >> 1], w[0][c >> 1], pick), __builtin_amdgcn_perm(w[3][c >> 1], w[2][c >> 1], pick)};
+            }
+        }
+        if ((tid & 127) == 0) {
+            tile.key_scale[unit] = to_log2;
+            tile.value_scale[unit] = 1.f;
+            tile.valid[unit] = 16;
         }
         if (odd) tile.odd = number;
     };
@@ -1010,7 +1013,10 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
             }
             float weight[NT][2][4];
             U32x4 upper[NT][1], lower[NT][1];
+            // (The wave that computes weights goes before one in its products: 105 -> 103 us for two chunks of 509 rows.)
+            __builtin_amdgcn_s_setprio(2);
             fp8_softmax<NT, kOut, 2>(columns, dot, key_scale, value_scale, weight, upper, lower);
+            __builtin_amdgcn_s_setprio(0);
 #pragma unroll
             for (int e = 0; e < kOut; ++e)
 #pragma unroll
@@ -1052,8 +1058,7 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
     };
 
     Stage stage;
-#pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) next_block[pass] = block_of(0, pass);
+    next_entry = old_tiles > 0 ? entry_of(0) : -1;
     if (tid < 2) tiles[tid].odd = -1;
     __syncthreads();
     if (all_tiles > 0) {
@@ -1109,9 +1114,9 @@ __global__ __launch_bounds__(64 * Waves) void attention_fp8_wide_kernel(const Fp
 // split joins that share of its item's columns.  (The last of the splits alone
 // would read 1 MB for 256 columns in 8 parts: one request of 2048 + 256 tokens
 // took 68 us with that.)
-template <int D, int NT, int Waves>
-__global__ __launch_bounds__(kJoinThreads) void attention_fp8_join_kernel(const Fp8AttentionParams p) {
-    constexpr int kTile = 16 * NT * Waves, kEntry = D + 4;
+template <int D>
+__global__ __launch_bounds__(kWideThreads) void attention_fp8_join_kernel(const Fp8AttentionParams p) {
+    constexpr int kTile = kWideTile, kEntry = D + 4;
     const int head = (int)(blockIdx.x % (unsigned)p.kv_heads);
     const PlanItem item = fp8_item<kTile>(p, (int)(blockIdx.x / (unsigned)p.kv_heads));
     const int request = __builtin_amdgcn_readfirstlane(item.request);
@@ -1122,7 +1127,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_fp8_join_kernel(const 
     const int item_column = __builtin_amdgcn_readfirstlane(item.index) * kTile, count = min(kTile, columns_in - item_column);
     float* const entries = p.partials + ((int64_t)head * p.entries + __builtin_amdgcn_readfirstlane(item.entry)) * kEntry;
     const __amdgpu_buffer_rsrc_t handoff = handoff_resource(entries, (uint32_t)min((int64_t)columns_in * splits * kEntry * 4, (int64_t)0xfffffffc));
-    fp8_join<D, kJoinThreads>(handoff, item_column + count * split / splits, item_column + count * (split + 1) / splits, splits,
+    fp8_join<D, kWideThreads>(handoff, item_column + count * split / splits, item_column + count * (split + 1) / splits, splits,
                               [&](int column) {
                                   return p.output + (int64_t)(first + column / group) * p.output_stride +
                                          ((int64_t)head * group + column % group) * D;
@@ -1157,9 +1162,9 @@ void launch_attention(const Fp8AttentionParams& p, hipStream_t stream) {
     else if (p.tile == 32)
         hipLaunchKernelGGL((attention_fp8_kernel<D, 2>), grid, threads, 0, stream, p);
     else {
-        hipLaunchKernelGGL((attention_fp8_wide_kernel<D, 2, 8>), grid, dim3(512), 0, stream, p);
+        hipLaunchKernelGGL((attention_fp8_wide_kernel<D>), grid, dim3(kWideThreads), 0, stream, p);
         if (p.splits > 1 || (p.items > 0 && p.plan_max_splits > 1))
-            hipLaunchKernelGGL((attention_fp8_join_kernel<D, 2, 8>), grid, dim3(kJoinThreads), 0, stream, p);
+            hipLaunchKernelGGL((attention_fp8_join_kernel<D>), grid, dim3(kWideThreads), 0, stream, p);
     }
 }
 
