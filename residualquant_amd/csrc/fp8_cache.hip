@@ -231,8 +231,11 @@ __device__ __forceinline__ PlanItem fp8_item(const Fp8AttentionParams& p, int ke
         const Fp8Request q = fp8_request(p, lane < requests ? lane : requests - 1);
         const int columns = lane < requests ? q.rows * group : 0;
         const PlanEntry own{(columns + Tile - 1) / Tile, fp8_steps(q.history) + fp8_steps(q.rows), q.first, q.history, columns};
-        const PlanSizes sizes{p.plan_target, p.splits, p.plan_min, 1 << 24, p.plan_max_splits, 0, 1, 9, 0};
-        return plan_find(requests, key, sizes, own);
+        const PlanSizes sizes = fp8_sizes(p);
+        PlanItem item = plan_find(requests, key, sizes, own);
+        // (Query starts that do not ascend could ask for more entries than the workspace has.)
+        if (item.splits > 1 && (item.entry < 0 || item.entry + (int64_t)item.rows * item.splits > p.entries)) item.request = -1;
+        return item;
     }
     // More requests than a wave has lanes: tile i of request b has slot
     // floor(first column of b / Tile) + b + i, each slot `splits` workgroups.

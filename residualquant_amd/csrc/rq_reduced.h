@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "rq_plan.h"
+
 namespace rq {
 
 // Projections with 4-bit weights and group scales (linear_int4.hip).
@@ -56,7 +58,6 @@ hipError_t launch_logprobs(const LogprobParams& p, hipStream_t stream);
 
 // Cache held in 8 bits (fp8_cache.hip): E4M3 codes [2, blocks, kv_heads, PT, D],
 // FP32 scales [2, blocks, kv_heads].
-constexpr int kFp8MaxDim = 128;
 struct Fp8WriteParams {
     const uint16_t* key;
     int64_t key_stride;
@@ -102,7 +103,7 @@ struct Fp8AttentionParams {
     // read in steps of 32 tokens.  Up to kPlanRequests requests, `items`
     // workgroups per K/V head are planned on the device; with more (items 0)
     // every tile takes `splits`.
-    int tile;                 // 16, 32 or 128 columns per workgroup
+    int tile;                 // 16, 32 or 256 columns per workgroup
     int items;
     int splits;               // of every tile of equal requests
     int plan_target, plan_min, plan_max_splits;  // PlanSizes, in steps
@@ -110,6 +111,9 @@ struct Fp8AttentionParams {
     float* partials;          // workspace [kv_heads, entries, D + 4]
     uint64_t call_tag;        // of this call (48 bits, rq_plan.h)
 };
+__host__ __device__ __forceinline__ PlanSizes fp8_sizes(const Fp8AttentionParams& p) {
+    return PlanSizes{p.plan_target, p.splits, p.plan_min, 1 << 24, p.plan_max_splits, 0, 1, 9, 0};
+}
 hipError_t launch_quantize_fp8(const Fp8WriteParams& p, hipStream_t stream);
 hipError_t launch_attention_fp8(const Fp8AttentionParams& p, hipStream_t stream);
 

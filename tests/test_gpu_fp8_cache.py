@@ -224,6 +224,59 @@ def test_attention_is_repeatable_and_takes_any_workspace(device):
     _check_attention(case, first)
 
 
+def test_attention_of_many_requests_with_many_columns(device):
+    """More requests than a wave has lanes, with 0 to 90 rows: several tiles, whole and with splits."""
+    g = torch.Generator().manual_seed(50)
+    for longest, seed in ((40, 51), (700, 52)):
+        histories = torch.randint(0, longest, (66,), generator=g).tolist()
+        rows = torch.randint(0, 91, (66,), generator=g).tolist()
+        rows[65] = 300
+        case = _case(histories, rows, 2, 1, 96, 16, seed=seed)
+        _check_attention(case, _attend(_to(case, device), device))
+
+
+def test_attention_of_a_chunk_in_graphs_that_share_a_workspace(device):
+    """Two graphs and eager calls, of one row and of many, take turns with one workspace; another stream."""
+    many = _to(_case([1800, 700], [120, 300], 2, 2, 128, 16, seed=53), device)
+    few = _to(_case([2000, 900, 4], [1, 1, 1], 2, 2, 128, 16, seed=54), device)
+    needed = max(ops.paged_attention_fp8_workspace_bytes(d["query"].size(0), 2, 2, 128, d["table"].size(1), 16)
+                 for d in (many, few))
+    workspace = torch.full((needed,), 0xFF, dtype=torch.uint8, device=device)
+    want = [_attend(d, device) for d in (many, few)]
+    outs = [torch.zeros_like(d["query"]) for d in (many, few)]
+    graphs = []
+    for d, out in zip((many, few), outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            _attend(d, device, workspace=workspace, output=out)
+        graphs.append(graph)
+    for turn in range(4):
+        for k in ((0, 1), (1, 0), (0, 0), (1, 1))[turn]:
+            outs[k].fill_(torch.nan)
+            graphs[k].replay()
+            assert torch.equal(outs[k], want[k]), f"turn {turn}"
+            other = (many, few)[1 - k]
+            assert torch.equal(_attend(other, device, workspace=workspace), want[1 - k]), f"eager, turn {turn}"
+    stream = torch.cuda.Stream(device=device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        got = _attend(many, device, workspace=workspace)
+    torch.cuda.current_stream(device).wait_stream(stream)
+    assert torch.equal(got, want[0])
+
+
+def test_attention_of_a_padded_batch(device):
+    """Rows behind the last request keep what they held; requests of no tokens are none's."""
+    case = _case([700, 0, 90, 0], [140, 0, 1, 0], 2, 2, 96, 32, seed=55)
+    d = _to(case, device)
+    pad = lambda t: torch.cat([t, torch.full((9, *t.shape[1:]), torch.nan, dtype=t.dtype, device=device)])  # noqa: E731
+    d |= {k: pad(d[k]) for k in ("query", "key", "value")}
+    out = torch.full_like(d["query"], 7.0)
+    _attend(d, device, output=out)
+    _check_attention(case, out[:141])
+    assert bool((out[141:] == 7.0).all())
+
+
 def test_attention_far_block(device):
     """A page whose byte offset passes 2^32."""
     blocks = (1 << 32) // (16 * 128) + 40  # one head: 2 KiB a page, two planes of over 4 GiB
