@@ -193,13 +193,14 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     __shared__ float2 wave_sums[kWaves];
     __shared__ uint64_t candidates[kMaxCandidates];
     __shared__ uint16_t listed[Threads];
-    __shared__ uint64_t threshold;
+    __shared__ int above[64];  // owners above each
     __shared__ int listed_count, candidate_count;
     const int64_t row_number = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const Row<Bf16> row(p, row_number);
     float token_logit = 0.f;
     int64_t token = 0;
+    if (tid < 64) above[tid] = 0;
     if (tid == 0) {
         token = p.tokens[row_number];
         token_logit = token >= 0 && token < p.vocab ? logit_at<Bf16>(row.base, token) : __builtin_nanf("");
@@ -298,20 +299,23 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     }
     if (p.top == 0) return;
 
-    // T: the `top`-th of the owners; the first of them every wave knows.
-    if (p.top > 1 && wave == 0) {
-        int above = 0;
-        for (int o = 0; o < 64; ++o) {
-            const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(owner >> 32), o) << 32) |
-                                   (uint32_t)__builtin_amdgcn_readlane((uint32_t)owner, o);
-            above += other > owner || (other == owner && o < lane) ? 1 : 0;
-        }
-        if (above == p.top - 1) threshold = owner;
-    }
+    // T: the `top`-th of the owners (the first of them every wave knows).  The waves share its comparisons out.
     uint64_t limit = ((uint64_t)ordered << 32) | wave_max_u32((uint32_t)(owner >> 32) == ordered ? (uint32_t)owner : 0u);
+    auto owner_of = [&](int o) {
+        return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(owner >> 32), o) << 32) |
+               (uint32_t)__builtin_amdgcn_readlane((uint32_t)owner, o);
+    };
     if (p.top > 1) {
+        int more = 0;
+#pragma unroll
+        for (int k = 0; k < 64 / kWaves; ++k) {
+            const int o = __builtin_amdgcn_readfirstlane(wave) * (64 / kWaves) + k;
+            const uint64_t other = owner_of(o);
+            more += other > owner || (other == owner && o < lane) ? 1 : 0;
+        }
+        if (more > 0) atomicAdd(&above[lane], more);
         __syncthreads();
-        limit = threshold;
+        limit = owner_of(__builtin_ctzll(__ballot(above[lane] == p.top - 1)));
     }
     if (own_key >= limit && largest_chunk != 0xffffffffu) listed[atomicAdd(&listed_count, 1)] = (uint16_t)tid;
     __syncthreads();
@@ -344,11 +348,17 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
         logprobs_plain<Bf16, Threads>(p, row_number, true, keys, reinterpret_cast<float*>(wave_sums));
         return;
     }
-    for (int c = tid; c < found; c += Threads) {
-        const uint64_t key = candidates[c];
-        int rank = 0;
-        for (int o = 0; o < found; ++o) rank += candidates[o] > key ? 1 : 0;
-        if (rank >= p.top) continue;
+    // 16 lanes count one candidate's rank.
+    for (int c0 = 0; c0 < found; c0 += Threads / 16) {
+        const int c = c0 + (tid >> 4);
+        const uint64_t key = c < found ? candidates[c] : ~0ull;
+        uint32_t rank = 0;
+        for (int o = tid & 15; o < found; o += 16) rank += candidates[o] > key ? 1 : 0;
+        rank += plan_dpp<0xB1>(rank);   // quad_perm [1,0,3,2]
+        rank += plan_dpp<0x4E>(rank);   // quad_perm [2,3,0,1]
+        rank += plan_dpp<0x124>(rank);  // row_ror:4
+        rank += plan_dpp<0x128>(rank);  // row_ror:8
+        if ((tid & 15) != 0 || c >= found || rank >= (uint32_t)p.top) continue;
         const uint32_t bits = (uint32_t)(key >> 32);
         const float x = __uint_as_float((bits >> 31) ? bits & 0x7fffffffu : ~bits);
         p.top_tokens[row_number * p.top + rank] = (int64_t)(0xffffffffu - (uint32_t)key);
