@@ -366,10 +366,16 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     }
 }
 
+// Four waves per row for short rows, and where enough rows run beside each
+// other; else eight.  (256 threads, 512, and 1024, whose start and barriers cost
+// more than they share out, in us.  1 row of 8000 logits with 8 alternatives: 6.5,
+// 7.2, 9.7; of 32000: 9.6, 9.0, 10.6; of 49152: 11.6, 10.4, 11.9.  600 rows of 50257
+// with 1: 23.5, 25.1, 38.9; 2041 rows: 50.9, 56.5, 101; 3000 rows of 151000 with 8:
+// 243, 220, 296.)
 template <bool Bf16>
 void launch_rows(const LogprobParams& p, hipStream_t stream) {
-    if (p.rows <= 256)
-        hipLaunchKernelGGL((logprobs_kernel<Bf16, 1024>), dim3((unsigned)p.rows), dim3(1024), 0, stream, p);
+    if (p.vocab <= 16384 || (p.rows > 256 && p.vocab <= 65536))
+        hipLaunchKernelGGL((logprobs_kernel<Bf16, 256>), dim3((unsigned)p.rows), dim3(256), 0, stream, p);
     else
         hipLaunchKernelGGL((logprobs_kernel<Bf16, 512>), dim3((unsigned)p.rows), dim3(512), 0, stream, p);
 }
