@@ -308,7 +308,7 @@ int rq_linear_rows(const void* x, int64_t x_stride, const void* weight, void* y,
  * with an invalid block) are skipped.  A block that is written must belong to
  * one request of the call.  The call may be repeated: it writes the same.
  * key, value: BF16 [rows, kv_heads, head_dim], 8-byte aligned, token strides
- * multiples of 4 elements.
+ * multiples of 4 elements; max_pages x page_tokens at most 2^30.
  */
 int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int64_t value_stride, int64_t rows,
                     int kv_heads, int head_dim, void* cache, float* scales, int64_t num_blocks, int page_tokens,

@@ -1178,9 +1178,10 @@ static int check_fp8_pages(const void* cache, const float* scales, int64_t num_b
     if (requests < 0 || requests > (int64_t)INT32_MAX / 4 ||
         (requests > 0 && (query_start_loc == nullptr || seq_lens == nullptr)))
         return fail(RQ_EINVAL, "Contiguous INT32 query starts with one final boundary required");
-    if ((rows > 0 && requests > 0 && block_table == nullptr) || max_pages < 0 || block_table_stride < max_pages ||
-        max_pages > (int64_t)INT32_MAX / page_tokens)
+    if ((rows > 0 && requests > 0 && block_table == nullptr) || max_pages < 0 || block_table_stride < max_pages)
         return fail(RQ_EINVAL, "INT32 page table with packed rows required");
+    // (The kernels count tokens, rounded up to steps and tiles ahead, in 31 bits.)
+    if (max_pages > ((int64_t)1 << 30) / page_tokens) return fail(RQ_EINVAL, "A page table of at most 2^30 tokens required");
     return RQ_OK;
 }
 

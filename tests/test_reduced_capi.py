@@ -76,6 +76,16 @@ def test_attention_refusals(lib):
     assert _attend(lib, rows=0) == _lib.RQ_OK
 
 
+def test_page_tables_past_2_to_the_30_tokens_are_refused(lib):
+    """The kernels count tokens in 31 bits, rounded up to steps and tiles ahead."""
+    for page in (16, 32):
+        pages = (1 << 30) // page + 1
+        assert _write(lib, page=page, max_pages=pages, table_stride=pages) == _lib.RQ_EINVAL
+        assert b"2^30 tokens" in lib.rq_last_error()
+        assert _attend(lib, page=page, max_pages=pages) == _lib.RQ_EINVAL
+        assert b"2^30 tokens" in lib.rq_last_error()
+
+
 def test_attention_workspace_depends_on_shapes_only(lib):
     sizes = [lib.rq_paged_attention_fp8_workspace_bytes(rows, 16, 16, 128, 512, 16) for rows in (1, 32, 1024)]
     assert sizes == [lib.rq_paged_attention_fp8_workspace_bytes(rows, 16, 16, 128, 512, 16) for rows in (1, 32, 1024)]
