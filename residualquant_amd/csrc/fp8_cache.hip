@@ -329,8 +329,9 @@ __device__ __forceinline__ void fp8_softmax(Fp8Columns<NT, Channels>& columns, c
     }
 }
 
-// Joins the splits' parts of columns from..to - 1, in the splits' order.
-template <int D, int Threads, class OutputRow>
+// Joins the splits' parts of columns from..to - 1, in the splits' order.  Shared:
+// they come from workgroups of the same launch, past the caches that are not coherent.
+template <int D, int Threads, bool Shared, class OutputRow>
 __device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int from, int to, int splits, OutputRow output_row) {
     constexpr int kEntry = D + 4;
     const int tid = threadIdx.x, channel = 8 * (tid & 15);
@@ -344,13 +345,23 @@ __device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int fro
         constexpr int kGroup = 4;
         float2 stats[kGroup];
         float4 low[kGroup], up[kGroup];
+        const auto load2 = [&](uint32_t place) {
+            if constexpr (Shared) return handoff_load2(handoff, place);
+            const U32x2 v = __builtin_amdgcn_raw_buffer_load_b64(handoff, place, 0, 0);
+            return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
+        };
+        const auto load4 = [&](uint32_t place) {
+            if constexpr (Shared) return handoff_load4(handoff, place);
+            const U32x4 v = __builtin_amdgcn_raw_buffer_load_b128(handoff, place, 0, 0);
+            return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+        };
         const auto load = [&](int first) {
 #pragma unroll
             for (int k = 0; k < kGroup; ++k) {
                 const uint32_t part = at + (uint32_t)min(first + k, splits - 1) * kEntry * 4;
-                stats[k] = handoff_load2(handoff, part);
-                low[k] = handoff_load4(handoff, part + 16 + 4 * channel);
-                up[k] = handoff_load4(handoff, part + 32 + 4 * channel);
+                stats[k] = load2(part);
+                low[k] = load4(part + 16 + 4 * channel);
+                up[k] = load4(part + 32 + 4 * channel);
             }
         };
         load(0);
@@ -358,7 +369,7 @@ __device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int fro
         for (int first = kGroup; first < splits; first += 8) {
             float largest[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) largest[k] = handoff_load2(handoff, at + (uint32_t)min(first + k, splits - 1) * kEntry * 4).x;
+            for (int k = 0; k < 8; ++k) largest[k] = load2(at + (uint32_t)min(first + k, splits - 1) * kEntry * 4).x;
 #pragma unroll
             for (int k = 0; k < 8; ++k) high = fmaxf(high, largest[k]);
         }
@@ -743,7 +754,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
     }
     if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
     // The last split to finish joins.
-    fp8_join<D, kStreamThreads>(handoff, item_column, min(item_column + kTile, columns_in), splits, output_row);
+    fp8_join<D, kStreamThreads, true>(handoff, item_column, min(item_column + kTile, columns_in), splits, output_row);
 }
 
 // ------------------------------------------------------------------ many columns
@@ -1130,7 +1141,7 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_join_kernel(const 
     const int item_column = __builtin_amdgcn_readfirstlane(item.index) * kTile, count = min(kTile, columns_in - item_column);
     float* const entries = p.partials + ((int64_t)head * p.entries + __builtin_amdgcn_readfirstlane(item.entry)) * kEntry;
     const __amdgpu_buffer_rsrc_t handoff = handoff_resource(entries, (uint32_t)min((int64_t)columns_in * splits * kEntry * 4, (int64_t)0xfffffffc));
-    fp8_join<D, kWideThreads>(handoff, item_column + count * split / splits, item_column + count * (split + 1) / splits, splits,
+    fp8_join<D, kWideThreads, false>(handoff, item_column + count * split / splits, item_column + count * (split + 1) / splits, splits,
                               [&](int column) {
                                   return p.output + (int64_t)(first + column / group) * p.output_stride +
                                          ((int64_t)head * group + column % group) * D;
