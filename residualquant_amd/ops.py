@@ -74,9 +74,12 @@ def _schedule(records: Sequence[Sequence[int]]):
     return _schedule_arrays(tuple([(int(r[0]), int(r[1])) for r in records]))
 
 
+_CURRENT = nullcontext()
+
+
 def _on_device(device: int):
     """A context on CUDA device ``device`` (nothing to do where it is current)."""
-    return nullcontext() if torch.cuda.current_device() == device else torch.cuda.device(device)
+    return _CURRENT if torch.cuda.current_device() == device else torch.cuda.device(device)
 
 
 def _stream(device: int) -> int:
@@ -343,29 +346,33 @@ def paged_attention_bf16(query: torch.Tensor, key: torch.Tensor, value: torch.Te
 
 
 def _validate_fp8_cache(cache, scales, device, kv_heads, head_dim):
+    """The cache's shape."""
     shape = cache.shape
-    _require(cache.get_device() == device and cache.dtype is torch.float8_e4m3fn and cache.is_contiguous()
-             and len(shape) == 5 and shape[0] == 2 and shape[2] == kv_heads and shape[4] == head_dim,
-             "Contiguous E4M3 [2, blocks, heads, page tokens, channels] cache required")
-    _require(scales.get_device() == device and scales.dtype is torch.float32 and scales.is_contiguous()
-             and scales.shape == shape[:3], "Contiguous FP32 [2, blocks, heads] scales on the cache device required")
+    if not (cache.get_device() == device and cache.dtype is torch.float8_e4m3fn and cache.is_contiguous()
+            and len(shape) == 5 and shape[0] == 2 and shape[2] == kv_heads and shape[4] == head_dim):
+        raise RuntimeError("Contiguous E4M3 [2, blocks, heads, page tokens, channels] cache required")
+    if not (scales.get_device() == device and scales.dtype is torch.float32 and scales.is_contiguous()
+            and scales.shape == shape[:3]):
+        raise RuntimeError("Contiguous FP32 [2, blocks, heads] scales on the cache device required")
     return shape
 
 
 def _validate_sequences(query_start_loc, seq_lens, block_table, device):
-    """The number of requests."""
+    """The number of requests, and the page table's width and row stride."""
     requests = seq_lens.numel()
-    _require(query_start_loc.get_device() == device and query_start_loc.dtype is torch.int32
-             and query_start_loc.dim() == 1 and query_start_loc.is_contiguous()
-             and query_start_loc.numel() == requests + 1,
-             "Contiguous INT32 query starts with one final boundary required")
-    _require(seq_lens.get_device() == device and seq_lens.dtype is torch.int32 and seq_lens.dim() == 1
-             and seq_lens.is_contiguous(), "Contiguous INT32 sequence lengths required")
-    _require(block_table.get_device() == device and block_table.dtype is torch.int32 and block_table.dim() == 2
-             and (block_table.stride(1) == 1 or block_table.size(1) <= 1) and block_table.size(0) >= requests
-             and (block_table.stride(0) >= block_table.size(1) or block_table.size(0) <= 1),
-             "INT32 page table with packed rows required")
-    return requests
+    if not (query_start_loc.get_device() == device and query_start_loc.dtype is torch.int32
+            and query_start_loc.dim() == 1 and query_start_loc.is_contiguous()
+            and query_start_loc.numel() == requests + 1):
+        raise RuntimeError("Contiguous INT32 query starts with one final boundary required")
+    if not (seq_lens.get_device() == device and seq_lens.dtype is torch.int32 and seq_lens.dim() == 1
+            and seq_lens.is_contiguous()):
+        raise RuntimeError("Contiguous INT32 sequence lengths required")
+    shape = block_table.shape
+    if block_table.get_device() == device and block_table.dtype is torch.int32 and len(shape) == 2:
+        (rows, pages), stride = shape, block_table.stride()
+        if (stride[1] == 1 or pages <= 1) and rows >= requests and (stride[0] >= pages or rows <= 1):
+            return requests, pages, max(stride[0], pages)
+    raise RuntimeError("INT32 page table with packed rows required")
 
 
 def quantize_fp8(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor,
@@ -389,13 +396,12 @@ def quantize_fp8(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, sc
     _require(value.get_device() == device and value_shape == shape, "K/V must have matching shapes and devices")
     rows, kv_heads, head_dim = shape
     _, blocks, _, page_tokens, _ = _validate_fp8_cache(cache, scales, device, kv_heads, head_dim)
-    requests = _validate_sequences(query_start_loc, seq_lens, block_table, device)
+    requests, pages, table_stride = _validate_sequences(query_start_loc, seq_lens, block_table, device)
     with _on_device(device):
         status = _lib.lib().rq_quantize_fp8(
             key.data_ptr(), key_stride, value.data_ptr(), value_stride, rows, kv_heads, head_dim, cache.data_ptr(),
             scales.data_ptr(), blocks, page_tokens, query_start_loc.data_ptr(), seq_lens.data_ptr(), requests,
-            block_table.data_ptr(), max(block_table.stride(0), block_table.size(1)), block_table.size(1),
-            _stream(device))
+            block_table.data_ptr(), table_stride, pages, _stream(device))
     _lib.check(status)
 
 
@@ -404,6 +410,13 @@ def paged_attention_fp8_workspace_bytes(rows: int, heads: int, kv_heads: int, he
     """Device workspace (bytes) for ``paged_attention_fp8``; depends on shapes only."""
     return int(_lib.lib().rq_paged_attention_fp8_workspace_bytes(rows, heads, kv_heads, head_dim, max_pages,
                                                                  page_tokens))
+
+
+@lru_cache(maxsize=256)
+def _fp8_workspace_bytes(device: int, *shape: int) -> int:
+    # (Computed for the compute units of the device.)
+    with _on_device(device):
+        return paged_attention_fp8_workspace_bytes(*shape)
 
 
 def paged_attention_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor,
@@ -431,27 +444,25 @@ def paged_attention_fp8(query: torch.Tensor, key: torch.Tensor, value: torch.Ten
     device = query.get_device()
     rows, heads, head_dim = shape
     kv_heads = key_shape[1]
-    _require(key.get_device() == device and value.get_device() == device and output.get_device() == device
-             and out_shape == shape and value_shape == key_shape and key_shape[0] == rows
-             and key_shape[2] == head_dim, "Q/K/V/output must have matching shapes and devices")
+    if not (key.get_device() == device and value.get_device() == device and output.get_device() == device
+            and out_shape == shape and value_shape == key_shape and key_shape[0] == rows
+            and key_shape[2] == head_dim):
+        raise RuntimeError("Q/K/V/output must have matching shapes and devices")
     _, blocks, _, page_tokens, _ = _validate_fp8_cache(cache, scales, device, kv_heads, head_dim)
-    requests = _validate_sequences(query_start_loc, seq_lens, block_table, device)
-    max_pages = block_table.size(1)
-    library = _lib.lib()
+    requests, max_pages, table_stride = _validate_sequences(query_start_loc, seq_lens, block_table, device)
     if workspace is None:
-        needed = library.rq_paged_attention_fp8_workspace_bytes(rows, heads, kv_heads, head_dim, max_pages, page_tokens)
-        workspace = torch.empty(needed, dtype=torch.uint8, device=query.device)
+        needed = _fp8_workspace_bytes(device, rows, heads, kv_heads, head_dim, max_pages, page_tokens)
+        workspace = query.new_empty(needed, dtype=torch.uint8)
     else:
         _require(workspace.get_device() == device and workspace.is_contiguous(),
                  "Contiguous attention workspace on the query device required")
     with _on_device(device):
-        status = library.rq_paged_attention_fp8(
+        status = _lib.lib().rq_paged_attention_fp8(
             query.data_ptr(), query_stride, key.data_ptr(), key_stride, value.data_ptr(), value_stride,
             output.data_ptr(), out_stride, rows, heads, kv_heads, head_dim, cache.data_ptr(), scales.data_ptr(),
             blocks, page_tokens, query_start_loc.data_ptr(), seq_lens.data_ptr(), requests, block_table.data_ptr(),
-            max(block_table.stride(0), max_pages), max_pages,
-            head_dim ** -0.5 if softmax_scale is None else float(softmax_scale), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _stream(device))
+            table_stride, max_pages, head_dim ** -0.5 if softmax_scale is None else float(softmax_scale),
+            workspace.data_ptr(), workspace.nbytes, _stream(device))
     _lib.check(status)
 
 

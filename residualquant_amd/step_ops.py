@@ -227,21 +227,27 @@ def linear_rows_int4(x: torch.Tensor, weight: Int4Weight, out: Optional[torch.Te
     The codes are exact in the products and the scales multiply each group's
     sum; the weight itself is never rounded to BF16.  ``x`` rows are 16-byte aligned.
     """
-    _rows(x, "x")
-    rows, in_features = x.shape
-    device = x.get_device()
-    _require(in_features == weight.in_features and weight.data.get_device() == device,
-             "x must have the weight's in_features and device")
+    # (A step makes hundreds of these calls: shapes and strides are read once.)
+    shape, strides = x.shape, x.stride()
+    if not (len(shape) == 2 and strides[1] == 1 and x.is_cuda and x.dtype is torch.bfloat16):
+        _rows(x, "x")
+    rows, in_features = shape
+    out_features, data, device = weight.out_features, weight.data, x.get_device()
+    if in_features != weight.in_features or data.get_device() != device:
+        raise RuntimeError("x must have the weight's in_features and device")
+    out_stride = out_features
     if out is None:
-        out = torch.empty((rows, weight.out_features), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((rows, out_features))
     else:
         _rows(out, "out")
-        _require(out.shape == (rows, weight.out_features) and out.device == x.device,
-                 "out must be [rows, out_features]")
+        if out.shape != (rows, out_features) or out.get_device() != device:
+            raise RuntimeError("out must be [rows, out_features]")
+        if rows > 1:
+            out_stride = out.stride(0)
     with _on_device(device):
         status = _lib.lib().rq_linear_rows_int4(
-            x.data_ptr(), x.stride(0) if rows > 1 else in_features, weight.data.data_ptr(), weight.data.numel(),
-            out.data_ptr(), out.stride(0) if rows > 1 else weight.out_features, rows, weight.out_features, in_features, weight.group, torch._C._cuda_getCurrentRawStream(device))
+            x.data_ptr(), strides[0] if rows > 1 else in_features, data.data_ptr(), data.numel(), out.data_ptr(),
+            out_stride, rows, out_features, in_features, weight.group, torch._C._cuda_getCurrentRawStream(device))
     _lib.check(status)
     return out
 
@@ -267,24 +273,25 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     add nothing to the entropy; a row of -inf alone, or with a NaN or +inf,
     gives NaN.  Equal logits rank by the lower token.
     """
-    _require(logits.is_cuda and logits.dim() == 2 and (logits.stride(1) == 1 or logits.size(1) == 1)
-             and logits.dtype in (torch.bfloat16, torch.float32),
-             "logits must be BF16 or FP32 [rows, vocab] on a HIP device with unit column stride")
-    rows, vocab = logits.shape
+    shape, strides, dtype = logits.shape, logits.stride(), logits.dtype
+    if not (logits.is_cuda and len(shape) == 2 and (strides[1] == 1 or shape[1] == 1)
+            and (dtype is torch.bfloat16 or dtype is torch.float32)):
+        raise RuntimeError("logits must be BF16 or FP32 [rows, vocab] on a HIP device with unit column stride")
+    rows, vocab = shape
     device = logits.get_device()
-    _require(tokens.get_device() == device and tokens.dtype is torch.int64 and tokens.dim() == 1
-             and tokens.is_contiguous() and tokens.numel() == rows,
-             "Contiguous INT64 tokens, one per row, on the logits' device required")
+    if not (tokens.get_device() == device and tokens.dtype is torch.int64 and tokens.dim() == 1
+            and tokens.is_contiguous() and tokens.numel() == rows):
+        raise RuntimeError("Contiguous INT64 tokens, one per row, on the logits' device required")
     top = int(top)
-    _require(0 <= top <= min(LOGPROBS_MAX_TOP, vocab),
-             f"0 to {LOGPROBS_MAX_TOP} alternatives, at most the vocabulary, required")
+    if not 0 <= top <= min(LOGPROBS_MAX_TOP, vocab):
+        raise RuntimeError(f"0 to {LOGPROBS_MAX_TOP} alternatives, at most the vocabulary, required")
     logprob = torch.empty(rows, dtype=torch.float32, device=logits.device)
     entropy = torch.empty_like(logprob)
-    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=logits.device)
-    top_tokens = torch.empty((rows, top), dtype=torch.int64, device=logits.device)
+    top_logprobs = logprob.new_empty((rows, top))
+    top_tokens = tokens.new_empty((rows, top))
     with _on_device(device):
         status = _lib.lib().rq_token_logprobs(
-            logits.data_ptr(), max(logits.stride(0), vocab), 0 if logits.dtype is torch.bfloat16 else 1, rows, vocab,
+            logits.data_ptr(), max(strides[0], vocab), 0 if dtype is torch.bfloat16 else 1, rows, vocab,
             tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), top, top_logprobs.data_ptr(),
             top_tokens.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
     _lib.check(status)
