@@ -462,12 +462,14 @@ void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
 //   2 rounds:  2048 x 5632, 64: 16.6 us (24.3); 4096 x 5632, 32: 16.7 (13.7)
 //   3 rounds:  11264 x 2048, 8: 6.8 us (7.4), 16: 9.0 (7.7); 6144 x 1024, 32: 5.7 (6.0)
 //   4 rounds:  16000 x 2048, 8: 8.3 us (7.1); 4096 x 1024, 64: 6.8 (6.5)
+// and with 4 waves: 16000 x 512, 16 (4 rounds): 4.9 us (5.3); 11264 x 512, 32 (6): 6.1 (6.8); 16000 x 512,
+// 32 (8): 7.2 (6.0).
 template <int Group>
 void launch_rows(const LinearInt4Params& p, hipStream_t stream) {
     const int blocks = (int)int4_blocks(p.in_features);
     const int64_t workgroups = int4_tiles(p.out_features) * ((p.rows + 15) / 16);
     const int64_t rounds = (workgroups + p.compute_units - 1) / p.compute_units;
-    const int64_t most = blocks <= 8 || (blocks <= 24 && p.rows <= 8) ? 3 : p.rows > 32 ? 2 : 1;
+    const int64_t most = blocks <= 4 ? 6 : blocks <= 8 || (blocks <= 24 && p.rows <= 8) ? 3 : p.rows > 32 ? 2 : 1;
     if (blocks <= 48 && rounds <= most) {
         // (Four waves where they hold all inputs: 6144 x 512, 16 rows 3.5 us against 4.6 with eight, which
         // at 1024 inputs take 3.3 against 3.6; sixteen past 24 blocks: 2048 x 4096, one row 4.7 against 4.9.)

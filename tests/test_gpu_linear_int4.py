@@ -81,10 +81,10 @@ def test_wide_and_deep_weights_are_exact_on_small_integers(device, rows, group, 
     assert torch.equal(got.cpu(), want.to(torch.bfloat16))
 
 
-@pytest.mark.parametrize("rows", [3, 40])
-def test_wide_weight_nan_and_infinity(device, rows):
+@pytest.mark.parametrize("rows,features", [(3, 256), (40, 256), (3, 1152), (16, 1152)])
+def test_wide_weight_nan_and_infinity(device, rows, features):
     """As the narrow ones: on the row of the NaN or infinity only, the others as without it."""
-    out, features = 16643, 256
+    out = 16643
     codes, scales = _weight(out, features, 64, seed=8)
     codes[codes == 0] = 1
     weight = step_ops.pack_weight_int4(codes.to(device), scales.to(device))
