@@ -291,7 +291,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     top_tokens = tokens.new_empty((rows, top))
     with _on_device(device):
         status = _lib.lib().rq_token_logprobs(
-            logits.data_ptr(), max(strides[0], vocab), 0 if dtype is torch.bfloat16 else 1, rows, vocab,
+            logits.data_ptr(), strides[0] if rows > 1 else vocab, 0 if dtype is torch.bfloat16 else 1, rows, vocab,
             tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), top, top_logprobs.data_ptr(),
             top_tokens.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
     _lib.check(status)

@@ -161,3 +161,14 @@ def test_streams_graphs_and_refusals(device):
                   dict(logits=x.t().contiguous().t()), dict(logits=x[0])):
         with pytest.raises(RuntimeError):
             step_ops.token_logprobs(**{"logits": x, "tokens": t, "top": 2, **wrong})
+
+
+def test_expanded_rows_are_refused(device):
+    """Rows that share memory (stride 0) are not rows of vocab logits; one row may have any stride."""
+    row, tokens = torch.randn(1, 500, device=device), torch.zeros(4, dtype=torch.int64, device=device)
+    with pytest.raises(RuntimeError, match="unit column stride"):
+        step_ops.token_logprobs(row.expand(4, 500), tokens)
+    with pytest.raises(RuntimeError, match="unit column stride"):
+        step_ops.token_logprobs(torch.randn(2000, device=device).as_strided((4, 500), (100, 1)), tokens)
+    odd = torch.randn(2000, device=device).as_strided((1, 500), (3, 1))
+    _check(odd.cpu().contiguous(), tokens[:1].cpu(), 3, device, got=step_ops.token_logprobs(odd, tokens[:1], top=3))
