@@ -15,6 +15,7 @@
 // as rows with NaN or infinities do) are ranked by counting.
 #include "rq_device.h"
 #include "rq_plan.h"
+#include "rq_rank.h"
 #include "rq_reduced.h"
 
 namespace rq {
@@ -32,17 +33,6 @@ __device__ __forceinline__ float logit_at(const void* logits, int64_t i) {
         return bf16_f32(static_cast<const uint16_t*>(logits)[i]);
     else
         return static_cast<const float*>(logits)[i];
-}
-
-// Order of values as numbers: -0 and +0 alike, NaN above all.
-__device__ __forceinline__ uint32_t ordered_bits(float x) {
-    const uint32_t u = __float_as_uint(x + 0.0f);
-    return x != x ? 0xffffffffu : (u >> 31) ? ~u : u | 0x80000000u;
-}
-
-// Order of (value, index): equal values by the lower index.
-__device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
-    return ((uint64_t)ordered_bits(x) << 32) | (0xffffffffu - index);
 }
 
 __device__ __forceinline__ uint64_t shuffle_xor_u64(uint64_t v, int d) {
@@ -170,13 +160,11 @@ __device__ __noinline__ void logprobs_plain(const LogprobParams& p, int64_t row,
                                                        : __builtin_nanf("");
         p.entropy[row] = log_sum - weighted / sum;
     }
-    uint64_t below = ~0ull;
+    uint64_t below = kAboveKeys;
     for (int k = 0; k < p.top; ++k) {
         uint64_t best = 0;
-        for (int64_t i = threadIdx.x; i < p.vocab; i += Threads) {
-            const uint64_t key = rank_key(logit_at<Bf16>(p.logits, base + i), (uint32_t)i);
-            if (key < below && key > best) best = key;
-        }
+        for (int64_t i = threadIdx.x; i < p.vocab; i += Threads)
+            best = next_rank(best, rank_key(logit_at<Bf16>(p.logits, base + i), (uint32_t)i), below);
         below = best = block_max_u64<Threads>(best, keys);
         if (threadIdx.x == 0) {
             const int64_t index = 0xffffffffu - (uint32_t)best;
@@ -351,7 +339,7 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     // 16 lanes count one candidate's rank.
     for (int c0 = 0; c0 < found; c0 += Threads / 16) {
         const int c = c0 + (tid >> 4);
-        const uint64_t key = c < found ? candidates[c] : ~0ull;
+        const uint64_t key = c < found ? candidates[c] : kAboveKeys;
         uint32_t rank = 0;
         for (int o = tid & 15; o < found; o += 16) rank += candidates[o] > key ? 1 : 0;
         rank += plan_dpp<0xB1>(rank);   // quad_perm [1,0,3,2]

@@ -172,3 +172,26 @@ def test_expanded_rows_are_refused(device):
         step_ops.token_logprobs(torch.randn(2000, device=device).as_strided((4, 500), (100, 1)), tokens)
     odd = torch.randn(2000, device=device).as_strided((1, 500), (3, 1))
     _check(odd.cpu().contiguous(), tokens[:1].cpu(), 3, device, got=step_ops.token_logprobs(odd, tokens[:1], top=3))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 32, 33, 3001])
+def test_nan_ranks_first_wherever_it_is(device, dtype, vocab):
+    """NaN at token 0, at the last and everywhere, beside infinities, with as many alternatives as there are tokens."""
+    logits, tokens = _logits(6, vocab, dtype, seed=vocab)
+    logits[0, 0] = torch.nan
+    logits[1, vocab - 1] = torch.nan
+    logits[2] = torch.nan
+    logits[3, ::2] = torch.nan
+    logits[4] = -torch.inf
+    logits[4, 0] = torch.nan
+    logits[5, vocab // 2] = torch.inf
+    top = min(32, vocab)
+    print(f"vocab={vocab} top={top} {dtype}", flush=True)
+    got = step_ops.token_logprobs(logits.to(device), tokens.to(device), top=top)
+    for row in range(6):
+        x = logits[row].float()
+        order = sorted(range(vocab), key=lambda i: (not x[i].isnan(), -x[i] if not x[i].isnan() else 0.0, i))
+        assert got.top_tokens[row].tolist() == order[:top], row
+    assert bool(got.logprob.isnan().all()) and bool(got.entropy.isnan().all())
+    assert bool(got.top_logprobs.isnan().all())
