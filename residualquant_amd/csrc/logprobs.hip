@@ -4,8 +4,11 @@
 //
 // One workgroup reads a row once, in chunks of 8 logits per thread.  A thread
 // keeps the sums against a reference that follows its running maximum only
-// when a logit exceeds it by 2^8 (log2 units), and its largest logit with the
-// chunk that holds it first.  Alternatives: the threads of one lane number
+// when a logit exceeds it by 5.5 (a weight of 2^8), and its largest logit with
+// the chunk that holds it first.  The reference is a logit itself and is
+// subtracted before the scale of e^ to 2^: one fma(x, log2(e), -reference)
+// would be an instruction less per logit, but leaves the maximum of a row
+// around 10^10 with e^ of the hundreds that log2(e) x is rounded by.  Alternatives: the threads of one lane number
 // form one of 64 owners.  With T the `top`-th largest of the owners' largest
 // (value, chunk) - greater values first, then lower chunks - at least `top`
 // logits lie at or above T, so every alternative does; and logits at or above
@@ -24,8 +27,8 @@ namespace {
 
 constexpr int kChunk = 8;
 constexpr int kMaxCandidates = 2048;
-constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
-constexpr float kSlack = 8.0f;
+constexpr float kLog2e = 1.44269504088896341f, kSlack = 5.5f;
+constexpr float kLowest = -3.402823466e+38f;
 
 template <bool Bf16>
 __device__ __forceinline__ float logit_at(const void* logits, int64_t i) {
@@ -90,12 +93,16 @@ struct Row {
     }
 };
 
-// a * b, 0 where a is 0 (whatever b).
-__device__ __forceinline__ float mul_zero(float a, float b) { return a == 0.f ? 0.f : a * b; }
-
-// Sums of e^(x - m) and of e^(x - m) (x - m) in log2 units, with m = high.
+// Sums of e^(x - m) and of e^(x - m) (x - m), with m = high.
 struct Sums {
     float high, sum, weighted;
+    // The sums against `above` >= high.  (A sum that is NaN stays; the difference may pass the range.)
+    __device__ __forceinline__ void refer_to(float above) {
+        const float down = high - above, keep = __builtin_amdgcn_exp2f(down * kLog2e);
+        weighted = keep == 0.f ? 0.f : (weighted + sum * down) * keep;
+        sum *= keep;
+        high = above;
+    }
 };
 
 // Sum over the wave, in every lane.
@@ -196,7 +203,7 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     }
 
     // One pass: the sums, and the thread's largest logit with its first chunk.
-    Sums own{-3.0e38f, 0.f, 0.f};
+    Sums own{kLowest, 0.f, 0.f};
     float largest = -__builtin_inff();
     uint32_t largest_chunk = 0xffffffffu;
     auto take = [&](int q, const float (&x)[kChunk]) {
@@ -206,17 +213,11 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
             largest_chunk = (uint32_t)q;
             largest = fmaxf(most, largest);
         }
-        if (__any(most * kLog2e > own.high + kSlack)) {
-            const float high = fmaxf(own.high, most * kLog2e);
-            const float down = own.high - high, keep = __builtin_amdgcn_exp2f(down);
-            own.weighted = (own.weighted + mul_zero(own.sum, down)) * keep;
-            own.sum *= keep;
-            own.high = high;
-        }
+        if (__any(most > own.high + kSlack)) own.refer_to(fmaxf(own.high, most));
 #pragma unroll
         for (int e = 0; e < kChunk; ++e) {
-            const float d = fmaf(x[e], kLog2e, -own.high);
-            const float w = __builtin_amdgcn_exp2f(d);
+            const float d = x[e] - own.high;
+            const float w = __builtin_amdgcn_exp2f(d * kLog2e);
             own.sum += w;
             own.weighted = fmaf(w, fmaxf(d, -1000.0f), own.weighted);  // 0 where w is 0, also at d = -inf
         }
@@ -263,27 +264,23 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
     for (int w = 1; w < kWaves; ++w) owner = keys[64 * w + lane] > owner ? keys[64 * w + lane] : owner;
     const uint32_t ordered = wave_max_u32((uint32_t)(owner >> 32));
     const float m = __uint_as_float((ordered >> 31) ? ordered & 0x7fffffffu : ~ordered);
-    // The thread's sums against m itself.  Its reference is a rounded m' log2(e); one
-    // rounding of the difference keeps large logits exact.
-    const float above_reference = fmaf(m, kLog2e, -own.high), keep = __builtin_amdgcn_exp2f(-above_reference);
-    const float weighted_here = own.sum == 0.f ? 0.f : (own.weighted - above_reference * own.sum) * keep;
-    const float sum_here = own.sum == 0.f ? 0.f : own.sum * keep;
-    const float wave_total = wave_sum(sum_here), wave_weighted = wave_sum(weighted_here);
+    own.refer_to(m);
+    const float wave_total = wave_sum(own.sum), wave_weighted = wave_sum(own.weighted);
     if (lane == 0) wave_sums[wave] = make_float2(wave_total, wave_weighted);
     __syncthreads();
     float2 part = make_float2(0.f, 0.f);
     if (lane < kWaves) part = wave_sums[lane];
     const float exact_sum = wave_sum(part.x), weighted = wave_sum(part.y);
     const float log_sum = logf(exact_sum);
-    // NaN, infinities (S is NaN), nothing but -inf (m), or values near the lowest.
-    if (!(m > -1.0e38f && m < 1.0e38f && exact_sum < 1.0e38f)) {
+    // NaN, infinities, nothing but -inf: S is NaN or m is not finite.  (Else S is 1 and more.)
+    if (!(fabsf(m) < __builtin_inff() && exact_sum >= 0.5f && exact_sum < 1.0e38f)) {
         __syncthreads();
         logprobs_plain<Bf16, Threads>(p, row_number, false, keys, reinterpret_cast<float*>(wave_sums));
         return;
     }
     if (tid == 0) {
         p.logprob[row_number] = token_logit - m - log_sum;
-        p.entropy[row_number] = log_sum - weighted * kLn2 / exact_sum;
+        p.entropy[row_number] = log_sum - weighted / exact_sum;
     }
     if (p.top == 0) return;
 

@@ -195,3 +195,46 @@ def test_nan_ranks_first_wherever_it_is(device, dtype, vocab):
         assert got.top_tokens[row].tolist() == order[:top], row
     assert bool(got.logprob.isnan().all()) and bool(got.entropy.isnan().all())
     assert bool(got.top_logprobs.isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [900, 50257])
+def test_logits_far_from_zero(device, dtype, vocab):
+    """Rows around +-5e9 and more, where log2(e) x has a rounding of hundreds: the maximum has e^0 all the same."""
+    for k, at in enumerate((5e9, 1e10, 2e10, 1e20, 1e30, 3e38, -5e10, -1e11, -1e12, -1e30, -3e38, 2.0 ** 100, -2.0 ** 100)):
+        logits, tokens = _logits(4, vocab, dtype, seed=30 + k)
+        logits = logits.float()
+        logits[0] += at                        # equal, or a unit apart
+        logits[1] = at * (1 + logits[1].abs() * 2.0 ** -10).clamp(max=1.1)
+        logits[2] = at
+        logits[3] = at * 0.75
+        logits[3, vocab // 3] = at
+        tokens[3] = vocab // 3
+        _check(logits.clamp(-3.38e38, 3.38e38).to(dtype), tokens, 3, device)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("mask", [-1e4, -1e10, -1e20, -1e30, -2.0 ** 120, -2.0 ** 126, -1e38, -2e38, -3.38e38])
+def test_finite_masks(device, dtype, mask):
+    """Ruled-out tokens held as a finite value, in stretches that whole threads see nothing else of, first, last or all."""
+    logits, tokens = _logits(6, 20011, dtype, seed=44)
+    logits[0, 5000:] = mask
+    logits[1, :15000] = mask
+    logits[2, torch.rand(20011, generator=torch.Generator().manual_seed(3)) < 0.9] = mask
+    logits[3, 4096:] = mask
+    logits[3, :4096:2] = mask
+    logits[4] = mask
+    logits[5] = mask
+    logits[5, 777] = 2.0
+    _check(logits, tokens, 4, device)
+
+
+def test_finite_masks_are_as_infinite_ones(device):
+    """A row masked with a finite value gives what the row masked with -inf gives, where neither value has a weight."""
+    logits, tokens = _logits(3, 49152, torch.float32, seed=45)
+    out = torch.rand(49152, generator=torch.Generator().manual_seed(4)) < 0.3
+    out[tokens] = False
+    want = step_ops.token_logprobs(logits.masked_fill(out, -torch.inf).to(device), tokens.to(device), top=8)
+    for mask in (-1e4, -1e10, -1e30, -1e38):
+        got = step_ops.token_logprobs(logits.masked_fill(out, mask).to(device), tokens.to(device), top=8)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), mask
