@@ -101,7 +101,8 @@ class LoopedDecoder:
 
     With ``top_logprobs`` (0 to 32) every step also leaves the log probability
     of each next token, the entropy and that many alternatives in ``logprobs``
-    (``step_ops.TokenLogprobs``)."""
+    (``step_ops.TokenLogprobs``); after ``capture()`` these are the captured
+    step's tensors, which every later step, eager or replayed, overwrites."""
 
     def __init__(self, config: LoopedConfig, batch: int, context: int, max_new_tokens: int,
                  device: torch.device, seed: int = 0, weights_from: Optional["LoopedDecoder"] = None,
@@ -303,7 +304,12 @@ class LoopedDecoder:
         # Greedy next token and the next position, slot and sequence length.
         self.tokens.copy_(logits.argmax(dim=-1))
         if self.top_logprobs is not None:
-            self.logprobs = step_ops.token_logprobs(logits, self.tokens, top=self.top_logprobs)
+            scored = step_ops.token_logprobs(logits, self.tokens, top=self.top_logprobs)
+            if capturing or self.graph is None:
+                self.logprobs = scored
+            else:  # an eager step beside a captured one, whose replays write these tensors
+                for held, fresh in zip(self.logprobs, scored):
+                    held.copy_(fresh)
         self.positions.add_(1)
         self.seq_lens.add_(1)
         self._update_slots()

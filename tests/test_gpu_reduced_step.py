@@ -155,3 +155,19 @@ def test_looped_decoder_of_many_rows_and_refusals(device):
         LoopedDecoder(_small_config(projection_bits=8), 1, 20, 4, device)
     with pytest.raises(ValueError, match="alternatives"):
         LoopedDecoder(_small_config(), 1, 20, 4, device, top_logprobs=33)
+
+
+def test_looped_decoder_logprobs_of_the_last_step_however_it_ran(device):
+    """Captured and eager steps in turn: ``logprobs`` is the last step's, also where the graph itself is replayed."""
+    decoder = LoopedDecoder(_small_config(), 3, 40, 9, device, seed=7, top_logprobs=4)
+    decoder.build_history(seed=5)
+    graph = decoder.capture()
+    for run in (decoder.replay, decoder.step, decoder.replay, decoder.step, decoder.step, graph.replay):
+        logits = run()
+        torch.cuda.synchronize()
+        logits = decoder.logits if logits is None else logits
+        check_logprobs(logits.cpu(), decoder.tokens.cpu(), 4, device, got=decoder.logprobs)
+    decoder.capture()
+    logits = decoder.replay()
+    torch.cuda.synchronize()
+    check_logprobs(logits.cpu(), decoder.tokens.cpu(), 4, device, got=decoder.logprobs)
