@@ -4,7 +4,7 @@
 // Packed layout, made once from the codes: tiles of 16 output rows, in a tile
 // blocks of 128 inputs of 1 KB each.  Lane l of a wave reads 16 bytes at
 // 16 l: word i holds the codes of row l % 16 at inputs 32 i + 8 (l / 16) + e,
-// e = 0..7 (code_shift), the A operand of v_mfma_f32_16x16x32 for 16 output
+// e = 0..7 (code_word), the A operand of v_mfma_f32_16x16x32 for 16 output
 // rows.  Rows and inputs past the weight hold code 0.  The scales follow (scale_place),
 // in the order in which the lanes of the product's result need them.
 #include <algorithm>
@@ -16,19 +16,20 @@ namespace rq {
 
 namespace {
 
-// The lowest bit of code e in its word.  The codes (plus 8, unsigned) of e =
-// 0, 2, 4, 6 fill the lower and of 1, 3, 5, 7 the upper half word, and the word
-// is rotated left by 3: the pair (0, 1) stands at bits 3 and 19, in the upper
-// mantissa bits of two BF16 numbers.
-__device__ __forceinline__ int code_shift(int e) { return (3 + 4 * (e >> 1) + 16 * (e & 1)) & 31; }
+__device__ __forceinline__ uint32_t rotate_right(uint32_t x, int n) { return __builtin_amdgcn_alignbit(x, x, n); }
 
-__device__ __forceinline__ uint32_t rotate_left(uint32_t x, int n) {
-    n &= 31;
-    return n == 0 ? x : (x << n) | (x >> (32 - n));
+// Code c as element e of its word: a sign s and three bits m, c = m or -m - 1.
+// Elements 0..3 have m in the lowest bits and s in the top bit of byte e, 4..7
+// the same after a rotation by 4 bits (code_bytes).
+__device__ __forceinline__ uint32_t code_word(int c, int e) {
+    const uint32_t byte = c < 0 ? 0x80u | (uint32_t)(-c - 1) : (uint32_t)c, word = byte << (8 * (e & 3));
+    return e < 4 ? word : rotate_right(word, 28);
 }
 
 __device__ __forceinline__ int code_at(uint32_t word, int e) {
-    return (int)(rotate_left(word, 32 - code_shift(e)) & 15u) - 8;
+    const uint32_t byte = (e < 4 ? word : rotate_right(word, 4)) >> (8 * (e & 3));
+    const int m = (int)(byte & 7u);
+    return byte & 0x80u ? -m - 1 : m;
 }
 
 __host__ __device__ __forceinline__ int64_t int4_tiles(int64_t out_features) { return (out_features + 15) / 16; }
@@ -79,7 +80,7 @@ __global__ __launch_bounds__(256) void pack_int4_kernel(const Int4PackParams p) 
         } else if (inside) {
             code = min(max((int)p.codes[n * p.in_features + k + e], -8), 7);
         }
-        word |= rotate_left((uint32_t)(code + 8), code_shift(e));
+        word |= code_word(code, e);
     }
     p.packed[w] = word;
 }
@@ -106,31 +107,28 @@ __device__ __forceinline__ F32x4 mfma(U32x4 a, U32x4 b, F32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
 }
 
-// The eight codes of a word as BF16 numbers 1 + (c + 8) / 16, in three shifts
-// and four v_and_or: a code takes the upper four mantissa bits of a 1.
-__device__ __forceinline__ U32x4 codes_bf16(uint32_t word) {
-    constexpr uint32_t kMantissa = 0x00780078u, kOne = 0x3f803f80u;
-    return U32x4{(word & kMantissa) | kOne, ((word >> 4) & kMantissa) | kOne, ((word >> 8) & kMantissa) | kOne,
-                 (__builtin_amdgcn_alignbit(word, word, 12) & kMantissa) | kOne};
+// Two E4M3 bytes (of the low or high half word of x) as two BF16, exactly.
+template <bool High>
+__device__ __forceinline__ uint32_t bf16x2_of_fp8(uint32_t x) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, High));
 }
 
-// y of `rows` rows and of the outputs 16 tile0.. of `tiles` tiles in plain steps, for results that are
-// not finite: the products of shifted codes overflow earlier than the sum
-// itself, and turn an infinity in x into NaN.
-__device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int tiles, int64_t first_row, int rows, int threads) {
-    const int64_t blocks = int4_blocks(p.in_features);
-    for (int64_t o = threadIdx.x; o < (int64_t)tiles * 16 * rows; o += threads) {
-        const int64_t tile = tile0 + o / 16 % tiles, n = 16 * tile + o % 16, m = first_row + o / (16 * tiles);
-        if (n >= p.out_features) continue;
-        float sum = 0.f;
-        for (int64_t k = 0; k < p.in_features; k += 8) {
-            const uint32_t word = p.packed[((tile * blocks + k / 128) * 64 + (n & 15) + 16 * (k / 8 % 4)) * 4 + k / 32 % 4];
-            const float scale = bf16_f32(p.packed_scales[scale_place(tile, blocks, k / p.group, p.group, (int)(n & 15))]);
-            for (int e = 0; e < 8; ++e) sum += (float)code_at(word, e) * (bf16_f32(p.x[m * p.x_stride + k + e]) * scale);
-        }
-        p.y[m * p.y_stride + n] = (uint16_t)bf16_rn(sum);
-    }
+// Four codes as E4M3 bytes of c x 2^-9: bytes 0..15 are the multiples 0..15 of
+// 2^-9 (the lowest exponents of E4M3 are linear), so the byte of |c| is |c|
+// itself, m + s, below the sign.
+__device__ __forceinline__ uint32_t code_bytes(uint32_t word) {
+    return (word & 0x87878787u) + ((word >> 7) & 0x01010101u);
 }
+
+// The eight codes of a word as BF16 numbers c x 2^-9, each exact: 13 vector
+// instructions.  (Seven make 1 + (c + 8) / 16, and c x from it less 1.5 x: then
+// every input counts with 24 times its size, also under a code of 0, and one
+// that is not finite takes the other codes' sums with it.)
+__device__ __forceinline__ U32x4 codes_bf16(uint32_t word) {
+    const uint32_t low = code_bytes(word), high = code_bytes(rotate_right(word, 4));
+    return U32x4{bf16x2_of_fp8<false>(low), bf16x2_of_fp8<true>(low), bf16x2_of_fp8<false>(high), bf16x2_of_fp8<true>(high)};
+}
+constexpr float kCodeUnit = 512.0f;  // of the sums
 
 // One workgroup of eight waves per 8 / WK x NB tiles of 16 outputs, for all
 // rows (T tiles of 16).  x passes through LDS, in chunks of `chunk_blocks`
@@ -139,10 +137,6 @@ __device__ void linear_int4_plain(const LinearInt4Params& p, int64_t tile0, int 
 // wave took most of the time (64 rows x 16 outputs x 2048 inputs, one
 // workgroup: 10.3 us, 8 of them for x).  WK waves share a tile's inputs out; a
 // wave keeps the codes of kAhead blocks in flight.
-//
-// With u = c + 8 and v = 1 + u / 16 (codes_bf16), sum c x = 16 (sum v x - 1.5
-// sum x): the second sum, from a constant operand, is the accumulator that the
-// first starts with, once per group for all tiles of a wave.
 typedef __attribute__((address_space(3))) void LdsVoid;
 
 // One DMA load: lane l's 16 bytes at `offset` of the resource go to lds + 16 l (lds wave-uniform).
@@ -196,8 +190,6 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
     const uint8_t* x_row[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) x_row[t] = lds + min(16 * t + i, rows - 1) * row_bytes + 16 * g;
-    // [block][group][row]: -1.5 sum x, behind the rows of x.
-    float* const starts = reinterpret_cast<float*>(lds + rows * row_bytes);
     auto compute = [&](const Codes& b, int block) {
         U32x4 x[T][4];
 #pragma unroll
@@ -206,17 +198,11 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
             for (int s = 0; s < 4; ++s) x[t][s] = *reinterpret_cast<const U32x4*>(x_row[t] + 256 * block + 64 * s);
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
-            F32x4 start[T];
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-                const float value = starts[(block * kPer + h) * (16 * T) + 16 * t + i];
-                start[t] = F32x4{value, value, value, value};
-            }
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
                 F32x4 sum[T];
 #pragma unroll
-                for (int t = 0; t < T; ++t) sum[t] = start[t];
+                for (int t = 0; t < T; ++t) sum[t] = F32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < kGroupSteps; ++s) {
                     const U32x4 a = codes_bf16(b.words[j][h * kGroupSteps + s]);
@@ -257,20 +243,6 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
         }
         wait_vector_memory();
         __syncthreads();
-        for (int b = wave; b < count; b += 8) {
-            const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
-#pragma unroll
-            for (int h = 0; h < kPer; ++h)
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    F32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int s = 0; s < kGroupSteps; ++s)
-                        sum = mfma(shift, *reinterpret_cast<const U32x4*>(x_row[t] + 256 * b + 64 * (h * kGroupSteps + s)), sum);
-                    if (g == 0) starts[(b * kPer + h) * (16 * T) + 16 * t + i] = sum[0];
-                }
-        }
-        __syncthreads();
         for (int b = begin; b < end; b += kAhead) {
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
@@ -281,22 +253,18 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
     }
 
     // ---------------------------------------------------------------- join
-    bool finite = true;
     auto write = [&](F32x4 sum, int64_t tile, int t) {
         const int64_t n = 16 * tile + 4 * g, m = 16 * t + i;
         if (m >= p.rows) return;
         if (p.aligned && n + 4 <= p.out_features) {
-            finite = finite && fabsf(sum[0]) < __builtin_inff() && fabsf(sum[1]) < __builtin_inff() &&
-                     fabsf(sum[2]) < __builtin_inff() && fabsf(sum[3]) < __builtin_inff();
             *reinterpret_cast<uint2*>(p.y + m * p.y_stride + n) =
-                make_uint2(bf16x2_rn(16.0f * sum[0], 16.0f * sum[1]), bf16x2_rn(16.0f * sum[2], 16.0f * sum[3]));
+                make_uint2(bf16x2_rn(kCodeUnit * sum[0], kCodeUnit * sum[1]), bf16x2_rn(kCodeUnit * sum[2], kCodeUnit * sum[3]));
             return;
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (n + r >= p.out_features) break;
-            finite = finite && fabsf(sum[r]) < __builtin_inff();
-            p.y[m * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * sum[r]);
+            p.y[m * p.y_stride + n + r] = (uint16_t)bf16_rn(kCodeUnit * sum[r]);
         }
     };
     if constexpr (WK == 1) {
@@ -320,15 +288,12 @@ __global__ __launch_bounds__(kLinearInt4Threads) void linear_int4_kernel(const L
             write(sum, tile0 + q / T, q % T);
         }
     }
-    const int64_t workgroup_tile = (int64_t)blockIdx.x * (8 / WK) * NB;
-    if (__syncthreads_or(!finite))
-        linear_int4_plain(p, workgroup_tile, (int)min((int64_t)(8 / WK) * NB, tiles - workgroup_tile), 0, rows, kLinearInt4Threads);
 }
 
 // One workgroup of W waves per tile of 16 outputs and 16 rows: x goes from
 // global memory to the operands without LDS, which saves few rows a copy and a
 // barrier.  All of a wave's blocks, at most kBlocks, are in flight at once;
-// past its last one a wave reads that block again, with scales of 0 (a branch
+// past its last one a wave reads that block again and leaves its sums out (a branch
 // around it would let the compiler move its loads behind the first block's products).
 template <int Group, int kBlocks, int W>
 __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt4Params p) {
@@ -352,8 +317,8 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
 #pragma unroll
         for (int h = 0; h < kPer; ++h) {
             const uint2 v = reinterpret_cast<const uint2*>(from)[h];
-            scales[a][2 * h] = begin + a < end ? v.x : 0u;
-            scales[a][2 * h + 1] = begin + a < end ? v.y : 0u;
+            scales[a][2 * h] = v.x;
+            scales[a][2 * h + 1] = v.y;
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
@@ -363,17 +328,11 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
     }
     __builtin_amdgcn_sched_barrier(0);
     F32x4 total = {0.f, 0.f, 0.f, 0.f};
-    const U32x4 shift = {0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u, 0xbfc0bfc0u};  // -1.5
 #pragma unroll
     for (int a = 0; a < kBlocks; ++a) {
         F32x4 sum[kPer];
 #pragma unroll
-        for (int h = 0; h < kPer; ++h) {
-            sum[h] = F32x4{0.f, 0.f, 0.f, 0.f};
-            // (Groups past the inputs hold no scale: 0 times what is read there again.)
-#pragma unroll
-            for (int s = 0; s < kGroupSteps; ++s) sum[h] = mfma(shift, x[a][h * kGroupSteps + s], sum[h]);
-        }
+        for (int h = 0; h < kPer; ++h) sum[h] = F32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < kGroupSteps; ++s)
 #pragma unroll
@@ -383,13 +342,14 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
         for (int h = 0; h < kPer; ++h) {
             const float scale[4] = {__uint_as_float(scales[a][2 * h] << 16), __uint_as_float(scales[a][2 * h] & 0xffff0000u),
                                     __uint_as_float(scales[a][2 * h + 1] << 16), __uint_as_float(scales[a][2 * h + 1] & 0xffff0000u)};
+            // (What was read again may hold infinities: no sum of it counts, not even times 0.)
+            const bool counts = begin + a < end && 128 * (begin + a) + Group * h < in_features;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) total[r] = fmaf(scale[r], sum[h][r], total[r]);
+            for (int r = 0; r < 4; ++r) total[r] = counts ? fmaf(scale[r], sum[h][r], total[r]) : total[r];
         }
     }
     partial[wave][lane] = total;
     __syncthreads();
-    bool finite = true;
     if (wave == 0 && i < rows) {
 #pragma unroll
         for (int w = 1; w < W; ++w) total += partial[w][lane];
@@ -397,15 +357,27 @@ __global__ __launch_bounds__(64 * W) void linear_int4_few_kernel(const LinearInt
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (n + r >= p.out_features) break;
-            finite = finite && fabsf(total[r]) < __builtin_inff();
-            p.y[(first_row + i) * p.y_stride + n + r] = (uint16_t)bf16_rn(16.0f * total[r]);
+            p.y[(first_row + i) * p.y_stride + n + r] = (uint16_t)bf16_rn(kCodeUnit * total[r]);
         }
     }
-    if (__syncthreads_or(!finite)) linear_int4_plain(p, tile, 1, first_row, rows, 64 * W);
 }
 
+// One workgroup per tile of 16 outputs, in plain steps: rows of x too far
+// apart for the others' addresses.
 __global__ __launch_bounds__(256) void linear_int4_plain_kernel(const LinearInt4Params p) {
-    linear_int4_plain(p, blockIdx.x, 1, 0, (int)p.rows, 256);
+    const int64_t blocks = int4_blocks(p.in_features), tile = blockIdx.x;
+    for (int o = threadIdx.x; o < 16 * (int)p.rows; o += 256) {
+        const int64_t n = 16 * tile + o % 16, m = o / 16;
+        if (n >= p.out_features) continue;
+        float sum = 0.f;
+        for (int64_t k = 0; k < p.in_features; k += 8) {
+            const uint32_t word = p.packed[((tile * blocks + k / 128) * 64 + (n & 15) + 16 * (k / 8 % 4)) * 4 + k / 32 % 4];
+            const float scale = bf16_f32(p.packed_scales[scale_place(tile, blocks, k / p.group, p.group, (int)(n & 15))]);
+            for (int e = 0; e < 8; ++e)
+                sum = fmaf(scale, (float)code_at(word, e) / kCodeUnit * bf16_f32(p.x[m * p.x_stride + k + e]), sum);
+        }
+        p.y[m * p.y_stride + n] = (uint16_t)bf16_rn(kCodeUnit * sum);
+    }
 }
 
 template <int Group, int T, int NB, int WK>
@@ -427,9 +399,8 @@ void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
     const int blocks = (int)int4_blocks(p.in_features);
     LinearInt4Params q = p;
     q.aligned = p.y_stride % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0;
-    // x of one chunk in LDS with its sums: all of it up to 152 KB, else chunks of at most that.
-    constexpr int kPer = 128 / Group;
-    auto chunk_bytes = [&](int64_t count) { return p.rows * ((count + 3) / 4 * 1024 + kRowPad) + count * kPer * 16 * T * 4; };
+    // x of one chunk in LDS: all of it up to 152 KB, else chunks of at most that.
+    auto chunk_bytes = [&](int64_t count) { return p.rows * ((count + 3) / 4 * 1024 + kRowPad); };
     q.chunk_blocks = blocks;
     while (chunk_bytes(q.chunk_blocks) > 152 * 1024) q.chunk_blocks = (q.chunk_blocks - 1) / 4 * 4;  // (whole KB of a row)
     const size_t bytes = chunk_bytes(q.chunk_blocks);

@@ -216,3 +216,78 @@ def test_empty_and_refusals(device):
     with pytest.raises(RuntimeError, match="out must be"):
         step_ops.linear_rows_int4(torch.zeros((2, 64), dtype=torch.bfloat16, device=device), weight,
                                   out=torch.zeros((2, 31), dtype=torch.bfloat16, device=device))
+
+
+# Beside the codes and through shared memory, whole and in chunks, for one to four row tiles.
+ROUTES = [(1, 40, 256, 32), (7, 130, 2048, 64), (16, 300, 5632, 128), (40, 70, 512, 32), (3, 24, 6400, 64),
+          (20, 9000, 1152, 32), (33, 5000, 2048, 64), (64, 1037, 6400, 128), (16, 16643, 1152, 64)]
+
+
+def _far(x):
+    """The same rows 2^24 elements apart."""
+    store = torch.zeros((x.size(0) - 1) * (1 << 24) + x.size(1), dtype=torch.bfloat16, device=x.device)
+    return store.as_strided(x.shape, (1 << 24, 1)).copy_(x)
+
+
+@pytest.mark.parametrize("rows,out,features,group", ROUTES)
+def test_inputs_under_codes_of_zero_add_nothing(device, rows, out, features, group):
+    """An input whose codes are all 0 may have any finite size: the outputs are those without it, bit for bit."""
+    print(f"rows={rows} out={out} in={features} group={group}", flush=True)
+    codes, scales = _weight(out, features, group, seed=rows + out)
+    places = [3, features // 2 + 1, features - 1]
+    codes[:, places] = 0
+    scales[:, 0] = 16.0
+    weight = step_ops.pack_weight_int4(codes.to(device), scales.to(device))
+    x = torch.randn((rows, features), generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16).to(device)
+    x[:, places] = 0
+    want = step_ops.linear_rows_int4(x, weight)
+    wide = rows <= 3 and step_ops.linear_rows_int4(_far(x), weight)
+    for value in (1e3, -1e5, 1e8, 1e20, -3.3e38):
+        x[:, places] = value
+        assert torch.equal(step_ops.linear_rows_int4(x, weight), want), value
+        if rows <= 3:
+            assert torch.equal(step_ops.linear_rows_int4(_far(x), weight), wide), value
+
+
+@pytest.mark.parametrize("rows,out,features,group", ROUTES)
+def test_linear_with_outliers(device, rows, out, features, group):
+    """Channels of 10^4 times the others' size.  The bound: one BF16 rounding, and each addition of a group's products
+    and of the groups' sums off by 2^-23 of the terms' own size (a product of a code and an input is exact)."""
+    codes, scales = _weight(out, features, group, seed=rows + out + 1)
+    codes[torch.rand(codes.shape, generator=torch.Generator().manual_seed(2)) < 0.3] = 0
+    x = torch.randn((rows, features), generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16)
+    x[:, 5::97] *= 1e4
+    held = scales.double().repeat_interleave(group, dim=1) * codes.double()
+    want = x.double() @ held.t()
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -23 * (group + features // group + 16) * (x.double().abs() @ held.abs().t())
+    got = step_ops.linear_rows_int4(x.to(device), step_ops.pack_weight_int4(codes.to(device), scales.to(device)))
+    over = (got.cpu().double() - want).abs() / bound
+    assert over.max() <= 1.0, f"{over.max():.2f} times the bound"
+
+
+@pytest.mark.parametrize("rows,out,features,group", ROUTES)
+def test_nan_and_infinity_leave_other_outputs_alone(device, rows, out, features, group):
+    """A row or an output with NaN or infinities is what float64 makes of it, and every other one as without, bit for bit."""
+    codes, scales = _weight(out, features, group, seed=rows + out + 2)
+    x = torch.randn((rows, features), generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16)
+    weight = step_ops.pack_weight_int4(codes.to(device), scales.to(device))
+    plain = step_ops.linear_rows_int4(x.to(device), weight).cpu()
+    held = codes.double() * scales.double().repeat_interleave(group, dim=1)
+    hit = rows // 2
+    rest = [m for m in range(rows) if m != hit]
+    for place, value in ((0, torch.inf), (features - 1, -torch.inf), (features // 3, torch.nan), (features // 2, 3.3e38)):
+        y = x.clone()
+        y[hit, place] = value
+        got = step_ops.linear_rows_int4(y.to(device), weight).cpu()
+        want = (y[hit].double() @ held.t()).to(torch.bfloat16)
+        assert torch.equal(got[hit].isnan(), want.isnan()), value
+        assert torch.equal(got[hit].isposinf(), want.isposinf()) and torch.equal(got[hit].isneginf(), want.isneginf()), value
+        assert torch.equal(got[rest], plain[rest]), value
+    scales[out // 2, -1], scales[out - 1, 0] = torch.nan, torch.inf
+    codes[out - 1, 0], codes[out - 1, 1:group] = 1, 0  # (an infinite scale times one term: no NaN from codes of 0)
+    x[:, 0] = x[:, 0].abs() + 1
+    plain = step_ops.linear_rows_int4(x.to(device), weight).cpu()
+    got = step_ops.linear_rows_int4(x.to(device), step_ops.pack_weight_int4(codes.to(device), scales.to(device))).cpu()
+    assert bool(got[:, out // 2].isnan().all()) and bool(got[:, out - 1].isposinf().all())
+    rest = [n for n in range(out - 1) if n != out // 2]
+    assert torch.equal(got[:, rest], plain[:, rest])
