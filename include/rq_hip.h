@@ -308,7 +308,8 @@ int rq_linear_rows(const void* x, int64_t x_stride, const void* weight, void* y,
  * with an invalid block) are skipped.  A block that is written must belong to
  * one request of the call.  The call may be repeated: it writes the same.
  * key, value: BF16 [rows, kv_heads, head_dim], 8-byte aligned, token strides
- * multiples of 4 elements; max_pages x page_tokens at most 2^30.
+ * multiples of 4 elements; max_pages x page_tokens at most 2^30, and
+ * rows / page_tokens + 2 x requests below 2^24.
  */
 int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int64_t value_stride, int64_t rows,
                     int kv_heads, int head_dim, void* cache, float* scales, int64_t num_blocks, int page_tokens,
@@ -347,7 +348,8 @@ size_t rq_paged_attention_fp8_workspace_bytes(int64_t rows, int heads, int kv_he
  * codes c in -8..7 and one BF16 scale per output row and group of 32, 64 or
  * 128 inputs (in_features a multiple of the group), laid out once for the
  * kernel in rq_int4_weight_bytes(...) bytes of 16-byte aligned device memory
- * (0 for an invalid shape).
+ * (0 for an invalid shape).  out_features up to 2^24, in_features up to 2^20,
+ * together fewer than 2^35 elements in whole tiles of 16 x 128.
  * rq_pack_weight_int4 takes codes (INT8 [out, in], limited to -8..7) and
  * scales (BF16 [out, in / group]); rq_quantize_weight_int4 a BF16 weight:
  * scale = bf16(largest |w| of the group / 7), code = w / scale to nearest,

@@ -1185,6 +1185,9 @@ static int check_fp8_pages(const void* cache, const float* scales, int64_t num_b
     return RQ_OK;
 }
 
+// Threads of one dimension of a launch stay below 2^32.
+static bool launchable(int64_t workgroups, int64_t threads) { return workgroups < (((int64_t)1 << 32) / threads); }
+
 static int check_bf16_rows(const void* data, int64_t stride, int64_t rows, int64_t heads, int head_dim) {
     if (stride < heads * head_dim || stride % 4 != 0)
         return fail(RQ_EINVAL, "BF16 [tokens, heads, channels] with packed trailing strides, a multiple of 4 elements "
@@ -1204,6 +1207,7 @@ int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int6
     if (status == RQ_OK) status = check_bf16_rows(value, value_stride, rows, kv_heads, head_dim);
     if (status != RQ_OK) return status;
     if (rows == 0 || requests == 0 || num_blocks == 0 || max_pages == 0) return ok();
+    if (!launchable(rows / page_tokens + 2 * requests, 256)) return fail(RQ_EINVAL, "Too many rows and requests for one call");
     rq::Fp8WriteParams p{};
     p.key = static_cast<const uint16_t*>(key);
     p.key_stride = key_stride;
@@ -1342,7 +1346,8 @@ int rq_paged_attention_fp8(const void* query, int64_t query_stride, const void* 
     p.call_tag = next_call_tag();
     plan_fp8(p);
     const int64_t workgroups = p.items > 0 ? p.items : (rows * (heads / kv_heads) / p.tile + requests) * p.splits;
-    if (workgroups > (int64_t)INT32_MAX / kv_heads) return fail(RQ_EINVAL, "Too many rows, heads and requests for one call");
+    if (workgroups > (int64_t)INT32_MAX / kv_heads || !launchable(workgroups * kv_heads, p.tile == kFp8MaxTile ? 512 : 256))
+        return fail(RQ_EINVAL, "Too many rows, heads and requests for one call");
     return check_launch(rq::launch_attention_fp8(p, stream), "8-bit attention launch");
 }
 
@@ -1350,10 +1355,11 @@ int rq_paged_attention_fp8(const void* query, int64_t query_stride, const void* 
 static int check_int4_shape(int64_t out_features, int64_t in_features, int group) {
     if (group != 32 && group != 64 && group != 128)
         return fail(RQ_ENOKERNEL, "No compiled 4-bit projection kernel for groups of %d (32, 64 or 128)", group);
+    // (Packed by one thread per 8 elements of whole tiles of 16 x 128.)
     if (out_features <= 0 || in_features <= 0 || in_features % group != 0 || out_features > (1 << 24) ||
-        in_features > (1 << 20) || out_features * in_features > ((int64_t)1 << 40))
+        in_features > (1 << 20) || !launchable(((out_features + 15) / 16) * ((in_features + 127) / 128), 256))
         return fail(RQ_EINVAL, "4-bit weights need out_features up to 2^24, in_features, a multiple of the group, up "
-                               "to 2^20 and at most 2^40 elements");
+                               "to 2^20 and fewer than 2^35 elements in whole tiles of 16 x 128");
     return RQ_OK;
 }
 

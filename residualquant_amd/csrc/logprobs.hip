@@ -16,6 +16,8 @@
 // any order.  Their chunks are read again, by all threads, and the few logits
 // found (at most kMaxCandidates, else the row takes one pass per alternative,
 // as rows with NaN or infinities do) are ranked by counting.
+#include <algorithm>
+
 #include "rq_device.h"
 #include "rq_plan.h"
 #include "rq_rank.h"
@@ -359,10 +361,21 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
 // 243, 220, 296.)
 template <bool Bf16>
 void launch_rows(const LogprobParams& p, hipStream_t stream) {
-    if (p.vocab <= 16384 || (p.rows > 256 && p.vocab <= 65536))
-        hipLaunchKernelGGL((logprobs_kernel<Bf16, 256>), dim3((unsigned)p.rows), dim3(256), 0, stream, p);
-    else
-        hipLaunchKernelGGL((logprobs_kernel<Bf16, 512>), dim3((unsigned)p.rows), dim3(512), 0, stream, p);
+    const bool four_waves = p.vocab <= 16384 || (p.rows > 256 && p.vocab <= 65536);
+    // (The threads of a launch stay below 2^32.)
+    constexpr int64_t kMostRows = 1 << 22;
+    for (int64_t first = 0; first < p.rows; first += kMostRows) {
+        LogprobParams q = p;
+        q.rows = std::min(p.rows - first, kMostRows);
+        q.logits = static_cast<const uint8_t*>(p.logits) + first * p.stride * (Bf16 ? 2 : 4);
+        q.tokens += first, q.logprob += first, q.entropy += first;
+        if (p.top > 0) q.top_logprobs += first * p.top, q.top_tokens += first * p.top;
+        const dim3 grid((unsigned)q.rows);
+        if (four_waves)
+            hipLaunchKernelGGL((logprobs_kernel<Bf16, 256>), grid, dim3(256), 0, stream, q);
+        else
+            hipLaunchKernelGGL((logprobs_kernel<Bf16, 512>), grid, dim3(512), 0, stream, q);
+    }
 }
 
 }  // namespace

@@ -238,3 +238,18 @@ def test_finite_masks_are_as_infinite_ones(device):
     for mask in (-1e4, -1e10, -1e30, -1e38):
         got = step_ops.token_logprobs(logits.masked_fill(out, mask).to(device), tokens.to(device), top=8)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), mask
+
+
+def test_more_rows_than_one_launch_takes(device):
+    """2^24 and some rows of two logits."""
+    rows = (1 << 24) + 3
+    g = torch.Generator(device=device).manual_seed(7)
+    logits = torch.randn((rows, 2), generator=g, device=device).to(torch.bfloat16)
+    tokens = torch.randint(0, 2, (rows,), generator=g, device=device)
+    got = step_ops.token_logprobs(logits, tokens, top=1)
+    # Against the small calls, which the tests above check: the last rows, and some around the launches' borders.
+    for first in (0, (1 << 22) - 20, (1 << 23) - 1, (1 << 24) - 30, rows - 40):
+        part = slice(first, first + 40)
+        want = step_ops.token_logprobs(logits[part], tokens[part], top=1)
+        assert all(torch.equal(a[part], b) for a, b in zip(got, want)), first
+    assert torch.equal(got.top_tokens[:, 0], (logits[:, 1] > logits[:, 0]).long())

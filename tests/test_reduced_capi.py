@@ -145,3 +145,21 @@ def test_python_refusals():
         step_ops.pack_weight_int4(torch.zeros((64, 64), dtype=torch.int8), torch.zeros((64, 2), dtype=torch.bfloat16))
     with pytest.raises(RuntimeError, match="on a HIP device"):
         step_ops.token_logprobs(torch.zeros((2, 64)), torch.zeros(2, dtype=torch.int64))
+
+
+def test_calls_past_a_launch_are_refused(lib):
+    """The threads of one launch stay below 2^32: larger calls are refused before they are launched."""
+    assert _write(lib, requests=1 << 23) == _lib.RQ_EINVAL
+    assert b"Too many rows and requests" in lib.rq_last_error()
+    for heads, kv_heads, rows in ((8, 4, (1 << 29) - 1), (64, 64, 1 << 26)):  # tiles of 256 columns, 512 threads
+        assert _attend(lib, rows=rows, heads=heads, kv_heads=kv_heads, query_stride=64 * 128, key_stride=64 * 128) == _lib.RQ_EINVAL
+
+    def decode(requests):  # one row each: tiles of 16 columns, 256 threads
+        return lib.rq_paged_attention_fp8(FAKE, 64 * 128, FAKE, 64 * 128, FAKE, 64 * 128, FAKE, 64 * 128, requests, 64, 64,
+                                          128, FAKE, FAKE, 8, 16, FAKE, FAKE, requests, FAKE, 1, 1, 0.1, FAKE, 1 << 40, None)
+
+    assert decode(1 << 18) == _lib.RQ_EINVAL
+    assert b"Too many rows, heads and requests" in lib.rq_last_error()
+    assert lib.rq_int4_weight_bytes(1 << 24, 1 << 11, 128) == 0
+    assert b"2^35 elements" in lib.rq_last_error()
+    assert lib.rq_int4_weight_bytes((1 << 24) - 16, 1 << 11, 128) > 0
