@@ -327,9 +327,9 @@ int rq_quantize_fp8(const void* key, int64_t key_stride, const void* value, int6
  * [rows, heads, head_dim], key, value [rows, kv_heads, head_dim], 8-byte
  * aligned, token strides multiples of 4 elements.  A request may have no new
  * rows; rows outside query_start_loc are left as they are; tokens on invalid
- * blocks are skipped.  Sums are FP32 and not yet divided by the softmax's sum:
- * the values of a request's tokens together must stay below 2^119 (BF16 reaches
- * 2^128).  `workspace`: device memory of
+ * blocks are skipped.  Sums are FP32, in units of 2^40 from a page scale above
+ * 2^72 or a new value of 2^80 on, so that no finite values pass their range.
+ * `workspace`: device memory of
  * rq_paged_attention_fp8_workspace_bytes(...), any address; calls that may
  * overlap need one each.
  */

@@ -167,6 +167,16 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams 
 // again as the rounding of the output).  The running maximum of a column moves
 // only when a score exceeds it by 2^8, so most steps neither exchange lanes
 // nor rescale; weights are then at most 2^8.
+//
+// Sums are not divided by the weights' sum before the end, so values near the
+// top of BF16 would pass FP32 although their average does not.  From the first
+// page scale above 2^72 or new value of 2^80 on, a wave counts O in units of
+// 2^40: 2^30 tokens of any size then stay in range, and what the units lose is
+// far below the rounding of such values.  The sign of a part's sum of weights
+// says in which unit its O is.  All of it lies on paths that are rare already
+// (tokens that do not count, values that are not finite): no time.  (A second
+// pass after an overflow: 11.4 us of 10.5 for one request of 2048 tokens, and 152
+// bytes of spilled registers where there are many columns.)
 
 typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 Bf16x2 __attribute__((ext_vector_type(2)));
@@ -175,6 +185,7 @@ typedef float F32x4 __attribute__((ext_vector_type(4)));
 constexpr int kStreamThreads = 256;
 constexpr float kLowest = -3.402823466e+38f;
 constexpr float kMaxSlack = 8.0f;  // log2 units
+constexpr float kHugeUnit = 0x1p40f, kHugeScale = 0x1p72f, kHugeValue = 0x1p80f;
 
 __device__ __forceinline__ F32x4 mfma(U32x4 a, U32x4 b, F32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
@@ -198,8 +209,14 @@ __device__ __forceinline__ void transpose_bytes(const uint32_t (&x)[4], uint32_t
     t[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
 }
 
-__device__ __forceinline__ bool not_finite_bf16x2(uint32_t x) {
-    return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
+// Values that the products leave out and that are added apart: of kHugeValue and more, infinities, NaN.
+__device__ __forceinline__ bool odd_bf16x2(uint32_t x) {
+    return (x & 0x7f80u) >= 0x6780u || (x & 0x7f800000u) >= 0x67800000u;
+}
+__device__ __forceinline__ uint32_t without_odd(uint32_t x) {
+    if ((x & 0x7f80u) >= 0x6780u) x &= 0xffff0000u;
+    if ((x & 0x7f800000u) >= 0x67800000u) x &= 0x0000ffffu;
+    return x;
 }
 
 // One request's new rows (as columns) and history.
@@ -269,7 +286,38 @@ struct Fp8Columns {
     F32x4 out[NT][Channels];  // [tile][e]
     float high[NT];  // the maximum that weights refer to (log2 units)
     float sum[NT];   // of this lane's tokens
+    float unit;      // by which O is multiplied (the same for the whole wave): 1 or 1 / kHugeUnit
+
+    __device__ __forceinline__ void clear() {
+        unit = 1.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            high[t] = kLowest;
+            sum[t] = 0.f;
+#pragma unroll
+            for (int e = 0; e < Channels; ++e) out[t][e] = F32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    __device__ __forceinline__ void make_room() {
+        if (unit != 1.0f) return;
+        unit = 1.0f / kHugeUnit;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < Channels; ++e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) out[t][e][r] *= 1.0f / kHugeUnit;
+    }
+    // A part's sum as it is handed on.
+    __device__ __forceinline__ float marked_sum(int t) const { return unit == 1.0f ? sum[t] : -sum[t]; }
 };
+
+// Of the parts of a column, `marks`: their sums' bits, or-ed (without branches, beside loads in flight).
+// What a part's O counts in the join's unit, and that unit over the sum.
+__device__ __forceinline__ float part_unit(uint32_t marks, float sum) {
+    return (int)(marks & ~__float_as_uint(sum)) < 0 ? 1.0f / kHugeUnit : 1.0f;
+}
+__device__ __forceinline__ float join_scale(uint32_t marks, float sum) { return ((int)marks < 0 ? kHugeUnit : 1.0f) / sum; }
 
 // Weights of U units of 16 tokens: of the products dot (masked: -inf) with their
 // K scales (positive, softmax scale and log2(e) included), as two BF16 parts of
@@ -366,21 +414,23 @@ __device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int fro
         };
         load(0);
         float high = kLowest;
+        uint32_t marks = 0;
         for (int first = kGroup; first < splits; first += 8) {
-            float largest[8];
+            float2 others[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) largest[k] = load2(at + (uint32_t)min(first + k, splits - 1) * kEntry * 4).x;
+            for (int k = 0; k < 8; ++k) others[k] = load2(at + (uint32_t)min(first + k, splits - 1) * kEntry * 4);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) high = fmaxf(high, largest[k]);
+            for (int k = 0; k < 8; ++k) high = fmaxf(high, others[k].x), marks |= __float_as_uint(others[k].y);
         }
 #pragma unroll
-        for (int k = 0; k < kGroup; ++k) high = fmaxf(high, stats[k].x);
+        for (int k = 0; k < kGroup; ++k) high = fmaxf(high, stats[k].x), marks |= __float_as_uint(stats[k].y);
         float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
         for (int first = 0;;) {
 #pragma unroll
             for (int k = 0; k < kGroup; ++k) {
-                const float keep = first + k >= splits ? 0.0f : stats[k].x == high ? 1.0f : __builtin_amdgcn_exp2f(stats[k].x - high);
-                sum += stats[k].y * keep;
+                float keep = first + k >= splits ? 0.0f : stats[k].x == high ? 1.0f : __builtin_amdgcn_exp2f(stats[k].x - high);
+                sum += fabsf(stats[k].y) * keep;
+                keep *= part_unit(marks, stats[k].y);
                 o[0] += low[k].x * keep, o[1] += low[k].y * keep, o[2] += low[k].z * keep, o[3] += low[k].w * keep;
                 o[4] += up[k].x * keep, o[5] += up[k].y * keep, o[6] += up[k].z * keep, o[7] += up[k].w * keep;
             }
@@ -388,7 +438,7 @@ __device__ __forceinline__ void fp8_join(__amdgpu_buffer_rsrc_t handoff, int fro
             if (first >= splits) break;
             load(first);
         }
-        const float scale = 1.0f / sum;
+        const float scale = join_scale(marks, sum);
         uint16_t* out = output_row(column) + channel;
         *reinterpret_cast<U32x2*>(out) = U32x2{bf16x2_rn(o[0] * scale, o[1] * scale), bf16x2_rn(o[2] * scale, o[3] * scale)};
         *reinterpret_cast<U32x2*>(out + 4) = U32x2{bf16x2_rn(o[4] * scale, o[5] * scale), bf16x2_rn(o[6] * scale, o[7] * scale)};
@@ -446,13 +496,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         }
     }
     Fp8Columns<NT, 8> columns;  // tile e: channels 8 (4 g + r) + e
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        columns.high[t] = kLowest;
-        columns.sum[t] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) columns.out[t][e] = F32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    columns.clear();
     const float to_log2 = p.softmax_scale * 1.44269504088896341f;
 
     // ---------------------------------------------------------------- history
@@ -525,17 +569,24 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
 #pragma unroll
                 for (int t = 0; t < NT; ++t) dot[t][u] = mfma(a, query[t][m], dot[t][u]);
             }
-            if (x.valid[u] < 16) {
+        }
+        // (Scalar instructions: positive floats compare as their bits.)
+        const bool whole = min(x.valid[0], x.valid[1]) == 16;
+        const bool huge = max(__float_as_uint(x.value_scale[0]), __float_as_uint(x.value_scale[1])) > __builtin_bit_cast(uint32_t, kHugeScale);
+        if (!whole || huge) {
+            if (huge) columns.make_room();
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         dot[t][u][r] = 4 * g + r < x.valid[u] ? dot[t][u][r] : -__builtin_inff();
-            }
         }
         float weight[NT][2][4];
         U32x4 upper[NT][1], lower[NT][1];
-        fp8_softmax<NT, 8, 2>(columns, dot, x.key_scale, x.value_scale, weight, upper, lower);
+        const float value_scale[2] = {x.value_scale[0] * columns.unit, x.value_scale[1] * columns.unit};
+        fp8_softmax<NT, 8, 2>(columns, dot, x.key_scale, value_scale, weight, upper, lower);
         uint32_t v[2][4][2];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
@@ -544,7 +595,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
 #pragma unroll
                 for (int w = 0; w < 2; ++w) v[u][r][w] = x.v[u][r][w];
         // Slots past the history may hold NaN, which a weight of zero does not remove.
-        if (x.valid[0] < 16 || x.valid[1] < 16) {
+        if (!whole) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -623,16 +674,16 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
             }
             float weight[NT][2][4];
             U32x4 upper[NT][1], lower[NT][1];
-            const float key_scale[2] = {to_log2, to_log2}, value_scale[2] = {1.f, 1.f};
+            const float key_scale[2] = {to_log2, to_log2}, value_scale[2] = {columns.unit, columns.unit};
             fp8_softmax<NT, 8, 2>(columns, dot, key_scale, value_scale, weight, upper, lower);
-            // Infinities and NaN, which a weight of zero does not remove, are added apart.
+            // Infinities and NaN, which a weight of zero does not remove, and huge values are added apart.
             bool odd_values = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) odd_values |= not_finite_bf16x2(v[u][r][w]);
+                    for (int w = 0; w < 4; ++w) odd_values |= odd_bf16x2(v[u][r][w]);
             const bool any_odd = __any(odd_values);
             if (any_odd) {
 #pragma unroll
@@ -640,12 +691,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            uint32_t x = v[u][r][w];
-                            if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
-                            if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
-                            v[u][r][w] = x;
-                        }
+                        for (int w = 0; w < 4; ++w) v[u][r][w] = without_odd(v[u][r][w]);
             }
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -661,6 +707,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
                 }
             }
             if (any_odd) {
+                columns.make_room();
                 for (int j = 0; j < 32; ++j) {
                     const int token = base + j;
                     if (token >= rows) break;
@@ -683,7 +730,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
                                 const int channel = 32 * g + 8 * r + e;
                                 if (channel >= D) continue;
                                 const float x = bf16_f32(row[channel]);
-                                if (!(fabsf(x) < __builtin_inff())) columns.out[t][e][r] += w * x;
+                                if (!(fabsf(x) < kHugeValue)) columns.out[t][e][r] += w * (x * columns.unit);
                             }
                     }
                 }
@@ -702,9 +749,9 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         return p.output + (int64_t)(first + column / group) * p.output_stride + ((int64_t)head * group + column % group) * D;
     };
     // Eight channels of a column: the output, or this split's part of it.
-    auto emit = [&](int column, int channel, const float (&o)[8], float high, float sum) {
+    auto emit = [&](int column, int channel, const float (&o)[8], float high, float sum, uint32_t marks) {
         if (splits == 1) {
-            const float scale = 1.0f / sum;
+            const float scale = join_scale(marks, sum);
             uint16_t* out = output_row(column) + channel;
             *reinterpret_cast<U32x2*>(out) = U32x2{bf16x2_rn(o[0] * scale, o[1] * scale), bf16x2_rn(o[2] * scale, o[3] * scale)};
             *reinterpret_cast<U32x2*>(out + 4) = U32x2{bf16x2_rn(o[4] * scale, o[5] * scale), bf16x2_rn(o[6] * scale, o[7] * scale)};
@@ -715,7 +762,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         handoff_store4(handoff, at + 32 + 4 * channel, o[4], o[5], o[6], o[7]);
         if (channel == 0) {
             handoff_store(handoff, at, high);
-            handoff_store(handoff, at + 4, sum);
+            handoff_store(handoff, at + 4, (int)marks < 0 ? -sum : sum);
         }
     };
     if (splits > 1 && tid == 0) tag_arrivals(arrivals, p.call_tag, arrivals_seen);
@@ -732,24 +779,27 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         }
         if (g == 0) {
             merged[wave][i][D] = columns.high[t];
-            merged[wave][i][D + 1] = columns.sum[t];
+            merged[wave][i][D + 1] = columns.marked_sum(t);
         }
         __syncthreads();
         const int local = tid >> 4, channel = 8 * (tid & 15), column = item_column + 16 * t + local;
         if (column < columns_in && channel < D) {
             float high = kLowest;
+            uint32_t marks = 0;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) high = fmaxf(high, merged[w][local][D]);
+            for (int w = 0; w < kWaves; ++w)
+                high = fmaxf(high, merged[w][local][D]), marks |= __float_as_uint(merged[w][local][D + 1]);
             float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) {
                 const float m = merged[w][local][D];
-                const float keep = m == high ? 1.0f : __builtin_amdgcn_exp2f(m - high);
-                sum += merged[w][local][D + 1] * keep;
+                float keep = m == high ? 1.0f : __builtin_amdgcn_exp2f(m - high);
+                sum += fabsf(merged[w][local][D + 1]) * keep;
+                keep *= part_unit(marks, merged[w][local][D + 1]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] += merged[w][local][channel + e] * keep;
             }
-            emit(column, channel, o, high, sum);
+            emit(column, channel, o, high, sum, marks);
         }
     }
     if (splits == 1 || !arrive_last_tagged(arrivals, splits, &last_flag)) return;
@@ -782,13 +832,15 @@ constexpr int kWideTile = kWideColumns * kWideThreads / 64;
 // Distinct for channels c..c + 7 (an operand read) and for every fourth (the transposing writes).
 __device__ __forceinline__ int v_swizzle(int channel) { return (channel ^ (channel >> 2)) & 7; }
 
+constexpr int kHugeFlag = 32;  // of a unit whose page has a V scale above kHugeScale
+
 template <int D>
 struct WideTile {
     U32x4 k[kWideTokens][16];  // [token][chunk of 8 channels, chunk ^ (token % 16)]
     U32x4 v[D][8];             // [channel][chunk of 8 tokens, chunk ^ v_swizzle(channel)]
     float key_scale[4], value_scale[4];  // of the tile's units of 16 tokens
-    int valid[4];              // tokens of the unit that count (0 to 16)
-    int odd;                   // the number of the last tile of new rows with infinities or NaN among its values
+    int valid[4];              // tokens of the unit that count (0 to 16), and kHugeFlag
+    int odd;                   // the number of the last tile of new rows with odd_bf16x2 among its values
 };
 
 template <int D>
@@ -841,13 +893,7 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
         }
     }
     Fp8Columns<NT, kOut> columns;  // tile e: channels 16 e + 4 g + r
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        columns.high[t] = kLowest;
-        columns.sum[t] = 0.f;
-#pragma unroll
-        for (int e = 0; e < kOut; ++e) columns.out[t][e] = F32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    columns.clear();
     const float to_log2 = p.softmax_scale * 1.44269504088896341f;
     const int page_shift = p.page_tokens == 16 ? 4 : 5;
     const int64_t plane_bytes = ((p.num_blocks * p.kv_heads) << page_shift) * D;
@@ -930,24 +976,21 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
             if ((tid & 127) == 0) {
                 tile.key_scale[unit] = stage_block >= 0 ? x.key_scale * to_log2 : 1.f;
                 tile.value_scale[unit] = stage_block >= 0 ? x.value_scale : 1.f;
-                tile.valid[unit] = valid;
+                tile.valid[unit] = valid | (stage_block >= 0 && x.value_scale > kHugeScale ? kHugeFlag : 0);
             }
             return;
         }
         if (filler) {
             tile.k[token][(2 * k_chunk) ^ k_token] = x.k[0];
             tile.k[token][(2 * k_chunk + 1) ^ k_token] = x.k[1];
-            // Infinities and NaN, which a weight of zero does not remove, are left out here and added apart.
+            // Infinities and NaN, which a weight of zero does not remove, and huge values are left out here and added apart.
             U32x2 w[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t v = x.v[r][h];
-                    odd |= not_finite_bf16x2(v);
-                    if ((v & 0x7f80u) == 0x7f80u) v &= 0xffff0000u;
-                    if ((v & 0x7f800000u) == 0x7f800000u) v &= 0x0000ffffu;
-                    w[r][h] = v;
+                    odd |= odd_bf16x2(x.v[r][h]);
+                    w[r][h] = without_odd(x.v[r][h]);
                 }
             }
 #pragma unroll
@@ -1007,14 +1050,15 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
             for (int e = 0; e < kOut; ++e) operand[e] = tile.v[16 * e + i][(4 * st + g) ^ v_swizzle(16 * e + i)];
             __builtin_amdgcn_sched_barrier(0);
             if (base < 0) {
-                if (__builtin_amdgcn_readfirstlane(valid[0] & valid[1]) != 16) {
+                if (__builtin_amdgcn_readfirstlane((valid[0] ^ 16) | (valid[1] ^ 16)) != 0) {
+                    if (__builtin_amdgcn_readfirstlane((valid[0] | valid[1]) & kHugeFlag) != 0) columns.make_room();
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int t = 0; t < NT; ++t)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                dot[t][u][r] = 4 * g + r < valid[u] ? dot[t][u][r] : -__builtin_inff();
+                                dot[t][u][r] = 4 * g + r < (valid[u] & (kHugeFlag - 1)) ? dot[t][u][r] : -__builtin_inff();
                 }
             } else if (base + 32 * st + 31 > column0 / group || base + 32 * st + 31 >= new_end) {
 #pragma unroll
@@ -1029,6 +1073,8 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
             U32x4 upper[NT][1], lower[NT][1];
             // (The wave that computes weights goes before one in its products: 105 -> 103 us for two chunks of 509 rows.)
             __builtin_amdgcn_s_setprio(2);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) value_scale[u] *= columns.unit;
             fp8_softmax<NT, kOut, 2>(columns, dot, key_scale, value_scale, weight, upper, lower);
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
@@ -1040,7 +1086,9 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
 #pragma unroll
                 for (int t = 0; t < NT; ++t) columns.out[t][e] = mfma(operand[e], lower[t][0], columns.out[t][e]);
             if (base >= 0 && tile.odd == number) {
-                // Infinities and NaN among the new values, for the columns that see them.
+                // Huge values, infinities and NaN among the new ones, for the columns that see them.
+                const float unit_of_weights = columns.unit;
+                columns.make_room();
                 for (int j = 0; j < 32; ++j) {
                     const int token = base + 32 * st + j;
                     if (token >= new_end) break;
@@ -1063,7 +1111,7 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
                                 const float x = bf16_f32(row[16 * e + 4 * g + r]);
-                                if (!(fabsf(x) < __builtin_inff())) columns.out[t][e][r] += w * x;
+                                if (!(fabsf(x) < kHugeValue)) columns.out[t][e][r] += w * (x * (columns.unit / unit_of_weights));
                             }
                     }
                 }
@@ -1102,7 +1150,7 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
         const int column = column0 + 16 * t + i;
         if (column >= columns_in) continue;
         if (splits == 1) {
-            const float scale = 1.0f / columns.sum[t];
+            const float scale = join_scale(__float_as_uint(columns.marked_sum(t)), columns.sum[t]);
             uint16_t* out = output_row(column) + 4 * g;
 #pragma unroll
             for (int e = 0; e < kOut; ++e) {
@@ -1119,7 +1167,7 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
         }
         if (g == 0) {
             handoff_store(handoff, at, columns.high[t]);
-            handoff_store(handoff, at + 4, columns.sum[t]);
+            handoff_store(handoff, at + 4, columns.marked_sum(t));
         }
     }
 }

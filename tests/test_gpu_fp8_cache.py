@@ -444,3 +444,34 @@ def test_refusals_on_the_device(device):
         call(query=three)
     with pytest.raises(RuntimeError):
         ops.quantize_fp8(d["key"], d["value"][:, :1], d["cache"], d["scales"], d["starts"], d["seq_lens"], d["table"])
+
+
+# ---------------------------------------------------------------- attention at the ends of the range
+
+
+@pytest.mark.parametrize("histories,rows", [([300, 181], [1, 1]), ([300, 181], [4, 37]), ([3000], [1]), ([2000, 60], [100, 130]),
+                                            ([0, 40], [1, 90])])
+def test_attention_of_huge_values(device, histories, rows):
+    """Values up to 2^127, all of one sign, whose sum passes FP32 and whose average does not; the heads beside
+    hold values of 1 and of 2^-100."""
+    print(f"histories={histories} rows={rows}", flush=True)
+    case = _case(histories, rows, 6, 3, 128, 16, seed=61)
+    raw = case["cache"].view(torch.uint8)
+    raw[1] &= 0x7F  # positive values
+    for head, power in enumerate((2.0 ** 124, 1.0, 2.0 ** -100)):
+        case["scales"][1, :, head] *= power
+        case["value"][:, head] = (case["value"][:, head].float().abs() * power).to(torch.bfloat16)
+    _check_attention(case, _attend(_to(case, device), device))
+
+
+@pytest.mark.parametrize("rows", [[1], [5], [40], [150]])
+@pytest.mark.parametrize("where", ["early", "late", "new"])
+def test_attention_of_huge_values_in_one_place(device, rows, where):
+    """One page or one new row of values near the top of BF16 among ordinary ones, seen by one wave or split only."""
+    case = _case([2600], rows, 2, 2, 96, 32, seed=62)
+    if where == "new":
+        case["value"][rows[0] // 2] = (case["value"][rows[0] // 2].float().abs() * 2.0 ** 125).to(torch.bfloat16)
+    else:
+        block = int(case["table"][0, 1 if where == "early" else 2600 // 32 - 2])
+        case["scales"][1, block] *= 2.0 ** 124
+    _check_attention(case, _attend(_to(case, device), device))
