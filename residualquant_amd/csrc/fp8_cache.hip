@@ -319,6 +319,14 @@ __device__ __forceinline__ float part_unit(uint32_t marks, float sum) {
 }
 __device__ __forceinline__ float join_scale(uint32_t marks, float sum) { return ((int)marks < 0 ? kHugeUnit : 1.0f) / sum; }
 
+// a * b, rounded also where a sum follows.  (A score less the maximum by one fma would be its product's
+// rounding away from 0 at the maximum itself: from scores of 2^31 on that is a weight of 2^128, or none.
+// No time in any kernel.)
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 // Weights of U units of 16 tokens: of the products dot (masked: -inf) with their
 // K scales (positive, softmax scale and log2(e) included), as two BF16 parts of
 // weight x V scale.  Channels: the product's tiles of 16.
@@ -358,7 +366,7 @@ __device__ __forceinline__ void fp8_softmax(Fp8Columns<NT, Channels>& columns, c
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                weight[t][u][r] = __builtin_amdgcn_exp2f(fmaf(dot[t][u][r], key_scale[u], -columns.high[t]));
+                weight[t][u][r] = __builtin_amdgcn_exp2f(rounded_product(dot[t][u][r], key_scale[u]) - columns.high[t]);
                 columns.sum[t] += weight[t][u][r];
             }
 #pragma unroll

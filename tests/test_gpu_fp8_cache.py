@@ -475,3 +475,55 @@ def test_attention_of_huge_values_in_one_place(device, rows, where):
         block = int(case["table"][0, 1 if where == "early" else 2600 // 32 - 2])
         case["scales"][1, block] *= 2.0 ** 124
     _check_attention(case, _attend(_to(case, device), device))
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [3, 30], [90, 1]])
+@pytest.mark.parametrize("size", [1e6, 1e10, 1e14, 1e25])
+def test_attention_of_large_scores(device, rows, size):
+    """Scores of 10^7 and more, whose largest stands alone: its value comes out."""
+    case = _case([300, 181], rows, 2, 2, 128, 16, seed=63)
+    case["query"] = (case["query"].float() * size).to(torch.bfloat16)
+    query, scales, table = case["query"].double(), case["scales"].double(), case["table"]
+    want, gaps = torch.zeros_like(query), []
+    for b, (h, n) in enumerate(zip([300, 181], rows)):
+        begin = sum(rows[:b])
+        blocks = table[b, [t // 16 for t in range(h)]].long()
+        slots = torch.tensor([t % 16 for t in range(h)])
+        for head in range(2):
+            held = [case["cache"].view(torch.uint8)[p, blocks, head, slots].view(torch.float8_e4m3fn).double()
+                    * scales[p, blocks, head][:, None] for p in range(2)]
+            for i in range(n):
+                k, v = (torch.cat([x, case[name][begin:begin + i + 1, head].double()]) for x, name in zip(held, ("key", "value")))
+                q = query[begin + i, head]
+                scores = k @ q * 128 ** -0.5
+                first, second = scores.topk(2).values
+                # Its lead over the rounding of a score: 128 products summed in float32, and a factor.
+                gaps.append((first - second) - 2 * 140 * 2.0 ** -24 * float((k.abs() @ q.abs()).max()) * 128 ** -0.5)
+                want[begin + i, head] = v[scores.argmax()]
+    clear = torch.tensor(gaps).view(-1) > 30
+    assert clear.float().mean() > 0.9
+    # (In the order of the gaps: request, head, row.)
+    order = [(sum(rows[:b]) + i, head) for b, n in enumerate(rows) for head in range(2) for i in range(n)]
+    got = _attend(_to(case, device), device).cpu().double()
+    for (row, head), sure in zip(order, clear.tolist()):
+        if sure:  # one BF16 rounding, and weights of two BF16 parts
+            assert bool(((got[row, head] - want[row, head]).abs() <= 2.0 ** -7 * want[row, head].abs() + 2.0 ** -10).all()), (row, head)
+    assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("rows", [[1], [40]])
+def test_attention_of_large_equal_scores(device, rows):
+    """Equal keys: equal weights, whatever the size of the scores."""
+    for sign, power in ((1, 12), (1, 30), (-1, 30), (1, 60), (-1, 60), (1, 100)):
+        case = _case([333], rows, 1, 1, 128, 16, seed=64)
+        case["cache"][0] = torch.ones(case["cache"][0].shape).to(torch.float8_e4m3fn)
+        case["scales"][0] = 2.0 ** -3
+        case["query"] = torch.full_like(case["query"], sign * 1.5 * 2.0 ** power)
+        case["key"] = torch.full_like(case["key"], -3.0 if sign > 0 else 6.0)  # far below the others
+        blocks = case["table"][0, [t // 16 for t in range(333)]].long()
+        slots = torch.tensor([t % 16 for t in range(333)])
+        v = case["cache"].view(torch.uint8)[1, blocks, 0, slots].view(torch.float8_e4m3fn).double()
+        v = v * case["scales"][1, blocks, 0].double()[:, None]
+        got = _attend(_to(case, device), device).cpu().double()
+        bound = 2.0 ** -8 * v.mean(0).abs() + (2.0 ** -16 + 100 * 2.0 ** -23) * v.abs().mean(0)
+        assert bool(((got[:, 0] - v.mean(0)).abs() <= bound).all()), (sign, power)
