@@ -327,6 +327,10 @@ __device__ __forceinline__ float rounded_product(float a, float b) {
     return a * b;
 }
 
+// A page's K scale with the softmax scale: positive also where the product is too small for FP32 (0 would
+// make NaN of the -inf of masked scores).
+__device__ __forceinline__ float factor_of_scores(float scale, float to_log2) { return fmaxf(scale * to_log2, 0x1p-149f); }
+
 // Weights of U units of 16 tokens: of the products dot (masked: -inf) with their
 // K scales (positive, softmax scale and log2(e) included), as two BF16 parts of
 // weight x V scale.  Channels: the product's tiles of 16.
@@ -529,7 +533,7 @@ __global__ __launch_bounds__(kStreamThreads) void attention_fp8_kernel(const Fp8
         place_low = (uint32_t)place;
         place_high = (uint32_t)((uint64_t)place >> 32);
         unit_valid = held ? (uint32_t)min(left, 16) : 0u;
-        unit_key_scale = held ? p.scales[index] * to_log2 : 1.f;
+        unit_key_scale = held ? factor_of_scores(p.scales[index], to_log2) : 1.f;
         unit_value_scale = held ? p.scales[index + p.num_blocks * p.kv_heads] : 1.f;
     };
     auto load = [&](Fp8Step<D>& x, int number) {
@@ -982,7 +986,7 @@ __global__ __launch_bounds__(kWideThreads) void attention_fp8_wide_kernel(const 
                     *v_place(tile, 4 * v_word + c, unit, v_quad) = U32x2{bf16x2_of_fp8<false>(y[c]), bf16x2_of_fp8<true>(y[c])};
             }
             if ((tid & 127) == 0) {
-                tile.key_scale[unit] = stage_block >= 0 ? x.key_scale * to_log2 : 1.f;
+                tile.key_scale[unit] = stage_block >= 0 ? factor_of_scores(x.key_scale, to_log2) : 1.f;
                 tile.value_scale[unit] = stage_block >= 0 ? x.value_scale : 1.f;
                 tile.valid[unit] = valid | (stage_block >= 0 && x.value_scale > kHugeScale ? kHugeFlag : 0);
             }

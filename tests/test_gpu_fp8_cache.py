@@ -527,3 +527,12 @@ def test_attention_of_large_equal_scores(device, rows):
         got = _attend(_to(case, device), device).cpu().double()
         bound = 2.0 ** -8 * v.mean(0).abs() + (2.0 ** -16 + 100 * 2.0 ** -23) * v.abs().mean(0)
         assert bool(((got[:, 0] - v.mean(0)).abs() <= bound).all()), (sign, power)
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [3, 90]])
+def test_attention_of_scores_that_vanish(device, rows):
+    """A softmax scale so small that a page's scale times it underflows: every token has the same weight."""
+    case = _case([300, 181], rows, 2, 2, 128, 16, seed=65)
+    case["scales"][0] *= 2.0 ** -20
+    for scale in (1e-30, 1e-38, 1e-44):
+        _check_attention(case, _attend(_to(case, device), device, softmax_scale=scale), scale=scale)
