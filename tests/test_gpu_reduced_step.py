@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from residualquant_amd import ops, step_ops
-from residualquant_amd.looped_decode import LoopedConfig, LoopedDecoder
+from residualquant_amd.looped_decode import LoopedConfig, LoopedDecoder, _project
 
 from . import fp8_reference as reference
 from .test_gpu_linear_int4 import _reference as linear_reference
@@ -171,3 +171,29 @@ def test_looped_decoder_logprobs_of_the_last_step_however_it_ran(device):
     logits = decoder.replay()
     torch.cuda.synchronize()
     check_logprobs(logits.cpu(), decoder.tokens.cpu(), 4, device, got=decoder.logprobs)
+
+
+@pytest.mark.parametrize("rows", [64, 65, 70, 130, 257])
+@pytest.mark.parametrize("out,features,group", [(1000, 512, 32), (512, 768, 64), (37, 5632, 128)])
+def test_projection_of_many_rows(device, rows, out, features, group):
+    """The decoder's projection at any number of rows: the weight itself is not rounded."""
+    g = torch.Generator().manual_seed(rows + out)
+    codes = torch.randint(-8, 8, (out, features), generator=g, dtype=torch.int8)
+    scales = (torch.rand((out, features // group), generator=g) * 0.02 + 0.001).to(torch.bfloat16)
+    x = torch.randn((rows, features), generator=g).to(torch.bfloat16)
+    got = _project(x.to(device), step_ops.pack_weight_int4(codes.to(device), scales.to(device))).cpu().double()
+    want, bound = linear_reference(x, codes, scales)
+    assert got.shape == want.shape
+    assert bool(((got - want).abs() <= bound).all()), ((got - want).abs() / bound).max()
+
+
+def test_looped_decoder_of_many_rows_repeats_its_replays(device):
+    """A step of 70 rows: captured and replayed, it gives what an eager twin gives."""
+    first, second = (LoopedDecoder(_small_config(projection_bits=4), 70, 20, 6, device, seed=8) for _ in range(2))
+    for decoder in (first, second):
+        decoder.build_history(seed=5)
+    first.capture()
+    for _ in range(3):
+        got, want = first.replay(), second.step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(first.tokens, second.tokens)
