@@ -164,9 +164,12 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams 
 // A page's K scale multiplies its scores (FP32), its V scale the weights
 // (FP32), which are then split into two BF16 parts (16 bits of the weight
 // multiply V; one part alone would round each weight by up to 2^-8, as much
-// again as the rounding of the output).  The running maximum of a column moves
-// only when a score exceeds it by 2^8, so most steps neither exchange lanes
-// nor rescale; weights are then at most 2^8.
+// again as the rounding of the output.  A third part, for all 24 bits, changes
+// one output of 600 by a BF16 step and the mean error against float64 in none of
+// its first five digits, and takes 59.0 us instead of 57.7 for eight requests of
+// five rows over 55 heads, 120 instead of 103 for two chunks of 509 rows).  The
+// running maximum of a column moves only when a score exceeds it by 2^8, so most
+// steps neither exchange lanes nor rescale; weights are then at most 2^8.
 //
 // Sums are not divided by the weights' sum before the end, so values near the
 // top of BF16 would pass FP32 although their average does not.  From the first

@@ -429,12 +429,12 @@ void launch_tiles(const LinearInt4Params& p, hipStream_t stream) {
 // x beside the codes, or through LDS: by the rounds of workgroups, one per tile
 // and 16 rows, that the compute units take without it.  Without LDS (against
 // with it), for outputs x inputs and rows:
-//   1 round:   2048 x 5632, 16: 8.8 us (9.4); 32: 9.0 (13.3)
-//   2 rounds:  2048 x 5632, 64: 16.6 us (24.3); 4096 x 5632, 32: 16.7 (13.7)
-//   3 rounds:  11264 x 2048, 8: 6.8 us (7.4), 16: 9.0 (7.7); 6144 x 1024, 32: 5.7 (6.0)
-//   4 rounds:  16000 x 2048, 8: 8.3 us (7.1); 4096 x 1024, 64: 6.8 (6.5)
-// and with 4 waves: 16000 x 512, 16 (4 rounds): 4.9 us (5.3); 11264 x 512, 32 (6): 6.1 (6.8); 16000 x 512,
-// 32 (8): 7.2 (6.0).
+//   1 round:   2048 x 5632, 16: 8.7 us (8.5); 32: 9.0 (11.3)
+//   2 rounds:  2048 x 5632, 64: 16.0 us (20.1); 4096 x 5632, 32: 16.0 (12.2)
+//   3 rounds:  11264 x 2048, 8: 7.2 us (7.4), 16: 9.2 (7.8); 12288 x 1024, 16: 6.0 (6.5); 6144 x 1024, 32: 6.0 (5.7)
+//   4 rounds:  16000 x 2048, 8: 8.5 us (7.4); 4096 x 1024, 64: 7.1 (5.9)
+// and with 4 waves: 6144 x 512, 16 (2 rounds): 3.5 us (4.3); 16000 x 512, 16 (4): 4.9 (4.8); 11264 x 512, 32 (6): 6.1
+// (5.9); 16000 x 512, 32 (8): 7.1 (5.2).
 template <int Group>
 void launch_rows(const LinearInt4Params& p, hipStream_t stream) {
     const int blocks = (int)int4_blocks(p.in_features);
@@ -442,8 +442,9 @@ void launch_rows(const LinearInt4Params& p, hipStream_t stream) {
     const int64_t rounds = (workgroups + p.compute_units - 1) / p.compute_units;
     const int64_t most = blocks <= 4 ? 6 : blocks <= 8 || (blocks <= 24 && p.rows <= 8) ? 3 : p.rows > 32 ? 2 : 1;
     if (blocks <= 48 && rounds <= most) {
-        // (Four waves where they hold all inputs: 6144 x 512, 16 rows 3.5 us against 4.6 with eight, which
-        // at 1024 inputs take 3.3 against 3.6; sixteen past 24 blocks: 2048 x 4096, one row 4.7 against 4.9.)
+        // (Four waves where they hold all inputs: 6144 x 512, 16 rows 3.5 us against 4.5 with eight, which
+        // at 1024 inputs take 4.6 against 4.8; sixteen past 24 blocks, for one row: 2048 x 5632 5.6 us against
+        // 5.8, 2048 x 4096 4.6 against 4.5; with 16 rows 8.8 against 8.6 and 6.6 against 6.5.)
         if (blocks <= 4)
             launch_few<Group, 1, 4>(p, stream);
         else if (blocks <= 8)

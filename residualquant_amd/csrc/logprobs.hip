@@ -355,10 +355,10 @@ __global__ __launch_bounds__(Threads) void logprobs_kernel(const LogprobParams p
 
 // Four waves per row for short rows, and where enough rows run beside each
 // other; else eight.  (256 threads, 512, and 1024, whose start and barriers cost
-// more than they share out, in us.  1 row of 8000 logits with 8 alternatives: 6.5,
-// 7.2, 9.7; of 32000: 9.6, 9.0, 10.6; of 49152: 11.6, 10.4, 11.9.  600 rows of 50257
-// with 1: 23.5, 25.1, 38.9; 2041 rows: 50.9, 56.5, 101; 3000 rows of 151000 with 8:
-// 243, 220, 296.)
+// more than they share out, in us.  1 row of 8000 logits with 8 alternatives: 6.6,
+// 7.3, 9.7; of 32000: 10.1, 9.4, 10.7; of 49152: 12.3, 10.7, 11.9.  600 rows of 50257
+// with 1: 26.9, 28.4, 43.0; 2041 rows: 54.6, 61.3, 108; 3000 rows of 151000 with 8:
+// 248, 225, 302.)
 template <bool Bf16>
 void launch_rows(const LogprobParams& p, hipStream_t stream) {
     const bool four_waves = p.vocab <= 16384 || (p.rows > 256 && p.vocab <= 65536);
