@@ -51,8 +51,10 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t x) {
     x = max(x, plan_dpp<0x4E>(x));   // quad_perm [2,3,0,1]
     x = max(x, plan_dpp<0x124>(x));  // row_ror:4
     x = max(x, plan_dpp<0x128>(x));  // row_ror:8
-    return max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
-               max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48)));
+    // (readlane gives an int: values of 2^31 and more would compare as negative ones.)
+    const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16);
+    const uint32_t c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+    return max(max(a, b), max(c, d));
 }
 
 // Inclusive sum over lanes 0..lane of the wave.

@@ -253,3 +253,24 @@ def test_more_rows_than_one_launch_takes(device):
         want = step_ops.token_logprobs(logits[part], tokens[part], top=1)
         assert all(torch.equal(a[part], b) for a, b in zip(got, want)), first
     assert torch.equal(got.top_tokens[:, 0], (logits[:, 1] > logits[:, 0]).long())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [9, 28, 200, 3001])
+def test_maxima_of_both_signs(device, dtype, vocab):
+    """Positive logits far above stretches of negative ones, wherever they stand: the row's maximum is the positive one."""
+    g = torch.Generator().manual_seed(vocab)
+    logits, tokens = [], []
+    for gap in (3.0, 40.0, 80.0, 84.0, 85.5, 87.0, 100.0, 1000.0):
+        for place in sorted({0, 1, vocab // 2, vocab - 1, *torch.randint(0, vocab, (6,), generator=g).tolist()}):
+            row = -gap * 0.5 - torch.rand(vocab, generator=g) * 3
+            row[place] = gap * 0.5
+            logits.append(row)
+            tokens.append(place)
+    logits, tokens = torch.stack(logits).to(dtype), torch.tensor(tokens)
+    _check(logits, tokens, min(3, vocab), device)
+    _check(logits, (tokens + 1) % vocab, 1, device)
+    only = torch.full((8, vocab), -torch.inf)
+    only[:, 0] = torch.arange(8) * 12.0
+    only[:, -1] = -3.0
+    _check(only.to(dtype), torch.zeros(8, dtype=torch.int64), 2, device)
