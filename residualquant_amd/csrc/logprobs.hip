@@ -8,14 +8,16 @@
 // the chunk that holds it first.  The reference is a logit itself and is
 // subtracted before the scale of e^ to 2^: one fma(x, log2(e), -reference)
 // would be an instruction less per logit, but leaves the maximum of a row
-// around 10^10 with e^ of the hundreds that log2(e) x is rounded by.  Alternatives: the threads of one lane number
-// form one of 64 owners.  With T the `top`-th largest of the owners' largest
-// (value, chunk) - greater values first, then lower chunks - at least `top`
-// logits lie at or above T, so every alternative does; and logits at or above
-// T belong to threads whose own largest is, some 20 to 40 of them in a row in
-// any order.  Their chunks are read again, by all threads, and the few logits
-// found (at most kMaxCandidates, else the row takes one pass per alternative,
-// as rows with NaN or infinities do) are ranked by counting.
+// around 10^10 with e^ of the hundreds that log2(e) x is rounded by.
+//
+// Alternatives: the threads of one lane number form one of 64 owners.  With T
+// the `top`-th largest of the owners' largest (value, chunk) - greater values
+// first, then lower chunks - at least `top` logits lie at or above T, so every
+// alternative does; and logits at or above T belong to threads whose own largest
+// is, some 20 to 40 of them in a row in any order.  Their chunks are read again,
+// by all threads, and the few logits found (at most kMaxCandidates, else the row
+// takes one pass per alternative, as rows with NaN or infinities do) are ranked
+// by counting.
 #include <algorithm>
 
 #include "rq_device.h"
