@@ -371,7 +371,7 @@ int rq_linear_rows_int4(const void* x, int64_t x_stride, const void* packed, siz
                         int64_t y_stride, int64_t rows, int64_t out_features, int64_t in_features, int group,
                         hipStream_t stream);
 
-/* Element types of rq_token_logprobs' logits. */
+/* Element types of logits and probabilities. */
 enum { RQ_DTYPE_BF16 = 0, RQ_DTYPE_F32 = 1 };
 
 /*
@@ -387,6 +387,96 @@ enum { RQ_DTYPE_BF16 = 0, RQ_DTYPE_F32 = 1 };
 int rq_token_logprobs(const void* logits, int64_t stride, int dtype, int64_t rows, int64_t vocab, const int64_t* tokens,
                       float* logprob, float* entropy, int top, float* top_logprobs, int64_t* top_tokens,
                       hipStream_t stream);
+
+/* Scales of an 8-bit weight: exponent bytes, 2^(byte - 127), or FP32. */
+enum { RQ_SCALE_E8M0 = 0, RQ_SCALE_F32 = 1 };
+
+/*
+ * Projections in 8-bit floating point: a weight [out_features, in_features]
+ * as OCP E4M3 codes cw and one scale sw per block of 128 outputs x 128 inputs
+ * (the last of each side may be smaller), laid out once for the kernels in
+ * rq_fp8_weight_bytes(...) bytes of 16-byte aligned device memory (0 for an
+ * invalid shape).  out_features up to 2^24, in_features up to 2^20, of any
+ * value, together fewer than 2^36 elements in whole tiles of 16 x 128.
+ * rq_pack_weight_fp8 takes codes [out, in] and scales
+ * [ceil(out / 128), ceil(in / 128)], both contiguous; rq_quantize_weight_fp8 a
+ * BF16 weight (scales are exponents: the least power of two s >= 2^-126 with
+ * |w| <= 448 s for every finite value of the block; NaN and infinities become
+ * NaN); rq_dequantize_weight_fp8 restores bf16(cw x sw).
+ * rq_linear_fp8: y[m, n] = bf16(sum_b sx[m, b] sw[n / 128, b] sum_k cx[m, k] cw[n, k])
+ * over blocks b of 128 inputs, for up to 2^20 BF16 rows x [rows, in_features],
+ * which it rounds itself: sx[m, b] is the least power of two >= 2^-126 with
+ * |x| <= 448 sx for the block's finite values, cx = e4m3(x / sx) to nearest,
+ * ties to even, NaN for what is not finite.  FP32 sums; results below the
+ * normal range of FP32 may be 0.  x of any even address and row stride
+ * (16-byte aligned rows are read faster).  `workspace`: device memory of
+ * rq_linear_fp8_workspace_bytes(...), any address; calls that may overlap need
+ * one each.
+ */
+size_t rq_fp8_weight_bytes(int64_t out_features, int64_t in_features, int scale_type);
+int rq_pack_weight_fp8(const void* codes, const void* scales, int scale_type, int64_t out_features, int64_t in_features,
+                       void* packed, size_t packed_bytes, hipStream_t stream);
+int rq_quantize_weight_fp8(const void* weight, int64_t out_features, int64_t in_features, void* packed,
+                           size_t packed_bytes, hipStream_t stream);
+int rq_dequantize_weight_fp8(const void* packed, size_t packed_bytes, int scale_type, int64_t out_features,
+                             int64_t in_features, void* weight, hipStream_t stream);
+size_t rq_linear_fp8_workspace_bytes(int64_t rows, int64_t in_features);
+int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t packed_bytes, int scale_type, void* y,
+                  int64_t y_stride, int64_t rows, int64_t out_features, int64_t in_features, void* workspace,
+                  size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * A call's new tokens from fused [q | k | v] BF16 rows [rows, (heads +
+ * 2 kv_heads) x head_dim]: q and k rotated to their positions into query
+ * [rows, heads, head_dim] and key [rows, kv_heads, head_dim], and k (rotated)
+ * and v appended to a paged cache on the way.  With scales, the cache holds
+ * E4M3 codes and is written as rq_quantize_fp8 does; with scales NULL it holds
+ * BF16 [2, num_blocks, kv_heads, page_tokens, head_dim] (16-byte aligned), as
+ * rq_paged_attention_bf16 reads it.  Requests, rows, slots and what is skipped
+ * as in rq_quantize_fp8 (a token without a page is still rotated; rows outside
+ * query_start_loc are left as they are).
+ * Rotation: of the first rotary_dim (a multiple of 16 up to head_dim) channels
+ * of a head the pairs (a, b) = (x[i], x[i + rotary_dim / 2]), interleaved
+ * (x[2 i], x[2 i + 1]), become bf16(a cos - b sin), bf16(b cos + a sin), each
+ * product and sum rounded to FP32; cos/sin FP32 [table_rows, rotary_dim / 2],
+ * 16-byte aligned, at the token's place in its request, or at
+ * positions[row] where positions are given (clamped to the tables).
+ * qkv, query and key 8-byte aligned, token strides multiples of 4 elements; no
+ * two of them overlap.
+ */
+int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads, int kv_heads, int head_dim,
+                   int rotary_dim, int interleaved, const float* cos_table, const float* sin_table, int64_t table_rows,
+                   const int64_t* positions, void* query, int64_t query_stride, void* key, int64_t key_stride,
+                   void* cache, float* scales, int64_t num_blocks, int page_tokens, const int32_t* query_start_loc,
+                   const int32_t* seq_lens, int64_t requests, const int32_t* block_table, int64_t block_table_stride,
+                   int64_t max_pages, hipStream_t stream);
+
+/*
+ * Verification of drafted tokens by given random numbers.  Request b's rows
+ * query_start_loc[b]..query_start_loc[b + 1] hold its last token and its
+ * drafts, tokens[row] each; target[row] (BF16 or FP32 [rows, vocab], unit
+ * column stride) is the target's distribution of the token behind that row,
+ * and draft[row], of the same type, the one that the next row's draft was
+ * drawn from (NULL: that draft was certain).  In order, the draft t behind row
+ * r is taken iff uniforms[r] x draft[r][t] < target[r][t] (draft 1 where it is
+ * NULL; a t outside the vocabulary has target 0).  The row of the first draft
+ * that is not taken, or the request's last row, is the final one: its token is
+ * drawn from the weights max(target - draft, 0) (draft NULL: target without t), in
+ * the last row from target, as the lowest token of positive weight whose
+ * running sum exceeds uniforms[the request's last row] x the sum (the last of
+ * positive weight if none does).  Entries that are negative, NaN or infinite
+ * count as 0; sums and products are FP64.
+ * accepted[b]: drafts taken.  out_tokens [rows]: row r's following token, for the
+ * rows before the final one their drafts, for it the drawn token (-1 if no
+ * weight is positive), -1 in all other rows.
+ * `workspace`: device memory of rq_verify_drafts_workspace_bytes(...), any
+ * address; calls that may overlap need one each.
+ */
+int rq_verify_drafts(const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int dtype,
+                     int64_t rows, int64_t vocab, const int64_t* tokens, const float* uniforms,
+                     const int32_t* query_start_loc, int64_t requests, int32_t* accepted, int64_t* out_tokens,
+                     void* workspace, size_t workspace_bytes, hipStream_t stream);
+size_t rq_verify_drafts_workspace_bytes(int64_t requests, int64_t vocab);
 
 /*
  * Kernel timing for measurement: when enabled, rq_attention and

@@ -44,6 +44,15 @@ EXPORTED_SYMBOLS = (
     "rq_dequantize_weight_int4",
     "rq_linear_rows_int4",
     "rq_token_logprobs",
+    "rq_fp8_weight_bytes",
+    "rq_pack_weight_fp8",
+    "rq_quantize_weight_fp8",
+    "rq_dequantize_weight_fp8",
+    "rq_linear_fp8_workspace_bytes",
+    "rq_linear_fp8",
+    "rq_rope_append",
+    "rq_verify_drafts",
+    "rq_verify_drafts_workspace_bytes",
     "rq_timing_enable",
     "rq_timing_read",
     "rq_set_split_target",
@@ -136,6 +145,25 @@ def _declare(l: ctypes.CDLL) -> None:
     l.rq_linear_rows_int4.argtypes = [vp, i64, vp, sz, vp, i64, i64, i64, i64, i32, vp]
     l.rq_token_logprobs.restype = i32
     l.rq_token_logprobs.argtypes = [vp, i64, i32, i64, i64, vp, vp, vp, i32, vp, vp, vp]
+    l.rq_fp8_weight_bytes.restype = sz
+    l.rq_fp8_weight_bytes.argtypes = [i64, i64, i32]
+    l.rq_pack_weight_fp8.restype = i32
+    l.rq_pack_weight_fp8.argtypes = [vp, vp, i32, i64, i64, vp, sz, vp]
+    l.rq_quantize_weight_fp8.restype = i32
+    l.rq_quantize_weight_fp8.argtypes = [vp, i64, i64, vp, sz, vp]
+    l.rq_dequantize_weight_fp8.restype = i32
+    l.rq_dequantize_weight_fp8.argtypes = [vp, sz, i32, i64, i64, vp, vp]
+    l.rq_linear_fp8_workspace_bytes.restype = sz
+    l.rq_linear_fp8_workspace_bytes.argtypes = [i64, i64]
+    l.rq_linear_fp8.restype = i32
+    l.rq_linear_fp8.argtypes = [vp, i64, vp, sz, i32, vp, i64, i64, i64, i64, vp, sz, vp]
+    l.rq_rope_append.restype = i32
+    l.rq_rope_append.argtypes = [vp, i64, i64, i32, i32, i32, i32, i32, vp, vp, i64, vp, vp, i64, vp, i64, vp, vp, i64,
+                                 i32, vp, vp, i64, vp, i64, i64, vp]
+    l.rq_verify_drafts.restype = i32
+    l.rq_verify_drafts.argtypes = [vp, i64, vp, i64, i32, i64, i64, vp, vp, vp, i64, vp, vp, vp, sz, vp]
+    l.rq_verify_drafts_workspace_bytes.restype = sz
+    l.rq_verify_drafts_workspace_bytes.argtypes = [i64, i64]
     l.rq_timing_enable.argtypes = [i32]
     l.rq_timing_read.restype = i32
     l.rq_timing_read.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]

@@ -1475,6 +1475,230 @@ int rq_token_logprobs(const void* logits, int64_t stride, int dtype, int64_t row
     return check_launch(rq::launch_logprobs(p, stream), "log probability launch");
 }
 
+// ------------------------------------------------- projections in 8-bit floating point
+
+// The largest sides and elements keep every index of the kernels in range.
+static int check_fp8_shape(int64_t out_features, int64_t in_features, int scale_type) {
+    if (scale_type != RQ_SCALE_E8M0 && scale_type != RQ_SCALE_F32)
+        return fail(RQ_EINVAL, "Scales as exponents (E8M0) or in FP32 required");
+    // (Packed by one thread per 16 elements of whole tiles of 16 x 128.)
+    if (out_features <= 0 || in_features <= 0 || out_features > (1 << 24) || in_features > (1 << 20) ||
+        !launchable(((out_features + 15) / 16) * ((in_features + 127) / 128), 128))
+        return fail(RQ_EINVAL, "8-bit weights need out_features up to 2^24, in_features up to 2^20 and fewer than 2^36 "
+                               "elements in whole tiles of 16 x 128");
+    return RQ_OK;
+}
+
+size_t rq_fp8_weight_bytes(int64_t out_features, int64_t in_features, int scale_type) {
+    if (check_fp8_shape(out_features, in_features, scale_type) != RQ_OK) return 0;
+    ok();
+    return rq::fp8_weight_bytes(out_features, in_features, scale_type == RQ_SCALE_E8M0);
+}
+
+static int fp8_pack_params(rq::Fp8PackParams* p, const void* packed, size_t packed_bytes, int64_t out_features,
+                           int64_t in_features, int scale_type) {
+    const int status = check_fp8_shape(out_features, in_features, scale_type);
+    if (status != RQ_OK) return status;
+    const size_t needed = rq::fp8_weight_bytes(out_features, in_features, scale_type == RQ_SCALE_E8M0);
+    if (packed == nullptr || (reinterpret_cast<uintptr_t>(packed) % 16) != 0 || packed_bytes < needed)
+        return fail(RQ_EINVAL, "16-byte aligned packed weight of %zu bytes required", needed);
+    *p = rq::Fp8PackParams{};
+    p->packed = static_cast<uint8_t*>(const_cast<void*>(packed));
+    p->packed_scales = p->packed + rq::fp8_code_bytes(out_features, in_features);
+    p->out_features = out_features;
+    p->in_features = in_features;
+    p->exponents = scale_type == RQ_SCALE_E8M0;
+    return RQ_OK;
+}
+
+int rq_pack_weight_fp8(const void* codes, const void* scales, int scale_type, int64_t out_features, int64_t in_features,
+                       void* packed, size_t packed_bytes, hipStream_t stream) {
+    rq::Fp8PackParams p;
+    const int status = fp8_pack_params(&p, packed, packed_bytes, out_features, in_features, scale_type);
+    if (status != RQ_OK) return status;
+    if (codes == nullptr || scales == nullptr || (!p.exponents && (reinterpret_cast<uintptr_t>(scales) % 4) != 0))
+        return fail(RQ_EINVAL, "E4M3 codes and their scales required");
+    p.codes = static_cast<const uint8_t*>(codes);
+    p.scales = scales;
+    return check_launch(rq::launch_pack_fp8(p, stream), "8-bit weight pack launch");
+}
+
+int rq_quantize_weight_fp8(const void* weight, int64_t out_features, int64_t in_features, void* packed,
+                           size_t packed_bytes, hipStream_t stream) {
+    rq::Fp8PackParams p;
+    const int status = fp8_pack_params(&p, packed, packed_bytes, out_features, in_features, RQ_SCALE_E8M0);
+    if (status != RQ_OK) return status;
+    if (weight == nullptr || (reinterpret_cast<uintptr_t>(weight) % 2) != 0)
+        return fail(RQ_EINVAL, "BF16 weight required");
+    p.weight = static_cast<const uint16_t*>(weight);
+    return check_launch(rq::launch_pack_fp8(p, stream), "8-bit weight quantize launch");
+}
+
+int rq_dequantize_weight_fp8(const void* packed, size_t packed_bytes, int scale_type, int64_t out_features,
+                             int64_t in_features, void* weight, hipStream_t stream) {
+    rq::Fp8PackParams p;
+    const int status = fp8_pack_params(&p, packed, packed_bytes, out_features, in_features, scale_type);
+    if (status != RQ_OK) return status;
+    if (weight == nullptr || (reinterpret_cast<uintptr_t>(weight) % 2) != 0)
+        return fail(RQ_EINVAL, "BF16 weight required");
+    return check_launch(rq::launch_unpack_fp8(p, static_cast<uint16_t*>(weight), stream), "8-bit weight restore launch");
+}
+
+size_t rq_linear_fp8_workspace_bytes(int64_t rows, int64_t in_features) {
+    if (rows <= 0 || rows > rq::kLinearFp8MaxRows || in_features <= 0 || in_features > (1 << 20)) return 256;
+    return 256 + rq::linear_fp8_workspace(rows, in_features);
+}
+
+int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t packed_bytes, int scale_type, void* y,
+                  int64_t y_stride, int64_t rows, int64_t out_features, int64_t in_features, void* workspace,
+                  size_t workspace_bytes, hipStream_t stream) {
+    if (rows < 0 || rows > rq::kLinearFp8MaxRows)
+        return fail(RQ_ENOKERNEL, "No compiled 8-bit projection kernel for %lld rows (at most %lld)", (long long)rows,
+                    (long long)rq::kLinearFp8MaxRows);
+    rq::Fp8PackParams w;
+    const int status = fp8_pack_params(&w, packed, packed_bytes, out_features, in_features, scale_type);
+    if (status != RQ_OK) return status;
+    if (x_stride < in_features || y_stride < out_features)
+        return fail(RQ_EINVAL, "x rows of in_features and y rows of out_features required");
+    if (rows == 0) return ok();
+    if (x == nullptr || y == nullptr || (reinterpret_cast<uintptr_t>(x) % 2) || (reinterpret_cast<uintptr_t>(y) % 2))
+        return fail(RQ_EINVAL, "BF16 x and a BF16 output required");
+    if (!launchable(((rows + 15) / 16) * ((in_features + 511) / 512), 256))
+        return fail(RQ_EINVAL, "Too many rows and inputs for one call");
+    const size_t needed = rq_linear_fp8_workspace_bytes(rows, in_features);
+    if (workspace == nullptr || workspace_bytes < needed)
+        return fail(RQ_ENOSPACE, "Projection workspace of %zu bytes required, %zu given", needed, workspace_bytes);
+    rq::LinearFp8Params p{};
+    p.x = static_cast<const uint16_t*>(x);
+    p.x_stride = x_stride;
+    p.packed = w.packed;
+    p.packed_scales = w.packed_scales;
+    p.y = static_cast<uint16_t*>(y);
+    p.y_stride = y_stride;
+    p.rows = rows;
+    p.out_features = out_features;
+    p.in_features = in_features;
+    p.exponents = w.exponents;
+    p.compute_units = compute_units();
+    p.x_codes = static_cast<uint8_t*>(workspace) + to_boundary(workspace);
+    p.x_scales = reinterpret_cast<uint32_t*>(p.x_codes + rq::fp8_code_bytes(rows, in_features));
+    return check_launch(rq::launch_linear_fp8(p, stream), "8-bit projection launch");
+}
+
+// ------------------------------------------------- rotated appends, verification of drafts
+
+// Whether `rows` rows of `width` elements of 2 bytes at two places share an address.
+static bool rows_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b, int64_t b_stride,
+                         int64_t b_width, int64_t rows) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t a1 = a0 + 2 * (uintptr_t)((rows - 1) * a_stride + a_width), b1 = b0 + 2 * (uintptr_t)((rows - 1) * b_stride + b_width);
+    return a0 < b1 && b0 < a1;
+}
+
+int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads, int kv_heads, int head_dim,
+                   int rotary_dim, int interleaved, const float* cos_table, const float* sin_table, int64_t table_rows,
+                   const int64_t* positions, void* query, int64_t query_stride, void* key, int64_t key_stride,
+                   void* cache, float* scales, int64_t num_blocks, int page_tokens, const int32_t* query_start_loc,
+                   const int32_t* seq_lens, int64_t requests, const int32_t* block_table, int64_t block_table_stride,
+                   int64_t max_pages, hipStream_t stream) {
+    // (BF16 pages have no scales: the cache itself stands in for their address.)
+    int status = check_fp8_pages(cache, scales != nullptr ? scales : static_cast<const float*>(cache), num_blocks, kv_heads,
+                                 head_dim, page_tokens, rows, query_start_loc, seq_lens, requests, block_table,
+                                 block_table_stride, max_pages);
+    if (status != RQ_OK) return status;
+    if (heads <= 0 || heads > 65535) return fail(RQ_EINVAL, "1 to 65535 query heads required");
+    if (rotary_dim <= 0 || rotary_dim % 16 != 0 || rotary_dim > head_dim)
+        return fail(RQ_EINVAL, "Rotated channels must be a multiple of 16, at most head_dim");
+    if (table_rows <= 0 || cos_table == nullptr || sin_table == nullptr || (reinterpret_cast<uintptr_t>(cos_table) % 16) ||
+        (reinterpret_cast<uintptr_t>(sin_table) % 16))
+        return fail(RQ_EINVAL, "16-byte aligned FP32 cos/sin tables of at least one position required");
+    const int64_t all_heads = heads + 2 * (int64_t)kv_heads;
+    status = check_bf16_rows(qkv, qkv_stride, rows, all_heads, head_dim);
+    if (status == RQ_OK) status = check_bf16_rows(query, query_stride, rows, heads, head_dim);
+    if (status == RQ_OK) status = check_bf16_rows(key, key_stride, rows, kv_heads, head_dim);
+    if (status != RQ_OK) return status;
+    if (positions != nullptr && (reinterpret_cast<uintptr_t>(positions) % 8) != 0)
+        return fail(RQ_EINVAL, "INT64 positions required");
+    if (rows == 0 || requests == 0) return ok();
+    if (rows_overlap(qkv, qkv_stride, all_heads * head_dim, query, query_stride, (int64_t)heads * head_dim, rows) ||
+        rows_overlap(qkv, qkv_stride, all_heads * head_dim, key, key_stride, (int64_t)kv_heads * head_dim, rows) ||
+        rows_overlap(query, query_stride, (int64_t)heads * head_dim, key, key_stride, (int64_t)kv_heads * head_dim, rows))
+        return fail(RQ_EINVAL, "The rotated query and key must not overlap each other or their input");
+    if (!launchable(rows / page_tokens + 2 * requests, 256)) return fail(RQ_EINVAL, "Too many rows and requests for one call");
+    rq::RopeAppendParams p{};
+    p.qkv = static_cast<const uint16_t*>(qkv);
+    p.qkv_stride = qkv_stride;
+    p.rows = rows;
+    p.heads = heads;
+    p.kv_heads = kv_heads;
+    p.head_dim = head_dim;
+    p.rotary = rotary_dim;
+    p.interleaved = interleaved != 0;
+    p.cos_table = cos_table;
+    p.sin_table = sin_table;
+    p.table_rows = table_rows;
+    p.positions = positions;
+    p.query = static_cast<uint16_t*>(query);
+    p.query_stride = query_stride;
+    p.key = static_cast<uint16_t*>(key);
+    p.key_stride = key_stride;
+    p.cache = cache;
+    p.scales = scales;
+    p.num_blocks = num_blocks;
+    p.page_tokens = page_tokens;
+    p.query_start_loc = query_start_loc;
+    p.seq_lens = seq_lens;
+    p.requests = requests;
+    p.block_table = block_table;
+    p.block_table_stride = block_table_stride;
+    p.max_pages = max_pages;
+    return check_launch(rq::launch_rope_append(p, stream), "rotated append launch");
+}
+
+size_t rq_verify_drafts_workspace_bytes(int64_t requests, int64_t vocab) {
+    if (requests <= 0 || requests > (int64_t)INT32_MAX / 4 || vocab <= 0 || vocab > (int64_t)INT32_MAX) return 256;
+    int64_t chunk = 0;
+    return 256 + (size_t)requests * rq::verify_chunks(requests, vocab, &chunk) * sizeof(double);
+}
+
+int rq_verify_drafts(const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int dtype,
+                     int64_t rows, int64_t vocab, const int64_t* tokens, const float* uniforms,
+                     const int32_t* query_start_loc, int64_t requests, int32_t* accepted, int64_t* out_tokens,
+                     void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (dtype != RQ_DTYPE_BF16 && dtype != RQ_DTYPE_F32) return fail(RQ_EINVAL, "BF16 or FP32 probabilities required");
+    const uintptr_t element = dtype == RQ_DTYPE_BF16 ? 2 : 4;
+    if (rows < 0 || rows > (int64_t)INT32_MAX || vocab <= 0 || vocab > (int64_t)INT32_MAX || target_stride < vocab ||
+        (draft != nullptr && draft_stride < vocab))
+        return fail(RQ_EINVAL, "Probabilities [rows, vocab] of at least one column with unit column stride required");
+    if (requests < 0 || requests > (int64_t)INT32_MAX / 4 || (requests > 0 && (query_start_loc == nullptr || accepted == nullptr)))
+        return fail(RQ_EINVAL, "Contiguous INT32 query starts with one final boundary required");
+    if (requests == 0) return ok();
+    if (rows > 0 && (target == nullptr || (reinterpret_cast<uintptr_t>(target) % element) ||
+                     (reinterpret_cast<uintptr_t>(draft) % element) || tokens == nullptr || uniforms == nullptr || out_tokens == nullptr))
+        return fail(RQ_EINVAL, "Probabilities, tokens, random numbers and outputs required");
+    rq::VerifyParams p{};
+    p.chunks = rq::verify_chunks(requests, vocab, &p.chunk);
+    if (!launchable(requests * p.chunks, 512)) return fail(RQ_EINVAL, "Too many requests and tokens for one call");
+    const size_t needed = rq_verify_drafts_workspace_bytes(requests, vocab);
+    if (workspace == nullptr || workspace_bytes < needed)
+        return fail(RQ_ENOSPACE, "Verification workspace of %zu bytes required, %zu given", needed, workspace_bytes);
+    p.target = target;
+    p.target_stride = target_stride;
+    p.draft = draft;
+    p.draft_stride = draft_stride;
+    p.bf16 = dtype == RQ_DTYPE_BF16;
+    p.rows = rows;
+    p.vocab = vocab;
+    p.tokens = tokens;
+    p.uniforms = uniforms;
+    p.query_start_loc = query_start_loc;
+    p.requests = requests;
+    p.accepted = accepted;
+    p.out_tokens = out_tokens;
+    p.sums = reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + to_boundary(workspace));
+    return check_launch(rq::launch_verify(p, stream), "draft verification launch");
+}
+
 void rq_timing_enable(int enabled) {
     std::lock_guard<std::mutex> lock(g_timing.mutex);
     g_timing.enabled = enabled != 0;

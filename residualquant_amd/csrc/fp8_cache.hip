@@ -4,16 +4,13 @@
 // quantize_fp8_kernel writes a call's new tokens, attention_fp8_kernel reads
 // the cache: the 8-bit member beside the packed (2 + 4 bit) and the BF16 pages.
 #include "rq_device.h"
+#include "rq_fp8.h"
 #include "rq_plan.h"
 #include "rq_reduced.h"
 
 namespace rq {
 
 namespace {
-
-typedef uint32_t U32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t U32x2 __attribute__((ext_vector_type(2)));
-typedef U32x4 U32x4At8 __attribute__((aligned(8)));  // 16 bytes on an 8-byte boundary
 
 // ------------------------------------------------------------------ write
 //
@@ -23,38 +20,10 @@ typedef U32x4 U32x4At8 __attribute__((aligned(8)));  // 16 bytes on an 8-byte bo
 // (n rows touch at most n / PT + 2 pages), so a wave finds its request by
 // counting.
 
-// The request of slot `slot` (the last whose first slot is at or below it).
-__device__ __forceinline__ int write_request(const int32_t* qsl, int requests, int page_shift, int slot) {
-    const int lane = threadIdx.x & 63;
-    int count = 0;
-    for (int b = 1 + lane; b < requests; b += 64) count += (int64_t)(qsl[b] >> page_shift) + 2 * (int64_t)b <= slot ? 1 : 0;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) count += __shfl_xor(count, d);
-    return __builtin_amdgcn_readfirstlane(count);
-}
-
-// The least power of two s >= 2^-126 with largest <= 448 s.  largest = m 2^e,
-// 1 <= m < 2, and 448 = 1.75 * 2^8: s is 2^(e - 8), twice that where m > 1.75.
-__device__ __forceinline__ float needed_scale(float largest) {
-    const uint32_t u = __float_as_uint(largest);
-    int exponent = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-    if (exponent < 1) exponent = 1;  // 2^-126
-    return __uint_as_float((uint32_t)exponent << 23);
-}
-
-// Four E4M3 codes (ties to even) of values within +-448; what is not finite becomes NaN.
-__device__ __forceinline__ uint32_t fp8x4_rn(float a, float b, float c, float d) {
-    auto nan_unless_finite = [](float x) { return fabsf(x) < __builtin_inff() ? x : __builtin_nanf(""); };
-    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(a), nan_unless_finite(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(c), nan_unless_finite(d), low, true);
-}
-
-__device__ __forceinline__ bool power_of_two(float x) { return (__float_as_uint(x) & 0x7fffffu) == 0; }
-
 template <int D, int PT>
 __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams p) {
     constexpr int kRow = D / 8;                      // chunks of 8 values per row
-    constexpr int kChunks = (PT * kRow + 63) / 64;   // per lane
+    constexpr int kChunks = kPageChunks<D, PT>;
     constexpr int kShift = PT == 16 ? 4 : 5;
     const int lane = threadIdx.x & 63;
     const int head = (int)blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -87,60 +56,7 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams 
         values[c] = U32x4{0u, 0u, 0u, 0u};
         if (r < rows) values[c] = *reinterpret_cast<const U32x4At8*>(in + r * stride + 8 * (chunk - r * kRow));
     }
-    float largest = 0.f;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = __uint_as_float(values[c][e] << 16), b = __uint_as_float(values[c][e] & 0xffff0000u);
-            largest = fmaxf(largest, fabsf(a) < __builtin_inff() ? fabsf(a) : 0.f);
-            largest = fmaxf(largest, fabsf(b) < __builtin_inff() ? fabsf(b) : 0.f);
-        }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
-    const float need = needed_scale(largest);
-    const float scale = slot > 0 && before >= need ? before : need;
-
-    if (slot > 0 && scale > before) {
-        const float shrink = before / scale;
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int chunk = 64 * c + lane;
-            if (chunk >= slot * kRow) continue;
-            U32x2* place = reinterpret_cast<U32x2*>(codes) + chunk;
-            U32x2 word = *place;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(word[w], false), high = __builtin_amdgcn_cvt_pk_f32_fp8(word[w], true);
-                word[w] = fp8x4_rn(low[0] * shrink, low[1] * shrink, high[0] * shrink, high[1] * shrink);
-            }
-            *place = word;
-        }
-    }
-    // A division by a power of two is a product (a scale that the caller made may be any number).
-    const bool exact = power_of_two(scale);
-    const float inverse = 1.0f / scale;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const int chunk = 64 * c + lane;
-        if (chunk >= rows * kRow) continue;
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[2 * e] = __uint_as_float(values[c][e] << 16);
-            x[2 * e + 1] = __uint_as_float(values[c][e] & 0xffff0000u);
-        }
-        if (exact) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= inverse;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] /= scale;
-        }
-        reinterpret_cast<U32x2*>(codes)[slot * kRow + chunk] =
-            U32x2{fp8x4_rn(x[0], x[1], x[2], x[3]), fp8x4_rn(x[4], x[5], x[6], x[7])};
-    }
-    if (lane == 0) p.scales[index] = scale;
+    write_fp8_page<D, PT>(values, codes, p.scales + index, before, slot, rows);
 }
 
 // ------------------------------------------------------------------ attention

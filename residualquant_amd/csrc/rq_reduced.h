@@ -56,6 +56,85 @@ struct LogprobParams {
 };
 hipError_t launch_logprobs(const LogprobParams& p, hipStream_t stream);
 
+// Projections in 8-bit floating point with block scales (linear_fp8.hip).
+constexpr int64_t kLinearFp8MaxRows = 1 << 20;
+struct Fp8PackParams {
+    const uint8_t* codes;     // E4M3 [out, in] with scales [out / 128, in / 128] (rounded up), or
+    const void* scales;       // E8M0 bytes or FP32
+    const uint16_t* weight;   // a BF16 weight [out, in] to quantize (E8M0 scales)
+    uint8_t* packed;
+    uint8_t* packed_scales;
+    int64_t out_features, in_features;
+    bool exponents;           // scales are E8M0
+};
+struct LinearFp8Params {
+    const uint16_t* x;        // BF16 [rows, in]
+    int64_t x_stride;
+    const uint8_t* packed;
+    const uint8_t* packed_scales;
+    uint16_t* y;              // BF16 [rows, out]
+    int64_t y_stride;
+    int64_t rows, out_features, in_features;
+    bool exponents;
+    int compute_units;        // of the launching device
+    uint8_t* x_codes;         // workspace: x as the weights are packed
+    uint32_t* x_scales;       // workspace [tiles of 16 rows][fours of blocks][16], four E8M0 bytes each
+};
+size_t fp8_code_bytes(int64_t rows, int64_t in_features);
+size_t fp8_weight_bytes(int64_t out_features, int64_t in_features, bool exponents);
+size_t linear_fp8_workspace(int64_t rows, int64_t in_features);
+hipError_t launch_pack_fp8(const Fp8PackParams& p, hipStream_t stream);
+hipError_t launch_unpack_fp8(const Fp8PackParams& p, uint16_t* weight, hipStream_t stream);
+hipError_t launch_linear_fp8(const LinearFp8Params& p, hipStream_t stream);
+
+// Rotation of a call's q and k, and K/V appended to a paged cache (rope_append.hip).
+struct RopeAppendParams {
+    const uint16_t* qkv;      // BF16 [rows, (heads + 2 kv_heads) D]
+    int64_t qkv_stride;
+    int64_t rows;
+    int heads, kv_heads, head_dim, rotary;
+    bool interleaved;
+    const float* cos_table;   // [table_rows, rotary / 2]
+    const float* sin_table;
+    int64_t table_rows;
+    const int64_t* positions; // [rows], or null: the tokens' places in their requests
+    uint16_t* query;
+    int64_t query_stride;
+    uint16_t* key;
+    int64_t key_stride;
+    void* cache;              // [2, blocks, kv_heads, PT, D], E4M3 with scales or BF16
+    float* scales;            // [2, blocks, kv_heads], null: BF16 pages
+    int64_t num_blocks;
+    int page_tokens;
+    const int32_t* query_start_loc;
+    const int32_t* seq_lens;
+    int64_t requests;
+    const int32_t* block_table;
+    int64_t block_table_stride;
+    int64_t max_pages;
+};
+hipError_t launch_rope_append(const RopeAppendParams& p, hipStream_t stream);
+
+// Verification of drafted tokens (verify.hip).
+struct VerifyParams {
+    const void* target;       // BF16 or FP32 [rows, vocab]
+    int64_t target_stride;
+    const void* draft;        // as target, or null
+    int64_t draft_stride;
+    bool bf16;
+    int64_t rows, vocab;
+    const int64_t* tokens;    // [rows]
+    const float* uniforms;    // [rows]
+    const int32_t* query_start_loc;
+    int64_t requests;
+    int32_t* accepted;        // [requests]
+    int64_t* out_tokens;      // [rows]
+    int64_t chunk, chunks;    // tokens whose weights a workgroup sums, and how many such of a row
+    double* sums;             // workspace [requests, chunks]
+};
+int64_t verify_chunks(int64_t requests, int64_t vocab, int64_t* chunk);
+hipError_t launch_verify(const VerifyParams& p, hipStream_t stream);
+
 // Cache held in 8 bits (fp8_cache.hip): E4M3 codes [2, blocks, kv_heads, PT, D],
 // FP32 scales [2, blocks, kv_heads].
 struct Fp8WriteParams {

@@ -405,6 +405,73 @@ def quantize_fp8(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor, sc
     _lib.check(status)
 
 
+def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache: torch.Tensor,
+                scales: Optional[torch.Tensor], query_start_loc: torch.Tensor, seq_lens: torch.Tensor,
+                block_table: torch.Tensor, positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+                query: Optional[torch.Tensor] = None,
+                key: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Rotate a call's new tokens and append their K/V to a paged cache on the way.
+
+    ``qkv`` holds fused BF16 rows ``[rows, (heads + 2 * kv_heads) * D]``.
+    Returns ``(query, key, value)``: the rotated q and k as ``[rows, heads,
+    D]`` and ``[rows, kv_heads, D]`` (new tensors, or those given, which must
+    not overlap ``qkv``) and the v part of ``qkv`` as a view; they are what
+    ``paged_attention_fp8`` takes.  The cache is ``[2, blocks, kv_heads,
+    page_tokens, D]``, E4M3 with its ``scales`` (written as ``quantize_fp8``
+    does) or BF16 with ``scales=None`` (``paged_attention_bf16``'s); requests
+    and pages as in ``quantize_fp8``.
+
+    Of the first ``2 * cos.size(1)`` channels (a multiple of 16) of each head
+    the pairs ``(x[i], x[i + cos.size(1)])``, with ``interleaved`` ``(x[2 i],
+    x[2 i + 1])``, are turned by the angles whose FP32 ``cos``/``sin`` ``[max_position,
+    channels / 2]`` hold in the row of the token's place in its request, or of
+    ``positions`` (INT64 ``[rows]``) where given (clamped to the tables).  Rows
+    outside ``query_start_loc`` are left as they are.
+    """
+    shape = qkv.shape
+    _require(qkv.is_cuda and qkv.dtype is torch.bfloat16 and len(shape) == 2 and qkv.stride(1) == 1,
+             "qkv must be BF16 [rows, channels] on a HIP device with unit channel stride")
+    device, rows = qkv.get_device(), shape[0]
+    _require(cache.get_device() == device and cache.dim() == 5, "Cache [2, blocks, kv_heads, page_tokens, D] on the Q/K/V device required")
+    _, blocks, kv_heads, page_tokens, head_dim = cache.shape
+    heads = shape[1] // head_dim - 2 * kv_heads if head_dim > 0 else 0
+    _require(heads > 0 and shape[1] == (heads + 2 * kv_heads) * head_dim,
+             "qkv rows must hold [q | k | v] of (heads + 2 * kv_heads) * head_dim channels")
+    if scales is None:
+        _require(cache.dtype is torch.bfloat16 and cache.size(0) == 2 and cache.is_contiguous(),
+                 "Contiguous BF16 [2, blocks, kv_heads, page_tokens, D] cache required (8-bit pages need their scales)")
+    else:
+        _validate_fp8_cache(cache, scales, device, kv_heads, head_dim)
+    requests, max_pages, table_stride = _validate_sequences(query_start_loc, seq_lens, block_table, device)
+    for table in (cos, sin):
+        _require(table.get_device() == device and table.dtype is torch.float32 and table.is_contiguous()
+                 and table.dim() == 2 and table.shape == cos.shape,
+                 "Contiguous FP32 [positions, channels / 2] cos/sin tables required")
+    if positions is not None:
+        _require(positions.get_device() == device and positions.dtype is torch.int64 and positions.is_contiguous()
+                 and positions.numel() == rows, "Contiguous INT64 positions, one per row, required")
+    if query is None:
+        query = qkv.new_empty((rows, heads, head_dim))
+    if key is None:
+        key = qkv.new_empty((rows, kv_heads, head_dim))
+    query_shape, query_stride = _validate_bf16_token_tensor(query)
+    key_shape, key_stride = _validate_bf16_token_tensor(key)
+    _require(query_shape == (rows, heads, head_dim) and key_shape == (rows, kv_heads, head_dim)
+             and query.get_device() == device and key.get_device() == device,
+             "query and key must be [rows, heads, D] and [rows, kv_heads, D] on the Q/K/V device")
+    width = shape[1]
+    with _on_device(device):
+        status = _lib.lib().rq_rope_append(
+            qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, kv_heads, head_dim, 2 * cos.size(1),
+            1 if interleaved else 0, cos.data_ptr(), sin.data_ptr(), cos.size(0),
+            positions.data_ptr() if positions is not None else None, query.data_ptr(), query_stride, key.data_ptr(),
+            key_stride, cache.data_ptr(), scales.data_ptr() if scales is not None else None, blocks, page_tokens,
+            query_start_loc.data_ptr(), seq_lens.data_ptr(), requests, block_table.data_ptr(), table_stride, max_pages,
+            _stream(device))
+    _lib.check(status)
+    return query, key, qkv[:, (heads + kv_heads) * head_dim:].view(rows, kv_heads, head_dim)
+
+
 def paged_attention_fp8_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_pages: int,
                                         page_tokens: int) -> int:
     """Device workspace (bytes) for ``paged_attention_fp8``; depends on shapes only."""

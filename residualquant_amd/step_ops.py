@@ -4,14 +4,16 @@ One Ouro layer (plugins/looped_transformers/src/looped_transformers/ouro.py:101-
 brackets its attention with vLLM's fused add + RMSNorm, the rotary embedding
 of Q and K, and Qwen2MLP's SiLU(gate) * up.  Beside them stand the projections at a few rows,
 with BF16 and with 4-bit weights, and the log probabilities of a step's
-tokens.  Each op here is a HIP launch through ``librq_hip.so`` (rq_rms_norm,
-rq_rope_qkv, rq_silu_mul, rq_linear_rows, rq_linear_rows_int4,
-rq_token_logprobs); there is no CPU or torch fallback.  Work is enqueued on the current HIP stream of the
+tokens, projections in 8-bit floating point for any number of rows and the
+verification of drafted tokens.  Each op here is a call of ``librq_hip.so``
+(rq_rms_norm, rq_rope_qkv, rq_silu_mul, rq_linear_rows, rq_linear_rows_int4,
+rq_linear_fp8, rq_token_logprobs, rq_verify_drafts); there is no CPU or torch fallback.  Work is enqueued on the current HIP stream of the
 input's device.
 """
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -252,6 +254,120 @@ def linear_rows_int4(x: torch.Tensor, weight: Int4Weight, out: Optional[torch.Te
     return out
 
 
+class Fp8Weight:
+    """A linear weight ``[out_features, in_features]`` in 8-bit floating point, laid out for ``linear_fp8``.
+
+    E4M3 codes with one scale per block of 128 outputs and 128 inputs, a power
+    of two (``exponents``) or FP32; made by ``quantize_weight_fp8`` or
+    ``pack_weight_fp8``.
+    """
+
+    def __init__(self, data: torch.Tensor, out_features: int, in_features: int, exponents: bool):
+        self.data, self.out_features, self.in_features, self.exponents = data, out_features, in_features, exponents
+        self.device = data.device
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.out_features, self.in_features
+
+    def dequantize(self) -> torch.Tensor:
+        """The BF16 weight ``[out_features, in_features]``: ``bf16(code * scale)``."""
+        weight = torch.empty(self.shape, dtype=torch.bfloat16, device=self.device)
+        with _on_device(self.data.get_device()):
+            status = _lib.lib().rq_dequantize_weight_fp8(self.data.data_ptr(), self.data.numel(),
+                                                         0 if self.exponents else 1, self.out_features,
+                                                         self.in_features, weight.data_ptr(), _stream(self.device))
+        _lib.check(status)
+        return weight
+
+
+def _fp8_weight(out_features: int, in_features: int, exponents: bool, device: torch.device) -> Fp8Weight:
+    needed = _lib.lib().rq_fp8_weight_bytes(out_features, in_features, 0 if exponents else 1)
+    if needed == 0:
+        raise RuntimeError(_lib.lib().rq_last_error().decode(errors="replace"))
+    return Fp8Weight(torch.empty(needed, dtype=torch.uint8, device=device), out_features, in_features, exponents)
+
+
+def quantize_weight_fp8(weight: torch.Tensor) -> Fp8Weight:
+    """A contiguous BF16 weight ``[out_features, in_features]`` in 8-bit floating point.
+
+    Per block of 128 x 128: scale = the least power of two with which the
+    block's values stay within 448, code = w / scale to nearest, ties to even.
+    """
+    _require(weight.is_cuda and weight.dtype == torch.bfloat16 and weight.dim() == 2 and weight.is_contiguous(),
+             "weight must be a contiguous BF16 [out_features, in_features] tensor on a HIP device")
+    packed = _fp8_weight(weight.size(0), weight.size(1), True, weight.device)
+    with _on_device(weight.get_device()):
+        status = _lib.lib().rq_quantize_weight_fp8(weight.data_ptr(), packed.out_features, packed.in_features,
+                                                   packed.data.data_ptr(), packed.data.numel(), _stream(weight.device))
+    _lib.check(status)
+    return packed
+
+
+def pack_weight_fp8(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Weight:
+    """A weight given as E4M3 ``codes`` ``[out_features, in_features]`` and ``scales``
+    ``[ceil(out_features / 128), ceil(in_features / 128)]``, FP32 or exponents (``float8_e8m0fnu``), both contiguous."""
+    _require(codes.is_cuda and codes.dtype == torch.float8_e4m3fn and codes.dim() == 2 and codes.is_contiguous(),
+             "codes must be a contiguous E4M3 [out_features, in_features] tensor on a HIP device")
+    _require(scales.device == codes.device and scales.dtype in (torch.float32, torch.float8_e8m0fnu)
+             and scales.is_contiguous() and scales.shape == (-(-codes.size(0) // 128), -(-codes.size(1) // 128)),
+             "scales must be a contiguous FP32 or E8M0 [ceil(out_features / 128), ceil(in_features / 128)] tensor on "
+             "the codes' device")
+    packed = _fp8_weight(codes.size(0), codes.size(1), scales.dtype == torch.float8_e8m0fnu, codes.device)
+    with _on_device(codes.get_device()):
+        status = _lib.lib().rq_pack_weight_fp8(codes.data_ptr(), scales.data_ptr(), 0 if packed.exponents else 1,
+                                               packed.out_features, packed.in_features, packed.data.data_ptr(),
+                                               packed.data.numel(), _stream(codes.device))
+    _lib.check(status)
+    return packed
+
+
+def linear_fp8_workspace_bytes(rows: int, in_features: int) -> int:
+    """Device workspace (bytes) for ``linear_fp8``; depends on shapes only."""
+    return int(_lib.lib().rq_linear_fp8_workspace_bytes(rows, in_features))
+
+
+def linear_fp8(x: torch.Tensor, weight: Fp8Weight, out: Optional[torch.Tensor] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``bf16(x @ weight.T)`` in 8-bit floating point for BF16 rows, one or a prompt's (rq_linear_fp8), FP32 accumulation.
+
+    ``x`` is rounded to E4M3 on the way, with a power-of-two scale for each row
+    and 128 inputs; a row with a NaN or an infinity gives NaN, others do not
+    change.  ``workspace``: uint8 memory of ``linear_fp8_workspace_bytes(rows,
+    in_features)`` bytes for this call alone, by default from torch's allocator.
+    """
+    shape, strides = x.shape, x.stride()
+    if not (len(shape) == 2 and strides[1] == 1 and x.is_cuda and x.dtype is torch.bfloat16):
+        _rows(x, "x")
+    rows, in_features = shape
+    out_features, data, device = weight.out_features, weight.data, x.get_device()
+    if in_features != weight.in_features or data.get_device() != device:
+        raise RuntimeError("x must have the weight's in_features and device")
+    out_stride = out_features
+    if out is None:
+        out = x.new_empty((rows, out_features))
+    else:
+        _rows(out, "out")
+        if out.shape != (rows, out_features) or out.get_device() != device:
+            raise RuntimeError("out must be [rows, out_features]")
+        if rows > 1:
+            out_stride = out.stride(0)
+    if workspace is None:
+        workspace = x.new_empty(_linear_fp8_workspace_bytes(rows, in_features), dtype=torch.uint8)
+    else:
+        _require(workspace.get_device() == device and workspace.is_contiguous(),
+                 "Contiguous projection workspace on x's device required")
+    with _on_device(device):
+        status = _lib.lib().rq_linear_fp8(
+            x.data_ptr(), strides[0] if rows > 1 else in_features, data.data_ptr(), data.numel(),
+            0 if weight.exponents else 1, out.data_ptr(), out_stride, rows, out_features, in_features,
+            workspace.data_ptr(), workspace.nbytes, torch._C._cuda_getCurrentRawStream(device))
+    _lib.check(status)
+    return out
+
+
+_linear_fp8_workspace_bytes = lru_cache(maxsize=256)(linear_fp8_workspace_bytes)
+
 LOGPROBS_MAX_TOP = 32
 
 
@@ -296,3 +412,75 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
             top_tokens.data_ptr(), torch._C._cuda_getCurrentRawStream(device))
     _lib.check(status)
     return TokenLogprobs(logprob, entropy, top_logprobs, top_tokens)
+
+
+class VerifiedDrafts(NamedTuple):
+    """How many drafts of each request were taken, and the tokens that follow its rows."""
+
+    accepted: torch.Tensor  # INT32 [requests]
+    tokens: torch.Tensor    # INT64 [rows]: the drafts taken, the token drawn behind them, then -1
+
+
+def verify_drafts_workspace_bytes(requests: int, vocab: int) -> int:
+    """Device workspace (bytes) for ``verify_drafts``; depends on shapes only."""
+    return int(_lib.lib().rq_verify_drafts_workspace_bytes(requests, vocab))
+
+
+_verify_workspace_bytes = lru_cache(maxsize=256)(verify_drafts_workspace_bytes)
+
+
+def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor, query_start_loc: torch.Tensor,
+                  draft: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> VerifiedDrafts:
+    """Judge drafted tokens by the target's probabilities, and draw the token that follows the last one taken.
+
+    Request b's rows ``query_start_loc[b]..query_start_loc[b+1]`` are its last
+    token and its drafts (``tokens``, INT64 ``[rows]``), as one call of the
+    attention takes them.  ``target`` (BF16 or FP32 ``[rows, vocab]``, unit
+    column stride) holds the target's distribution of the token behind each
+    row, ``draft`` (of the same type) the distribution that the next row's draft was
+    drawn from; without it the drafts were certain (looked up, or greedy).
+    ``uniforms`` are FP32 random numbers of [0, 1), one per row.  In order, the
+    draft behind row r is taken iff ``uniforms[r] * draft < target`` at it; at
+    the first that is not, a token is drawn from what the target has above the
+    draft, behind the last draft from the target, by ``uniforms`` of the
+    request's last row: the lowest token whose running sum exceeds that share
+    of the sum.  Sums are FP64.  Row r of the result's ``tokens`` is the token
+    behind row r: drafts taken, the drawn token (-1 if no weight is positive),
+    then -1 (also in rows outside ``query_start_loc``).  Probabilities need not
+    sum to 1; entries that are negative, NaN or infinite count as 0.
+    """
+    shape, strides, dtype = target.shape, target.stride(), target.dtype
+    if not (target.is_cuda and len(shape) == 2 and (strides[1] == 1 or shape[1] == 1)
+            and (dtype is torch.bfloat16 or dtype is torch.float32)):
+        raise RuntimeError("target must be BF16 or FP32 [rows, vocab] on a HIP device with unit column stride")
+    rows, vocab = shape
+    device = target.get_device()
+    if draft is not None:
+        _require(draft.get_device() == device and draft.dtype is dtype and draft.shape == shape
+                 and (draft.stride(1) == 1 or vocab == 1), "draft must match target in shape, type and device")
+    _require(tokens.get_device() == device and tokens.dtype is torch.int64 and tokens.dim() == 1
+             and tokens.is_contiguous() and tokens.numel() == rows,
+             "Contiguous INT64 tokens, one per row, on the target's device required")
+    _require(uniforms.get_device() == device and uniforms.dtype is torch.float32 and uniforms.dim() == 1
+             and uniforms.is_contiguous() and uniforms.numel() == rows,
+             "Contiguous FP32 uniforms, one per row, on the target's device required")
+    _require(query_start_loc.get_device() == device and query_start_loc.dtype is torch.int32
+             and query_start_loc.dim() == 1 and query_start_loc.is_contiguous() and query_start_loc.numel() > 0,
+             "Contiguous INT32 query starts with one final boundary required")
+    requests = query_start_loc.numel() - 1
+    accepted = query_start_loc.new_empty(requests)
+    # (Without requests no kernel runs.)
+    following = torch.empty_like(tokens) if requests > 0 else torch.full_like(tokens, -1)
+    if workspace is None:
+        workspace = tokens.new_empty(_verify_workspace_bytes(requests, vocab), dtype=torch.uint8)
+    else:
+        _require(workspace.get_device() == device and workspace.is_contiguous(),
+                 "Contiguous verification workspace on the target's device required")
+    with _on_device(device):
+        status = _lib.lib().rq_verify_drafts(
+            target.data_ptr(), strides[0] if rows > 1 else vocab, draft.data_ptr() if draft is not None else None,
+            draft.stride(0) if draft is not None and rows > 1 else vocab, 0 if dtype is torch.bfloat16 else 1, rows,
+            vocab, tokens.data_ptr(), uniforms.data_ptr(), query_start_loc.data_ptr(), requests, accepted.data_ptr(),
+            following.data_ptr(), workspace.data_ptr(), workspace.nbytes, torch._C._cuda_getCurrentRawStream(device))
+    _lib.check(status)
+    return VerifiedDrafts(accepted, following)
