@@ -397,7 +397,7 @@ enum { RQ_SCALE_E8M0 = 0, RQ_SCALE_F32 = 1 };
  * (the last of each side may be smaller), laid out once for the kernels in
  * rq_fp8_weight_bytes(...) bytes of 16-byte aligned device memory (0 for an
  * invalid shape).  out_features up to 2^24, in_features up to 2^20, of any
- * value, together fewer than 2^36 elements in whole tiles of 16 x 128.
+ * value, together fewer than 2^36 elements in whole tiles of 64 x 128.
  * rq_pack_weight_fp8 takes codes [out, in] and scales
  * [ceil(out / 128), ceil(in / 128)], both contiguous; rq_quantize_weight_fp8 a
  * BF16 weight (scales are exponents: the least power of two s >= 2^-126 with
@@ -410,8 +410,8 @@ enum { RQ_SCALE_E8M0 = 0, RQ_SCALE_F32 = 1 };
  * ties to even, NaN for what is not finite.  FP32 sums; results below the
  * normal range of FP32 may be 0.  x of any even address and row stride
  * (16-byte aligned rows are read faster).  `workspace`: device memory of
- * rq_linear_fp8_workspace_bytes(...), any address; calls that may overlap need
- * one each.
+ * rq_linear_fp8_workspace_bytes(...) (0 for a few rows), any address; calls
+ * that may overlap need one each.
  */
 size_t rq_fp8_weight_bytes(int64_t out_features, int64_t in_features, int scale_type);
 int rq_pack_weight_fp8(const void* codes, const void* scales, int scale_type, int64_t out_features, int64_t in_features,

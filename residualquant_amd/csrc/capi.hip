@@ -1483,9 +1483,9 @@ static int check_fp8_shape(int64_t out_features, int64_t in_features, int scale_
         return fail(RQ_EINVAL, "Scales as exponents (E8M0) or in FP32 required");
     // (Packed by one thread per 16 elements of whole tiles of 16 x 128.)
     if (out_features <= 0 || in_features <= 0 || out_features > (1 << 24) || in_features > (1 << 20) ||
-        !launchable(((out_features + 15) / 16) * ((in_features + 127) / 128), 128))
+        !launchable(((out_features + 63) / 64) * ((in_features + 127) / 128), 512))
         return fail(RQ_EINVAL, "8-bit weights need out_features up to 2^24, in_features up to 2^20 and fewer than 2^36 "
-                               "elements in whole tiles of 16 x 128");
+                               "elements in whole tiles of 64 x 128");
     return RQ_OK;
 }
 
@@ -1545,8 +1545,9 @@ int rq_dequantize_weight_fp8(const void* packed, size_t packed_bytes, int scale_
 }
 
 size_t rq_linear_fp8_workspace_bytes(int64_t rows, int64_t in_features) {
-    if (rows <= 0 || rows > rq::kLinearFp8MaxRows || in_features <= 0 || in_features > (1 << 20)) return 256;
-    return 256 + rq::linear_fp8_workspace(rows, in_features);
+    if (rows <= 0 || rows > rq::kLinearFp8MaxRows || in_features <= 0 || in_features > (1 << 20)) return 0;
+    const size_t bytes = rq::linear_fp8_workspace(rows, in_features);
+    return bytes > 0 ? 256 + bytes : 0;
 }
 
 int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t packed_bytes, int scale_type, void* y,
@@ -1566,7 +1567,7 @@ int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t pa
     if (!launchable(((rows + 15) / 16) * ((in_features + 511) / 512), 256))
         return fail(RQ_EINVAL, "Too many rows and inputs for one call");
     const size_t needed = rq_linear_fp8_workspace_bytes(rows, in_features);
-    if (workspace == nullptr || workspace_bytes < needed)
+    if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
         return fail(RQ_ENOSPACE, "Projection workspace of %zu bytes required, %zu given", needed, workspace_bytes);
     rq::LinearFp8Params p{};
     p.x = static_cast<const uint16_t*>(x);
@@ -1580,8 +1581,7 @@ int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t pa
     p.in_features = in_features;
     p.exponents = w.exponents;
     p.compute_units = compute_units();
-    p.x_codes = static_cast<uint8_t*>(workspace) + to_boundary(workspace);
-    p.x_scales = reinterpret_cast<uint32_t*>(p.x_codes + rq::fp8_code_bytes(rows, in_features));
+    if (needed > 0) p.x_codes = static_cast<uint8_t*>(workspace) + to_boundary(workspace);
     return check_launch(rq::launch_linear_fp8(p, stream), "8-bit projection launch");
 }
 

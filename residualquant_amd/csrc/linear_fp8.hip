@@ -9,6 +9,13 @@
 // holds row i, inputs 32 g + 16 h + 0..15 in the 16 bytes at 1024 h + 16 l, h = 0,
 // 1.  (An instruction sums over all 128 inputs, so their order matters only in
 // that both operands have the same.)  Rows and inputs past the matrix hold 0.
+// Of 32 outputs, tile t (0, 1) holds the outputs 8 g + 4 t + r as its rows 4 g + r: a
+// lane of the result, which has rows 4 g + 0..3 of a tile, then has 8 neighbouring
+// outputs of both tiles, and a row's 32 outputs are stored as 64 bytes at once.
+// Weights lie as [64 outputs][block][tile][2 KB], x as [block][tile][2 KB]: what the
+// waves read at a time is whole stretches of 8 KB and more, which all channels of
+// the L2 cache hold alike.  (With each tile's blocks in a row, at 2048 inputs a tile
+// begins every 32 KB, and workgroups at the same block met in half the channels.)
 // The instruction multiplies by powers of two as it goes: sx always, sw if it
 // is an exponent; an FP32 sw multiplies each block's FP32 sum instead.
 //
@@ -20,6 +27,7 @@
 // codes converted to BF16 operands would not (3e-7), at half the rate and with a
 // conversion per two codes.
 #include <algorithm>
+#include <type_traits>
 
 #include "rq_device.h"
 #include "rq_fp8.h"
@@ -35,6 +43,18 @@ typedef int I32x8 __attribute__((ext_vector_type(8)));
 constexpr int kBlock = 128, kTileBytes = 16 * kBlock;
 
 __host__ __device__ __forceinline__ int64_t tiles_of(int64_t rows) { return (rows + 15) / 16; }
+// (Whole groups of 64, as the waves of the product for many rows take them.)
+__host__ __device__ __forceinline__ int64_t out_tiles_of(int64_t out_features) { return (out_features + 63) / 64 * 4; }
+// The output that row `row` of a tile stands for.
+__device__ __forceinline__ int64_t output_of(int64_t tile, int row) {
+    return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (int)(tile & 1) + (row & 3);
+}
+// Places of a weight's tile and of a tile of x, in tiles.
+__device__ __forceinline__ int64_t weight_place(int64_t tile, int64_t blocks, int64_t block) {
+    return 4 * ((tile >> 2) * blocks + block) + (tile & 3);
+}
+__device__ __forceinline__ int64_t row_place(int64_t tile, int64_t row_tiles, int64_t block) { return block * row_tiles + tile; }
+
 __host__ __device__ __forceinline__ int64_t blocks_of(int64_t in_features) { return (in_features + kBlock - 1) / kBlock; }
 // Scales lie in fours, one word per row (or block row) and four blocks.
 __host__ __device__ __forceinline__ int64_t fours_of(int64_t in_features) { return (blocks_of(in_features) + 3) / 4; }
@@ -50,7 +70,7 @@ __device__ __forceinline__ float finite_size(float x) { return fabsf(x) < __buil
 
 // One thread per 16 bytes of the packed codes.
 __global__ __launch_bounds__(256) void pack_fp8_kernel(const Fp8PackParams p) {
-    const int64_t blocks = blocks_of(p.in_features), pieces = tiles_of(p.out_features) * blocks * (kTileBytes / 16);
+    const int64_t blocks = blocks_of(p.in_features), pieces = out_tiles_of(p.out_features) * blocks * (kTileBytes / 16);
     const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t high = (p.out_features + kBlock - 1) / kBlock, wide = 4 * fours_of(p.in_features);
     if (w < high * wide) {
@@ -62,7 +82,7 @@ __global__ __launch_bounds__(256) void pack_fp8_kernel(const Fp8PackParams p) {
     }
     if (w >= pieces) return;
     const int lane = (int)w & 63, half = (int)(w >> 6) & 1;
-    const int64_t block = (w >> 7) % blocks, n = 16 * ((w >> 7) / blocks) + (lane & 15);
+    const int64_t block = (w >> 9) % blocks, n = output_of(4 * ((w >> 9) / blocks) + ((w >> 7) & 3), lane & 15);
     const int64_t k = kBlock * block + 32 * (lane >> 4) + 16 * half;
     U32x4 piece = {0u, 0u, 0u, 0u};
     if (n < p.out_features)
@@ -92,27 +112,27 @@ __global__ __launch_bounds__(256) void quantize_weight_fp8_kernel(const Fp8PackP
             for (int64_t b = blocks; b < wide; ++b) p.packed_scales[high * wide + b] = 127;
     }
     const float inverse = inverse_scale(exponent);
-    const int64_t tiles = tiles_of(p.out_features);
+    const int64_t tiles = out_tiles_of(p.out_features);
     for (int w = threadIdx.x; w < 8 * (kTileBytes / 16); w += 256) {
         const int lane = w & 63, half = (w >> 6) & 1;
-        const int64_t tile = 8 * high + (w >> 7), n = 16 * tile + (lane & 15), k = kBlock * block + 32 * (lane >> 4) + 16 * half;
+        const int64_t tile = 8 * high + (w >> 7), n = output_of(tile, lane & 15), k = kBlock * block + 32 * (lane >> 4) + 16 * half;
         if (tile >= tiles) continue;
         float x[16];
         for (int e = 0; e < 16; ++e)
             x[e] = n < p.out_features && k + e < p.in_features ? bf16_f32(p.weight[n * p.in_features + k + e]) * inverse : 0.f;
         U32x4 piece;
         for (int e = 0; e < 4; ++e) piece[e] = fp8x4_rn(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-        reinterpret_cast<U32x4*>(p.packed)[((tile * blocks + block) * 2 + half) * 64 + lane] = piece;
+        reinterpret_cast<U32x4*>(p.packed)[(weight_place(tile, blocks, block) * 2 + half) * 64 + lane] = piece;
     }
 }
 
 // The BF16 weight [out, in] of a packed one: bf16(code x scale).  One thread per 16 bytes.
 __global__ __launch_bounds__(256) void unpack_fp8_kernel(const Fp8PackParams p, uint16_t* weight) {
-    const int64_t blocks = blocks_of(p.in_features), pieces = tiles_of(p.out_features) * blocks * (kTileBytes / 16);
+    const int64_t blocks = blocks_of(p.in_features), pieces = out_tiles_of(p.out_features) * blocks * (kTileBytes / 16);
     const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (w >= pieces) return;
     const int lane = (int)w & 63, half = (int)(w >> 6) & 1;
-    const int64_t block = (w >> 7) % blocks, n = 16 * ((w >> 7) / blocks) + (lane & 15);
+    const int64_t block = (w >> 9) % blocks, n = output_of(4 * ((w >> 9) / blocks) + ((w >> 7) & 3), lane & 15);
     const int64_t k = kBlock * block + 32 * (lane >> 4) + 16 * half;
     if (n >= p.out_features) return;
     const int64_t at = n / kBlock * (4 * fours_of(p.in_features)) + block;
@@ -130,6 +150,44 @@ __global__ __launch_bounds__(256) void unpack_fp8_kernel(const Fp8PackParams p, 
 
 // ------------------------------------------------------------------ rows
 
+// Eight neighbouring values of a row as they lie there (0 past its end); Wide: from 16-byte aligned addresses.
+template <bool Wide>
+__device__ __forceinline__ U32x4 load_values(const uint16_t* row, int64_t k, int64_t in_features) {
+    if (Wide && k + 8 <= in_features) return *reinterpret_cast<const U32x4*>(row + k);
+    U32x4 raw;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        raw[e] = (k + 2 * e < in_features ? row[k + 2 * e] : 0u) | (k + 2 * e + 1 < in_features ? (uint32_t)row[k + 2 * e + 1] << 16 : 0u);
+    return raw;
+}
+
+// A block of a row, eight values in each of 16 neighbouring lanes: its scale's byte, and these values' codes.
+struct RowCodes {
+    int exponent;
+    uint2 codes;
+};
+__device__ __forceinline__ RowCodes quantize_row_block(U32x4 raw) {
+    float x[8], largest = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(raw[e] << 16);
+        x[2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_size(x[e]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+    RowCodes r;
+    r.exponent = scale_exponent(largest);
+    const float inverse = inverse_scale(r.exponent);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= inverse;
+    r.codes = make_uint2(fp8x4_rn(x[0], x[1], x[2], x[3]), fp8x4_rn(x[4], x[5], x[6], x[7]));
+    return r;
+}
+// Where the codes of row i's values 8 j.. of a block lie in its tile.
+__device__ __forceinline__ int code_place(int i, int j) { return 1024 * ((j >> 1) & 1) + 16 * (i + 16 * (j >> 2)) + 8 * (j & 1); }
+
 // One workgroup per tile of 16 rows and four blocks of 128 inputs; 16 lanes per row of a block.
 template <bool Wide>
 __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const LinearFp8Params p) {
@@ -137,39 +195,18 @@ __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const LinearFp8P
     const int64_t blocks = blocks_of(p.in_features), fours = fours_of(p.in_features);
     const int64_t four = blockIdx.x % fours, tile = blockIdx.x / fours, m = 16 * tile + i;
     const uint16_t* row = p.x + m * p.x_stride;
+    U32x4 x[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) x[b] = load_values<Wide>(row, kBlock * (4 * four + b) + 8 * j, m < p.rows ? p.in_features : 0);
     uint32_t word = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-        const int64_t block = 4 * four + b, k = kBlock * block + 8 * j;
-        float x[8];
-        if (Wide && m < p.rows && k + 8 <= p.in_features) {
-            const U32x4 raw = *reinterpret_cast<const U32x4*>(row + k);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[2 * e] = __uint_as_float(raw[e] << 16);
-                x[2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = m < p.rows && k + e < p.in_features ? bf16_f32(row[k + e]) : 0.f;
-        }
-        float largest = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_size(x[e]));
-#pragma unroll
-        for (int d = 8; d; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
-        const int exponent = scale_exponent(largest);
-        const float inverse = inverse_scale(exponent);
-        word |= (uint32_t)exponent << (8 * b);
-        if (block < blocks) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= inverse;
-            const uint2 codes = make_uint2(fp8x4_rn(x[0], x[1], x[2], x[3]), fp8x4_rn(x[4], x[5], x[6], x[7]));
-            uint8_t* to = p.x_codes + (tile * blocks + block) * kTileBytes;
-            *reinterpret_cast<uint2*>(to + 1024 * ((j >> 1) & 1) + 16 * (i + 16 * (j >> 2)) + 8 * (j & 1)) = codes;
-        }
+        const RowCodes r = quantize_row_block(x[b]);
+        word |= (uint32_t)r.exponent << (8 * b);
+        if (4 * four + b < blocks)
+            *reinterpret_cast<uint2*>(p.x_codes + row_place(tile, tiles_of(p.rows), 4 * four + b) * kTileBytes + code_place(i, j)) = r.codes;
     }
-    if (j == 0) p.x_scales[(tile * fours + four) * 16 + i] = word;
+    if (j == 0) p.x_scales[(four * tiles_of(p.rows) + tile) * 16 + i] = word;
 }
 
 // ------------------------------------------------------------------ product
@@ -180,78 +217,491 @@ __device__ __forceinline__ I32x8 operand(const uint8_t* tile, int lane) {
 }
 
 // 16 outputs (a) x 16 rows (b) over 128 inputs; lane (i, g) of the result: row i, outputs 4 g + 0..3.
+// The scales are bytes A and B of their words.
+template <int A = 0, int B = 0>
 __device__ __forceinline__ F32x4 mfma(I32x8 a, I32x8 b, F32x4 c, uint32_t scale_a, uint32_t scale_b) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, (int)scale_a, 0, (int)scale_b);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, A, (int)scale_a, B, (int)scale_b);
 }
 
-// One workgroup of eight waves per 16 outputs and T tiles of 16 rows; the waves share the inputs out.
-template <int T, bool Exponents>
-__global__ __launch_bounds__(512) void linear_fp8_kernel(const LinearFp8Params p) {
-    __shared__ F32x4 partial[8][T][64];
+// Up to some hundred rows: one workgroup of eight waves per J tiles of outputs and T tiles of 16 rows. The
+// waves share the inputs out, each with operands straight from global memory (whole
+// stretches of 2 KB) and a block's in flight while the one before is multiplied,
+// and join through LDS.
+template <int J, int T, bool Exponents>
+__global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Params p) {
+    __shared__ F32x4 partial[8][J * T][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int blocks = (int)blocks_of(p.in_features), fours = (int)fours_of(p.in_features);
-    const int64_t tile = blockIdx.x, row_tiles = tiles_of(p.rows), first = (int64_t)blockIdx.y * T;
+    const int64_t row_tiles = tiles_of(p.rows), row_groups = (row_tiles + T - 1) / T;
+    const int64_t tile0 = J * (blockIdx.x / row_groups), row_tile0 = T * (blockIdx.x % row_groups);
     const int begin = blocks * wave / 8, end = blocks * (wave + 1) / 8;
-    F32x4 total[T];
+    typedef std::conditional_t<Exponents, uint32_t, float> Scale;
+    struct Block {
+        I32x8 a[J], x[T];
+        uint32_t words[T];
+        Scale scale;
+    };
+    auto load = [&](Block& to, int b) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) total[t] = F32x4{0.f, 0.f, 0.f, 0.f};
-    const int64_t scales = tile / 8 * (4 * fours);
-    for (int b = begin; b < end; ++b) {
-        const I32x8 a = operand(p.packed + (tile * blocks + b) * kTileBytes, lane);
+        for (int j = 0; j < J; ++j) to.a[j] = operand(p.packed + weight_place(tile0 + j, blocks, b) * kTileBytes, lane);
 #pragma unroll
         for (int t = 0; t < T; ++t) {
-            const int64_t m = min(first + t, row_tiles - 1);
-            const I32x8 x = operand(p.x_codes + (m * blocks + b) * kTileBytes, lane);
-            const uint32_t x_scale = p.x_scales[(m * fours + (b >> 2)) * 16 + i] >> (8 * (b & 3));
-            if constexpr (Exponents) {
-                total[t] = mfma(a, x, total[t], p.packed_scales[scales + b], x_scale);
-            } else {
-                const F32x4 sum = mfma(a, x, F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scale);
-                const float scale = reinterpret_cast<const float*>(p.packed_scales)[scales + b];
+            const int64_t m = min(row_tile0 + t, row_tiles - 1);
+            to.x[t] = operand(p.x_codes + row_place(m, row_tiles, b) * kTileBytes, lane);
+            to.words[t] = p.x_scales[((b >> 2) * row_tiles + m) * 16 + i];
+        }
+        if constexpr (Exponents)
+            to.scale = reinterpret_cast<const uint32_t*>(p.packed_scales)[tile0 / 8 * fours + (b >> 2)];
+        else
+            to.scale = reinterpret_cast<const float*>(p.packed_scales)[tile0 / 8 * (4 * fours) + b];
+    };
+    F32x4 total[J][T];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) total[t][r] = fmaf(scale, sum[r], total[t][r]);
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int t = 0; t < T; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Block& of, int b) {
+        const int shift = 8 * (b & 3);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                if constexpr (Exponents) {
+                    total[j][t] = mfma(of.a[j], of.x[t], total[j][t], of.scale >> shift, of.words[t] >> shift);
+                } else {
+                    const F32x4 sum = mfma(of.a[j], of.x[t], F32x4{0.f, 0.f, 0.f, 0.f}, 127u, of.words[t] >> shift);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(of.scale, sum[r], total[j][t][r]);
+                }
             }
+    };
+    // (Loads without a condition, past the end the last block again: after a load that one path leaves out every wait
+    // is for all loads in flight.)
+    Block now, next;
+    load(now, min(begin, blocks - 1));
+    for (int b = begin; b < end; b += 2) {
+        load(next, min(b + 1, blocks - 1));
+        multiply(now, b);
+        load(now, min(b + 2, blocks - 1));
+        if (b + 1 < end) multiply(next, b + 1);
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int t = 0; t < T; ++t) partial[wave][j * T + t][lane] = total[j][t];
+    __syncthreads();
+    // The waves share the tiles out, a pair with neighbouring outputs at a time.
+    constexpr int kPair = J > 1 ? 2 : 1;
+    for (int q = wave; q < J / kPair * T; q += 8) {
+        const int j = kPair * (q / T), t = q % T;
+        F32x4 sum[kPair];
+#pragma unroll
+        for (int h = 0; h < kPair; ++h) {
+            sum[h] = partial[0][(j + h) * T + t][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) sum[h] += partial[w][(j + h) * T + t][lane];
+        }
+        const int64_t n = output_of(tile0 + j, 4 * g), m = 16 * (row_tile0 + t) + i;
+        if (m >= p.rows) continue;
+        uint16_t* const to = p.y + m * p.y_stride + n;
+        if (kPair == 2 && p.aligned && n + 8 <= p.out_features) {
+            const F32x4 u = sum[0], v = sum[kPair - 1];
+            *reinterpret_cast<U32x4*>(to) = U32x4{bf16x2_rn(u[0], u[1]), bf16x2_rn(u[2], u[3]), bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3])};
+            continue;
+        }
+#pragma unroll
+        for (int h = 0; h < kPair; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n + 4 * h + r < p.out_features) to[4 * h + r] = (uint16_t)bf16_rn(sum[h][r]);
+    }
+}
+
+// A few rows: one launch. Workgroups of eight waves round x into LDS as operands,
+// each for itself, while their first weights are on the way, and take tiles of outputs
+// one after the other; the waves share the inputs out and join through LDS.
+// (One row, 2048 -> 6144: 4.1 us, 2048 -> 50257 17.6; with two tiles at a time 4.4 and
+// 22.8, with four 6.0 and 25; with three and six blocks of weights in flight
+// 4.4 and 18.9, 5.7 and 26.5.)
+constexpr int kFewAhead = 2;     // blocks of weights in flight
+constexpr int kFewAtOnce = 128;  // rows of blocks of x
+constexpr int kFewMaxBlocks = 64;  // that LDS holds
+template <bool Exponents, bool Wide>
+__global__ __launch_bounds__(512) void linear_fp8_few_kernel(const LinearFp8Params p) {
+    extern __shared__ __align__(16) uint8_t few_lds[];  // x's codes [block][2 KB], its scales' bytes [block][16]
+    __shared__ F32x4 partial[2][8][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int i = lane & 15, g = lane >> 4, rows = (int)p.rows;
+    const int blocks = (int)blocks_of(p.in_features), fours = (int)fours_of(p.in_features);
+    uint8_t* const bytes = few_lds + blocks * kTileBytes;
+    const int begin = blocks * wave / 8, end = blocks * (wave + 1) / 8;
+    const int64_t tiles = out_tiles_of(p.out_features);
+    int64_t tile = blockIdx.x;
+    typedef std::conditional_t<Exponents, uint32_t, float> Scale;
+    struct Block {
+        I32x8 a;
+        Scale scale;
+    };
+    auto load = [&](Block& to, int b) {
+        b = min(b, blocks - 1);
+        to.a = operand(p.packed + weight_place(tile, blocks, b) * kTileBytes, lane);
+        if constexpr (Exponents)
+            to.scale = p.packed_scales[tile / 8 * (4 * fours) + b];
+        else
+            to.scale = reinterpret_cast<const float*>(p.packed_scales)[tile / 8 * (4 * fours) + b];
+    };
+    Block held[kFewAhead];
+#pragma unroll
+    for (int a = 0; a < kFewAhead; ++a) load(held[a], begin + a);
+    // 16 lanes per row of a block, the values of kFewAtOnce such rows in flight together.
+    const int j16 = tid & 15;
+    for (int q = tid >> 4; q < rows * blocks; q += kFewAtOnce) {
+        U32x4 x[kFewAtOnce / 32];
+#pragma unroll
+        for (int h = 0; h < kFewAtOnce / 32; ++h) {
+            const int r = min(q + 32 * h, rows * blocks - 1);
+            x[h] = load_values<Wide>(p.x + r / blocks * p.x_stride, kBlock * (r % blocks) + 8 * j16, p.in_features);
+        }
+#pragma unroll
+        for (int h = 0; h < kFewAtOnce / 32; ++h) {
+            const int r = q + 32 * h, row = r / blocks, b = r % blocks;
+            if (r >= rows * blocks) break;
+            const RowCodes codes = quantize_row_block(x[h]);
+            *reinterpret_cast<uint2*>(few_lds + b * kTileBytes + code_place(row, j16)) = codes.codes;
+            if (j16 == 0) bytes[16 * b + row] = (uint8_t)codes.exponent;
         }
     }
+    lds_barrier();
+    int side = 0;
+    while (true) {
+        F32x4 total = {0.f, 0.f, 0.f, 0.f};
+        for (int b = begin; b < end; b += kFewAhead) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) partial[wave][t][lane] = total[t];
-    __syncthreads();
-    for (int t = wave; t < T; t += 8) {
-        F32x4 sum = partial[0][t][lane];
+            for (int a = 0; a < kFewAhead; ++a) {
+                // (Rows past the last hold what LDS held: their results are not stored.)
+                if (b + a < end) {
+                    const I32x8 x = operand(few_lds + (b + a) * kTileBytes, lane);
+                    const uint32_t x_scale = bytes[16 * (b + a) + i];
+                    if constexpr (Exponents) {
+                        total = mfma(held[a].a, x, total, held[a].scale, x_scale);
+                    } else {
+                        const F32x4 sum = mfma(held[a].a, x, F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scale);
 #pragma unroll
-        for (int w = 1; w < 8; ++w) sum += partial[w][t][lane];
-        const int64_t n = 16 * tile + 4 * g, m = 16 * (first + t) + i;
-        if (m >= p.rows) continue;
+                        for (int r = 0; r < 4; ++r) total[r] = fmaf(held[a].scale, sum[r], total[r]);
+                    }
+                }
+                load(held[a], b + a + kFewAhead);
+            }
+        }
+        const int64_t own = tile;
+        tile += gridDim.x;
+        if (tile < tiles) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < p.out_features) p.y[m * p.y_stride + n + r] = (uint16_t)bf16_rn(sum[r]);
+            for (int a = 0; a < kFewAhead; ++a) load(held[a], begin + a);
+        }
+        partial[side][wave][lane] = total;
+        lds_barrier();
+        if (wave == 0) {
+            F32x4 sum = partial[side][0][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) sum += partial[side][w][lane];
+            const int64_t n = output_of(own, 4 * g);
+            if (i < rows) {
+                uint16_t* const to = p.y + i * p.y_stride + n;
+                if (p.aligned && n + 4 <= p.out_features) {
+                    *reinterpret_cast<uint2*>(to) = make_uint2(bf16x2_rn(sum[0], sum[1]), bf16x2_rn(sum[2], sum[3]));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (n + r < p.out_features) to[r] = (uint16_t)bf16_rn(sum[r]);
+                }
+            }
+        }
+        if (tile >= tiles) return;
+        side ^= 1;  // (whose last readers passed the barrier above)
     }
+}
+
+// Many rows: workgroups of four waves take tiles of 256 outputs and 16 NT rows, a
+// wave 64 outputs.  x passes LDS, where the four waves of its rows
+// read it, in a ring of four blocks of inputs with a barrier every two; the weights
+// go from global memory to the operands, since their order there is the operands'
+// own and only two waves share them.  (Through LDS both would take it 128 bytes a
+// cycle, all that it has, at the matrix instructions' full rate.)  What a block
+// reads from global memory was asked for a block ahead, and a tile's first block
+// before the results of the tile before it are stored.
+template <bool Exponents, int NT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_fp8_wide_kernel(const LinearFp8Params p) {
+    constexpr int kPieces = NT * kTileBytes / 16 / 256;  // 16-byte pieces of x per thread and block
+    __shared__ __align__(16) uint8_t lds[4][NT * kTileBytes];
+    __shared__ uint32_t x_words[2][16 * NT];  // scales of its rows, for four blocks each
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int blocks = (int)blocks_of(p.in_features), fours = (int)fours_of(p.in_features);
+    const int64_t out_groups = (p.out_features + 255) / 256, row_groups = (p.rows + 16 * NT - 1) / (16 * NT);
+    const int64_t out_tiles = out_tiles_of(p.out_features), row_tiles = tiles_of(p.rows);
+    // (In 32 bits: rows_at_once.)
+    const uint32_t x_stride = (uint32_t)row_tiles * kTileBytes, words_stride = (uint32_t)row_tiles * 64;
+
+    // Neighbouring workgroups run on different XCDs: each XCD takes a stretch of the
+    // tiles, eight row groups wide, whose weights and rows its workgroups share.
+    const int64_t tiles = out_groups * row_groups, per = (tiles + 7) / 8;
+    const int64_t stop = min(((int64_t)(blockIdx.x & 7) + 1) * per, tiles);
+    const int step_of_tiles = gridDim.x >> 3;
+    int64_t tile0, row_tile0;  // of this wave's outputs, of the rows
+    __amdgpu_buffer_rsrc_t weights, x_all, x_scales;
+    typedef std::conditional_t<Exponents, uint32_t, F32x4> Scales;  // of the weight, for four blocks
+    const Scales* scales_of;
+    // Tiles past the weight's last read as 0, past x's as other rows or 0: neither is stored.
+    auto take = [&](int64_t number) {
+        const int64_t band = number / (8 * out_groups), in_band = number - band * 8 * out_groups;
+        const int64_t high = min((int64_t)8, row_groups - 8 * band);
+        const int64_t out_group = in_band / high, row_group = 8 * band + in_band % high;
+        tile0 = 16 * out_group + 4 * wave;
+        row_tile0 = NT * row_group;
+        auto resource = [](const void* base, int64_t bytes) { return handoff_resource(base, (uint32_t)bytes); };
+        weights = resource(p.packed + min(tile0, out_tiles) * blocks * kTileBytes, tile0 < out_tiles ? 4 * blocks * kTileBytes : 0);
+        x_all = resource(p.x_codes + row_tile0 * kTileBytes, (blocks * row_tiles - row_tile0) * kTileBytes);
+        x_scales = resource(p.x_scales + row_tile0 * 16, (fours * row_tiles - row_tile0) * 64);
+        scales_of = reinterpret_cast<const Scales*>(p.packed_scales) + (tile0 < out_tiles ? tile0 / 8 : 0) * fours;
+    };
+
+    F32x4 total[4][NT];
+    I32x8 a[2][4];
+    U32x4 piece[kPieces];
+    uint32_t word;  // of x's scales, on its way to LDS
+    Scales w_scales;
+    auto load_x = [&](int b) {
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+            piece[c] = __builtin_amdgcn_raw_buffer_load_b128(x_all, 16 * tid, 4096 * c + b * x_stride, 0);
+    };
+    auto store_x = [&](int buffer) {
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) *reinterpret_cast<U32x4*>(&lds[buffer][16 * (256 * c + tid)]) = piece[c];
+    };
+    auto load_a = [&](I32x8 (&to)[4], int b) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t at = (4 * b + j) * kTileBytes;
+            const U32x4 low = __builtin_amdgcn_raw_buffer_load_b128(weights, 16 * lane, at, 0);
+            const U32x4 high = __builtin_amdgcn_raw_buffer_load_b128(weights, 16 * lane + 1024, at, 0);
+            to[j] = I32x8{(int)low[0], (int)low[1], (int)low[2], (int)low[3], (int)high[0], (int)high[1], (int)high[2], (int)high[3]};
+        }
+    };
+    auto load_word = [&](int four) {
+        word = __builtin_amdgcn_raw_buffer_load_b32(x_scales, 4 * tid, four * words_stride, 0);
+    };
+    auto store_word = [&](int four) {
+        if (tid < 16 * NT) x_words[four & 1][tid] = word;
+    };
+    auto load_scales = [&](int four) {
+        Scales v = scales_of[four];
+        if constexpr (Exponents)
+            v = __builtin_amdgcn_readfirstlane(v);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v[e])));
+        return v;
+    };
+    // Block 4 four + S.  (Blocks past the last are read as they come and not used: within the resources, or 0.)
+    auto step = [&](auto place, int four) {
+        constexpr int S = decltype(place)::value;
+        const int b = 4 * four + S;
+        store_x((S + 2) & 3);
+        load_x(b + 3);
+        load_a(a[(S + 1) & 1], b + 1);
+        if constexpr (S == 0) load_word(four + 1);
+        if constexpr (S == 2) store_word(four + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* from = lds[S];
+        const uint32_t* from_words = &x_words[four & 1][i];
+        I32x8 x[2];
+        uint32_t x_scale[2];
+        x[0] = operand(from, lane);
+        x_scale[0] = from_words[0];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (t + 1 < NT) {
+                x[(t + 1) & 1] = operand(from + (t + 1) * kTileBytes, lane);
+                x_scale[(t + 1) & 1] = from_words[16 * (t + 1)];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (Exponents) {
+                    total[j][t] = mfma<S, S>(a[S & 1][j], x[t & 1], total[j][t], w_scales, x_scale[t & 1]);
+                } else {
+                    const F32x4 sum = mfma<0, S>(a[S & 1][j], x[t & 1], F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scale[t & 1]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(w_scales[S], sum[r], total[j][t][r]);
+                }
+            }
+        }
+        // The operands of a row tile are read while the products of the one before run.
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+        for (int t = 0; t < NT - 1; ++t) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        if constexpr (S & 1) lds_barrier();
+    };
+
+    int64_t number = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (number >= stop) return;
+    auto begin = [&] {
+        take(number);
+        load_x(0);
+        load_a(a[0], 0);
+        load_word(0);
+    };
+    begin();
+    while (true) {
+        w_scales = load_scales(0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
+        store_x(0);
+        store_word(0);
+        load_x(1);
+        store_x(1);
+        load_x(2);
+        lds_barrier();
+        for (int four = 0; four < fours; ++four) {
+            step(std::integral_constant<int, 0>{}, four);
+            if (4 * four + 1 < blocks) step(std::integral_constant<int, 1>{}, four);
+            if (4 * four + 2 < blocks) step(std::integral_constant<int, 2>{}, four);
+            if (4 * four + 3 < blocks) step(std::integral_constant<int, 3>{}, four);
+            w_scales = load_scales(min(four + 1, fours - 1));
+        }
+        // The next tile's first block, then this one's results.
+        const int64_t out_at = 16 * tile0 + 8 * g, row_at = 16 * row_tile0 + i;
+        number += step_of_tiles;
+        const bool more = number < stop;
+        if (more) begin();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int64_t m = row_at + 16 * t;
+            if (m >= p.rows) continue;
+            uint16_t* const to = p.y + m * p.y_stride + out_at;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const F32x4 u = total[2 * h][t], v = total[2 * h + 1][t];
+                if (p.aligned && out_at + 32 * h + 8 <= p.out_features) {
+                    *reinterpret_cast<U32x4*>(to + 32 * h) =
+                        U32x4{bf16x2_rn(u[0], u[1]), bf16x2_rn(u[2], u[3]), bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3])};
+                    continue;
+                }
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (out_at + 32 * h + r < p.out_features) to[32 * h + r] = (uint16_t)bf16_rn(r < 4 ? u[r] : v[r - 4]);
+            }
+        }
+        if (!more) return;
+        // (A step of the last pair may still be reading its buffers.)
+        lds_barrier();
+    }
+}
+
+template <bool Exponents, bool Wide>
+void launch_few(const LinearFp8Params& p, hipStream_t stream) {
+    const size_t lds = blocks_of(p.in_features) * (kTileBytes + 16);
+    const unsigned grid = (unsigned)std::min<int64_t>(out_tiles_of(p.out_features), 2 * p.compute_units);
+    hipLaunchKernelGGL((linear_fp8_few_kernel<Exponents, Wide>), dim3(grid), dim3(512), lds, stream, p);
+}
+
+template <bool Exponents, int J, int T>
+void launch_split(const LinearFp8Params& p, hipStream_t stream) {
+    const int64_t groups = out_tiles_of(p.out_features) / J * ((tiles_of(p.rows) + T - 1) / T);
+    hipLaunchKernelGGL((linear_fp8_split_kernel<J, T, Exponents>), dim3((unsigned)groups), dim3(512), 0, stream, p);
+}
+
+// Two workgroups per compute unit, in whole rounds of the XCDs.
+template <bool Exponents, int NT>
+void launch_wide(const LinearFp8Params& p, hipStream_t stream) {
+    const int64_t tiles = ((p.out_features + 255) / 256) * ((p.rows + 16 * NT - 1) / (16 * NT));
+    const unsigned grid = (unsigned)std::min<int64_t>((tiles + 7) / 8 * 8, std::max(p.compute_units / 8, 1) * 16);
+    hipLaunchKernelGGL((linear_fp8_wide_kernel<Exponents, NT>), dim3(grid), dim3(256), 0, stream, p);
+}
+
+// The kernel for rows in operand order: by what its rounds of workgroups take, two
+// per compute unit or one in the last, a block of inputs at a time. Measured in us per
+// block with one workgroup on a compute unit and with two, and per round (the join,
+// the first loads); of 38 shapes from 32 to 8192 rows the choice takes the fastest
+// of the six, or up to 10% longer. (1018 rows, 2048 -> 11264: tiles of 256 x 96 31.5 us, x 64
+// 33.2, x 128 39.1, 64 x 64 74. 40 rows, 5632 -> 2048: 32 x 32 6.1, 64 x 64 10.3. 512 rows,
+// 5632 -> 2048: 64 x 64 18.6, 256 x 64 30.9.)
+struct Tiling {
+    int outs, rows;
+    float one, two, round;
+};
+template <bool Exponents>
+int fastest_tiling(const LinearFp8Params& p) {
+    constexpr Tiling kTilings[6] = {
+        {32, 32, 0.10f, 0.30f, 0.3f},
+        {32, 64, 0.17f, 0.36f, 0.6f},
+        {64, 64, 0.27f, 0.54f, 1.2f},
+        {256, 64, Exponents ? 0.55f : 0.63f, Exponents ? 1.05f : 1.13f, 0.3f},
+        {256, 96, Exponents ? 0.70f : 0.85f, Exponents ? 1.45f : 1.67f, 0.3f},
+        {256, 128, Exponents ? 0.85f : 1.33f, Exponents ? 1.75f : 2.15f, 0.3f},
+    };
+    const float blocks = (float)blocks_of(p.in_features);
+    int best = 0;
+    float least = 0.f;
+    for (int c = 0; c < 6; ++c) {
+        const Tiling& t = kTilings[c];
+        const int64_t groups = ((p.out_features + t.outs - 1) / t.outs) * ((p.rows + t.rows - 1) / t.rows);
+        const int64_t pairs = groups / (2 * p.compute_units), rest = groups % (2 * p.compute_units);
+        const float pair = t.two * blocks + 2 * t.round;
+        const float time = (float)pairs * pair + (rest > p.compute_units ? pair : rest > 0 ? t.one * blocks + t.round : 0.f);
+        if (c == 0 || time < least) best = c, least = time;
+    }
+    return best;
 }
 
 template <bool Exponents>
 void launch_product(const LinearFp8Params& p, hipStream_t stream) {
-    const int64_t row_tiles = tiles_of(p.rows);
-    const unsigned tiles = (unsigned)tiles_of(p.out_features);
-    if (row_tiles == 1)
-        hipLaunchKernelGGL((linear_fp8_kernel<1, Exponents>), dim3(tiles), dim3(512), 0, stream, p);
-    else if (row_tiles == 2)
-        hipLaunchKernelGGL((linear_fp8_kernel<2, Exponents>), dim3(tiles), dim3(512), 0, stream, p);
-    else
-        hipLaunchKernelGGL((linear_fp8_kernel<4, Exponents>), dim3(tiles, (unsigned)((row_tiles + 3) / 4)), dim3(512), 0, stream, p);
+    switch (fastest_tiling<Exponents>(p)) {
+        case 0: return launch_split<Exponents, 2, 2>(p, stream);
+        case 1: return launch_split<Exponents, 2, 4>(p, stream);
+        case 2: return launch_split<Exponents, 4, 4>(p, stream);
+        case 3: return launch_wide<Exponents, 4>(p, stream);
+        case 4: return launch_wide<Exponents, 6>(p, stream);
+        default: return launch_wide<Exponents, 8>(p, stream);
+    }
 }
+
+// Rows of one launch: the wide kernels address the codes of x in 31 bits.
+int64_t rows_at_once(int64_t in_features) { return (((int64_t)1 << 31) - 1) / (blocks_of(in_features) * kBlock) / 128 * 128; }
 
 }  // namespace
 
-size_t fp8_code_bytes(int64_t rows, int64_t in_features) { return (size_t)tiles_of(rows) * blocks_of(in_features) * kTileBytes; }
+static size_t fp8_row_bytes(int64_t rows, int64_t in_features) { return (size_t)tiles_of(rows) * blocks_of(in_features) * kTileBytes; }
+
+size_t fp8_code_bytes(int64_t out_features, int64_t in_features) {
+    return (size_t)out_tiles_of(out_features) * blocks_of(in_features) * kTileBytes;
+}
 
 size_t fp8_weight_bytes(int64_t out_features, int64_t in_features, bool exponents) {
     return fp8_code_bytes(out_features, in_features) +
            (size_t)((out_features + kBlock - 1) / kBlock) * fours_of(in_features) * (exponents ? 4 : 16);
 }
 
+// Whether every workgroup rounds x for itself, or a launch before the product does: by
+// x's blocks. (2048 -> 6144: 1 row 4.1 us against 8.4, 8 rows 7.3 against 8.2, 16 rows
+// 9.8 against 7.9; 5632 -> 2048: 2 rows 5.4 against 8.8, 4 rows 7.1 against 8.6.)
+static bool few_rows(int64_t rows, int64_t in_features) {
+    const int64_t blocks = blocks_of(in_features);
+    return rows <= 16 && blocks <= kFewMaxBlocks && rows * blocks <= kFewAtOnce;
+}
+
 size_t linear_fp8_workspace(int64_t rows, int64_t in_features) {
-    return fp8_code_bytes(rows, in_features) + (size_t)tiles_of(rows) * fours_of(in_features) * 64;
+    if (few_rows(rows, in_features)) return 0;
+    rows = std::min(rows, rows_at_once(in_features));
+    return fp8_row_bytes(rows, in_features) + (size_t)tiles_of(rows) * fours_of(in_features) * 64;
 }
 
 hipError_t launch_pack_fp8(const Fp8PackParams& p, hipStream_t stream) {
@@ -260,29 +710,42 @@ hipError_t launch_pack_fp8(const Fp8PackParams& p, hipStream_t stream) {
         hipLaunchKernelGGL(quantize_weight_fp8_kernel, dim3((unsigned)(high * blocks_of(p.in_features))), dim3(256), 0, stream, p);
     } else {
         // (128 pieces a tile: more threads than the scales, four of which a tile may pad.)
-        const int64_t pieces = tiles_of(p.out_features) * blocks_of(p.in_features) * (kTileBytes / 16);
+        const int64_t pieces = out_tiles_of(p.out_features) * blocks_of(p.in_features) * (kTileBytes / 16);
         hipLaunchKernelGGL(pack_fp8_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, p);
     }
     return hipGetLastError();
 }
 
 hipError_t launch_unpack_fp8(const Fp8PackParams& p, uint16_t* weight, hipStream_t stream) {
-    const int64_t pieces = tiles_of(p.out_features) * blocks_of(p.in_features) * (kTileBytes / 16);
+    const int64_t pieces = out_tiles_of(p.out_features) * blocks_of(p.in_features) * (kTileBytes / 16);
     hipLaunchKernelGGL(unpack_fp8_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, p, weight);
     return hipGetLastError();
 }
 
-hipError_t launch_linear_fp8(const LinearFp8Params& p, hipStream_t stream) {
-    const dim3 grid((unsigned)(fours_of(p.in_features) * tiles_of(p.rows)));
+hipError_t launch_linear_fp8(const LinearFp8Params& given, hipStream_t stream) {
+    LinearFp8Params p = given;
+    p.aligned = p.y_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
     const bool wide = p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
-    if (wide)
-        hipLaunchKernelGGL(quantize_rows_fp8_kernel<true>, grid, dim3(256), 0, stream, p);
-    else
-        hipLaunchKernelGGL(quantize_rows_fp8_kernel<false>, grid, dim3(256), 0, stream, p);
-    if (p.exponents)
-        launch_product<true>(p, stream);
-    else
-        launch_product<false>(p, stream);
+    if (few_rows(p.rows, p.in_features)) {
+        if (wide)
+            p.exponents ? launch_few<true, true>(p, stream) : launch_few<false, true>(p, stream);
+        else
+            p.exponents ? launch_few<true, false>(p, stream) : launch_few<false, false>(p, stream);
+        return hipGetLastError();
+    }
+    const int64_t most = rows_at_once(p.in_features);
+    for (int64_t first = 0; first < given.rows; first += most) {
+        p.rows = std::min(given.rows - first, most);
+        p.x = given.x + first * p.x_stride;
+        p.y = given.y + first * p.y_stride;
+        p.x_scales = reinterpret_cast<uint32_t*>(p.x_codes + fp8_row_bytes(p.rows, p.in_features));
+        const dim3 grid((unsigned)(fours_of(p.in_features) * tiles_of(p.rows)));
+        if (wide)
+            hipLaunchKernelGGL(quantize_rows_fp8_kernel<true>, grid, dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL(quantize_rows_fp8_kernel<false>, grid, dim3(256), 0, stream, p);
+        p.exponents ? launch_product<true>(p, stream) : launch_product<false>(p, stream);
+    }
     return hipGetLastError();
 }
 

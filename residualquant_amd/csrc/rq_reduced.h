@@ -77,10 +77,11 @@ struct LinearFp8Params {
     int64_t rows, out_features, in_features;
     bool exponents;
     int compute_units;        // of the launching device
-    uint8_t* x_codes;         // workspace: x as the weights are packed
-    uint32_t* x_scales;       // workspace [tiles of 16 rows][fours of blocks][16], four E8M0 bytes each
+    uint8_t* x_codes;         // workspace: x in operand order
+    uint32_t* x_scales;       // set by the launch: workspace [fours of blocks][tiles of 16 rows][16], four E8M0 bytes each
+    bool aligned;             // set by the launch: 16-byte stores of y
 };
-size_t fp8_code_bytes(int64_t rows, int64_t in_features);
+size_t fp8_code_bytes(int64_t out_features, int64_t in_features);
 size_t fp8_weight_bytes(int64_t out_features, int64_t in_features, bool exponents);
 size_t linear_fp8_workspace(int64_t rows, int64_t in_features);
 hipError_t launch_pack_fp8(const Fp8PackParams& p, hipStream_t stream);

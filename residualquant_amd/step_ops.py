@@ -323,7 +323,7 @@ def pack_weight_fp8(codes: torch.Tensor, scales: torch.Tensor) -> Fp8Weight:
 
 
 def linear_fp8_workspace_bytes(rows: int, in_features: int) -> int:
-    """Device workspace (bytes) for ``linear_fp8``; depends on shapes only."""
+    """Device workspace (bytes) for ``linear_fp8``; depends on shapes only (none for a few rows)."""
     return int(_lib.lib().rq_linear_fp8_workspace_bytes(rows, in_features))
 
 
@@ -352,16 +352,21 @@ def linear_fp8(x: torch.Tensor, weight: Fp8Weight, out: Optional[torch.Tensor] =
             raise RuntimeError("out must be [rows, out_features]")
         if rows > 1:
             out_stride = out.stride(0)
-    if workspace is None:
-        workspace = x.new_empty(_linear_fp8_workspace_bytes(rows, in_features), dtype=torch.uint8)
-    else:
+    memory, memory_bytes = None, 0
+    if workspace is not None:
         _require(workspace.get_device() == device and workspace.is_contiguous(),
                  "Contiguous projection workspace on x's device required")
+        memory, memory_bytes = workspace.data_ptr(), workspace.nbytes
+    else:
+        memory_bytes = _linear_fp8_workspace_bytes(rows, in_features)
+        if memory_bytes > 0:
+            workspace = x.new_empty(memory_bytes, dtype=torch.uint8)
+            memory = workspace.data_ptr()
     with _on_device(device):
         status = _lib.lib().rq_linear_fp8(
             x.data_ptr(), strides[0] if rows > 1 else in_features, data.data_ptr(), data.numel(),
             0 if weight.exponents else 1, out.data_ptr(), out_stride, rows, out_features, in_features,
-            workspace.data_ptr(), workspace.nbytes, torch._C._cuda_getCurrentRawStream(device))
+            memory, memory_bytes, torch._C._cuda_getCurrentRawStream(device))
     _lib.check(status)
     return out
 

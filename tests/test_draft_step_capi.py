@@ -22,25 +22,25 @@ def lib():
 
 
 def test_weight_bytes(lib):
-    # Codes in whole tiles of 16 x 128, scales in fours of blocks.
-    assert lib.rq_fp8_weight_bytes(1, 1, 0) == 16 * 128 + 4
-    assert lib.rq_fp8_weight_bytes(1, 1, 1) == 16 * 128 + 16
+    # Codes in whole tiles of 64 x 128, scales in fours of blocks.
+    assert lib.rq_fp8_weight_bytes(1, 1, 0) == 64 * 128 + 4
+    assert lib.rq_fp8_weight_bytes(1, 1, 1) == 64 * 128 + 16
     assert lib.rq_fp8_weight_bytes(2048, 5632, 0) == 2048 * 5632 + 16 * 44
-    assert lib.rq_fp8_weight_bytes(130, 129, 1) == 144 * 256 + 2 * 16
+    assert lib.rq_fp8_weight_bytes(130, 129, 1) == 192 * 256 + 2 * 16
     for wrong in ((0, 128, 0), (16, 0, 0), (16, 128, 2), (16, 128, -1), ((1 << 24) + 1, 128, 0), (16, (1 << 20) + 1, 0),
                   (1 << 24, 1 << 20, 0)):
         assert lib.rq_fp8_weight_bytes(*wrong) == 0, wrong
         assert lib.rq_last_error()
 
 
-def _linear(lib, *, x=FAKE, x_stride=256, packed=FAKE, packed_bytes=1 << 40, scale_type=0, y=FAKE, y_stride=40, rows=2,
+def _linear(lib, *, x=FAKE, x_stride=256, packed=FAKE, packed_bytes=1 << 40, scale_type=0, y=FAKE, y_stride=40, rows=200,
             out=40, features=256, workspace=FAKE, workspace_bytes=1 << 40):
     return lib.rq_linear_fp8(x, x_stride, packed, packed_bytes, scale_type, y, y_stride, rows, out, features, workspace,
                              workspace_bytes, None)
 
 
 def test_projection_refusals(lib):
-    needed = lib.rq_linear_fp8_workspace_bytes(2, 256)
+    needed = lib.rq_linear_fp8_workspace_bytes(200, 256)
     for wrong, code, words in (
             (dict(rows=-1), _lib.RQ_ENOKERNEL, b"No compiled 8-bit projection"),
             (dict(rows=(1 << 20) + 1), _lib.RQ_ENOKERNEL, b"No compiled 8-bit projection"),
@@ -49,7 +49,7 @@ def test_projection_refusals(lib):
             (dict(features=0), _lib.RQ_EINVAL, b"8-bit weights need"),
             (dict(packed=None), _lib.RQ_EINVAL, b"packed weight"),
             (dict(packed=FAKE + 8), _lib.RQ_EINVAL, b"packed weight"),
-            (dict(packed_bytes=48 * 256 + 3), _lib.RQ_EINVAL, b"packed weight"),
+            (dict(packed_bytes=64 * 256 + 3), _lib.RQ_EINVAL, b"packed weight"),
             (dict(x_stride=255), _lib.RQ_EINVAL, b"x rows"),
             (dict(y_stride=39), _lib.RQ_EINVAL, b"y rows"),
             (dict(x=None), _lib.RQ_EINVAL, b"BF16 x"),
@@ -61,6 +61,7 @@ def test_projection_refusals(lib):
         assert _linear(lib, **wrong) == code, wrong
         assert words in lib.rq_last_error(), (wrong, lib.rq_last_error())
     assert _linear(lib, rows=0) == _lib.RQ_OK
+    assert lib.rq_linear_fp8_workspace_bytes(1, 2048) == 0  # (rounded by every workgroup)
 
 
 def test_packing_refusals(lib):

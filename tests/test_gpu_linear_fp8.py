@@ -185,6 +185,18 @@ def test_strides_and_alignment(device, rows, offset, pad):
     assert bool((memory[:5] == 0x7f).all()) and bool((memory[5 + needed:] == 0x7f).all())
 
 
+def test_more_rows_than_one_launch_takes(device):
+    """x of 2^31 codes and more goes in parts; sums of whole numbers are exact."""
+    features, rows = 1 << 20, 2100
+    weight = torch.zeros((16, features), dtype=torch.bfloat16, device=device)
+    weight[:, ::1 << 10] = torch.arange(16, device=device)[:, None].to(torch.bfloat16)
+    x = torch.ones((rows, features), dtype=torch.bfloat16, device=device)
+    x[:, 0] = (torch.arange(rows, device=device) % 8 - 4).to(torch.bfloat16)
+    got = step_ops.linear_fp8(x, step_ops.quantize_weight_fp8(weight))
+    want = (1023.0 + x[:, :1].float()) * torch.arange(16, device=device)
+    assert torch.equal(got, want.to(torch.bfloat16))
+
+
 def test_no_rows(device):
     weight, _ = make_weight(20, 30, "exponents", seed=1, device=device)
     assert step_ops.linear_fp8(torch.empty((0, 30), dtype=torch.bfloat16, device=device), weight).shape == (0, 20)
@@ -239,7 +251,7 @@ def test_refusals(device):
         with pytest.raises(RuntimeError):
             step_ops.linear_fp8(x, weight, out=out)
     with pytest.raises(RuntimeError, match="workspace"):
-        step_ops.linear_fp8(x, weight, workspace=torch.empty(300, dtype=torch.uint8, device=device))
+        step_ops.linear_fp8(make_x(100, 130, seed=1).to(device), weight, workspace=torch.empty(300, dtype=torch.uint8, device=device))
     codes = torch.zeros((20, 130), dtype=torch.float8_e4m3fn, device=device)
     for scales in (torch.ones((1, 1), device=device), torch.ones((2, 1), device=device), torch.ones((1, 2)),
                    torch.ones((1, 2), dtype=torch.bfloat16, device=device)):
