@@ -452,7 +452,7 @@ int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads,
                    int64_t max_pages, hipStream_t stream);
 
 /*
- * Verification of drafted tokens by given random numbers.  Request b's rows
+ * Verification of drafted tokens by given random numbers (vocab up to 2^27).  Request b's rows
  * query_start_loc[b]..query_start_loc[b + 1] hold its last token and its
  * drafts, tokens[row] each; target[row] (BF16 or FP32 [rows, vocab], unit
  * column stride) is the target's distribution of the token behind that row,

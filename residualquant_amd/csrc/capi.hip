@@ -1655,10 +1655,13 @@ int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads,
     return check_launch(rq::launch_rope_append(p, stream), "rotated append launch");
 }
 
+// (A row's chunks, of at least 4096 tokens where there are many, are counted in 16 bits.)
+constexpr int64_t kVerifyMaxVocab = (int64_t)1 << 27;
+
 size_t rq_verify_drafts_workspace_bytes(int64_t requests, int64_t vocab) {
-    if (requests <= 0 || requests > (int64_t)INT32_MAX / 4 || vocab <= 0 || vocab > (int64_t)INT32_MAX) return 256;
-    int64_t chunk = 0;
-    return 256 + (size_t)requests * rq::verify_chunks(requests, vocab, &chunk) * sizeof(double);
+    if (requests <= 0 || requests > (int64_t)INT32_MAX / 4 || vocab <= 0 || vocab > kVerifyMaxVocab) return 256;
+    const int64_t chunks = std::max(rq::verify_chunks(requests, vocab, false), rq::verify_chunks(requests, vocab, true));
+    return 256 + (size_t)requests * (chunks + rq::kVerifyArrivalStride) * 8;  // arrival words, and sums
 }
 
 int rq_verify_drafts(const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int dtype,
@@ -1667,9 +1670,9 @@ int rq_verify_drafts(const void* target, int64_t target_stride, const void* draf
                      void* workspace, size_t workspace_bytes, hipStream_t stream) {
     if (dtype != RQ_DTYPE_BF16 && dtype != RQ_DTYPE_F32) return fail(RQ_EINVAL, "BF16 or FP32 probabilities required");
     const uintptr_t element = dtype == RQ_DTYPE_BF16 ? 2 : 4;
-    if (rows < 0 || rows > (int64_t)INT32_MAX || vocab <= 0 || vocab > (int64_t)INT32_MAX || target_stride < vocab ||
+    if (rows < 0 || rows > (int64_t)INT32_MAX || vocab <= 0 || vocab > kVerifyMaxVocab || target_stride < vocab ||
         (draft != nullptr && draft_stride < vocab))
-        return fail(RQ_EINVAL, "Probabilities [rows, vocab] of at least one column with unit column stride required");
+        return fail(RQ_EINVAL, "Probabilities [rows, vocab] of 1 to 2^27 columns with unit column stride required");
     if (requests < 0 || requests > (int64_t)INT32_MAX / 4 || (requests > 0 && (query_start_loc == nullptr || accepted == nullptr)))
         return fail(RQ_EINVAL, "Contiguous INT32 query starts with one final boundary required");
     if (requests == 0) return ok();
@@ -1677,8 +1680,8 @@ int rq_verify_drafts(const void* target, int64_t target_stride, const void* draf
                      (reinterpret_cast<uintptr_t>(draft) % element) || tokens == nullptr || uniforms == nullptr || out_tokens == nullptr))
         return fail(RQ_EINVAL, "Probabilities, tokens, random numbers and outputs required");
     rq::VerifyParams p{};
-    p.chunks = rq::verify_chunks(requests, vocab, &p.chunk);
-    if (!launchable(requests * p.chunks, 512)) return fail(RQ_EINVAL, "Too many requests and tokens for one call");
+    p.chunks = rq::verify_chunks(requests, vocab, dtype == RQ_DTYPE_BF16);
+    if (!launchable(requests * p.chunks, 256)) return fail(RQ_EINVAL, "Too many requests and tokens for one call");
     const size_t needed = rq_verify_drafts_workspace_bytes(requests, vocab);
     if (workspace == nullptr || workspace_bytes < needed)
         return fail(RQ_ENOSPACE, "Verification workspace of %zu bytes required, %zu given", needed, workspace_bytes);
@@ -1695,7 +1698,9 @@ int rq_verify_drafts(const void* target, int64_t target_stride, const void* draf
     p.requests = requests;
     p.accepted = accepted;
     p.out_tokens = out_tokens;
-    p.sums = reinterpret_cast<double*>(static_cast<uint8_t*>(workspace) + to_boundary(workspace));
+    p.arrivals = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(workspace) + to_boundary(workspace));
+    p.sums = reinterpret_cast<double*>(p.arrivals + requests * rq::kVerifyArrivalStride);
+    p.call_tag = next_call_tag();
     return check_launch(rq::launch_verify(p, stream), "draft verification launch");
 }
 

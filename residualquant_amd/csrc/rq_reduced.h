@@ -130,10 +130,14 @@ struct VerifyParams {
     int64_t requests;
     int32_t* accepted;        // [requests]
     int64_t* out_tokens;      // [rows]
-    int64_t chunk, chunks;    // tokens whose weights a workgroup sums, and how many such of a row
+    int64_t chunks;           // of a row
+    int each;                 // set by the launch: chunks per workgroup
+    uint64_t* arrivals;       // workspace [requests] words of a cache line each, tagged arrival counts (rq_plan.h)
     double* sums;             // workspace [requests, chunks]
+    uint64_t call_tag;        // of this call (48 bits, rq_plan.h)
 };
-int64_t verify_chunks(int64_t requests, int64_t vocab, int64_t* chunk);
+constexpr int kVerifyArrivalStride = 16;  // words of 8 bytes
+int64_t verify_chunks(int64_t requests, int64_t vocab, bool bf16);
 hipError_t launch_verify(const VerifyParams& p, hipStream_t stream);
 
 // Cache held in 8 bits (fp8_cache.hip): E4M3 codes [2, blocks, kv_heads, PT, D],
