@@ -1624,7 +1624,9 @@ int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads,
         rows_overlap(qkv, qkv_stride, all_heads * head_dim, key, key_stride, (int64_t)kv_heads * head_dim, rows) ||
         rows_overlap(query, query_stride, (int64_t)heads * head_dim, key, key_stride, (int64_t)kv_heads * head_dim, rows))
         return fail(RQ_EINVAL, "The rotated query and key must not overlap each other or their input");
-    if (!launchable(rows / page_tokens + 2 * requests, 256)) return fail(RQ_EINVAL, "Too many rows and requests for one call");
+    // (Four heads of a page per workgroup, or more.)
+    if (!launchable(rows / page_tokens + 2 * requests, 256) || all_heads > 4 * 65535)
+        return fail(RQ_EINVAL, "Too many rows, heads and requests for one call");
     rq::RopeAppendParams p{};
     p.qkv = static_cast<const uint16_t*>(qkv);
     p.qkv_stride = qkv_stride;

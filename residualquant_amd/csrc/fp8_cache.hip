@@ -56,7 +56,10 @@ __global__ __launch_bounds__(256) void quantize_fp8_kernel(const Fp8WriteParams 
         values[c] = U32x4{0u, 0u, 0u, 0u};
         if (r < rows) values[c] = *reinterpret_cast<const U32x4At8*>(in + r * stride + 8 * (chunk - r * kRow));
     }
-    write_fp8_page<D, PT>(values, codes, p.scales + index, before, slot, rows);
+    write_fp8_page<D, PT>(values, codes, p.scales + index, before, slot, [&](int c) {
+        const int chunk = 64 * c + lane;
+        return chunk < rows * kRow ? chunk : -1;
+    });
 }
 
 // ------------------------------------------------------------------ attention

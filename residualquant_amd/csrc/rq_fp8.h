@@ -43,16 +43,16 @@ __device__ __forceinline__ uint32_t fp8x4_rn(float a, float b, float c, float d)
 
 __device__ __forceinline__ bool power_of_two(float x) { return (__float_as_uint(x) & 0x7fffffu) == 0; }
 
-// A page's rows slot..slot + rows - 1 from `values` (zeros past them), its scale, and where that grows its earlier
-// rows once more.
-template <int D, int PT>
-__device__ __forceinline__ void write_fp8_page(const U32x4 (&values)[kPageChunks<D, PT>], uint8_t* codes, float* page_scale,
-                                               float before, int slot, int rows) {
+// A page's rows from `slot` on from `values` (zeros where there are none), its scale, and where that grows its
+// earlier rows once more.  place(c): which chunk of the new rows values[c] is, -1: none.
+template <int D, int PT, int Held, class Place>
+__device__ __forceinline__ void write_fp8_page(const U32x4 (&values)[Held], uint8_t* codes, float* page_scale, float before,
+                                               int slot, Place place) {
     constexpr int kRow = D / 8, kChunks = kPageChunks<D, PT>;
     const int lane = threadIdx.x & 63;
     float largest = 0.f;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+    for (int c = 0; c < Held; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float a = __uint_as_float(values[c][e] << 16), b = __uint_as_float(values[c][e] & 0xffff0000u);
@@ -70,23 +70,23 @@ __device__ __forceinline__ void write_fp8_page(const U32x4 (&values)[kPageChunks
         for (int c = 0; c < kChunks; ++c) {
             const int chunk = 64 * c + lane;
             if (chunk >= slot * kRow) continue;
-            U32x2* place = reinterpret_cast<U32x2*>(codes) + chunk;
-            U32x2 word = *place;
+            U32x2* held = reinterpret_cast<U32x2*>(codes) + chunk;
+            U32x2 word = *held;
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(word[w], false), high = __builtin_amdgcn_cvt_pk_f32_fp8(word[w], true);
                 word[w] = fp8x4_rn(low[0] * shrink, low[1] * shrink, high[0] * shrink, high[1] * shrink);
             }
-            *place = word;
+            *held = word;
         }
     }
     // A division by a power of two is a product (a scale that the caller made may be any number).
     const bool exact = power_of_two(scale);
     const float inverse = 1.0f / scale;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const int chunk = 64 * c + lane;
-        if (chunk >= rows * kRow) continue;
+    for (int c = 0; c < Held; ++c) {
+        const int chunk = place(c);
+        if (chunk < 0) continue;
         float x[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

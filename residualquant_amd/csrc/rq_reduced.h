@@ -113,6 +113,7 @@ struct RopeAppendParams {
     const int32_t* block_table;
     int64_t block_table_stride;
     int64_t max_pages;
+    int span;                 // set by the launch: heads (q's, k's and v's in a row) per workgroup
 };
 hipError_t launch_rope_append(const RopeAppendParams& p, hipStream_t stream);
 
