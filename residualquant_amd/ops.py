@@ -428,48 +428,59 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache: 
     ``positions`` (INT64 ``[rows]``) where given (clamped to the tables).  Rows
     outside ``query_start_loc`` are left as they are.
     """
-    shape = qkv.shape
-    _require(qkv.is_cuda and qkv.dtype is torch.bfloat16 and len(shape) == 2 and qkv.stride(1) == 1,
-             "qkv must be BF16 [rows, channels] on a HIP device with unit channel stride")
-    device, rows = qkv.get_device(), shape[0]
-    _require(cache.get_device() == device and cache.dim() == 5, "Cache [2, blocks, kv_heads, page_tokens, D] on the Q/K/V device required")
-    _, blocks, kv_heads, page_tokens, head_dim = cache.shape
-    heads = shape[1] // head_dim - 2 * kv_heads if head_dim > 0 else 0
-    _require(heads > 0 and shape[1] == (heads + 2 * kv_heads) * head_dim,
-             "qkv rows must hold [q | k | v] of (heads + 2 * kv_heads) * head_dim channels")
-    if scales is None:
-        _require(cache.dtype is torch.bfloat16 and cache.size(0) == 2 and cache.is_contiguous(),
-                 "Contiguous BF16 [2, blocks, kv_heads, page_tokens, D] cache required (8-bit pages need their scales)")
-    else:
+    # (A decode step's call runs 5 us on the GPU: each tensor's shape and strides are read once.)
+    shape, strides = qkv.shape, qkv.stride()
+    if not (len(shape) == 2 and strides[1] == 1 and qkv.is_cuda and qkv.dtype is torch.bfloat16):
+        raise RuntimeError("qkv must be BF16 [rows, channels] on a HIP device with unit channel stride")
+    device, (rows, width), cache_shape = qkv.get_device(), shape, cache.shape
+    if len(cache_shape) != 5:
+        raise RuntimeError("Cache [2, blocks, kv_heads, page_tokens, D] required")
+    _, blocks, kv_heads, page_tokens, head_dim = cache_shape
+    heads = width // head_dim - 2 * kv_heads if head_dim > 0 else 0
+    if not (heads > 0 and width == (heads + 2 * kv_heads) * head_dim):
+        raise RuntimeError("qkv rows must hold [q | k | v] of (heads + 2 * kv_heads) * head_dim channels")
+    if scales is not None:
         _validate_fp8_cache(cache, scales, device, kv_heads, head_dim)
+    elif not (cache.get_device() == device and cache.dtype is torch.bfloat16 and cache_shape[0] == 2
+              and cache.is_contiguous()):
+        raise RuntimeError("Contiguous BF16 [2, blocks, kv_heads, page_tokens, D] cache required (8-bit pages need "
+                           "their scales)")
     requests, max_pages, table_stride = _validate_sequences(query_start_loc, seq_lens, block_table, device)
-    for table in (cos, sin):
-        _require(table.get_device() == device and table.dtype is torch.float32 and table.is_contiguous()
-                 and table.dim() == 2 and table.shape == cos.shape,
-                 "Contiguous FP32 [positions, channels / 2] cos/sin tables required")
+    table_shape = cos.shape
+    if not (len(table_shape) == 2 and sin.shape == table_shape and cos.dtype is torch.float32
+            and sin.dtype is torch.float32 and cos.get_device() == device and sin.get_device() == device
+            and cos.is_contiguous() and sin.is_contiguous()):
+        raise RuntimeError("Contiguous FP32 [positions, channels / 2] cos/sin tables required")
+    positions_pointer = None
     if positions is not None:
         _require(positions.get_device() == device and positions.dtype is torch.int64 and positions.is_contiguous()
                  and positions.numel() == rows, "Contiguous INT64 positions, one per row, required")
+        positions_pointer = positions.data_ptr()
+    query_stride, key_stride = heads * head_dim, kv_heads * head_dim
     if query is None:
         query = qkv.new_empty((rows, heads, head_dim))
+    else:
+        given, query_stride = _validate_bf16_token_tensor(query)
+        _require(given == (rows, heads, head_dim) and query.get_device() == device,
+                 "query must be [rows, heads, D] on the Q/K/V device")
     if key is None:
         key = qkv.new_empty((rows, kv_heads, head_dim))
-    query_shape, query_stride = _validate_bf16_token_tensor(query)
-    key_shape, key_stride = _validate_bf16_token_tensor(key)
-    _require(query_shape == (rows, heads, head_dim) and key_shape == (rows, kv_heads, head_dim)
-             and query.get_device() == device and key.get_device() == device,
-             "query and key must be [rows, heads, D] and [rows, kv_heads, D] on the Q/K/V device")
-    width = shape[1]
+    else:
+        given, key_stride = _validate_bf16_token_tensor(key)
+        _require(given == (rows, kv_heads, head_dim) and key.get_device() == device,
+                 "key must be [rows, kv_heads, D] on the Q/K/V device")
+    row_stride = strides[0] if rows > 1 else width
     with _on_device(device):
         status = _lib.lib().rq_rope_append(
-            qkv.data_ptr(), qkv.stride(0) if rows > 1 else width, rows, heads, kv_heads, head_dim, 2 * cos.size(1),
-            1 if interleaved else 0, cos.data_ptr(), sin.data_ptr(), cos.size(0),
-            positions.data_ptr() if positions is not None else None, query.data_ptr(), query_stride, key.data_ptr(),
-            key_stride, cache.data_ptr(), scales.data_ptr() if scales is not None else None, blocks, page_tokens,
-            query_start_loc.data_ptr(), seq_lens.data_ptr(), requests, block_table.data_ptr(), table_stride, max_pages,
-            _stream(device))
+            qkv.data_ptr(), row_stride, rows, heads, kv_heads, head_dim, 2 * table_shape[1], 1 if interleaved else 0,
+            cos.data_ptr(), sin.data_ptr(), table_shape[0], positions_pointer, query.data_ptr(), query_stride,
+            key.data_ptr(), key_stride, cache.data_ptr(), None if scales is None else scales.data_ptr(), blocks,
+            page_tokens, query_start_loc.data_ptr(), seq_lens.data_ptr(), requests, block_table.data_ptr(), table_stride,
+            max_pages, _stream(device))
     _lib.check(status)
-    return query, key, qkv[:, (heads + kv_heads) * head_dim:].view(rows, kv_heads, head_dim)
+    value = qkv.as_strided((rows, kv_heads, head_dim), (row_stride, head_dim, 1),
+                           qkv.storage_offset() + (heads + kv_heads) * head_dim)
+    return query, key, value
 
 
 def paged_attention_fp8_workspace_bytes(rows: int, heads: int, kv_heads: int, head_dim: int, max_pages: int,

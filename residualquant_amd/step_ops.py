@@ -460,32 +460,41 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Te
         raise RuntimeError("target must be BF16 or FP32 [rows, vocab] on a HIP device with unit column stride")
     rows, vocab = shape
     device = target.get_device()
+    draft_pointer, draft_stride = None, vocab
     if draft is not None:
-        _require(draft.get_device() == device and draft.dtype is dtype and draft.shape == shape
-                 and (draft.stride(1) == 1 or vocab == 1), "draft must match target in shape, type and device")
-    _require(tokens.get_device() == device and tokens.dtype is torch.int64 and tokens.dim() == 1
-             and tokens.is_contiguous() and tokens.numel() == rows,
-             "Contiguous INT64 tokens, one per row, on the target's device required")
-    _require(uniforms.get_device() == device and uniforms.dtype is torch.float32 and uniforms.dim() == 1
-             and uniforms.is_contiguous() and uniforms.numel() == rows,
-             "Contiguous FP32 uniforms, one per row, on the target's device required")
-    _require(query_start_loc.get_device() == device and query_start_loc.dtype is torch.int32
-             and query_start_loc.dim() == 1 and query_start_loc.is_contiguous() and query_start_loc.numel() > 0,
-             "Contiguous INT32 query starts with one final boundary required")
-    requests = query_start_loc.numel() - 1
+        strides_of_draft = draft.stride()
+        if not (draft.shape == shape and draft.dtype is dtype and draft.get_device() == device
+                and (strides_of_draft[1] == 1 or vocab == 1)):
+            raise RuntimeError("draft must match target in shape, type and device")
+        draft_pointer = draft.data_ptr()
+        if rows > 1:
+            draft_stride = strides_of_draft[0]
+    if not (tokens.get_device() == device and tokens.dtype is torch.int64 and tokens.dim() == 1
+            and tokens.is_contiguous() and tokens.numel() == rows):
+        raise RuntimeError("Contiguous INT64 tokens, one per row, on the target's device required")
+    if not (uniforms.get_device() == device and uniforms.dtype is torch.float32 and uniforms.dim() == 1
+            and uniforms.is_contiguous() and uniforms.numel() == rows):
+        raise RuntimeError("Contiguous FP32 uniforms, one per row, on the target's device required")
+    starts = query_start_loc.numel()
+    if not (query_start_loc.get_device() == device and query_start_loc.dtype is torch.int32
+            and query_start_loc.dim() == 1 and query_start_loc.is_contiguous() and starts > 0):
+        raise RuntimeError("Contiguous INT32 query starts with one final boundary required")
+    requests = starts - 1
     accepted = query_start_loc.new_empty(requests)
     # (Without requests no kernel runs.)
     following = torch.empty_like(tokens) if requests > 0 else torch.full_like(tokens, -1)
     if workspace is None:
-        workspace = tokens.new_empty(_verify_workspace_bytes(requests, vocab), dtype=torch.uint8)
+        memory_bytes = _verify_workspace_bytes(requests, vocab)
+        workspace = tokens.new_empty((memory_bytes + 7) // 8)
     else:
         _require(workspace.get_device() == device and workspace.is_contiguous(),
                  "Contiguous verification workspace on the target's device required")
+        memory_bytes = workspace.nbytes
     with _on_device(device):
         status = _lib.lib().rq_verify_drafts(
-            target.data_ptr(), strides[0] if rows > 1 else vocab, draft.data_ptr() if draft is not None else None,
-            draft.stride(0) if draft is not None and rows > 1 else vocab, 0 if dtype is torch.bfloat16 else 1, rows,
-            vocab, tokens.data_ptr(), uniforms.data_ptr(), query_start_loc.data_ptr(), requests, accepted.data_ptr(),
-            following.data_ptr(), workspace.data_ptr(), workspace.nbytes, torch._C._cuda_getCurrentRawStream(device))
+            target.data_ptr(), strides[0] if rows > 1 else vocab, draft_pointer, draft_stride,
+            0 if dtype is torch.bfloat16 else 1, rows, vocab, tokens.data_ptr(), uniforms.data_ptr(),
+            query_start_loc.data_ptr(), requests, accepted.data_ptr(), following.data_ptr(), workspace.data_ptr(),
+            memory_bytes, torch._C._cuda_getCurrentRawStream(device))
     _lib.check(status)
     return VerifiedDrafts(accepted, following)
