@@ -6,9 +6,11 @@
 //
 // Both operands lie in tiles of 16 rows x 128 inputs, 2 KB each, in the order in
 // which v_mfma_scale_f32_16x16x128 takes them: lane l = (i = l % 16, g = l / 16)
-// holds row i, inputs 32 g + 16 h + 0..15 in the 16 bytes at 1024 h + 16 l, h = 0,
-// 1.  (An instruction sums over all 128 inputs, so their order matters only in
-// that both operands have the same.)  Rows and inputs past the matrix hold 0.
+// holds row i, inputs 8 g.. and 32 + 8 g.. (eight each) in the 16 bytes at 16 l, 64 +
+// 8 g.. and 96 + 8 g.. at 1024 + 16 l.  (An instruction sums over all 128 inputs, so
+// their order matters only in that both operands have the same; in this one, four
+// lanes together read 64 bytes of a BF16 row at a time.)  Rows and inputs past the matrix
+// hold 0.
 // Of 32 outputs, tile t (0, 1) holds the outputs 8 g + 4 t + r as its rows 4 g + r: a
 // lane of the result, which has rows 4 g + 0..3 of a tile, then has 8 neighbouring
 // outputs of both tiles, and a row's 32 outputs are stored as 64 bytes at once.
@@ -19,8 +21,8 @@
 // The instruction multiplies by powers of two as it goes: sx always, sw if it
 // is an exponent; an FP32 sw multiplies each block's FP32 sum instead.
 //
-// What the 8-bit instructions cost in exactness: beside FP32 sums they line 16
-// products up with the largest and cut what lies below 2^-13 of its power of two.
+// What the 8-bit instructions cost in exactness: beside FP32 sums they line the 16
+// products of a lane's piece up with the largest and cut what lies below 2^-13 of its power of two.
 // Against sums in 64 bits results are off by 1.4e-5 (normal values) to 5.6e-5 (codes of
 // all sizes) in the 2-norm, at 128 as at 2048 inputs, a hundredth of what the
 // rounding to BF16 is off by (1.7e-3). v_mfma_f32_16x16x32_fp8_fp8 cuts alike;
@@ -41,6 +43,9 @@ typedef float F32x4 __attribute__((ext_vector_type(4)));
 typedef int I32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kBlock = 128, kTileBytes = 16 * kBlock;
+
+// The input of byte e (0..15) of lane group g's piece `half`, within its block.
+__device__ __forceinline__ int input_of(int half, int g, int e) { return 64 * half + 32 * (e >> 3) + 8 * g + (e & 7); }
 
 __host__ __device__ __forceinline__ int64_t tiles_of(int64_t rows) { return (rows + 15) / 16; }
 // (Whole groups of 64, as the waves of the product for many rows take them.)
@@ -83,11 +88,12 @@ __global__ __launch_bounds__(256) void pack_fp8_kernel(const Fp8PackParams p) {
     if (w >= pieces) return;
     const int lane = (int)w & 63, half = (int)(w >> 6) & 1;
     const int64_t block = (w >> 9) % blocks, n = output_of(4 * ((w >> 9) / blocks) + ((w >> 7) & 3), lane & 15);
-    const int64_t k = kBlock * block + 32 * (lane >> 4) + 16 * half;
     U32x4 piece = {0u, 0u, 0u, 0u};
     if (n < p.out_features)
-        for (int e = 0; e < 16; ++e)
-            if (k + e < p.in_features) piece[e >> 2] |= (uint32_t)p.codes[n * p.in_features + k + e] << (8 * (e & 3));
+        for (int e = 0; e < 16; ++e) {
+            const int64_t k = kBlock * block + input_of(half, lane >> 4, e);
+            if (k < p.in_features) piece[e >> 2] |= (uint32_t)p.codes[n * p.in_features + k] << (8 * (e & 3));
+        }
     reinterpret_cast<U32x4*>(p.packed)[w] = piece;
 }
 
@@ -115,11 +121,13 @@ __global__ __launch_bounds__(256) void quantize_weight_fp8_kernel(const Fp8PackP
     const int64_t tiles = out_tiles_of(p.out_features);
     for (int w = threadIdx.x; w < 8 * (kTileBytes / 16); w += 256) {
         const int lane = w & 63, half = (w >> 6) & 1;
-        const int64_t tile = 8 * high + (w >> 7), n = output_of(tile, lane & 15), k = kBlock * block + 32 * (lane >> 4) + 16 * half;
+        const int64_t tile = 8 * high + (w >> 7), n = output_of(tile, lane & 15);
         if (tile >= tiles) continue;
         float x[16];
-        for (int e = 0; e < 16; ++e)
-            x[e] = n < p.out_features && k + e < p.in_features ? bf16_f32(p.weight[n * p.in_features + k + e]) * inverse : 0.f;
+        for (int e = 0; e < 16; ++e) {
+            const int64_t k = kBlock * block + input_of(half, lane >> 4, e);
+            x[e] = n < p.out_features && k < p.in_features ? bf16_f32(p.weight[n * p.in_features + k]) * inverse : 0.f;
+        }
         U32x4 piece;
         for (int e = 0; e < 4; ++e) piece[e] = fp8x4_rn(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
         reinterpret_cast<U32x4*>(p.packed)[(weight_place(tile, blocks, block) * 2 + half) * 64 + lane] = piece;
@@ -133,7 +141,6 @@ __global__ __launch_bounds__(256) void unpack_fp8_kernel(const Fp8PackParams p, 
     if (w >= pieces) return;
     const int lane = (int)w & 63, half = (int)(w >> 6) & 1;
     const int64_t block = (w >> 9) % blocks, n = output_of(4 * ((w >> 9) / blocks) + ((w >> 7) & 3), lane & 15);
-    const int64_t k = kBlock * block + 32 * (lane >> 4) + 16 * half;
     if (n >= p.out_features) return;
     const int64_t at = n / kBlock * (4 * fours_of(p.in_features)) + block;
     float scale;
@@ -144,8 +151,10 @@ __global__ __launch_bounds__(256) void unpack_fp8_kernel(const Fp8PackParams p, 
         scale = reinterpret_cast<const float*>(p.packed_scales)[at];
     }
     const U32x4 piece = reinterpret_cast<const U32x4*>(p.packed)[w];
-    for (int e = 0; e < 16 && k + e < p.in_features; ++e)
-        weight[n * p.in_features + k + e] = (uint16_t)bf16_rn(e4m3_f32((piece[e >> 2] >> (8 * (e & 3))) & 0xffu) * scale);
+    for (int e = 0; e < 16; ++e) {
+        const int64_t k = kBlock * block + input_of(half, lane >> 4, e);
+        if (k < p.in_features) weight[n * p.in_features + k] = (uint16_t)bf16_rn(e4m3_f32((piece[e >> 2] >> (8 * (e & 3))) & 0xffu) * scale);
+    }
 }
 
 // ------------------------------------------------------------------ rows
@@ -167,26 +176,25 @@ struct RowCodes {
     uint2 codes;
 };
 __device__ __forceinline__ RowCodes quantize_row_block(U32x4 raw) {
-    float x[8], largest = 0.f;
+    auto largest_of = [&](bool finite) {
+        uint32_t most = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        x[2 * e] = __uint_as_float(raw[e] << 16);
-        x[2 * e + 1] = __uint_as_float(raw[e] & 0xffff0000u);
-    }
+        for (int e = 0; e < 4; ++e) most = larger_sizes(most, finite ? finite_sizes(raw[e]) : raw[e] & 0x7fff7fffu);
+        most = max(most >> 16, most & 0xffffu);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) largest = fmaxf(largest, finite_size(x[e]));
-#pragma unroll
-    for (int d = 8; d; d >>= 1) largest = fmaxf(largest, __shfl_xor(largest, d));
+        for (int d = 8; d; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+        return most;
+    };
+    uint32_t most = largest_of(false);
+    if (__any(most >= kBf16Infinity)) most = largest_of(true);
     RowCodes r;
-    r.exponent = scale_exponent(largest);
-    const float inverse = inverse_scale(r.exponent);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] *= inverse;
-    r.codes = make_uint2(fp8x4_rn(x[0], x[1], x[2], x[3]), fp8x4_rn(x[4], x[5], x[6], x[7]));
+    const float scale = needed_scale(__uint_as_float(most << 16));
+    r.exponent = (int)(__float_as_uint(scale) >> 23);
+    r.codes = make_uint2(fp8x4_of_bf16(raw[0], raw[1], scale), fp8x4_of_bf16(raw[2], raw[3], scale));
     return r;
 }
 // Where the codes of row i's values 8 j.. of a block lie in its tile.
-__device__ __forceinline__ int code_place(int i, int j) { return 1024 * ((j >> 1) & 1) + 16 * (i + 16 * (j >> 2)) + 8 * (j & 1); }
+__device__ __forceinline__ int code_place(int i, int j) { return 1024 * (j >> 3) + 16 * (i + 16 * (j & 3)) + 8 * ((j >> 2) & 1); }
 
 // One workgroup per tile of 16 rows and four blocks of 128 inputs; 16 lanes per row of a block.
 template <bool Wide>
@@ -318,24 +326,19 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
     }
 }
 
-// A few rows: one launch. Workgroups of eight waves round x into LDS as operands,
-// each for itself, while their first weights are on the way, and take tiles of outputs
-// one after the other; the waves share the inputs out and join through LDS.
-// (One row, 2048 -> 6144: 4.1 us, 2048 -> 50257 17.6; with two tiles at a time 4.4 and
-// 22.8, with four 6.0 and 25; with three and six blocks of weights in flight
-// 4.4 and 18.9, 5.7 and 26.5.)
-constexpr int kFewAhead = 2;     // blocks of weights in flight
-constexpr int kFewAtOnce = 128;  // rows of blocks of x
-constexpr int kFewMaxBlocks = 64;  // that LDS holds
-template <bool Exponents, bool Wide>
-__global__ __launch_bounds__(512) void linear_fp8_few_kernel(const LinearFp8Params p) {
-    extern __shared__ __align__(16) uint8_t few_lds[];  // x's codes [block][2 KB], its scales' bytes [block][16]
-    __shared__ F32x4 partial[2][8][64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// Few rows: one launch. Workgroups of W waves take tiles of 16 outputs one
+// after the other, for all rows (T tiles of 16); the waves share the inputs out and
+// join through LDS. A wave rounds its at most B blocks of x once, straight into operands
+// that stay in its registers, while its first weights are on the way; a tile's weights are all asked
+// for while the tile before it is joined. (x rounded into LDS by all waves: 8 rows, 2048 -> 6144
+// 7.3 us, and 4.7 so.)
+template <int T, int W, int B, bool Exponents>
+__global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8Params p) {
+    __shared__ F32x4 partial[2][W][T][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4, rows = (int)p.rows;
     const int blocks = (int)blocks_of(p.in_features), fours = (int)fours_of(p.in_features);
-    uint8_t* const bytes = few_lds + blocks * kTileBytes;
-    const int begin = blocks * wave / 8, end = blocks * (wave + 1) / 8;
+    const int begin = blocks * wave / W, count = blocks * (wave + 1) / W - begin;
     const int64_t tiles = out_tiles_of(p.out_features);
     int64_t tile = blockIdx.x;
     typedef std::conditional_t<Exponents, uint32_t, float> Scale;
@@ -343,72 +346,126 @@ __global__ __launch_bounds__(512) void linear_fp8_few_kernel(const LinearFp8Para
         I32x8 a;
         Scale scale;
     };
+    // (Loads without a condition, past the end the last block again: after a load that one path leaves out every wait
+    // is for all loads in flight.)
     auto load = [&](Block& to, int b) {
-        b = min(b, blocks - 1);
+        b = min(begin + b, blocks - 1);
         to.a = operand(p.packed + weight_place(tile, blocks, b) * kTileBytes, lane);
         if constexpr (Exponents)
             to.scale = p.packed_scales[tile / 8 * (4 * fours) + b];
         else
             to.scale = reinterpret_cast<const float*>(p.packed_scales)[tile / 8 * (4 * fours) + b];
     };
-    Block held[kFewAhead];
+    Block held[B];
+    // Lane (i, g): row i of a tile, inputs 32 h + 8 g.. of a block (eight each), h = 0..3.
+    constexpr uint32_t kOutside = 0xfffffff0u;
+    const int in_features = (int)p.in_features;
+    const __amdgpu_buffer_rsrc_t x_all = handoff_resource(p.x, (uint32_t)((p.rows - 1) * p.x_stride + p.in_features) * 2);
+    struct Raw {
+        U32x4 piece[4];
+    };
+    auto load_raw = [&](int q) {
+        const int b = q / T, row = 16 * (q % T) + i, k = kBlock * (begin + b) + 8 * g;
+        // (What lies outside of x reads as 0.)
+        const uint32_t at = row < rows && b < count ? (uint32_t)(row * p.x_stride + k) * 2 : kOutside;
+        Raw raw;
+        if (!p.wide) {
+            const uint16_t* const from = p.x + row * p.x_stride;
 #pragma unroll
-    for (int a = 0; a < kFewAhead; ++a) load(held[a], begin + a);
-    // 16 lanes per row of a block, the values of kFewAtOnce such rows in flight together.
-    const int j16 = tid & 15;
-    for (int q = tid >> 4; q < rows * blocks; q += kFewAtOnce) {
-        U32x4 x[kFewAtOnce / 32];
-#pragma unroll
-        for (int h = 0; h < kFewAtOnce / 32; ++h) {
-            const int r = min(q + 32 * h, rows * blocks - 1);
-            x[h] = load_values<Wide>(p.x + r / blocks * p.x_stride, kBlock * (r % blocks) + 8 * j16, p.in_features);
+            for (int h = 0; h < 4; ++h)
+                raw.piece[h] = load_values<false>(from, k + 32 * h, row < rows && b < count ? in_features : 0);
+            return raw;
         }
 #pragma unroll
-        for (int h = 0; h < kFewAtOnce / 32; ++h) {
-            const int r = q + 32 * h, row = r / blocks, b = r % blocks;
-            if (r >= rows * blocks) break;
-            const RowCodes codes = quantize_row_block(x[h]);
-            *reinterpret_cast<uint2*>(few_lds + b * kTileBytes + code_place(row, j16)) = codes.codes;
-            if (j16 == 0) bytes[16 * b + row] = (uint8_t)codes.exponent;
+        for (int h = 0; h < 4; ++h)
+            raw.piece[h] = __builtin_amdgcn_raw_buffer_load_b128(x_all, k + 32 * h < in_features ? at + 64 * h : kOutside, 0, 0);
+        return raw;
+    };
+    I32x8 x[B][T];
+    uint32_t x_scales[(B * T + 3) / 4];  // four bytes each
+    auto round = [&](const Raw& raw, int q) {
+        auto largest_of = [&](bool finite) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    most = larger_sizes(most, finite ? finite_sizes(raw.piece[h][e]) : raw.piece[h][e] & 0x7fff7fffu);
+            most = max(most >> 16, most & 0xffffu);
+            most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+            return max(most, (uint32_t)__shfl_xor((int)most, 32));
+        };
+        uint32_t most = largest_of(false);
+        if (__any(most >= kBf16Infinity)) most = largest_of(true);
+        const float scale = needed_scale(__uint_as_float(most << 16));
+        if (q % 4 == 0) x_scales[q / 4] = 0;
+        x_scales[q / 4] |= (__float_as_uint(scale) >> 23) << (8 * (q % 4));
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            x[q / T][q % T][2 * h] = (int)fp8x4_of_bf16(raw.piece[h][0], raw.piece[h][1], scale);
+            x[q / T][q % T][2 * h + 1] = (int)fp8x4_of_bf16(raw.piece[h][2], raw.piece[h][3], scale);
         }
-    }
-    lds_barrier();
+    };
+    // x, which lies in the L2 cache once the first workgroups have read it, is asked for first and rounded while the
+    // weights are on the way: loads return in their order.
+    constexpr int kFirst = B * T < 4 ? B * T : 4;
+    Raw raw[kFirst];
+#pragma unroll
+    for (int q = 0; q < kFirst; ++q) raw[q] = load_raw(q);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < B; ++b) load(held[b], b);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < kFirst; ++q) round(raw[q], q);
+#pragma unroll
+    for (int q = kFirst; q < B * T; ++q) round(load_raw(q), q);
     int side = 0;
     while (true) {
-        F32x4 total = {0.f, 0.f, 0.f, 0.f};
-        for (int b = begin; b < end; b += kFewAhead) {
+        F32x4 total[T];
 #pragma unroll
-            for (int a = 0; a < kFewAhead; ++a) {
-                // (Rows past the last hold what LDS held: their results are not stored.)
-                if (b + a < end) {
-                    const I32x8 x = operand(few_lds + (b + a) * kTileBytes, lane);
-                    const uint32_t x_scale = bytes[16 * (b + a) + i];
-                    if constexpr (Exponents) {
-                        total = mfma(held[a].a, x, total, held[a].scale, x_scale);
-                    } else {
-                        const F32x4 sum = mfma(held[a].a, x, F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scale);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) total[r] = fmaf(held[a].scale, sum[r], total[r]);
-                    }
-                }
-                load(held[a], b + a + kFewAhead);
-            }
-        }
+        for (int t = 0; t < T; ++t) total[t] = F32x4{0.f, 0.f, 0.f, 0.f};
         const int64_t own = tile;
         tile += gridDim.x;
-        if (tile < tiles) {
+        const bool more = tile < tiles;
+        if (!more) tile = own;
+        auto multiply = [&](auto place) {
+            constexpr int Q = decltype(place)::value, b = Q / T, t = Q % T;
+            if constexpr (Exponents) {
+                total[t] = mfma<0, Q % 4>(held[b].a, x[b][t], total[t], held[b].scale, x_scales[Q / 4]);
+            } else {
+                const F32x4 sum = mfma<0, Q % 4>(held[b].a, x[b][t], F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scales[Q / 4]);
 #pragma unroll
-            for (int a = 0; a < kFewAhead; ++a) load(held[a], begin + a);
-        }
-        partial[side][wave][lane] = total;
+                for (int r = 0; r < 4; ++r) total[t][r] = fmaf(held[b].scale, sum[r], total[t][r]);
+            }
+        };
+        auto block = [&](auto number) {
+            constexpr int b = decltype(number)::value;
+            // (What lies past the wave's last block may hold NaN: no product of it, not even with 0.)
+            if (b < count) {
+                multiply(std::integral_constant<int, b * T>{});
+                if constexpr (T > 1) multiply(std::integral_constant<int, b * T + 1>{});
+                if constexpr (T > 2) multiply(std::integral_constant<int, b * T + 2>{});
+                if constexpr (T > 3) multiply(std::integral_constant<int, b * T + 3>{});
+            }
+            load(held[b], b);  // the next tile's
+        };
+        block(std::integral_constant<int, 0>{});
+        if constexpr (B > 1) block(std::integral_constant<int, 1>{});
+        if constexpr (B > 2) block(std::integral_constant<int, 2>{});
+        if constexpr (B > 3) block(std::integral_constant<int, 3>{});
+#pragma unroll
+        for (int t = 0; t < T; ++t) partial[side][wave][t][lane] = total[t];
         lds_barrier();
-        if (wave == 0) {
-            F32x4 sum = partial[side][0][lane];
+        if (wave < T) {
+            const int t = wave;
+            F32x4 sum = partial[side][0][t][lane];
 #pragma unroll
-            for (int w = 1; w < 8; ++w) sum += partial[side][w][lane];
+            for (int w = 1; w < W; ++w) sum += partial[side][w][t][lane];
             const int64_t n = output_of(own, 4 * g);
-            if (i < rows) {
-                uint16_t* const to = p.y + i * p.y_stride + n;
+            const int row = 16 * t + i;
+            if (row < rows) {
+                uint16_t* const to = p.y + row * p.y_stride + n;
                 if (p.aligned && n + 4 <= p.out_features) {
                     *reinterpret_cast<uint2*>(to) = make_uint2(bf16x2_rn(sum[0], sum[1]), bf16x2_rn(sum[2], sum[3]));
                 } else {
@@ -418,7 +475,7 @@ __global__ __launch_bounds__(512) void linear_fp8_few_kernel(const LinearFp8Para
                 }
             }
         }
-        if (tile >= tiles) return;
+        if (!more) return;
         side ^= 1;  // (whose last readers passed the barrier above)
     }
 }
@@ -606,11 +663,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 }
 
-template <bool Exponents, bool Wide>
+// One workgroup per compute unit at most: x is read and rounded by each. (16 rows, 2048 -> 11264: 6.1 us, with
+// two 7.8; 2048 -> 50257 18.6 and 18.8.)
+template <bool Exponents, int T, int W, int B>
+void launch_few_of(const LinearFp8Params& p, hipStream_t stream) {
+    const unsigned grid = (unsigned)std::min<int64_t>(out_tiles_of(p.out_features), p.compute_units);
+    hipLaunchKernelGGL((linear_fp8_few_kernel<T, W, B, Exponents>), dim3(grid), dim3(64 * W), 0, stream, p);
+}
+template <bool Exponents>
 void launch_few(const LinearFp8Params& p, hipStream_t stream) {
-    const size_t lds = blocks_of(p.in_features) * (kTileBytes + 16);
-    const unsigned grid = (unsigned)std::min<int64_t>(out_tiles_of(p.out_features), 2 * p.compute_units);
-    hipLaunchKernelGGL((linear_fp8_few_kernel<Exponents, Wide>), dim3(grid), dim3(512), lds, stream, p);
+    const int64_t blocks = blocks_of(p.in_features);
+    if (p.rows > 32)
+        return blocks <= 8 ? launch_few_of<Exponents, 3, 8, 1>(p, stream) : launch_few_of<Exponents, 3, 8, 2>(p, stream);
+    if (p.rows > 16) {
+        if (blocks <= 8) return launch_few_of<Exponents, 2, 8, 1>(p, stream);
+        return blocks <= 16 ? launch_few_of<Exponents, 2, 8, 2>(p, stream) : launch_few_of<Exponents, 2, 16, 2>(p, stream);
+    }
+    if (blocks <= 8)
+        launch_few_of<Exponents, 1, 8, 1>(p, stream);
+    else if (blocks <= 16)
+        launch_few_of<Exponents, 1, 8, 2>(p, stream);
+    else if (blocks <= 32)
+        launch_few_of<Exponents, 1, 16, 2>(p, stream);
+    else if (blocks <= 48)
+        launch_few_of<Exponents, 1, 16, 3>(p, stream);
+    else
+        launch_few_of<Exponents, 1, 16, 4>(p, stream);
 }
 
 template <bool Exponents, int J, int T>
@@ -690,12 +768,15 @@ size_t fp8_weight_bytes(int64_t out_features, int64_t in_features, bool exponent
            (size_t)((out_features + kBlock - 1) / kBlock) * fours_of(in_features) * (exponents ? 4 : 16);
 }
 
-// Whether every workgroup rounds x for itself, or a launch before the product does: by
-// x's blocks. (2048 -> 6144: 1 row 4.1 us against 8.4, 8 rows 7.3 against 8.2, 16 rows
-// 9.8 against 7.9; 5632 -> 2048: 2 rows 5.4 against 8.8, 4 rows 7.1 against 8.6.)
+// Whether every workgroup rounds x for itself, or a launch before the product does:
+// by x's blocks. (2048 -> 6144: 1 row 4.0 us against 8.2, 16 rows 5.3 against 7.1, 24 rows 6.9
+// against 8.1; 2048 -> 2048: 40 rows 8.2 against 8.1; 5632 -> 2048: 1 row 5.8 against
+// 10.1, 4 rows 6.3 against 9.9, 16 rows 9.1 against 9.2; 8192 -> 8192: 16 rows 18.3
+// against 15.8.)
+constexpr int64_t kFewMaxRows = 48, kFewMaxBlocks = 64, kFewMost = 512;
 static bool few_rows(int64_t rows, int64_t in_features) {
     const int64_t blocks = blocks_of(in_features);
-    return rows <= 16 && blocks <= kFewMaxBlocks && rows * blocks <= kFewAtOnce;
+    return rows <= kFewMaxRows && blocks <= kFewMaxBlocks && rows * blocks <= kFewMost;
 }
 
 size_t linear_fp8_workspace(int64_t rows, int64_t in_features) {
@@ -725,12 +806,11 @@ hipError_t launch_unpack_fp8(const Fp8PackParams& p, uint16_t* weight, hipStream
 hipError_t launch_linear_fp8(const LinearFp8Params& given, hipStream_t stream) {
     LinearFp8Params p = given;
     p.aligned = p.y_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
-    const bool wide = p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+    p.wide = p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
     if (few_rows(p.rows, p.in_features)) {
-        if (wide)
-            p.exponents ? launch_few<true, true>(p, stream) : launch_few<false, true>(p, stream);
-        else
-            p.exponents ? launch_few<true, false>(p, stream) : launch_few<false, false>(p, stream);
+        // (Whole pieces of eight inputs, within 2^31 bytes.)
+        p.wide = p.wide && p.in_features % 8 == 0 && p.rows * p.x_stride < ((int64_t)1 << 30);
+        p.exponents ? launch_few<true>(p, stream) : launch_few<false>(p, stream);
         return hipGetLastError();
     }
     const int64_t most = rows_at_once(p.in_features);
@@ -740,7 +820,7 @@ hipError_t launch_linear_fp8(const LinearFp8Params& given, hipStream_t stream) {
         p.y = given.y + first * p.y_stride;
         p.x_scales = reinterpret_cast<uint32_t*>(p.x_codes + fp8_row_bytes(p.rows, p.in_features));
         const dim3 grid((unsigned)(fours_of(p.in_features) * tiles_of(p.rows)));
-        if (wide)
+        if (p.wide)
             hipLaunchKernelGGL(quantize_rows_fp8_kernel<true>, grid, dim3(256), 0, stream, p);
         else
             hipLaunchKernelGGL(quantize_rows_fp8_kernel<false>, grid, dim3(256), 0, stream, p);

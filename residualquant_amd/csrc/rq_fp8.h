@@ -41,6 +41,30 @@ __device__ __forceinline__ uint32_t fp8x4_rn(float a, float b, float c, float d)
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(nan_unless_finite(c), nan_unless_finite(d), low, true);
 }
 
+// Four E4M3 codes of two words of two BF16 values over a power of two, |x| <= 448 of
+// it: what fp8x4_rn makes of the quotients, infinities and NaN included (checked on the
+// device for all values at powers from 2^-126 to 2^120), without unpacking them.
+__device__ __forceinline__ uint32_t fp8x4_of_bf16(uint32_t low, uint32_t high, float scale) {
+    typedef __bf16 Bf16x2 __attribute__((ext_vector_type(2)));
+    typedef short I16x2 __attribute__((ext_vector_type(2)));
+    I16x2 codes = {0, 0};
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(codes, __builtin_bit_cast(Bf16x2, low), scale, false);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(codes, __builtin_bit_cast(Bf16x2, high), scale, true);
+    return __builtin_bit_cast(uint32_t, codes);
+}
+
+// The larger sizes of pairs of BF16 values, as bits (infinities and NaN are the largest).
+__device__ __forceinline__ uint32_t larger_sizes(uint32_t a, uint32_t b) {
+    typedef uint16_t U16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(U16x2, a), __builtin_bit_cast(U16x2, b)));
+}
+constexpr uint32_t kBf16Infinity = 0x7f80u;
+// A pair's sizes, 0 in the place of what is not finite.
+__device__ __forceinline__ uint32_t finite_sizes(uint32_t x) {
+    x &= 0x7fff7fffu;
+    return ((x & 0xffffu) < kBf16Infinity ? x & 0xffffu : 0u) | (x < (kBf16Infinity << 16) ? x & 0xffff0000u : 0u);
+}
+
 __device__ __forceinline__ bool power_of_two(float x) { return (__float_as_uint(x) & 0x7fffffu) == 0; }
 
 // A page's rows from `slot` on from `values` (zeros where there are none), its scale, and where that grows its
