@@ -49,14 +49,17 @@ LINEAR_ROWS_MAX = 8
 
 
 def _project(x: torch.Tensor, weight) -> torch.Tensor:
-    """``x @ weight.T`` for a linear weight held ``[out, in]``, in BF16 or in 4 bits (``Int4Weight``).
+    """``x @ weight.T`` for a linear weight held ``[out, in]``, in BF16, in 4 bits (``Int4Weight``) or as E4M3 (``Fp8Weight``).
 
     At up to eight rows the product is a weight stream: ``step_ops.linear_rows``
     reads every weight row once with 16-byte loads and FP32 accumulation.
     Larger batches take hipBLASLt through ``F.linear``.  A 4-bit weight takes
     ``step_ops.linear_rows_int4``, above 64 rows in near-equal parts (2048 to
     11264 features: 29 us for 128 rows and 111 for 512; its codes restored to
-    BF16, each rounded, and a library product would take 39 and 50)."""
+    BF16, each rounded, and a library product would take 39 and 50).  An E4M3
+    weight takes ``step_ops.linear_fp8`` for any rows, which it rounds too."""
+    if isinstance(weight, step_ops.Fp8Weight):
+        return step_ops.linear_fp8(x, weight)
     rows, in_features = x.shape
     if isinstance(weight, step_ops.Int4Weight):
         if rows <= step_ops.LINEAR_INT4_MAX_ROWS:
@@ -82,7 +85,8 @@ class LoopedConfig:
     Ouro-1.4B MLP width at the same hidden size) is an assumption, as are
     ``rope_theta`` and ``rms_eps``.  ``projection_bits`` 4 holds the
     projections and the vocabulary projection as 4-bit codes with a BF16 scale
-    per ``projection_group`` inputs.
+    per ``projection_group`` inputs; 8 with ``projection_format`` "e4m3" as
+    E4M3 codes with a power-of-two scale per 128 x 128.
     """
 
     layers: int = 48
@@ -100,6 +104,7 @@ class LoopedConfig:
     page_tokens: int = 16
     projection_bits: int = 16
     projection_group: int = 32
+    projection_format: str = "int"
 
 
 class LoopedDecoder:
@@ -115,8 +120,8 @@ class LoopedDecoder:
                  top_logprobs: Optional[int] = None):
         if config.loops != len(config.schedule):
             raise ValueError("one packed record per loop is required")
-        if config.projection_bits not in (4, 16):
-            raise ValueError("projections are held in 16 or 4 bits")
+        if (config.projection_bits, config.projection_format) not in ((16, "int"), (4, "int"), (8, "e4m3")):
+            raise ValueError("projections are held in 16 or 4 bits, or in 8 with projection_format \"e4m3\"")
         if top_logprobs is not None and not 0 <= top_logprobs <= min(step_ops.LOGPROBS_MAX_TOP, config.vocab):
             raise ValueError(f"0 to {step_ops.LOGPROBS_MAX_TOP} alternatives, at most the vocabulary, required")
         self.top_logprobs = top_logprobs
@@ -129,7 +134,9 @@ class LoopedDecoder:
         def weight(fan_out, fan_in):
             scale = 1.0 / math.sqrt(fan_in)
             drawn = (torch.randn((fan_out, fan_in), generator=generator, device=device) * scale).to(torch.bfloat16)
-            return step_ops.quantize_weight_int4(drawn, c.projection_group) if c.projection_bits == 4 else drawn
+            if c.projection_bits == 4:
+                return step_ops.quantize_weight_int4(drawn, c.projection_group)
+            return step_ops.quantize_weight_fp8(drawn) if c.projection_bits == 8 else drawn
 
         q_size = c.heads * c.head_dim
         if weights_from is not None:
@@ -204,8 +211,8 @@ class LoopedDecoder:
         model's loops, as the reference binds them (install_model.py:154-196).
         4-D value rotations are folded into this decoder's QKV and O weights
         (weights.py:8-37), in place: call before building the history, and
-        before sharing the weights with another decoder (weights held in 4
-        bits cannot take them)."""
+        before sharing the weights with another decoder (weights held in 4 or
+        8 bits cannot take them)."""
         c = self.config
         q_size = c.heads * c.head_dim
         prepared, folded = artifact_module.prepare_value_rotation(artifact)
