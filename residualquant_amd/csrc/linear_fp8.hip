@@ -44,6 +44,10 @@ typedef int I32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kBlock = 128, kTileBytes = 16 * kBlock;
 
+// Behind x's codes and scales in the workspace: what the wide kernels read past the last row tile, of the
+// codes up to seven tiles.
+constexpr int kPastRows = 8 * kTileBytes;
+
 // The input of byte e (0..15) of lane group g's piece `half`, within its block.
 __device__ __forceinline__ int input_of(int half, int g, int e) { return 64 * half + 32 * (e >> 3) + 8 * g + (e & 7); }
 
@@ -358,7 +362,7 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
     };
     Block held[B];
     // Lane (i, g): row i of a tile, inputs 32 h + 8 g.. of a block (eight each), h = 0..3.
-    constexpr uint32_t kOutside = 0xfffffff0u;
+    constexpr uint32_t kOutside = 1u << 31;  // past x's bytes, with what is added below too
     const int in_features = (int)p.in_features;
     const __amdgpu_buffer_rsrc_t x_all = handoff_resource(p.x, (uint32_t)((p.rows - 1) * p.x_stride + p.in_features) * 2);
     struct Raw {
@@ -510,7 +514,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     __amdgpu_buffer_rsrc_t weights, x_all, x_scales;
     typedef std::conditional_t<Exponents, uint32_t, F32x4> Scales;  // of the weight, for four blocks
     const Scales* scales_of;
-    // Tiles past the weight's last read as 0, past x's as other rows or 0: neither is stored.
+    // Every read is of memory that is there: past the weight's last tiles those again, past x's row
+    // tiles what comes behind them (kPastRows), past the last block of x the last.  (What is the same for all lanes,
+    // an offset in a scalar register, comes off a resource's size before the comparison, below zero
+    // too: only the lanes' own offsets are guarded by it.)  None of that is stored.
     auto take = [&](int64_t number) {
         const int64_t band = number / (8 * out_groups), in_band = number - band * 8 * out_groups;
         const int64_t high = min((int64_t)8, row_groups - 8 * band);
@@ -518,10 +525,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         tile0 = 16 * out_group + 4 * wave;
         row_tile0 = NT * row_group;
         auto resource = [](const void* base, int64_t bytes) { return handoff_resource(base, (uint32_t)bytes); };
-        weights = resource(p.packed + min(tile0, out_tiles) * blocks * kTileBytes, tile0 < out_tiles ? 4 * blocks * kTileBytes : 0);
-        x_all = resource(p.x_codes + row_tile0 * kTileBytes, (blocks * row_tiles - row_tile0) * kTileBytes);
-        x_scales = resource(p.x_scales + row_tile0 * 16, (fours * row_tiles - row_tile0) * 64);
-        scales_of = reinterpret_cast<const Scales*>(p.packed_scales) + (tile0 < out_tiles ? tile0 / 8 : 0) * fours;
+        const int64_t own = min(tile0, out_tiles - 4);
+        weights = resource(p.packed + own * blocks * kTileBytes, 4 * blocks * kTileBytes);
+        x_all = resource(p.x_codes + row_tile0 * kTileBytes, (blocks * row_tiles - row_tile0) * kTileBytes + kPastRows);
+        x_scales = resource(p.x_scales + row_tile0 * 16, (fours * row_tiles - row_tile0) * 64 + kPastRows);
+        scales_of = reinterpret_cast<const Scales*>(p.packed_scales) + own / 8 * fours;
     };
 
     F32x4 total[4][NT];
@@ -541,9 +549,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     auto load_a = [&](I32x8 (&to)[4], int b) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t at = (4 * b + j) * kTileBytes;
-            const U32x4 low = __builtin_amdgcn_raw_buffer_load_b128(weights, 16 * lane, at, 0);
-            const U32x4 high = __builtin_amdgcn_raw_buffer_load_b128(weights, 16 * lane + 1024, at, 0);
+            // (The lane's offset holds the block, so that past the last block it is past the resource and reads 0.)
+            const uint32_t at = 16 * lane + 4 * b * kTileBytes + (j & 1) * kTileBytes, pair = (j >> 1) * 2 * kTileBytes;
+            const U32x4 low = __builtin_amdgcn_raw_buffer_load_b128(weights, at, pair, 0);
+            const U32x4 high = __builtin_amdgcn_raw_buffer_load_b128(weights, at + 1024, pair, 0);
             to[j] = I32x8{(int)low[0], (int)low[1], (int)low[2], (int)low[3], (int)high[0], (int)high[1], (int)high[2], (int)high[3]};
         }
     };
@@ -562,14 +571,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v[e])));
         return v;
     };
-    // Block 4 four + S.  (Blocks past the last are read as they come and not used: within the resources, or 0.)
+    // Block 4 four + S.
     auto step = [&](auto place, int four) {
         constexpr int S = decltype(place)::value;
         const int b = 4 * four + S;
         store_x((S + 2) & 3);
-        load_x(b + 3);
+        load_x(min(b + 3, blocks - 1));
         load_a(a[(S + 1) & 1], b + 1);
-        if constexpr (S == 0) load_word(four + 1);
+        if constexpr (S == 0) load_word(min(four + 1, fours - 1));
         if constexpr (S == 2) store_word(four + 1);
         __builtin_amdgcn_sched_barrier(0);
         const uint8_t* from = lds[S];
@@ -623,9 +632,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             for (int t = 0; t < NT; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
         store_x(0);
         store_word(0);
-        load_x(1);
+        load_x(min(1, blocks - 1));
         store_x(1);
-        load_x(2);
+        load_x(min(2, blocks - 1));
         lds_barrier();
         for (int four = 0; four < fours; ++four) {
             step(std::integral_constant<int, 0>{}, four);
@@ -782,7 +791,7 @@ static bool few_rows(int64_t rows, int64_t in_features) {
 size_t linear_fp8_workspace(int64_t rows, int64_t in_features) {
     if (few_rows(rows, in_features)) return 0;
     rows = std::min(rows, rows_at_once(in_features));
-    return fp8_row_bytes(rows, in_features) + (size_t)tiles_of(rows) * fours_of(in_features) * 64;
+    return fp8_row_bytes(rows, in_features) + (size_t)tiles_of(rows) * fours_of(in_features) * 64 + kPastRows;
 }
 
 hipError_t launch_pack_fp8(const Fp8PackParams& p, hipStream_t stream) {

@@ -118,6 +118,31 @@ def test_exact_sums(device, rows, out, features, kind):
     assert torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("kind", ["exponents", "float"])
+@pytest.mark.parametrize("rows,out,features", [(130, 3150, 100), (257, 2050, 200), (257, 2114, 300), (130, 6300, 640), (500, 8300, 100),
+                                               (500, 8300, 200), (510, 8400, 520), (700, 8300, 100), (700, 8300, 300),
+                                               (1500, 8270, 384), (2050, 8300, 1100)])
+def test_exact_sums_of_large_tiles(device, rows, out, features, kind):
+    """As above where tiles of 256 outputs are taken, which end past the weight, past x's rows and within the blocks
+    read ahead; what lies around the results stays as it was."""
+    print(f"rows={rows} out={out} in={features} {kind}", flush=True)
+    g = torch.Generator().manual_seed(rows + features)
+    codes = torch.randint(-3, 4, (out, features), generator=g).float().to(torch.float8_e4m3fn)
+    shape = (-(-out // BLOCK), -(-features // BLOCK))
+    exponents = torch.randint(-3, 4, shape, generator=g)
+    scales = (exponents + 127).to(torch.uint8).view(torch.float8_e8m0fnu) if kind == "exponents" else torch.exp2(exponents.float())
+    x = torch.randint(-8, 9, (rows, features), generator=g).to(torch.bfloat16)
+    full = torch.exp2(exponents.float()).repeat_interleave(BLOCK, 0)[:out].repeat_interleave(BLOCK, 1)[:, :features]
+    # (Whole multiples of 2^-3, up to 1100 x 24 x 2^3 < 2^18: FP32 holds every sum.)
+    want = (x.float() @ (codes.float() * full).t()).to(torch.bfloat16)
+    around = torch.full((rows + 2, out + 5), 7.0, device=device, dtype=torch.bfloat16)
+    step_ops.linear_fp8(x.to(device), step_ops.pack_weight_fp8(codes.to(device), scales.to(device)), out=around[1:-1, 2:-3])
+    around = around.cpu()
+    assert torch.equal(around[1:-1, 2:-3], want)
+    around[1:-1, 2:-3] = 7.0
+    assert torch.equal(around, torch.full_like(around, 7.0))
+
+
 @pytest.mark.parametrize("out,features", [(1, 1), (16, 128), (130, 300), (257, 1025)])
 def test_weight_quantize_and_restore(device, out, features):
     g = torch.Generator().manual_seed(out)
