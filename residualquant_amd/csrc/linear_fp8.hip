@@ -48,6 +48,10 @@ constexpr int kBlock = 128, kTileBytes = 16 * kBlock;
 // codes up to seven tiles.
 constexpr int kPastRows = 8 * kTileBytes;
 
+// Results at any element (rows of an odd number of outputs begin at any).
+typedef U32x4 U32x4At2 __attribute__((aligned(2)));
+typedef U32x2 U32x2At2 __attribute__((aligned(2)));
+
 // The input of byte e (0..15) of lane group g's piece `half`, within its block.
 __device__ __forceinline__ int input_of(int half, int g, int e) { return 64 * half + 32 * (e >> 3) + 8 * g + (e & 7); }
 
@@ -317,9 +321,9 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
         const int64_t n = output_of(tile0 + j, 4 * g), m = 16 * (row_tile0 + t) + i;
         if (m >= p.rows) continue;
         uint16_t* const to = p.y + m * p.y_stride + n;
-        if (kPair == 2 && p.aligned && n + 8 <= p.out_features) {
+        if (kPair == 2 && n + 8 <= p.out_features) {
             const F32x4 u = sum[0], v = sum[kPair - 1];
-            *reinterpret_cast<U32x4*>(to) = U32x4{bf16x2_rn(u[0], u[1]), bf16x2_rn(u[2], u[3]), bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3])};
+            *reinterpret_cast<U32x4At2*>(to) = U32x4{bf16x2_rn(u[0], u[1]), bf16x2_rn(u[2], u[3]), bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3])};
             continue;
         }
 #pragma unroll
@@ -470,8 +474,8 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
             const int row = 16 * t + i;
             if (row < rows) {
                 uint16_t* const to = p.y + row * p.y_stride + n;
-                if (p.aligned && n + 4 <= p.out_features) {
-                    *reinterpret_cast<uint2*>(to) = make_uint2(bf16x2_rn(sum[0], sum[1]), bf16x2_rn(sum[2], sum[3]));
+                if (n + 4 <= p.out_features) {
+                    *reinterpret_cast<U32x2At2*>(to) = U32x2{bf16x2_rn(sum[0], sum[1]), bf16x2_rn(sum[2], sum[3])};
                 } else {
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -656,8 +660,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const F32x4 u = total[2 * h][t], v = total[2 * h + 1][t];
-                if (p.aligned && out_at + 32 * h + 8 <= p.out_features) {
-                    *reinterpret_cast<U32x4*>(to + 32 * h) =
+                if (out_at + 32 * h + 8 <= p.out_features) {
+                    *reinterpret_cast<U32x4At2*>(to + 32 * h) =
                         U32x4{bf16x2_rn(u[0], u[1]), bf16x2_rn(u[2], u[3]), bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3])};
                     continue;
                 }
@@ -673,7 +677,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // One workgroup per compute unit at most: x is read and rounded by each. (16 rows, 2048 -> 11264: 6.1 us, with
-// two 7.8; 2048 -> 50257 18.6 and 18.8.)
+// two 7.8; 2048 -> 50257 21.4 and 20.7.)
 template <bool Exponents, int T, int W, int B>
 void launch_few_of(const LinearFp8Params& p, hipStream_t stream) {
     const unsigned grid = (unsigned)std::min<int64_t>(out_tiles_of(p.out_features), p.compute_units);
@@ -814,7 +818,6 @@ hipError_t launch_unpack_fp8(const Fp8PackParams& p, uint16_t* weight, hipStream
 
 hipError_t launch_linear_fp8(const LinearFp8Params& given, hipStream_t stream) {
     LinearFp8Params p = given;
-    p.aligned = p.y_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
     p.wide = p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
     if (few_rows(p.rows, p.in_features)) {
         // (Whole pieces of eight inputs, within 2^31 bytes.)
