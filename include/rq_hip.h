@@ -409,7 +409,7 @@ enum { RQ_SCALE_E8M0 = 0, RQ_SCALE_F32 = 1 };
  * |x| <= 448 sx for the block's finite values, cx = e4m3(x / sx) to nearest,
  * ties to even, NaN for what is not finite.  FP32 sums; results below the
  * normal range of FP32 may be 0.  x of any even address and row stride
- * (16-byte aligned rows are read faster).  `workspace`: device memory of
+ * (16-byte aligned rows are read faster); it and y do not overlap.  `workspace`: device memory of
  * rq_linear_fp8_workspace_bytes(...) (0 for a few rows), any address; calls
  * that may overlap need one each.
  */
@@ -468,7 +468,7 @@ int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads,
  * count as 0; sums and products are FP64.
  * accepted[b]: drafts taken.  out_tokens [rows]: row r's following token, for the
  * rows before the final one their drafts, for it the drawn token (-1 if no
- * weight is positive), -1 in all other rows.
+ * weight is positive), -1 in all other rows; it does not overlap tokens.
  * `workspace`: device memory of rq_verify_drafts_workspace_bytes(...), any
  * address; calls that may overlap need one each.
  */

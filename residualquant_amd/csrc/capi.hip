@@ -1475,6 +1475,18 @@ int rq_token_logprobs(const void* logits, int64_t stride, int dtype, int64_t row
     return check_launch(rq::launch_logprobs(p, stream), "log probability launch");
 }
 
+// Whether `rows` rows of `width` elements of 2 bytes at two places share an address (columns of rows of
+// one stride may lie side by side).
+static bool rows_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b, int64_t b_stride,
+                         int64_t b_width, int64_t rows) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t a1 = a0 + 2 * (uintptr_t)((rows - 1) * a_stride + a_width), b1 = b0 + 2 * (uintptr_t)((rows - 1) * b_stride + b_width);
+    if (a0 >= b1 || b0 >= a1) return false;
+    if (a_stride != b_stride || rows == 1) return true;
+    const uintptr_t stride = 2 * (uintptr_t)a_stride, behind = b0 > a0 ? (b0 - a0) % stride : (stride - (a0 - b0) % stride) % stride;
+    return behind < 2 * (uintptr_t)a_width || behind + 2 * (uintptr_t)b_width > stride;
+}
+
 // ------------------------------------------------- projections in 8-bit floating point
 
 // The largest sides and elements keep every index of the kernels in range.
@@ -1569,6 +1581,8 @@ int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t pa
     const size_t needed = rq_linear_fp8_workspace_bytes(rows, in_features);
     if (needed > 0 && (workspace == nullptr || workspace_bytes < needed))
         return fail(RQ_ENOSPACE, "Projection workspace of %zu bytes required, %zu given", needed, workspace_bytes);
+    if (rows_overlap(x, x_stride, in_features, y, y_stride, out_features, rows))
+        return fail(RQ_EINVAL, "x and the output must not overlap");
     rq::LinearFp8Params p{};
     p.x = static_cast<const uint16_t*>(x);
     p.x_stride = x_stride;
@@ -1586,14 +1600,6 @@ int rq_linear_fp8(const void* x, int64_t x_stride, const void* packed, size_t pa
 }
 
 // ------------------------------------------------- rotated appends, verification of drafts
-
-// Whether `rows` rows of `width` elements of 2 bytes at two places share an address.
-static bool rows_overlap(const void* a, int64_t a_stride, int64_t a_width, const void* b, int64_t b_stride,
-                         int64_t b_width, int64_t rows) {
-    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
-    const uintptr_t a1 = a0 + 2 * (uintptr_t)((rows - 1) * a_stride + a_width), b1 = b0 + 2 * (uintptr_t)((rows - 1) * b_stride + b_width);
-    return a0 < b1 && b0 < a1;
-}
 
 int rq_rope_append(const void* qkv, int64_t qkv_stride, int64_t rows, int heads, int kv_heads, int head_dim,
                    int rotary_dim, int interleaved, const float* cos_table, const float* sin_table, int64_t table_rows,
@@ -1687,6 +1693,8 @@ int rq_verify_drafts(const void* target, int64_t target_stride, const void* draf
     const size_t needed = rq_verify_drafts_workspace_bytes(requests, vocab);
     if (workspace == nullptr || workspace_bytes < needed)
         return fail(RQ_ENOSPACE, "Verification workspace of %zu bytes required, %zu given", needed, workspace_bytes);
+    if (rows > 0 && tokens < out_tokens + rows && out_tokens < tokens + rows)
+        return fail(RQ_EINVAL, "Tokens and the tokens that follow them must not overlap");
     p.target = target;
     p.target_stride = target_stride;
     p.draft = draft;

@@ -333,7 +333,7 @@ def linear_fp8(x: torch.Tensor, weight: Fp8Weight, out: Optional[torch.Tensor] =
 
     ``x`` is rounded to E4M3 on the way, with a power-of-two scale for each row
     and 128 inputs; a row with a NaN or an infinity gives NaN, others do not
-    change.  ``workspace``: uint8 memory of ``linear_fp8_workspace_bytes(rows,
+    change.  ``out`` must not overlap ``x``.  ``workspace``: uint8 memory of ``linear_fp8_workspace_bytes(rows,
     in_features)`` bytes for this call alone, by default from torch's allocator.
     """
     shape, strides = x.shape, x.stride()

@@ -165,3 +165,20 @@ def test_tensors_on_the_host_are_refused():
                                          torch.zeros((1, 4), dtype=torch.int32))):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_results_over_their_inputs_are_refused(lib):
+    # A few rows take no workspace; a results' row is 40 wide, an input's 256.
+    for wrong in (dict(y=FAKE), dict(y=FAKE + 2 * 255), dict(y=FAKE + 2 * (3 * 256 + 255)), dict(x=FAKE + 2 * (3 * 40 + 39), y=FAKE),
+                  dict(y=FAKE + 2 * 300, x_stride=512, y_stride=512, out=257), dict(y=FAKE, x=FAKE + 2 * 39, x_stride=512, y_stride=512),
+                  dict(y=FAKE + 2 * 260, x_stride=512, y_stride=500)):
+        assert _linear(lib, **{**dict(rows=4, workspace=None), **wrong}) == _lib.RQ_EINVAL, wrong
+        assert b"overlap" in lib.rq_last_error(), wrong
+    for out in (FAKE, FAKE + 8 * 3, FAKE - 8 * 3):
+        assert _verify(lib, target=1 << 30, draft=None, tokens=FAKE, out=out) == _lib.RQ_EINVAL
+        assert b"overlap" in lib.rq_last_error()
+    # Rotated rows side by side in rows of one stride pass (here as far as the next check, of the sizes of a grid).
+    side = dict(query=0x200000, key=0x200000 + 2 * 512, query_stride=768, key_stride=768, requests=1 << 24)
+    assert _append(lib, **side) == _lib.RQ_EINVAL and b"Too many rows" in lib.rq_last_error()
+    for wrong in (dict(key=0x200000 + 2 * 508), dict(query=0x200000 + 2 * 252, key=0x200000), dict(key=0x200000 + 2 * 516)):
+        assert _append(lib, **{**side, **wrong}) == _lib.RQ_EINVAL and b"overlap" in lib.rq_last_error(), wrong

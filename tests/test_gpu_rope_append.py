@@ -228,6 +228,19 @@ def test_captured_and_replayed(device, eight):
         assert scales is None or torch.equal(call.scales, scales)
 
 
+def test_query_and_key_side_by_side(device):
+    call = Call(device, [5, 33], [4, 9], 4, 2, 128, 16, True)
+    cos, sin = tables(50, 128, device)
+    before, scales = call.cache.clone(), call.scales.clone()
+    rest = (call.starts, call.seq_lens, call.table)
+    query, key, _ = ops.rope_append(call.qkv, cos, sin, call.cache, call.scales, *rest)
+    both = torch.full((13, 6 * 128 + 4), 7.0, dtype=torch.bfloat16, device=device)
+    ops.rope_append(call.qkv, cos, sin, before, scales, *rest, query=both[:, :512].view(13, 4, 128), key=both[:, 512:768].view(13, 2, 128))
+    assert torch.equal(both[:, :512], query.reshape(13, -1)) and torch.equal(both[:, 512:768], key.reshape(13, -1))
+    assert torch.equal(before.view(torch.uint8), call.cache.view(torch.uint8)) and torch.equal(scales, call.scales)
+    assert bool((both[:, 768:] == 7.0).all())
+
+
 def test_refusals(device):
     call = Call(device, [5, 33], [4, 9], 4, 2, 128, 16, True)
     cos, sin = tables(50, 128, device)
