@@ -167,10 +167,8 @@ __global__ __launch_bounds__(256) void unpack_fp8_kernel(const Fp8PackParams p, 
 
 // ------------------------------------------------------------------ rows
 
-// Eight neighbouring values of a row as they lie there (0 past its end); Wide: from 16-byte aligned addresses.
-template <bool Wide>
+// Eight neighbouring values of a row of any alignment and length (0 past its end).
 __device__ __forceinline__ U32x4 load_values(const uint16_t* row, int64_t k, int64_t in_features) {
-    if (Wide && k + 8 <= in_features) return *reinterpret_cast<const U32x4*>(row + k);
     U32x4 raw;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -178,51 +176,60 @@ __device__ __forceinline__ U32x4 load_values(const uint16_t* row, int64_t k, int
     return raw;
 }
 
-// A block of a row, eight values in each of 16 neighbouring lanes: its scale's byte, and these values' codes.
-struct RowCodes {
-    int exponent;
-    uint2 codes;
-};
-__device__ __forceinline__ RowCodes quantize_row_block(U32x4 raw) {
+// A block of a row, 32 values in each of the lanes i, i + 16, i + 32, i + 48 of a wave: its scale, and these
+// values' operands.
+__device__ __forceinline__ float quantize_row_block(const U32x4 (&raw)[4], I32x8& codes) {
     auto largest_of = [&](bool finite) {
         uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) most = larger_sizes(most, finite ? finite_sizes(raw[e]) : raw[e] & 0x7fff7fffu);
-        most = max(most >> 16, most & 0xffffu);
+        for (int h = 0; h < 4; ++h)
 #pragma unroll
-        for (int d = 8; d; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-        return most;
+            for (int e = 0; e < 4; ++e) most = larger_sizes(most, finite ? finite_sizes(raw[h][e]) : raw[h][e] & 0x7fff7fffu);
+        most = max(most >> 16, most & 0xffffu);
+        most = max(most, (uint32_t)__shfl_xor((int)most, 16));
+        return max(most, (uint32_t)__shfl_xor((int)most, 32));
     };
     uint32_t most = largest_of(false);
     if (__any(most >= kBf16Infinity)) most = largest_of(true);
-    RowCodes r;
     const float scale = needed_scale(__uint_as_float(most << 16));
-    r.exponent = (int)(__float_as_uint(scale) >> 23);
-    r.codes = make_uint2(fp8x4_of_bf16(raw[0], raw[1], scale), fp8x4_of_bf16(raw[2], raw[3], scale));
-    return r;
-}
-// Where the codes of row i's values 8 j.. of a block lie in its tile.
-__device__ __forceinline__ int code_place(int i, int j) { return 1024 * (j >> 3) + 16 * (i + 16 * (j & 3)) + 8 * ((j >> 2) & 1); }
-
-// One workgroup per tile of 16 rows and four blocks of 128 inputs; 16 lanes per row of a block.
-template <bool Wide>
-__global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const LinearFp8Params p) {
-    const int tid = threadIdx.x, j = tid & 15, i = tid >> 4;
-    const int64_t blocks = blocks_of(p.in_features), fours = fours_of(p.in_features);
-    const int64_t four = blockIdx.x % fours, tile = blockIdx.x / fours, m = 16 * tile + i;
-    const uint16_t* row = p.x + m * p.x_stride;
-    U32x4 x[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) x[b] = load_values<Wide>(row, kBlock * (4 * four + b) + 8 * j, m < p.rows ? p.in_features : 0);
-    uint32_t word = 0;
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        const RowCodes r = quantize_row_block(x[b]);
-        word |= (uint32_t)r.exponent << (8 * b);
-        if (4 * four + b < blocks)
-            *reinterpret_cast<uint2*>(p.x_codes + row_place(tile, tiles_of(p.rows), 4 * four + b) * kTileBytes + code_place(i, j)) = r.codes;
+    for (int h = 0; h < 4; ++h) {
+        codes[2 * h] = (int)fp8x4_of_bf16(raw[h][0], raw[h][1], scale);
+        codes[2 * h + 1] = (int)fp8x4_of_bf16(raw[h][2], raw[h][3], scale);
     }
-    if (j == 0) p.x_scales[(four * tiles_of(p.rows) + tile) * 16 + i] = word;
+    return scale;
+}
+
+// One workgroup per tile of 16 rows and four blocks of 128 inputs, a wave a block: lane (i, g) the operands
+// of row i, inputs 32 h + 8 g.. (eight each). Eights: whole pieces of eight inputs, read at any alignment and
+// without a condition (16-byte loads that one path leaves out wait one by one).
+template <bool Eights>
+__global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const LinearFp8Params p) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int64_t blocks = blocks_of(p.in_features), fours = fours_of(p.in_features), row_tiles = tiles_of(p.rows);
+    const int64_t four = blockIdx.x % fours, tile = blockIdx.x / fours, m = 16 * tile + i, b = 4 * four + wave;
+    const int64_t in_features = m < p.rows ? p.in_features : 0;
+    const int64_t k = kBlock * b + 8 * g;
+    U32x4 raw[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+        if constexpr (Eights)
+            raw[h] = *reinterpret_cast<const U32x4At2*>(p.x + (k + 32 * h < in_features ? m * p.x_stride + k + 32 * h : 0));
+        else
+            raw[h] = load_values(p.x + m * p.x_stride, k + 32 * h, in_features);
+    }
+    if constexpr (Eights)
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+            if (k + 32 * h >= in_features) raw[h] = U32x4{0u, 0u, 0u, 0u};
+    I32x8 codes;
+    const float scale = quantize_row_block(raw, codes);
+    if (b < blocks) {
+        uint8_t* const to = p.x_codes + row_place(tile, row_tiles, b) * kTileBytes + 16 * lane;
+        *reinterpret_cast<U32x4*>(to) = U32x4{(uint32_t)codes[0], (uint32_t)codes[1], (uint32_t)codes[2], (uint32_t)codes[3]};
+        *reinterpret_cast<U32x4*>(to + 1024) = U32x4{(uint32_t)codes[4], (uint32_t)codes[5], (uint32_t)codes[6], (uint32_t)codes[7]};
+    }
+    if (g == 0) reinterpret_cast<uint8_t*>(p.x_scales)[4 * ((four * row_tiles + tile) * 16 + i) + wave] = (uint8_t)(__float_as_uint(scale) >> 23);
 }
 
 // ------------------------------------------------------------------ product
@@ -381,7 +388,7 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
             const uint16_t* const from = p.x + row * p.x_stride;
 #pragma unroll
             for (int h = 0; h < 4; ++h)
-                raw.piece[h] = load_values<false>(from, k + 32 * h, row < rows && b < count ? in_features : 0);
+                raw.piece[h] = load_values(from, k + 32 * h, row < rows && b < count ? in_features : 0);
             return raw;
         }
 #pragma unroll
@@ -392,27 +399,9 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
     I32x8 x[B][T];
     uint32_t x_scales[(B * T + 3) / 4];  // four bytes each
     auto round = [&](const Raw& raw, int q) {
-        auto largest_of = [&](bool finite) {
-            uint32_t most = 0;
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    most = larger_sizes(most, finite ? finite_sizes(raw.piece[h][e]) : raw.piece[h][e] & 0x7fff7fffu);
-            most = max(most >> 16, most & 0xffffu);
-            most = max(most, (uint32_t)__shfl_xor((int)most, 16));
-            return max(most, (uint32_t)__shfl_xor((int)most, 32));
-        };
-        uint32_t most = largest_of(false);
-        if (__any(most >= kBf16Infinity)) most = largest_of(true);
-        const float scale = needed_scale(__uint_as_float(most << 16));
+        const float scale = quantize_row_block(raw.piece, x[q / T][q % T]);
         if (q % 4 == 0) x_scales[q / 4] = 0;
         x_scales[q / 4] |= (__float_as_uint(scale) >> 23) << (8 * (q % 4));
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            x[q / T][q % T][2 * h] = (int)fp8x4_of_bf16(raw.piece[h][0], raw.piece[h][1], scale);
-            x[q / T][q % T][2 * h + 1] = (int)fp8x4_of_bf16(raw.piece[h][2], raw.piece[h][3], scale);
-        }
     };
     // x, which lies in the L2 cache once the first workgroups have read it, is asked for first and rounded while the
     // weights are on the way: loads return in their order.
@@ -818,10 +807,10 @@ hipError_t launch_unpack_fp8(const Fp8PackParams& p, uint16_t* weight, hipStream
 
 hipError_t launch_linear_fp8(const LinearFp8Params& given, hipStream_t stream) {
     LinearFp8Params p = given;
-    p.wide = p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
     if (few_rows(p.rows, p.in_features)) {
         // (Whole pieces of eight inputs, within 2^31 bytes.)
-        p.wide = p.wide && p.in_features % 8 == 0 && p.rows * p.x_stride < ((int64_t)1 << 30);
+        p.wide = p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.in_features % 8 == 0 &&
+                 p.rows * p.x_stride < ((int64_t)1 << 30);
         p.exponents ? launch_few<true>(p, stream) : launch_few<false>(p, stream);
         return hipGetLastError();
     }
@@ -832,7 +821,7 @@ hipError_t launch_linear_fp8(const LinearFp8Params& given, hipStream_t stream) {
         p.y = given.y + first * p.y_stride;
         p.x_scales = reinterpret_cast<uint32_t*>(p.x_codes + fp8_row_bytes(p.rows, p.in_features));
         const dim3 grid((unsigned)(fours_of(p.in_features) * tiles_of(p.rows)));
-        if (p.wide)
+        if (p.in_features % 8 == 0)
             hipLaunchKernelGGL(quantize_rows_fp8_kernel<true>, grid, dim3(256), 0, stream, p);
         else
             hipLaunchKernelGGL(quantize_rows_fp8_kernel<false>, grid, dim3(256), 0, stream, p);

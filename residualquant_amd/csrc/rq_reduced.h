@@ -79,7 +79,7 @@ struct LinearFp8Params {
     int compute_units;        // of the launching device
     uint8_t* x_codes;         // workspace: x in operand order
     uint32_t* x_scales;       // set by the launch: workspace [fours of blocks][tiles of 16 rows][16], four E8M0 bytes each
-    bool wide;                // set by the launch: 16-byte loads of x
+    bool wide;                // set by the launch: 16-byte loads of a few rows of x
 };
 size_t fp8_code_bytes(int64_t out_features, int64_t in_features);
 size_t fp8_weight_bytes(int64_t out_features, int64_t in_features, bool exponents);
