@@ -771,10 +771,11 @@ size_t fp8_weight_bytes(int64_t out_features, int64_t in_features, bool exponent
 }
 
 // Whether every workgroup rounds x for itself, or a launch before the product does:
-// by x's blocks. (2048 -> 6144: 1 row 4.0 us against 8.2, 16 rows 5.3 against 7.1, 24 rows 6.9
-// against 8.1; 2048 -> 2048: 40 rows 8.2 against 8.1; 5632 -> 2048: 1 row 5.8 against
-// 10.1, 4 rows 6.3 against 9.9, 16 rows 9.1 against 9.2; 8192 -> 8192: 16 rows 18.3
-// against 15.8.)
+// by x's blocks. (2048 -> 6144: 1 row 4.4 us against 6.9, 16 rows 5.4 against 7.1, 24 rows 7.1
+// against 7.5, 40 rows 9.8 against 8.5; 2048 -> 2048: 32 rows 6.9 both; 5632 -> 2048: 1 row 5.9 against
+// 8.8, 11 rows 7.9 against 9.0, 16 rows 9.2 against 9.1; 2048 -> 50257: 32 rows 24.5 against 26.1. At
+// the most blocks the outputs decide too: 8192 inputs, 8 rows, 2048 outputs 9.6 against 10.5, 8192 outputs
+// 17.2 against 15.6; the workspace would then depend on them.)
 constexpr int64_t kFewMaxRows = 48, kFewMaxBlocks = 64, kFewMost = 512;
 static bool few_rows(int64_t rows, int64_t in_features) {
     const int64_t blocks = blocks_of(in_features);
