@@ -79,7 +79,8 @@ _CURRENT = nullcontext()
 
 def _on_device(device: int):
     """A context on CUDA device ``device`` (nothing to do where it is current)."""
-    return _CURRENT if torch.cuda.current_device() == device else torch.cuda.device(device)
+    # (torch.cuda.current_device() would ask first whether the device is initialised, which a tensor on it answers.)
+    return _CURRENT if torch._C._cuda_getDevice() == device else torch.cuda.device(device)
 
 
 def _stream(device: int) -> int:
