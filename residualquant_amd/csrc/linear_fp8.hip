@@ -665,8 +665,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
 }
 
-// One workgroup per compute unit at most: x is read and rounded by each. (16 rows, 2048 -> 11264: 6.1 us, with
-// two 7.8; 2048 -> 50257 21.4 and 20.7.)
+// One workgroup per compute unit at most: x is read and rounded by each. (32 rows, 2048 -> 11264: 8.9 us, with
+// two 12.3; -> 50257 24.7 and 25.1, 16 rows 21.2 and 21.1.)
 template <bool Exponents, int T, int W, int B>
 void launch_few_of(const LinearFp8Params& p, hipStream_t stream) {
     const unsigned grid = (unsigned)std::min<int64_t>(out_tiles_of(p.out_features), p.compute_units);
