@@ -315,12 +315,11 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
         for (int t = 0; t < T; ++t) partial[wave][j * T + t][lane] = total[j][t];
     __syncthreads();
     // The waves share the tiles out, a pair with neighbouring outputs at a time.
-    constexpr int kPair = J > 1 ? 2 : 1;
-    for (int q = wave; q < J / kPair * T; q += 8) {
-        const int j = kPair * (q / T), t = q % T;
-        F32x4 sum[kPair];
+    for (int q = wave; q < J / 2 * T; q += 8) {
+        const int j = 2 * (q / T), t = q % T;
+        F32x4 sum[2];
 #pragma unroll
-        for (int h = 0; h < kPair; ++h) {
+        for (int h = 0; h < 2; ++h) {
             sum[h] = partial[0][(j + h) * T + t][lane];
 #pragma unroll
             for (int w = 1; w < 8; ++w) sum[h] += partial[w][(j + h) * T + t][lane];
@@ -328,16 +327,14 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
         const int64_t n = output_of(tile0 + j, 4 * g), m = 16 * (row_tile0 + t) + i;
         if (m >= p.rows) continue;
         uint16_t* const to = p.y + m * p.y_stride + n;
-        if (kPair == 2 && n + 8 <= p.out_features) {
-            const F32x4 u = sum[0], v = sum[kPair - 1];
+        if (n + 8 <= p.out_features) {
+            const F32x4 u = sum[0], v = sum[1];
             *reinterpret_cast<U32x4At2*>(to) = U32x4{bf16x2_rn(u[0], u[1]), bf16x2_rn(u[2], u[3]), bf16x2_rn(v[0], v[1]), bf16x2_rn(v[2], v[3])};
             continue;
         }
 #pragma unroll
-        for (int h = 0; h < kPair; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (n + 4 * h + r < p.out_features) to[4 * h + r] = (uint16_t)bf16_rn(sum[h][r]);
+        for (int r = 0; r < 8; ++r)
+            if (n + r < p.out_features) to[r] = (uint16_t)bf16_rn(r < 4 ? sum[0][r] : sum[1][r - 4]);
     }
 }
 
@@ -443,7 +440,6 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
                 multiply(std::integral_constant<int, b * T>{});
                 if constexpr (T > 1) multiply(std::integral_constant<int, b * T + 1>{});
                 if constexpr (T > 2) multiply(std::integral_constant<int, b * T + 2>{});
-                if constexpr (T > 3) multiply(std::integral_constant<int, b * T + 3>{});
             }
             load(held[b], b);  // the next tile's
         };
