@@ -427,7 +427,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache: 
     x[2 i + 1])``, are turned by the angles whose FP32 ``cos``/``sin`` ``[max_position,
     channels / 2]`` hold in the row of the token's place in its request, or of
     ``positions`` (INT64 ``[rows]``) where given (clamped to the tables).  Rows
-    outside ``query_start_loc`` are left as they are.
+    outside ``query_start_loc`` are left as they are (in new tensors, without values).
     """
     # (A decode step's call runs 5 us on the GPU: each tensor's shape and strides are read once.)
     shape, strides = qkv.shape, qkv.stride()
