@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
@@ -300,3 +302,25 @@ def test_refusals(device):
         step_ops.pack_weight_fp8(codes.float(), torch.ones((1, 2), device=device))
     with pytest.raises(RuntimeError, match="8-bit weights need"):
         step_ops.quantize_weight_fp8(torch.empty((0, 16), dtype=torch.bfloat16, device=device))
+
+
+def test_seeded_random_shapes(device):
+    """Exact sums over sizes, strides and alignments drawn from the whole range, beside each other in one process."""
+    rng = random.Random(7)
+    for call in range(80):
+        rows, out, features = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 13.5)), int(2 ** rng.uniform(0, 13))
+        kind, pad, lead, beside = rng.choice("ef"), rng.choice([0, 0, 1, 3, 8]), rng.choice([0, 0, 1, 4, 8]), rng.choice([0, 0, 1, 2, 8])
+        print(f"call={call} rows={rows} out={out} in={features} {kind} pad={pad} lead={lead} beside={beside}", flush=True)
+        g = torch.Generator(device=device).manual_seed(call)
+        codes = torch.randint(-3, 4, (out, features), generator=g, device=device).float().to(torch.float8_e4m3fn)
+        exponents = torch.randint(-2, 3, (-(-out // BLOCK), -(-features // BLOCK)), generator=g, device=device)
+        scales = (exponents + 127).to(torch.uint8).view(torch.float8_e8m0fnu) if kind == "e" else torch.exp2(exponents.float())
+        x = torch.zeros(rows * (features + pad) + lead, dtype=torch.bfloat16, device=device)[lead:].view(rows, -1)[:, :features]
+        x.copy_(torch.randint(-8, 9, (rows, features), generator=g, device=device))
+        full = torch.exp2(exponents.double()).repeat_interleave(BLOCK, 0)[:out].repeat_interleave(BLOCK, 1)[:, :features]
+        want = (x.double() @ (codes.double() * full).t()).float().to(torch.bfloat16)
+        around = torch.full((rows + 2, out + beside), 7.0, dtype=torch.bfloat16, device=device)
+        step_ops.linear_fp8(x, step_ops.pack_weight_fp8(codes, scales), out=around[1:-1, :out])
+        assert torch.equal(around[1:-1, :out], want)
+        around[1:-1, :out] = 7.0
+        assert bool((around == 7.0).all())
