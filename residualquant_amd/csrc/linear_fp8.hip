@@ -18,8 +18,11 @@
 // waves read at a time is whole stretches of 8 KB and more, which all channels of
 // the L2 cache hold alike.  (With each tile's blocks in a row, at 2048 inputs a tile
 // begins every 32 KB, and workgroups at the same block met in half the channels.)
-// The instruction multiplies by powers of two as it goes: sx always, sw if it
-// is an exponent; an FP32 sw multiplies each block's FP32 sum instead.
+// The instruction multiplies by powers of two as it goes: sx and sw, if that is an
+// exponent. An FP32 sw is split in two: its power of two goes the same way and the factor of [1, 2)
+// that is left multiplies the block's FP32 sum, so that this is in range wherever the
+// block's part of the result is. (With sw multiplied afterwards, scales of 2^-12 and results
+// from 2^116 on, the sum before passed 2^128.)
 //
 // What the 8-bit instructions cost in exactness: beside FP32 sums they line the 16
 // products of a lane's piece up with the largest and cut what lies below 2^-13 of its power of two.
@@ -76,6 +79,13 @@ __host__ __device__ __forceinline__ int64_t fours_of(int64_t in_features) { retu
 __device__ __forceinline__ int scale_exponent(float largest) { return (int)(__float_as_uint(needed_scale(largest)) >> 23); }
 // 2^(127 - byte): what a value is multiplied by before its rounding, exactly (byte <= 247).
 __device__ __forceinline__ float inverse_scale(int exponent) { return __uint_as_float((uint32_t)(254 - exponent) << 23); }
+
+// An FP32 scale as 2^(power - 127) x factor, exactly: |factor| in [1, 2), below for a subnormal scale; what is
+// not finite stays in the factor.
+__device__ __forceinline__ uint32_t scale_power(float scale) {
+    return min(max((__float_as_uint(scale) >> 23) & 0xffu, 1u), 254u);
+}
+__device__ __forceinline__ float scale_factor(float scale, uint32_t power) { return __builtin_amdgcn_ldexpf(scale, 127 - (int)power); }
 
 __device__ __forceinline__ float finite_size(float x) { return fabsf(x) < __builtin_inff() ? fabsf(x) : 0.f; }
 
@@ -286,6 +296,9 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
         for (int t = 0; t < T; ++t) total[j][t] = F32x4{0.f, 0.f, 0.f, 0.f};
     auto multiply = [&](const Block& of, int b) {
         const int shift = 8 * (b & 3);
+        uint32_t power = 0;
+        float factor = 0.f;
+        if constexpr (!Exponents) power = scale_power(of.scale), factor = scale_factor(of.scale, power);
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -293,9 +306,9 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
                 if constexpr (Exponents) {
                     total[j][t] = mfma(of.a[j], of.x[t], total[j][t], of.scale >> shift, of.words[t] >> shift);
                 } else {
-                    const F32x4 sum = mfma(of.a[j], of.x[t], F32x4{0.f, 0.f, 0.f, 0.f}, 127u, of.words[t] >> shift);
+                    const F32x4 sum = mfma(of.a[j], of.x[t], F32x4{0.f, 0.f, 0.f, 0.f}, power, of.words[t] >> shift);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(of.scale, sum[r], total[j][t][r]);
+                    for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(factor, sum[r], total[j][t][r]);
                 }
             }
     };
@@ -428,9 +441,11 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
             if constexpr (Exponents) {
                 total[t] = mfma<0, Q % 4>(held[b].a, x[b][t], total[t], held[b].scale, x_scales[Q / 4]);
             } else {
-                const F32x4 sum = mfma<0, Q % 4>(held[b].a, x[b][t], F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scales[Q / 4]);
+                const uint32_t power = scale_power(held[b].scale);
+                const float factor = scale_factor(held[b].scale, power);
+                const F32x4 sum = mfma<0, Q % 4>(held[b].a, x[b][t], F32x4{0.f, 0.f, 0.f, 0.f}, power, x_scales[Q / 4]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) total[t][r] = fmaf(held[b].scale, sum[r], total[t][r]);
+                for (int r = 0; r < 4; ++r) total[t][r] = fmaf(factor, sum[r], total[t][r]);
             }
         };
         auto block = [&](auto number) {
@@ -525,7 +540,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     I32x8 a[2][4];
     U32x4 piece[kPieces];
     uint32_t word;  // of x's scales, on its way to LDS
-    Scales w_scales;
+    Scales w_scales;  // FP32: their factors
+    uint32_t w_powers = 0;  // FP32: their powers of two, a byte each
     auto load_x = [&](int b) {
 #pragma unroll
         for (int c = 0; c < kPieces; ++c)
@@ -552,13 +568,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (tid < 16 * NT) x_words[four & 1][tid] = word;
     };
     auto load_scales = [&](int four) {
-        Scales v = scales_of[four];
-        if constexpr (Exponents)
-            v = __builtin_amdgcn_readfirstlane(v);
-        else
+        const Scales v = scales_of[four];
+        if constexpr (Exponents) {
+            w_scales = __builtin_amdgcn_readfirstlane(v);
+        } else {
+            uint32_t powers = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v[e])));
-        return v;
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t power = scale_power(v[e]);
+                w_scales[e] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(scale_factor(v[e], power))));
+                powers |= power << (8 * e);
+            }
+            w_powers = powers;
+        }
     };
     // Block 4 four + S.
     auto step = [&](auto place, int four) {
@@ -576,6 +598,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         uint32_t x_scale[2];
         x[0] = operand(from, lane);
         x_scale[0] = from_words[0];
+        // FP32 scales: a row tile's sums are added while the next one's products run, if the registers last (of 128 rows
+        // 38 would spill: right behind each product then).
+        constexpr bool kLater = !Exponents && NT < 8;
+        F32x4 sum[4];
+        auto add = [&](int j, int t) {
+            if constexpr (!Exponents)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(w_scales[S], sum[j][r], total[j][t][r]);
+        };
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if (t + 1 < NT) {
@@ -587,20 +618,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 if constexpr (Exponents) {
                     total[j][t] = mfma<S, S>(a[S & 1][j], x[t & 1], total[j][t], w_scales, x_scale[t & 1]);
                 } else {
-                    const F32x4 sum = mfma<0, S>(a[S & 1][j], x[t & 1], F32x4{0.f, 0.f, 0.f, 0.f}, 127u, x_scale[t & 1]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) total[j][t][r] = fmaf(w_scales[S], sum[r], total[j][t][r]);
+                    if (kLater && t > 0) add(j, t - 1);
+                    sum[j] = mfma<S, S>(a[S & 1][j], x[t & 1], F32x4{0.f, 0.f, 0.f, 0.f}, w_powers, x_scale[t & 1]);
+                    if (!kLater) add(j, t);
                 }
             }
         }
+        if constexpr (kLater)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) add(j, NT - 1);
         // The operands of a row tile are read while the products of the one before run.
         __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
-        for (int t = 0; t < NT - 1; ++t) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+        for (int t = 0; t < NT; ++t) {
+            if (t < NT - 1) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+            if constexpr (kLater) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (t > 0) __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
+            } else {
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+            }
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
         if constexpr (S & 1) lds_barrier();
     };
 
@@ -614,7 +655,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     };
     begin();
     while (true) {
-        w_scales = load_scales(0);
+        load_scales(0);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -630,7 +671,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
             if (4 * four + 1 < blocks) step(std::integral_constant<int, 1>{}, four);
             if (4 * four + 2 < blocks) step(std::integral_constant<int, 2>{}, four);
             if (4 * four + 3 < blocks) step(std::integral_constant<int, 3>{}, four);
-            w_scales = load_scales(min(four + 1, fours - 1));
+            load_scales(min(four + 1, fours - 1));
         }
         // The next tile's first block, then this one's results.
         const int64_t out_at = 16 * tile0 + 8 * g, row_at = 16 * row_tile0 + i;

@@ -1,0 +1,93 @@
+"""Scales of any size in 8-bit projections (step_ops.linear_fp8): blocks, rows and results far from 1."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from residualquant_amd import step_ops
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 128
+
+# One row, few, some (rounded by a launch before) and many rows; tiles of 256 outputs from the sixth on.
+SIZES = [(1, 40, 300), (9, 200, 5000), (20, 300, 1000), (40, 150, 1500), (129, 140, 513), (257, 2050, 200), (130, 6300, 640),
+         (700, 8300, 300), (2050, 8300, 384)]
+
+# Powers of x, of the codes and of the scales: where the block's sum without its scale passes 2^128, where it lies
+# below 2^-126, and where only the scale is far from 1 (a subnormal one, the largest).
+POWERS = [(118, 6, -20), (113, 6, -30), (120, 0, -100), (-120, -9, 60), (-118, -9, 120), (100, 0, -140), (-125, 0, 125), (0, 0, 0),
+          (60, 6, 40)]
+
+
+@pytest.mark.parametrize("rows,out,features", SIZES)
+@pytest.mark.parametrize("of_x,of_codes,of_scales", POWERS)
+def test_float_scales_of_any_size(device, rows, out, features, of_x, of_codes, of_scales):
+    """Whole numbers times powers of two, and scales of three bits: with its scale FP32 holds every sum exactly (24 x 5000
+    x 2^2 eighths < 2^24), so the result is the formula's, rounded once, wherever it lies in FP32's normal range."""
+    print(f"rows={rows} out={out} in={features} x 2^{of_x} codes 2^{of_codes} scales 2^{of_scales}", flush=True)
+    g = torch.Generator().manual_seed(rows + of_x)
+    whole = torch.randint(-3, 4, (out, features), generator=g).float()
+    codes = (whole * 2.0 ** of_codes).to(torch.float8_e4m3fn)
+    assert torch.equal(codes.float(), whole * 2.0 ** of_codes)
+    shape = (-(-out // BLOCK), -(-features // BLOCK))
+    parts = torch.tensor([1.0, 1.25, 1.5, 1.75, -1.0, -1.5, 2.0, 0.0])[torch.randint(0, 8, shape, generator=g)]
+    scales = (parts.double() * 2.0 ** of_scales).float()
+    assert torch.equal(scales.double(), parts.double() * 2.0 ** of_scales)
+    small = torch.randint(-8, 9, (rows, features), generator=g).float()
+    x = (small.double() * 2.0 ** of_x).to(torch.bfloat16)
+    assert torch.equal(x.double(), small.double() * 2.0 ** of_x)
+    full = parts.repeat_interleave(BLOCK, 0)[:out].repeat_interleave(BLOCK, 1)[:, :features]
+    sums = small @ (whole * full).t()  # exact: quarters below 2^24
+    want = (sums.double() * 2.0 ** (of_x + of_codes + of_scales)).float()
+    assert bool(want.isfinite().all())
+    got = step_ops.linear_fp8(x.to(device), step_ops.pack_weight_fp8(codes.to(device), scales.to(device)))
+    assert torch.equal(got.cpu(), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("kind", ["exponents", "float"])
+@pytest.mark.parametrize("rows,out,features", [(1, 200, 300), (33, 300, 640), (200, 300, 640), (600, 2200, 640)])
+def test_scales_that_are_none_and_the_largest(device, rows, out, features, kind):
+    """A NaN scale makes its outputs NaN and no other; an infinite one (FP32) gives what its block's sum times infinity is;
+    beside codes of 0 the largest scales and rows give 0."""
+    g = torch.Generator().manual_seed(rows)
+    whole = torch.randint(1, 4, (out, features), generator=g).float()
+    whole[:, 256:] = 0.0  # of the last block(s)
+    codes = whole.to(torch.float8_e4m3fn)
+    shape = (-(-out // BLOCK), -(-features // BLOCK))
+    x = torch.randint(1, 9, (rows, features), generator=g).to(torch.bfloat16)
+    x[:, 256:] = 3.0e38
+    x[rows // 2:] = -x[rows // 2:]
+    values = torch.ones(shape, dtype=torch.float64)
+    values[0, 1], values[1, 0] = torch.nan, torch.nan if kind == "exponents" else torch.inf
+    if kind == "exponents":
+        raw = torch.full(shape, 127, dtype=torch.uint8)
+        raw[:, 2:], raw[0, 1], raw[1, 0] = 254, 255, 255
+        scales = raw.view(torch.float8_e8m0fnu)
+    else:
+        scales = values.float()
+        scales[:, 2:] = 3.4e38
+    want = torch.zeros((rows, out), dtype=torch.float64)
+    for block in range(2):  # (the others' codes are 0)
+        part = slice(block * BLOCK, (block + 1) * BLOCK)
+        sums = x[:, part].double() @ whole[:, part].double().t()
+        want += sums * values[:, block].repeat_interleave(BLOCK)[None, :out]
+    got = step_ops.linear_fp8(x.to(device), step_ops.pack_weight_fp8(codes.to(device), scales.to(device))).cpu()
+    want = want.float().to(torch.bfloat16)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(nan=5.0, posinf=torch.inf, neginf=-torch.inf),
+                       want.nan_to_num(nan=5.0, posinf=torch.inf, neginf=-torch.inf))
+
+
+def test_least_exponent(device):
+    """An exponent byte of 0 is 2^-127, in the product and restored."""
+    codes = torch.full((16, 128), 448.0).to(torch.float8_e4m3fn)
+    scales = torch.zeros((1, 1), dtype=torch.uint8).view(torch.float8_e8m0fnu)
+    packed = step_ops.pack_weight_fp8(codes.to(device), scales.to(device))
+    assert bool((packed.dequantize().double().cpu() == 448.0 * 2.0 ** -127).all())
+    for rows in (1, 100):
+        x = torch.zeros((rows, 128), dtype=torch.bfloat16)
+        x[:, 5] = 2.0 ** 100
+        got = step_ops.linear_fp8(x.to(device), packed).double().cpu()
+        assert bool((got == 448.0 * 2.0 ** -27).all())
