@@ -91,3 +91,35 @@ def test_least_exponent(device):
         x[:, 5] = 2.0 ** 100
         got = step_ops.linear_fp8(x.to(device), packed).double().cpu()
         assert bool((got == 448.0 * 2.0 ** -27).all())
+
+
+@pytest.mark.parametrize("kind", ["exponents", "float"])
+@pytest.mark.parametrize("rows", [1, 33, 200, 600])
+def test_small_products_beside_large_ones_that_cancel(device, rows, kind):
+    """448 x 448 and its negative leave small products alone.  Of the 16 that one lane multiplies (of each 64 inputs the
+    runs of eight at 8 g and at 32 + 8 g) those of 2^-13 of the largest's power of two and more are kept, each is off
+    by less than that, and others are not touched.
+
+    448 x 448 = 1.53 x 2^17: 2^4 x 1 beside it is exact, 16 products are off by at most 16 x 2^4 = 2^8 together."""
+    out, features = 144, 256
+    whole = torch.ones((out, features))
+    whole[:, 3], whole[:, 128 + 3] = 448.0, -448.0
+    codes = whole.to(torch.float8_e4m3fn)
+    shape = (2, 2)
+    scales = torch.full(shape, 127, dtype=torch.uint8).view(torch.float8_e8m0fnu) if kind == "exponents" else torch.ones(shape)
+    packed = step_ops.pack_weight_fp8(codes.to(device), scales.to(device))
+    x = torch.zeros((rows, features), dtype=torch.bfloat16)
+    x[:, 3], x[:, 128 + 3] = 448.0, 448.0
+
+    def product(x):
+        return step_ops.linear_fp8(x.to(device), packed).double().cpu()
+
+    assert bool((product(x) == 0).all())
+    beside, apart = x.clone(), x.clone()
+    beside[:, 4] = 16.0  # (among the same 16)
+    assert bool((product(beside) == 16.0).all())
+    apart[:, 20], apart[:, 128 + 90] = 2.0 ** -6, 2.0 ** -5  # (among others)
+    assert bool((product(apart) == 3 * 2.0 ** -6).all())
+    small = x.clone()
+    small[:, 4:8], small[:, 32:40] = 1.0, 3.0
+    assert bool(((product(small) - 28.0).abs() <= 2.0 ** 8 + 2.0 ** -8 * 284).all())
