@@ -258,8 +258,7 @@ __device__ __forceinline__ F32x4 mfma(I32x8 a, I32x8 b, F32x4 c, uint32_t scale_
 
 // Up to some hundred rows: one workgroup of eight waves per J tiles of outputs and T tiles of 16 rows. The
 // waves share the inputs out, each with operands straight from global memory (whole
-// stretches of 2 KB) and a block's in flight while the one before is multiplied,
-// and join through LDS.
+// stretches of 2 KB), two blocks in turn, and join through LDS.
 template <int J, int T, bool Exponents>
 __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Params p) {
     __shared__ F32x4 partial[8][J * T][64];
@@ -312,8 +311,9 @@ __global__ __launch_bounds__(512) void linear_fp8_split_kernel(const LinearFp8Pa
                 }
             }
     };
-    // (Loads without a condition, past the end the last block again: after a load that one path leaves out every wait
-    // is for all loads in flight.)
+    // (Past the end the last block is loaded again. The compiler moves next's loads into the branch that multiplies it,
+    // behind the loads of the block after it, and the wait there is for all of them: a pair of blocks pays one round
+    // trip that no product covers.)
     Block now, next;
     load(now, min(begin, blocks - 1));
     for (int b = begin; b < end; b += 2) {
@@ -492,10 +492,12 @@ __global__ __launch_bounds__(64 * W) void linear_fp8_few_kernel(const LinearFp8P
 // wave 64 outputs.  x passes LDS, where the four waves of its rows
 // read it, in a ring of four blocks of inputs with a barrier every two; the weights
 // go from global memory to the operands, since their order there is the operands'
-// own and only two waves share them.  (Through LDS both would take it 128 bytes a
+// own and no two waves of a workgroup share them.  (Through LDS both would take it 128 bytes a
 // cycle, all that it has, at the matrix instructions' full rate.)  What a block
 // reads from global memory was asked for a block ahead, and a tile's first block
-// before the results of the tile before it are stored.
+// before the results of the tile before it are stored.  (Two waits are for every load in
+// flight: the next four blocks' scales are made uniform as soon as they are asked for, and a
+// tile begins with the rows of two blocks loaded and stored in turn.)
 template <bool Exponents, int NT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_fp8_wide_kernel(const LinearFp8Params p) {
     constexpr int kPieces = NT * kTileBytes / 16 / 256;  // 16-byte pieces of x per thread and block
@@ -747,8 +749,10 @@ void launch_wide(const LinearFp8Params& p, hipStream_t stream) {
 // The kernel for rows in operand order: by what its rounds of workgroups take, two
 // per compute unit or one in the last, a block of inputs at a time. Measured in us per
 // block with one workgroup on a compute unit and with two, and per round (the join,
-// the first loads); of 38 shapes from 32 to 8192 rows the choice takes the fastest
-// of the six, or up to 10% longer. (1018 rows, 2048 -> 11264: tiles of 256 x 96 31.5 us, x 64
+// the first loads; two of 64 x 64 take 256 KB of LDS and follow one another); of 38 shapes
+// from 32 to 8192 rows the choice takes the fastest of the six, or up to 10% longer. Fewer rows over inputs too
+// long for the kernel above are not among these: up to 16 multiply a tile of x twice (1 row, 16384 -> 2048
+// 15.8 us, 16 rows 16.1, 31 rows, 8192 -> 2048 11.7). (1018 rows, 2048 -> 11264: tiles of 256 x 96 31.5 us, x 64
 // 33.2, x 128 39.1, 64 x 64 74. 40 rows, 5632 -> 2048: 32 x 32 6.1, 64 x 64 10.3. 512 rows,
 // 5632 -> 2048: 64 x 64 18.6, 256 x 64 30.9.)
 struct Tiling {

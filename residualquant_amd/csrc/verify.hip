@@ -10,8 +10,9 @@
 // and counts itself; the last of a request's workgroups finds the chunk and then,
 // reading it once more, the token in it. (A launch of its own for the draw, a wave per
 // request: 14.1 us for one request of 49152 tokens, 50.9 for 64 of 151000.) Bytes
-// bound many requests, the chain of dependent loads (query starts, tokens and numbers,
-// their probabilities, the row, the sums, the chunk) a few.
+// bound many requests, the chain of dependent loads a few: query starts, tokens, their
+// probabilities, the numbers they are judged by, the request's last number, the row, the
+// sums, the chunk. (Both kinds of numbers need the query starts alone, but are waited for in this order.)
 //
 // Sums are FP64: in FP32 their rounding, some 10^-7 of the whole, would move one
 // border in thirty among 150000 tokens past a given u; in FP64 none.
@@ -313,8 +314,9 @@ int loads_of(int64_t requests, int64_t vocab, bool bf16) {
     return requests * ((vocab + least - 1) / least) <= 1024 ? 1 : 4;
 }
 
-// Workgroups of a request: 1024 over all requests, but at least 8 and at most 64, as
-// each finds the final row for itself and all count in one word. (One workgroup per
+// Workgroups of a request: 1024 over all requests, but at least 8 (or one a chunk) and at most 64, as
+// each finds the final row for itself and all count in one word; an eighth of the chunks
+// where there are more than 512, as a workgroup takes at most kMostChunks. (One workgroup per
 // chunk, the words of eight requests in a cache line: 64 requests of 151000 tokens 47.2 us
 // and 18.1, 4 of them 21.1 and 9.6. At most 16, a line for each word: 18.5 and 13.1; 32: 18.2 and 10.8;
 // 64, words side by side: 18.5 and 12.4.)
